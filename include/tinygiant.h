@@ -411,6 +411,107 @@ void tg_sampler_destroy(tg_sampler *s);
 int tg_head_sample(tg_head *h, const float *x, float eps, float temperature, double top_p, double u,
                    float *logits, int32_t *token);
 
+/* ------------------------------------------------------------------ */
+/* attention block on the device: paged Q4_0 KV cache, int8 products    */
+/* ------------------------------------------------------------------ */
+/* What tg_attention_decode (tinygiant/engine.py:199-227) does for one token
+ * on host memory, as device calls for ragged batches.  All of them take
+ * device pointers and a HIP stream, run on that stream's device (the calling
+ * thread's current device for NULL), keep the thread's current device,
+ * allocate nothing, read no host copy of device data and are asynchronous;
+ * captured into a HIP graph they replay on whatever the buffers then hold.
+ * Element types: */
+#define TG_T_F32 0
+#define TG_T_F16 1
+#define TG_T_BF16 2
+
+/* One layer of a paged cache and a ragged batch over it.
+ *
+ * pages: [n_pages][n_kv_heads][page_tokens / 16] tiles of 16 tokens, 18 *
+ * head_dim bytes each (16-byte aligned; head_dim 64, 128 or 256; page_tokens
+ * a multiple of 16).  A tile holds Q4_0 blocks of 32 values (value = scale *
+ * (code - 8), scale fp16): the K codes (8 * head_dim bytes), the V codes (8 *
+ * head_dim), the K scales (head_dim), the V scales (head_dim), ordered so
+ * that a wave's 16-byte loads are operands of the matrix instructions
+ * (halfwords of 4 codes, code n in bits 4 n.., NG = head_dim / 32):
+ *   K, token r, dim 32 g + 8 h + 2 n + p: halfword ((h 16 + r) NG + g) 2 + p
+ *   V, token r, dim 16 (4 b + n) + c:
+ *       halfword (((r / 4) 16 + c) 2 + (r % 4) / 2) NG + 2 b + r % 2
+ *   K scale, token r, block g: half r NG + g
+ *   V scale, token r, block g: half ((r / 2) NG + g) 2 + r % 2
+ *
+ * Sequence s has kv_len[s] cached tokens, the batch's own among them; token
+ * p of it sits in page table[s * table_stride + p / page_tokens].  Rows
+ * cu[s] .. cu[s + 1] - 1 of the row tensors are its last tokens, the last
+ * one at position kv_len[s] - 1; rows from cu[n_seqs] on (padding) are
+ * neither read nor written.  Two sequences may share pages that the call
+ * only reads.  table, cu and kv_len are read on the device: a page outside
+ * 0..n_pages-1, or a position at or beyond table_cols * page_tokens, that a
+ * call needs makes NaN of the rows that need it (and is not written); no
+ * memory outside the arguments is touched. */
+typedef struct {
+    void *pages;
+    const int32_t *table;   /* [n_seqs][table_cols], rows table_stride apart */
+    const int32_t *cu;      /* [n_seqs + 1], from 0, not decreasing */
+    const int32_t *kv_len;  /* [n_seqs] */
+    int64_t n_pages;
+    int32_t page_tokens, n_kv_heads, head_dim;
+    int32_t table_cols, table_stride;
+    int32_t n_seqs, n_tokens; /* sequences, rows of the row tensors */
+} tg_kv_batch;
+
+/* New rows into the cache.  q [n_tokens][n_heads][head_dim], k and v
+ * [n_tokens][n_kv_heads][head_dim] of one element type, rows *_stride
+ * elements apart (multiples of 4, pointers aligned to 4 elements), so that
+ * views of one projection's rows do.  Per head: x <- x / rms(x) * norm_w
+ * (q_norm, k_norm: head_dim floats, NULL: no norm; eps), then the rotation of
+ * tg_attention_decode by the row of the token's position (rope_cos, rope_sin
+ * [max_pos][head_dim / 2]; both NULL: none), in fp32; q is rounded to its
+ * type into q_out (may be q), k and v (v as it is) are held in Q4_0: values
+ * beyond fp16's range saturate to +-65504, NaN makes its block NaN.  A token
+ * at a position below 0 or at or beyond max_pos is not written and its q_out
+ * row is NaN.  q may be NULL with n_heads 0. */
+int tg_kv_append_q4_dev(const tg_kv_batch *b, int type, const void *q,
+                        int64_t q_stride, const void *k, int64_t k_stride,
+                        const void *v, int64_t v_stride, void *q_out,
+                        int64_t q_out_stride, int n_heads,
+                        const float *q_norm, const float *k_norm, float eps,
+                        const float *rope_cos, const float *rope_sin,
+                        int max_pos, void *stream);
+/* The values the cache holds for the batch's rows, fp16 k and v [n_tokens]
+ * [n_kv_heads][head_dim] (16-byte aligned).  With cu counting whole sequences
+ * it reads them back whole (tg_arena_read_layer's role for the cache). */
+int tg_kv_read_q4_dev(const tg_kv_batch *b, void *k, void *v, void *stream);
+/* Causal grouped-query attention of the batch's rows over the cache: row at
+ * position p sees positions 0..p; out = softmax(scale * q . k) v, q and out
+ * [n_tokens][n_heads][head_dim] fp16 or bf16, rows *_stride elements apart
+ * (multiples of 8, pointers 16-byte aligned), out not overlapping q.  A row
+ * at a position below 0 sees nothing and is zero.  n_heads is a multiple of
+ * n_kv_heads.  max_len: about the longest kv_len (0: table_cols *
+ * page_tokens); it sets how the work is split, results hold for any.
+ * workspace: at least tg_attn_q4_workspace bytes, 16-byte aligned, free
+ * again when the call's work is done. */
+size_t tg_attn_q4_workspace(const tg_kv_batch *b, int n_heads, int max_len);
+int tg_attn_q4_dev(const tg_kv_batch *b, int type, const void *q,
+                   int64_t q_stride, int n_heads, float scale, void *out,
+                   int64_t out_stride, int max_len, void *workspace,
+                   size_t workspace_bytes, void *stream);
+/* out [M][N] = x [M][K] times int8 weights w [N][K] (scale w_scale[n] per
+ * channel), activations quantised per row on the way: xn = x / rms(x) *
+ * norm_w (norm_w K floats, NULL: xn = x; eps), a = max |xn|, q = rint(127 xn /
+ * a) (decided as in 64 bits), out = (sum_k q w) * (a / 127) * w_scale[n] +
+ * residual (NULL: none; of out's type, may be out).  The int32 sums are
+ * exact.  A row that holds NaN or inf is NaN.  x and out of any element
+ * type, rows *_stride elements apart; out overlaps neither x nor w.  w
+ * 16-byte aligned, K a multiple of 16 up to 131072.  workspace as above. */
+size_t tg_matmul_i8_workspace(int M, int N, int K);
+int tg_matmul_i8_dev(const void *x, int x_type, int64_t x_stride,
+                     const float *norm_w, float eps, const int8_t *w,
+                     const float *w_scale, const void *residual,
+                     int64_t residual_stride, void *out, int out_type,
+                     int64_t out_stride, int M, int N, int K, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

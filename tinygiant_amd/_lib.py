@@ -22,6 +22,7 @@ CI = ctypes.c_int
 CF = ctypes.c_float
 SZ = ctypes.c_size_t
 U64 = ctypes.c_uint64
+I64 = ctypes.c_int64
 CD = ctypes.c_double
 
 # (name, restype, argtypes) of the reference ABI, tinygiant/_lib.py:39-74
@@ -101,6 +102,12 @@ NEW_SYMBOLS = [
     ("tg_mirror_mode", CI, [CI]),
     ("tg_debug_fault_inject", CI, [ctypes.c_uint32, CI]),
     ("tg_clock_mfma_mhz", CI, [CI, VP, VP, VP]),
+    ("tg_kv_append_q4_dev", CI, [VP, CI, VP, I64, VP, I64, VP, I64, VP, I64, CI, VP, VP, CF, VP, VP, CI, VP]),
+    ("tg_kv_read_q4_dev", CI, [VP, VP, VP, VP]),
+    ("tg_attn_q4_workspace", SZ, [VP, CI, CI]),
+    ("tg_attn_q4_dev", CI, [VP, CI, VP, I64, CI, CF, VP, I64, CI, VP, SZ, VP]),
+    ("tg_matmul_i8_workspace", SZ, [CI, CI, CI]),
+    ("tg_matmul_i8_dev", CI, [VP, CI, I64, VP, CF, VP, VP, VP, I64, VP, CI, I64, CI, CI, CI, VP, SZ, VP]),
 ]
 
 ALL_SYMBOLS = LEGACY_SYMBOLS + UNREGISTERED_SYMBOLS + NEW_SYMBOLS

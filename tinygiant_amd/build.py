@@ -16,7 +16,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libtinygiant.so"
-SOURCES = ["tg_kernels.hip", "tg_moe.hip", "tg_mfma.hip", "tg_legacy.hip", "tg_sample.hip", "tg_abi.hip"]
+SOURCES = ["tg_kernels.hip", "tg_moe.hip", "tg_mfma.hip", "tg_legacy.hip", "tg_sample.hip", "tg_attn.hip",
+           "tg_linear.hip", "tg_abi.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("TG_OFFLOAD_ARCH", "gfx950")
@@ -59,7 +60,9 @@ EXTRA_FLAGS = {"tg_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-a
                "tg_moe.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
                "tg_kernels.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
                "tg_legacy.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
-               "tg_sample.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"]}
+               "tg_sample.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
+               "tg_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-kernarg-preload-count=16"],
+               "tg_linear.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-kernarg-preload-count=16"]}
 
 
 def build(verbose: bool = False) -> Path:

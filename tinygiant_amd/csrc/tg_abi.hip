@@ -2437,3 +2437,186 @@ extern "C" int tg_head_sample(tg_head *h, const float *x, float eps, float tempe
     if (logits) HIP_TRY(hipMemcpyAsync(logits, h->logits, sizeof(float) * (size_t)h->vocab, hipMemcpyDeviceToHost, st));
     return sampler_run(h->smp, h->logits, temperature, top_p, u, token, nullptr);
 }
+
+// ------------------------------------------------------- attention block
+// The stream's device (the thread's current one for the null stream) is made
+// current for the launches and the thread's own put back.
+struct DeviceOf {
+    int prev = -1, rc = TG_OK;
+    explicit DeviceOf(hipStream_t st) {
+        int n = 0, cur = 0, dev = 0;
+        if (hipGetDeviceCount(&n) != hipSuccess || n <= 0) {
+            (void)hipGetLastError();
+            rc = set_err(TG_E_NODEVICE, "no HIP device visible");
+            return;
+        }
+        if (!st) return;
+        hipError_t e = hipGetDevice(&cur);
+        if (e == hipSuccess) e = hipStreamGetDevice(st, &dev);
+        if (e == hipSuccess && dev != cur) {
+            e = hipSetDevice(dev);
+            if (e == hipSuccess) prev = cur;
+        }
+        if (e != hipSuccess) rc = set_err(TG_E_HIP, "device of the stream: %s", hipGetErrorString(e));
+    }
+    ~DeviceOf() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+};
+
+static bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+static size_t type_size(int type) { return type == TG_T_F32 ? 4 : 2; }
+
+// Checks a batch and gives it in the kernels' form.
+static int kv_batch(const char *fn, const tg_kv_batch *b, tg::KvBatch *k) {
+    if (!b) return set_err(TG_E_INVALID, "%s: batch is NULL", fn);
+    if (b->n_seqs < 0 || b->n_tokens < 0)
+        return set_err(TG_E_INVALID, "%s: n_seqs %d, n_tokens %d", fn, b->n_seqs, b->n_tokens);
+    if (b->head_dim != 64 && b->head_dim != 128 && b->head_dim != 256)
+        return set_err(TG_E_INVALID, "%s: head_dim %d is not 64, 128 or 256", fn, b->head_dim);
+    if (b->page_tokens < 16 || b->page_tokens % 16)
+        return set_err(TG_E_INVALID, "%s: page_tokens %d is not a multiple of 16", fn, b->page_tokens);
+    if (b->n_kv_heads < 1 || b->n_kv_heads > 1024 || b->n_pages < 1 || b->n_pages > INT32_MAX)
+        return set_err(TG_E_INVALID, "%s: n_kv_heads %d, n_pages %lld", fn, b->n_kv_heads, (long long)b->n_pages);
+    if (b->table_cols < 1 || b->table_stride < b->table_cols || (int64_t)b->table_cols * b->page_tokens > INT32_MAX)
+        return set_err(TG_E_INVALID, "%s: table_cols %d (rows %d apart) of %d tokens", fn, b->table_cols,
+                       b->table_stride, b->page_tokens);
+    if (!b->pages || !b->table || !b->cu || !b->kv_len) return set_err(TG_E_INVALID, "%s: a NULL pointer in the batch", fn);
+    if (!aligned(b->pages, 16)) return set_err(TG_E_INVALID, "%s: pages are not 16-byte aligned", fn);
+    *k = tg::KvBatch{static_cast<uint8_t *>(b->pages), b->table, b->cu, b->kv_len, b->n_pages, b->page_tokens,
+                     b->n_kv_heads, b->head_dim, b->table_cols, b->table_stride, b->n_seqs, b->n_tokens};
+    return TG_OK;
+}
+
+// rows of `heads` heads whose kernel loads `n` elements at a time
+static int kv_rows(const char *fn, const char *name, const void *p, int64_t stride, int heads, int D, int type, int n) {
+    if (!p) return set_err(TG_E_INVALID, "%s: %s is NULL", fn, name);
+    if (stride < (int64_t)heads * D || stride % n || !aligned(p, n * type_size(type)))
+        return set_err(TG_E_INVALID, "%s: %s rows %lld elements apart, at least %lld and a multiple of %d aligned to %d bytes",
+                       fn, name, (long long)stride, (long long)heads * D, n, (int)(n * type_size(type)));
+    return TG_OK;
+}
+
+extern "C" int tg_kv_append_q4_dev(const tg_kv_batch *b, int type, const void *q, int64_t q_stride, const void *k,
+                                   int64_t k_stride, const void *v, int64_t v_stride, void *q_out,
+                                   int64_t q_out_stride, int n_heads, const float *q_norm, const float *k_norm,
+                                   float eps, const float *rope_cos, const float *rope_sin, int max_pos,
+                                   void *stream) {
+    const char *fn = "tg_kv_append_q4_dev";
+    tg::KvBatch kb;
+    int rc = kv_batch(fn, b, &kb);
+    if (rc) return rc;
+    if (type != TG_T_F32 && type != TG_T_F16 && type != TG_T_BF16)
+        return set_err(TG_E_INVALID, "%s: element type %d", fn, type);
+    if (n_heads < 0 || n_heads > 4096 || (n_heads > 0) != (q != nullptr))
+        return set_err(TG_E_INVALID, "%s: n_heads %d with q %s", fn, n_heads, q ? "given" : "NULL");
+    if (q && (rc = kv_rows(fn, "q", q, q_stride, n_heads, kb.D, type, 4))) return rc;
+    if (q && (rc = kv_rows(fn, "q_out", q_out, q_out_stride, n_heads, kb.D, type, 4))) return rc;
+    if ((rc = kv_rows(fn, "k", k, k_stride, kb.n_kv, kb.D, type, 4))) return rc;
+    if ((rc = kv_rows(fn, "v", v, v_stride, kb.n_kv, kb.D, type, 4))) return rc;
+    if ((rope_cos != nullptr) != (rope_sin != nullptr))
+        return set_err(TG_E_INVALID, "%s: one of rope_cos and rope_sin is NULL", fn);
+    if (!aligned(q_norm, 16) || !aligned(k_norm, 16) || !aligned(rope_cos, 16) || !aligned(rope_sin, 16))
+        return set_err(TG_E_INVALID, "%s: norm weights and rotation tables are 16-byte aligned", fn);
+    if (max_pos < 1 && rope_cos) return set_err(TG_E_INVALID, "%s: max_pos %d", fn, max_pos);
+    if (!kb.n_tokens || !kb.n_seqs) return TG_OK;
+    DeviceOf dev(as_stream(stream));
+    if (dev.rc) return dev.rc;
+    const tg::AppendArgs a{{q, q_stride}, {k, k_stride}, {v, v_stride}, q_out, q_out_stride, n_heads, q_norm, k_norm,
+                           eps, rope_cos, rope_sin, rope_cos ? max_pos : INT32_MAX};
+    PROFILED("kv_append", as_stream(stream), tg::launch_kv_append(kb, type, a, as_stream(stream)));
+    return TG_OK;
+}
+
+extern "C" int tg_kv_read_q4_dev(const tg_kv_batch *b, void *k, void *v, void *stream) {
+    const char *fn = "tg_kv_read_q4_dev";
+    tg::KvBatch kb;
+    int rc = kv_batch(fn, b, &kb);
+    if (rc) return rc;
+    if (!k || !v || !aligned(k, 16) || !aligned(v, 16))
+        return set_err(TG_E_INVALID, "%s: k or v is NULL or not 16-byte aligned", fn);
+    if (!kb.n_tokens || !kb.n_seqs) return TG_OK;
+    DeviceOf dev(as_stream(stream));
+    if (dev.rc) return dev.rc;
+    PROFILED("kv_read", as_stream(stream), tg::launch_kv_read(kb, k, v, as_stream(stream)));
+    return TG_OK;
+}
+
+// what the attention's workspace and launch both need: heads and max_len in range
+static int attn_args(const char *fn, const tg_kv_batch *b, int n_heads, int *max_len, tg::KvBatch *kb) {
+    int rc = kv_batch(fn, b, kb);
+    if (rc) return rc;
+    if (n_heads < 1 || n_heads > 4096 || n_heads % kb->n_kv)
+        return set_err(TG_E_INVALID, "%s: n_heads %d is not a multiple of %d key heads up to 4096", fn, n_heads, kb->n_kv);
+    if (*max_len < 0) return set_err(TG_E_INVALID, "%s: max_len %d", fn, *max_len);
+    const int cap = kb->table_cols * kb->page_tokens;
+    if (*max_len == 0 || *max_len > cap) *max_len = cap;
+    return TG_OK;
+}
+
+extern "C" size_t tg_attn_q4_workspace(const tg_kv_batch *b, int n_heads, int max_len) {
+    tg::KvBatch kb;
+    if (attn_args("tg_attn_q4_workspace", b, n_heads, &max_len, &kb)) return 0;
+    return tg::attn_workspace(kb, n_heads, max_len);
+}
+
+extern "C" int tg_attn_q4_dev(const tg_kv_batch *b, int type, const void *q, int64_t q_stride, int n_heads, float scale,
+                              void *out, int64_t out_stride, int max_len, void *workspace, size_t workspace_bytes,
+                              void *stream) {
+    const char *fn = "tg_attn_q4_dev";
+    tg::KvBatch kb;
+    int rc = attn_args(fn, b, n_heads, &max_len, &kb);
+    if (rc) return rc;
+    if (type != TG_T_F16 && type != TG_T_BF16)
+        return set_err(TG_E_INVALID, "%s: element type %d is not fp16 or bf16", fn, type);
+    if ((rc = kv_rows(fn, "q", q, q_stride, n_heads, kb.D, type, 8))) return rc;
+    if ((rc = kv_rows(fn, "out", out, out_stride, n_heads, kb.D, type, 8))) return rc;
+    if (!(scale > 0.0f && scale < INFINITY)) return set_err(TG_E_INVALID, "%s: scale %g", fn, (double)scale);
+    if (!kb.n_tokens || !kb.n_seqs) return TG_OK;
+    const size_t need = tg::attn_workspace(kb, n_heads, max_len);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+        return set_err(TG_E_INVALID, "%s: workspace of %zu bytes, %zu and 16-byte alignment needed", fn,
+                       workspace ? workspace_bytes : (size_t)0, need);
+    DeviceOf dev(as_stream(stream));
+    if (dev.rc) return dev.rc;
+    PROFILED("attn", as_stream(stream), tg::launch_attn(kb, type, {q, q_stride}, n_heads, scale, out, out_stride,
+                                                        max_len, workspace, as_stream(stream)));
+    return TG_OK;
+}
+
+static int matmul_shape(const char *fn, int M, int N, int K) {
+    if (M < 0 || N < 1 || K < 16 || K % 16 || K > 131072)
+        return set_err(TG_E_INVALID, "%s: M %d, N %d, K %d (a multiple of 16 up to 131072)", fn, M, N, K);
+    return TG_OK;
+}
+
+extern "C" size_t tg_matmul_i8_workspace(int M, int N, int K) {
+    return matmul_shape("tg_matmul_i8_workspace", M, N, K) ? 0 : tg::matmul_i8_workspace(M, N, K);
+}
+
+extern "C" int tg_matmul_i8_dev(const void *x, int x_type, int64_t x_stride, const float *norm_w, float eps,
+                                const int8_t *w, const float *w_scale, const void *residual, int64_t residual_stride,
+                                void *out, int out_type, int64_t out_stride, int M, int N, int K, void *workspace,
+                                size_t workspace_bytes, void *stream) {
+    const char *fn = "tg_matmul_i8_dev";
+    int rc = matmul_shape(fn, M, N, K);
+    if (rc) return rc;
+    for (int t : {x_type, out_type})
+        if (t != TG_T_F32 && t != TG_T_F16 && t != TG_T_BF16) return set_err(TG_E_INVALID, "%s: element type %d", fn, t);
+    if (!x || !w || !w_scale || !out) return set_err(TG_E_INVALID, "%s: a NULL pointer", fn);
+    if (!aligned(w, 16)) return set_err(TG_E_INVALID, "%s: w is not 16-byte aligned", fn);
+    if (x_stride < K || out_stride < N || (residual && residual_stride < N))
+        return set_err(TG_E_INVALID, "%s: rows overlap (x %lld, out %lld apart)", fn, (long long)x_stride, (long long)out_stride);
+    if (!M) return TG_OK;
+    const size_t need = tg::matmul_i8_workspace(M, N, K);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+        return set_err(TG_E_INVALID, "%s: workspace of %zu bytes, %zu and 16-byte alignment needed", fn,
+                       workspace ? workspace_bytes : (size_t)0, need);
+    DeviceOf dev(as_stream(stream));
+    if (dev.rc) return dev.rc;
+    const tg::MatmulI8Args a{x, x_type, x_stride, norm_w, eps, w, w_scale, residual, residual_stride,
+                             out, out_type, out_stride, M, N, K};
+    PROFILED("matmul_i8", as_stream(stream), tg::launch_matmul_i8(a, workspace, as_stream(stream)));
+    return TG_OK;
+}

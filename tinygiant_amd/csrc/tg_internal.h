@@ -381,4 +381,52 @@ hipError_t launch_down_grouped(const uint8_t *layer_pl, const Shape &s, int n, c
 hipError_t launch_combine(const float *D, const float *w, int T, int H, int k, const float *resid, float *out,
                           hipStream_t st);
 
+// ---------------------------------------------------------------- attention block (tg_attn.hip, tg_linear.hip)
+// tg_kv_batch as the kernels take it
+struct KvBatch {
+    uint8_t *pages;
+    const int32_t *table, *cu, *kv_len;
+    int64_t n_pages;
+    int page_tokens, n_kv, D;
+    int table_cols, table_stride;
+    int n_seqs, n_tokens;
+};
+// strided rows of heads: element (t, h, d) at p[t * stride + h * D + d]
+struct KvRows {
+    const void *p;
+    int64_t stride;
+};
+struct AppendArgs {
+    KvRows q, k, v;
+    void *q_out;
+    int64_t q_out_stride;
+    int n_heads;
+    const float *q_norm, *k_norm;
+    float eps;
+    const float *cos, *sin;
+    int max_pos;
+};
+hipError_t launch_kv_append(const KvBatch &b, int type, const AppendArgs &a, hipStream_t st);
+hipError_t launch_kv_read(const KvBatch &b, void *k, void *v, hipStream_t st);
+size_t attn_workspace(const KvBatch &b, int n_heads, int max_len);
+hipError_t launch_attn(const KvBatch &b, int type, KvRows q, int n_heads, float scale, void *out, int64_t out_stride,
+                       int max_len, void *ws, hipStream_t st);
+struct MatmulI8Args {
+    const void *x;
+    int x_type;
+    int64_t x_stride;
+    const float *norm_w;
+    float eps;
+    const int8_t *w;
+    const float *w_scale;
+    const void *res;
+    int64_t res_stride;
+    void *out;
+    int out_type;
+    int64_t out_stride;
+    int M, N, K;
+};
+size_t matmul_i8_workspace(int M, int N, int K);
+hipError_t launch_matmul_i8(const MatmulI8Args &a, void *ws, hipStream_t st);
+
 }  // namespace tg
