@@ -429,7 +429,8 @@ int tg_head_sample(tg_head *h, const float *x, float eps, float temperature, dou
  *
  * pages: [n_pages][n_kv_heads][page_tokens / 16] tiles of 16 tokens, 18 *
  * head_dim bytes each (16-byte aligned; head_dim 64, 128 or 256; page_tokens
- * a multiple of 16).  A tile holds Q4_0 blocks of 32 values (value = scale *
+ * a multiple of 16 up to 65536, table_cols * page_tokens at most 2^30).  A
+ * tile holds Q4_0 blocks of 32 values (value = scale *
  * (code - 8), scale fp16): the K codes (8 * head_dim bytes), the V codes (8 *
  * head_dim), the K scales (head_dim), the V scales (head_dim), ordered so
  * that a wave's 16-byte loads are operands of the matrix instructions

@@ -97,8 +97,8 @@ class PagedKV:
                  device="cuda", pages=None):
         if head_dim not in (64, 128, 256):
             raise ValueError(f"head_dim {head_dim} is not 64, 128 or 256")
-        if page_tokens < 16 or page_tokens % 16:
-            raise ValueError(f"page_tokens {page_tokens} is not a multiple of 16")
+        if page_tokens % 16 or not 16 <= page_tokens <= 65536:
+            raise ValueError(f"page_tokens {page_tokens} is not a multiple of 16 up to 65536")
         if min(n_layers, n_pages, n_kv_heads) < 1:
             raise ValueError(f"n_layers {n_layers}, n_pages {n_pages}, n_kv_heads {n_kv_heads}")
         shape = (n_layers, n_pages, n_kv_heads, page_tokens // 16, 18 * head_dim)

@@ -2475,11 +2475,11 @@ static int kv_batch(const char *fn, const tg_kv_batch *b, tg::KvBatch *k) {
         return set_err(TG_E_INVALID, "%s: n_seqs %d, n_tokens %d", fn, b->n_seqs, b->n_tokens);
     if (b->head_dim != 64 && b->head_dim != 128 && b->head_dim != 256)
         return set_err(TG_E_INVALID, "%s: head_dim %d is not 64, 128 or 256", fn, b->head_dim);
-    if (b->page_tokens < 16 || b->page_tokens % 16)
-        return set_err(TG_E_INVALID, "%s: page_tokens %d is not a multiple of 16", fn, b->page_tokens);
+    if (b->page_tokens < 16 || b->page_tokens % 16 || b->page_tokens > 65536)
+        return set_err(TG_E_INVALID, "%s: page_tokens %d is not a multiple of 16 up to 65536", fn, b->page_tokens);
     if (b->n_kv_heads < 1 || b->n_kv_heads > 1024 || b->n_pages < 1 || b->n_pages > INT32_MAX)
         return set_err(TG_E_INVALID, "%s: n_kv_heads %d, n_pages %lld", fn, b->n_kv_heads, (long long)b->n_pages);
-    if (b->table_cols < 1 || b->table_stride < b->table_cols || (int64_t)b->table_cols * b->page_tokens > INT32_MAX)
+    if (b->table_cols < 1 || b->table_stride < b->table_cols || (int64_t)b->table_cols * b->page_tokens > 1 << 30)
         return set_err(TG_E_INVALID, "%s: table_cols %d (rows %d apart) of %d tokens", fn, b->table_cols,
                        b->table_stride, b->page_tokens);
     if (!b->pages || !b->table || !b->cu || !b->kv_len) return set_err(TG_E_INVALID, "%s: a NULL pointer in the batch", fn);
