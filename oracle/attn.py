@@ -85,8 +85,9 @@ class Cache:
             out.append((code - 8) * np.repeat(tile[sat].view(np.float16).astype(np.float64), 32))
         return out
 
-    def rows(self, table_row, n):
-        """K and V [n_kv, n, D] float64 of a sequence's first n tokens."""
+    def rows(self, table_row, n, steps=False):
+        """K and V [n_kv, n, D] float64 of a sequence's first n tokens;
+        steps: the scales of their blocks instead, spread over the dims."""
         t = np.arange(n)
         page = np.asarray(table_row)[t // self.page_tokens]
         tile = self.pages[page, :, t % self.page_tokens // 16].view(np.uint16)  # [n, n_kv, 9 D]
@@ -95,22 +96,25 @@ class Cache:
         for code_at, nib, scale_at in ((0, 1, 4), (2, 3, 5)):
             at = np.stack([pl[code_at] for pl in places])[t % 16][:, None]
             sat = np.stack([pl[scale_at] for pl in places])[t % 16][:, None]
+            d = np.repeat(np.take_along_axis(tile, sat, axis=2).view(np.float16).astype(np.float64), 32, axis=2)
             code = (np.take_along_axis(tile, at, axis=2).astype(np.int64) >> (4 * places[0][nib])) & 15
-            d = np.take_along_axis(tile, sat, axis=2).view(np.float16).astype(np.float64)
-            out.append(np.moveaxis((code - 8) * np.repeat(d, 32, axis=2), 1, 0))
+            out.append(np.moveaxis(d if steps else (code - 8) * d, 1, 0))
         return out
 
 
-def attend(q, k, v, n_new, scale):
+def attend(q, k, v, n_new, scale, steps=None):
     """q [n_new, heads, D], the last rows of a sequence with k, v [n_kv, n,
     D]: row i sees positions 0 .. n - n_new + i.  Returns in float64 out
     [n_new, heads, D], sum p |v| of the same shape, and the largest scale *
-    sum |q_i k_i| that each row sees [n_new, heads, 1] (for error bounds)."""
+    sum |q_i k_i| that each row sees [n_new, heads, 1] (for error bounds).
+    steps (the scales of k's and v's blocks): two more for bounds, sum p
+    |step of v| and the largest scale * max |q| * sum of |steps of k|'s
+    blocks that a row sees."""
     n_kv, n, D = k.shape
     heads = q.shape[1]
     G = heads // n_kv
-    out, size = np.zeros((2, n_new, heads, D))
-    top = np.zeros((n_new, heads, 1))
+    out, size, vstep = np.zeros((3, n_new, heads, D))
+    top, kstep = np.zeros((2, n_new, heads, 1))
     hide = np.arange(n)[None, :] > np.arange(n - n_new, n)[:, None]
     blind = hide.all(axis=1) if n else np.ones(n_new, bool)
     for h in range(heads if n else 0):
@@ -123,7 +127,11 @@ def attend(q, k, v, n_new, scale):
         out[:, h], size[:, h] = w @ v[h // G], w @ np.abs(v[h // G])
         a = np.where(hide, 0, scale * (np.abs(x) @ np.abs(k[h // G]).T))
         top[:, h, 0] = a.max(axis=1)
-    return out, size, top
+        if steps:
+            vstep[:, h] = w @ np.abs(steps[1][h // G])
+            a = np.where(hide, 0, np.abs(steps[0][h // G][:, ::32]).sum(axis=1)[None, :])
+            kstep[:, h, 0] = scale * np.abs(x).max(axis=1) * a.max(axis=1)
+    return (out, size, top, vstep, kstep) if steps else (out, size, top)
 
 
 def codes_i8(x, norm=None, eps=1e-6):

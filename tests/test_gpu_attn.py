@@ -2,15 +2,21 @@
 oracle/attn.py.
 
 The cache's bytes and the rotated q are compared exactly: both sides round
-each step alike.  Attention's tolerance counts the kernels' roundings, u =
-2^-11 being half a step of fp16 (weights and values are fp16 operands of the
-matrix instructions; keys too where rows are many):
-  weights  a score is off by at most 2 u S (S: the largest scale * sum |q_i
-           k_i| of the row) plus 2^-18 (S + 1) of fp32 sums and exponents, so a
-           weight by the factor e^(2 delta), and by u when it becomes a half
-  values   by u each
-and these move the output by at most that times sum p |v|; the result is
-then rounded by half a step of its type."""
+each step alike.  Attention's tolerance counts the kernels' roundings, u = 2^-11 being half a
+step of fp16 (weights and values are fp16 operands of the matrix
+instructions; keys and queries too where rows are many):
+  scores   off by at most 2 u S (S: the largest scale * sum |q_i k_i| of the
+           row), 2^-18 (S + 1) of fp32 sums and exponents, and, where the codes are
+           operands themselves, 2^-11 of the largest query value times one step of
+           each block: the instruction aligns 32 products to the largest one,
+           a subnormal operand (code 2^-18) counting as 2^-14, and cuts 2^-24 below
+           it, so 32 * 2^-38 * 16 / 2^-18 steps are lost (16 lies between the two
+           kinds of codes).  A weight is off by the factor e^(2 delta).
+  weights  u as a half; values u as a half; and again 2 * 32 * 2^-38 / 2^-22 = 2^-10 of one
+           step of each value block where the codes are operands (the codes' sum
+           and its offset's).
+These move the output by at most that times sum p |v| (p times one step); the
+result is then rounded by half a step of its type."""
 import numpy as np
 import pytest
 import torch
@@ -74,11 +80,13 @@ def check_attend(s, q, qn, out, scale=None, bad=()):
             continue
         k, v = s.cache.rows(s.table[i], n)
         rows = slice(s.cu[i], s.cu[i + 1])
-        ref, size, top = A.attend(qn[rows], k, v, new, s.D ** -0.5 if scale is None else scale)
-        delta = 2 * u * top + 2.0 ** -18 * (top + 1)
-        tol = size * (np.expm1(2 * delta) + 2 * u) + half * np.abs(ref) * (1 + 1e-3) + 2.0 ** -24
+        ref, size, top, vstep, kstep = A.attend(qn[rows], k, v, new, s.D ** -0.5 if scale is None else scale,
+                                                steps=s.cache.rows(s.table[i], n, steps=True))
+        delta = 2 * u * top + 2.0 ** -18 * (top + 1) + 2.0 ** -11 * kstep
+        tol = size * (np.expm1(2 * delta) + 2 * u) + 2.0 ** -10 * vstep + half * np.abs(ref) * (1 + 1e-3) + 2.0 ** -24
         off = np.abs(got[rows] - ref)
-        assert (off <= tol).all(), (i, n, new, float((off / tol).max()), np.unravel_index((off / tol).argmax(), off.shape))
+        at = np.unravel_index((off / tol).argmax(), off.shape)
+        assert off[at] <= tol[at], (i, n, new, at, got[rows][at], ref[at], size[at], top[at[0], at[1]], float(off[at] / tol[at]))
         # and on the whole far inside it where scores are ordinary (up to S = 64 their fp32 sums are off by at most
         # 2^-18 S = u / 2): independent roundings, not a bias
         if ref.size > 2000 and top.max() <= 64:
@@ -104,6 +112,9 @@ ATTEND = [
     (256, 1, 2, 64, [333, 64], [200, 64], "bf16"),
     (128, 2, 1, 16, [10, 4], [30, 20], "f16"),                     # more rows than tokens: the first see nothing
     (128, 1, 7, 16, [1], [300], "bf16"),
+    (64, 8, 2, 16, [5 + i % 37 for i in range(80)] + [3000, 1700], [1] * 82, "f16"),  # more tiles than shares, two long ones
+    (64, 1, 3, 32, [900 + 13 * i for i in range(10)], [1, 2, 3, 4, 5, 6, 7, 8, 9, 10], "bf16"),
+    (128, 1, 4, 16, [i % 5 * 100 for i in range(130)], [1] * 130, "f16"),             # more sequences than lanes, some empty
     (64, 1, 8, 16, [0], [40], "f16"),
 ]
 

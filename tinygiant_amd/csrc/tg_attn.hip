@@ -12,6 +12,7 @@
 #include "../../include/tinygiant.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tg {
 
@@ -306,19 +307,26 @@ __global__ __launch_bounds__(256) void k_kv_read(KvBatch b, _Float16 *k, _Float1
 // lane / 16) supplies key token c (16 bytes of a tile: its codes 8 h .. 8 h +
 // 7 of each block) and receives column c of tokens 4 h .. 4 h + 3, which is
 // just the layout the weights need as the B operand of O^T = V^T P^T.
-// The codes stay integers: a nibble masked in place is the fp16 subnormal
-// code * 2^-24 (bits 0..3) or code * 2^-20 (bits 4..7), which the matrix
-// instructions take exactly; the query operand carries the factor 16 between
-// the two, the sum starts at -8 times the query's block sum, and the block's
+// The codes stay integers: a nibble shifted to bits 2..5 or 6..9 of a half and
+// masked is the fp16 subnormal code * 2^-22 or code * 2^-18, which the matrix
+// instructions take; the query operand carries the factor 16 between the
+// two, the sum starts at -8 times the query's block sum, and the block's
 // scale multiplies the fp32 sum.  So keys and queries are exact: a query row
 // is scaled by a power of two to below 2^15 (its largest value in 2^10 ..
-// 2^11), which drops nothing above 2^-24 of that.
+// 2^11), which drops nothing above 2^-24 of that.  What the instruction adds up
+// is aligned to its largest product, a subnormal counting as 2^-14, and cut
+// 2^-24 below it: 32 addends lose at most 2^-11 of the largest query value times one
+// step of the block (measured: a tenth of it).  Unshifted nibbles (bits
+// 0..3 and 4..7) would lose four times that and save one shift in 5 operations.
 //
-// Weights are exp2(s - m + 4) with m raised (and the sums rescaled) only
-// where a score passes m + 11: they stay below 2^15 as fp16 operands, and
-// with m at most 11 below the largest score a weight is a normal fp16 down to
-// 2^-18 of it.  Values are dequantised to fp16 (one rounding, 2^-11), the
-// weights rounded to fp16 (2^-11); sums, maxima and outputs are fp32.
+// Weights and values.  A value block's scale d multiplies the weight, p' =
+// exp2(s - m + A) d, one rounding to fp16, once for its two column tiles, and
+// the codes stay the integers they are, again as subnormals; a constant operand of -8
+// takes the codes' offset off within the same step, so no sum grows with it.
+// A = 11 - e where every scale so far is below 2^e, and m is raised (and the sums rescaled)
+// only where a score passes m + 4: p' stays below 2^15, and with the largest weight
+// at 2^5 or more it is a normal fp16 down to 2^-19 of that, the smallest
+// subnormal at 2^-29.  Sums, maxima and outputs are fp32.
 //
 // A value block that is not finite makes the token's scores NaN and its values 0, so
 // that rows which see the token are NaN and rows which do not are as ever.
@@ -328,7 +336,9 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float AT_NONE = -3.402823466e38f;  // m of a column that has seen nothing
-constexpr float AT_LIFT = 4.0f, AT_ROOM = 11.0f;
+constexpr uint32_t AT_EVEN = 0x003C003Cu, AT_ODD = 0x03C003C0u;  // codes in bits 2..5, 6..9 of both halves
+constexpr float AT_ROOM = 6.0f;
+constexpr int AT_TOP = 9;                    // A + e
 
 TG_DEV f16x2 as_h2(uint32_t v) { return __builtin_bit_cast(f16x2, v); }
 TG_DEV uint32_t as_u(f16x2 v) { return __builtin_bit_cast(uint32_t, v); }
@@ -341,35 +351,133 @@ TG_DEV uint32_t pack_h2(float a, float b) {
     return as_u(__builtin_convertvector(v, f16x2));
 }
 
-// a half whose exponent is all ones, in either half of v
-TG_DEV bool odd_half(uint32_t v) { return (v & 0x7C00u) == 0x7C00u || (v & 0x7C000000u) == 0x7C000000u; }
+// a value that is the same in every lane, told to the compiler
+TG_DEV int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// Column tile `z` of the launch: its sequence (or -1) and its number there.
+// The maximum of v over the four lanes that share a column (lane % 16)
+TG_DEV float col_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+TG_DEV float col_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(q[0]) + __uint_as_float(q[1]);
+}
+
+// One sequence as a lane of the planning scan holds it
+struct SeqWork {
+    int lo, n, len, tiles, steps;
+};
+TG_DEV SeqWork seq_work(const KvBatch &b, int G, int j) {
+    const bool in = j < b.n_seqs;
+    const int jj = in ? j : 0;  // three loads side by side, not one behind the other
+    const int c0 = b.cu[jj], c1 = b.cu[jj + 1], cl = b.kv_len[jj];
+    SeqWork w;
+    w.lo = min(max(c0, 0), b.n_tokens);
+    w.n = in ? min(max(c1, w.lo), b.n_tokens) - w.lo : 0;
+    w.len = max(cl, 0);
+    w.tiles = (int)(((int64_t)w.n * G + 15) / 16);
+    w.steps = max(1, (min(w.len, b.table_cols * b.page_tokens + 1) + 31) / 32);
+    return w;
+}
+
+// Inclusive sums over the wave's lanes (rows of 16 by shifts, then across rows)
+template <class T>
+TG_DEV T wave_scan(T v) {
+    auto from = [&](auto ctrl, auto rows, auto zero) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value,
+                                                                 decltype(rows)::value, 0xF, decltype(zero)::value));
+    };
+    using std::integral_constant;
+    constexpr integral_constant<int, 0xF> all{};
+    constexpr std::true_type zero{};
+    v += from(integral_constant<int, 0x111>{}, all, zero);
+    v += from(integral_constant<int, 0x112>{}, all, zero);
+    v += from(integral_constant<int, 0x114>{}, all, zero);
+    v += from(integral_constant<int, 0x118>{}, all, zero);
+    v += from(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{}, std::false_type{});
+    v += from(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{}, std::false_type{});
+    return v;
+}
+template <class T>
+TG_DEV T wave_sum(T v) { return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(v)), 63)); }
+
+// How the launch is cut.  Sequence s has `tiles` column tiles of `steps` steps
+// of 32 tokens.  A block takes at most `each` steps of one tile, the fewest
+// (from an even share on, an eighth more at a time) with which all the pieces of a key head are
+// `share` blocks or less, so that one round of the device's CUs does them
+// all and the longest block is as short as that allows; where there are more tiles than that anyway, an
+// even share of two rounds.  Every block works this out for itself from cu and kv_len (a wave's
+// scan), so a launch follows lengths that only the device knows.
+constexpr int AT_MIN = 4;
 struct ColTile {
     int seq, tile, lo, n, len;
+    int split, splits, per;  // this split of the tile's, tokens of one split
+    int part;                // the tile's first partial result (splits > 1)
+    int join, joins;         // its place among the tiles that are split, and how many those are
 };
-TG_DEV ColTile col_tile(const KvBatch &b, int G, int cols, int z, int lane) {
-    ColTile r{-1, 0, 0, 0, 0};
-    for (int j0 = 0; j0 < b.n_seqs; j0 += 64) {
-        const int j = j0 + lane;
-        const bool in = j < b.n_seqs;
-        const int lo = in ? min(max(b.cu[j], 0), b.n_tokens) : 0;
-        const int hi = in ? min(max(b.cu[j + 1], lo), b.n_tokens) : 0;
-        const int len = in ? max(b.kv_len[j], 0) : 0;
-        const int first = (int)((int64_t)lo * G / cols) + j;
-        const uint64_t m = __ballot(in && first <= z);
-        if (m) {
-            // cu does not decrease, so neither does first: the last lane of m
-            const int k = 63 - __builtin_clzll(m);
-            r.seq = j0 + k;
-            r.tile = z - __builtin_amdgcn_readlane(first, k);
-            r.lo = __builtin_amdgcn_readlane(lo, k);
-            r.n = __builtin_amdgcn_readlane(hi, k) - r.lo;
-            r.len = __builtin_amdgcn_readlane(len, k);
-        }
-        if (m != ~0ull) break;
+// splits of `steps` steps where a block takes 1 / inv of them (the same in every block; per covers them all)
+TG_DEV int splits_of(int steps, float inv) { return max(1, (int)ceilf((float)steps * inv)); }
+
+// 1 / (the most steps of one block)
+TG_DEV float block_share(const KvBatch &b, int G, int share, int lane, const SeqWork &w0) {
+    if (share == 0) return 0.0f;  // no splits
+    float all = (float)w0.tiles * (float)w0.steps;
+    int tiles = min(w0.tiles, 1 << 20);
+    for (int j = lane + 64; j < (b.n_seqs + 63) / 64 * 64; j += 64) {
+        const SeqWork w = seq_work(b, G, j);
+        all += (float)w.tiles * (float)w.steps;
+        tiles = min(tiles + w.tiles, 1 << 20);
     }
-    if (r.seq >= 0 && (int64_t)r.tile * cols >= (int64_t)r.n * G) r.seq = -1;
+    all = wave_sum(all);
+    const float even = all / (float)share;
+    if (wave_sum(tiles) > share) return 1.0f / fmaxf((float)AT_MIN, even * 0.5f);
+    float each = fmaxf((float)AT_MIN, even);
+    if (b.n_seqs > 64) return 1.0f / (each * 1.5f);
+    for (int i = 0; i < 16 && wave_sum(w0.tiles * splits_of(w0.steps, 1.0f / each)) > share; i++) each *= 1.125f;
+    return 1.0f / each;
+}
+
+// Block x of the launch; seq -1 where there is none.
+TG_DEV ColTile col_tile(const KvBatch &b, int G, int share, int x, int lane) {
+    const SeqWork w0 = seq_work(b, G, lane);
+    const float inv = block_share(b, G, share, lane, w0);
+    ColTile r{-1, 0, 0, 0, 0, 0, 1, 0, 0, 0, 0};
+    int before = 0, parts = 0, joins = 0;
+    for (int j0 = 0; j0 < b.n_seqs; j0 += 64) {
+        const SeqWork w = j0 == 0 ? w0 : seq_work(b, G, j0 + lane);
+        const int splits = splits_of(w.steps, inv);
+        const int mine = w.tiles * splits, mparts = splits > 1 ? mine : 0;
+        const int items = wave_scan(mine), ps = wave_scan(mparts);
+        const int mjoins = splits > 1 ? w.tiles : 0, js = wave_scan(mjoins);
+        const uint64_t m = __ballot(before + items > x);
+        if (m && before <= x) {
+            const int k = __builtin_ctzll(m);
+            const int sp = __builtin_amdgcn_readlane(splits, k), st = __builtin_amdgcn_readlane(w.steps, k);
+            const int local = x - before - __builtin_amdgcn_readlane(items, k) + __builtin_amdgcn_readlane(mine, k);
+            r.seq = j0 + k;
+            r.tile = local / sp;
+            r.split = local - r.tile * sp;
+            r.lo = __builtin_amdgcn_readlane(w.lo, k);
+            r.n = __builtin_amdgcn_readlane(w.n, k);
+            r.len = __builtin_amdgcn_readlane(w.len, k);
+            r.splits = sp;
+            r.per = (st + sp - 1) / sp * 32;
+            r.part = parts + __builtin_amdgcn_readlane(ps, k) - __builtin_amdgcn_readlane(mparts, k) + r.tile * sp;
+            r.join = joins + __builtin_amdgcn_readlane(js, k) - __builtin_amdgcn_readlane(mjoins, k) + r.tile;
+        }
+        before += __builtin_amdgcn_readlane(items, 63);
+        parts += __builtin_amdgcn_readlane(ps, 63);
+        joins += __builtin_amdgcn_readlane(js, 63);
+    }
+    // what follows from these is scalar work and real branches
+    r.seq = uni(r.seq), r.tile = uni(r.tile), r.lo = uni(r.lo), r.n = uni(r.n), r.len = uni(r.len);
+    r.split = uni(r.split), r.splits = uni(r.splits), r.per = uni(r.per), r.part = uni(r.part);
+    r.join = uni(r.join), r.joins = joins;
     return r;
 }
 
@@ -384,7 +492,7 @@ template <int D>
 struct KvStep {
     static constexpr int NG = D / 32, SW = D / 64;  // scale words per lane and step
     uint32_t k[2][NG], v[2][2][NG / 2], s[SW];
-    bool bad[2];
+    bool bad[2];  // the tile's page is none (D = 64: of the lane's own tile)
 };
 
 template <int N>
@@ -409,240 +517,318 @@ TG_DEV void load_words(const void *p, uint32_t *w) {
 // through a wave's corner of LDS because 16 lanes need the same ones.  Chunks
 // of one column tile are joined by k_attn_join, or written out at once where
 // one chunk is all.
+// What k_attn_join needs of one column tile that is split: its first column
+// (row * G + head of the key head's), how many, its first partial result, and
+// how many to join (0: the first holds all that the tile sees).
+struct JoinTile {
+    int col, cols, part, splits;
+};
 struct AttnOut {
     void *p;
     int64_t stride;
-    float *part;  // [column tile][key head][split][16][D + 2]
+    JoinTile *join;  // [joins][key head]
+    int joins;       // no more tiles than this are split
+    float *part;     // [split][key head] of 16 x D sums, then 16 pairs (m, l)
 };
+template <int D>
+constexpr int AT_PART = 16 * D + 32;  // floats of one split
 
 template <int D, bool BF>
-__global__ __launch_bounds__(256, 2) void k_attn_split(KvBatch b, KvRows q, int G, float scale, int chunk, int nsplit,
-                                                       AttnOut o) {
+__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_attn_split(KvBatch b, KvRows q, int G, float scale, int share,
+                                                                      FastDiv tpp, AttnOut o) {
     constexpr int NG = D / 32, ND = D / 16, SW = D / 64;
+    constexpr int NB = D == 256 ? 2 : 3;  // steps held: one at work, the others on their way
     __shared__ __align__(16) uint8_t sm[4 * 16 * D * 4 + 4 * 16 * 8];
-    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int lane = threadIdx.x % 64, wave = uni(threadIdx.x / 64);
     const int c = lane % 16, h = lane / 16;
-    const int z = blockIdx.x, hk = blockIdx.y, split = blockIdx.z;
-    const ColTile ct = col_tile(b, G, 16, z, lane);
+    const int hk = blockIdx.y;
+    const ColTile ct = col_tile(b, G, share, blockIdx.x, lane);
+    if ((int)blockIdx.x >= ct.joins && (int)blockIdx.x < o.joins && threadIdx.x == 0)
+        o.join[(size_t)blockIdx.x * b.n_kv + hk] = JoinTile{0, 0, 0, 0};
     if (ct.seq < 0) return;
     // this lane's column
     const int f = ct.tile * 16 + c, last = min(ct.n * G - 1, ct.tile * 16 + 15);
     const bool col = f < ct.n * G;
     const int row = ct.lo + (col ? f / G : 0), head = hk * G + (col ? f % G : 0);
     const int pos = col ? ct.len - ct.n + f / G : -1;
-    const int seen = tokens_seen(b, ct, last / G);
-    const int t0 = split * chunk, t1 = split == nsplit - 1 ? seen : min(seen, t0 + chunk);
-    if (t0 >= t1 && split > 0) return;  // a column tile that sees nothing is split 0's to write
+    const int seen = uni(tokens_seen(b, ct, last / G)), all = uni(ct.len - ct.n + (ct.tile * 16) / G);  // first column's position
+    const int t0 = ct.split * ct.per, t1 = min(seen, t0 + ct.per);
+    if (ct.splits > 1 && ct.split == 0 && threadIdx.x == 0)
+        o.join[(size_t)ct.join * b.n_kv + hk] =
+            JoinTile{ct.lo * G + ct.tile * 16, last - ct.tile * 16 + 1, ct.part, seen <= ct.per ? 0 : (seen + ct.per - 1) / ct.per};
+    if (t0 >= t1) {
+        // nothing to see here; a column tile that sees nothing at all is split 0's to write
+        if (ct.split == 0) {
+            for (int i = threadIdx.x; i < 16 * D / 4; i += 256) {
+                const int ff = ct.tile * 16 + i / (D / 4);
+                if (ff >= ct.n * G) break;
+                store4<BF ? TG_T_BF16 : TG_T_F16>(o.p, (int64_t)(ct.lo + ff / G) * o.stride + (int64_t)(hk * G + ff % G) * D + i % (D / 4) * 4, f32x4{0, 0, 0, 0});
+            }
+        }
+        return;
+    }
+
+    uint32_t qw[NG][4];
+    {
+        const uint16_t *qp = static_cast<const uint16_t *>(q.p) + (int64_t)row * q.stride + (int64_t)head * D;
+#pragma unroll
+        for (int g = 0; g < NG; g++) load_words<4>(qp + 32 * g + 8 * h, qw[g]);
+    }
+
+    // a stretch of tokens c0 .. c1 - 1 whose pages the lanes hold, one each
+    const int ntile = (int)tpp.d, span = min(ct.per, 63 * 16 * ntile & ~31);
+    const size_t head_bytes = (size_t)ntile * (18 * D), page_bytes = head_bytes * b.n_kv;
+    const uint8_t *base = b.pages + hk * head_bytes;
+    int c0 = t0, c1 = 0, page0 = 0, mine = 0, st = 0, s1 = 0;
+    KvStep<D> k[NB];
+    auto load = [&](KvStep<D> &k, int step) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            int t = step * 2 + x;
+            t = (t * 16 < c1 ? t : c0 / 16) - page0 * ntile;  // behind the end: any tile, its tokens are masked
+            const int pi = (int)fdiv((uint32_t)t, tpp), pg = __builtin_amdgcn_readlane(mine, pi);
+            const uint8_t *p = base + (size_t)max(pg, 0) * page_bytes + (size_t)(t - pi * ntile) * (18 * D);
+            load_words<NG>(p + lane * (NG * 4), k.k[x]);
+            load_words<NG>(p + 8 * D + lane * (NG * 4), &k.v[x][0][0]);
+            // lane's share of the scales: the step's 4 D bytes over 64 lanes; a page that is none has NaN ones
+            const uint32_t *sp = reinterpret_cast<const uint32_t *>(p + 16 * D);
+            if (SW == 1) {
+                const uint32_t v = sp[lane % 32];
+                if (lane / 32 == x) k.s[0] = v, k.bad[0] = pg < 0;
+            } else {
+                k.bad[x] = pg < 0;
+#pragma unroll
+                for (int i = 0; i < SW / 2; i++) k.s[x * (SW / 2) + i] = sp[lane * (SW / 2) + i];
+            }
+        }
+        // loads leave in the order of their steps, so that the wait for one step leaves those behind it under way
+        asm volatile("" ::: "memory");
+    };
+    auto begin = [&]() {
+        c1 = min(t1, c0 + span);
+        page0 = uni(c0 / 16 / ntile);
+        mine = (page0 + lane) * 16 * ntile < c1 ? page_of(b, ct.seq, (page0 + lane) * 16 * ntile) : 0;
+        s1 = (c1 + 31) / 32;
+        st = c0 / 32 + wave;
+#pragma unroll
+        for (int i = 0; i < NB - 1; i++) load(k[i], st + 4 * i);
+    };
+    begin();
 
     // queries: operand slots 8 h .. 8 h + 7 of each block, and the start of the sums
     f16x8 qf[NG];
     f32x4 start[NG];
     float cs;
     {
-        const uint16_t *qp = static_cast<const uint16_t *>(q.p) + (int64_t)row * q.stride + (int64_t)head * D;
-        float x[NG][8], top = 0.0f;
+        uint32_t mag = 0;  // magnitudes order as the integers they are stored as
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-            uint32_t w[4];
-            load_words<4>(qp + 32 * g + 8 * h, w);
+        for (int g = 0; g < NG; g++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint16_t u = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
-                x[g][e] = col ? (BF ? bf2f(u) : h2f(u)) : 0.0f;
-                top = fmaxf(top, fabsf(x[g][e]));
+            for (int e = 0; e < 4; e++) {
+                if (!col) qw[g][e] = 0;
+                mag = max(mag, max(qw[g][e] & 0x7FFFu, (qw[g][e] >> 16) & 0x7FFFu));
             }
-        }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 16));
+        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
+        const float top = BF ? bf2f((uint16_t)mag) : h2f((uint16_t)mag);
         int e2 = 0;
         (void)frexpf(top, &e2);  // top = m 2^e2, m in [0.5, 1)
         const int a = top > 0.0f && top < INFINITY ? 11 - e2 : 0;
-        cs = ldexpf(scale * 1.44269504f, 20 - a);
+        cs = ldexpf(scale * 1.44269504f, 18 - a);
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const _Float16 v = (_Float16)ldexpf(x[g][e], a + ((e / 2) % 2 ? 0 : 4));
+                const uint16_t u = (uint16_t)(qw[g][e / 2] >> (16 * (e % 2)));
+                const _Float16 v = (_Float16)ldexpf(BF ? bf2f(u) : h2f(u), a + ((e / 2) % 2 ? 0 : 4));
                 qf[g][e] = v;
                 sum += (e / 2) % 2 ? (float)v * 16.0f : (float)v;
             }
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            const float st = sum * (-8.0f / 16777216.0f);
-            start[g] = f32x4{st, st, st, st};
+            sum = col_sum(sum);
+            const float s0 = sum * (-8.0f / 4194304.0f);
+            start[g] = f32x4{s0, s0, s0, s0};
         }
     }
 
     uint32_t *sl = reinterpret_cast<uint32_t *>(sm) + wave * (16 * D);  // this wave's corner
+    // word w of a tile's 2 D bytes of scales that this lane's i-th word is, and its tile
+    auto word_of = [&](int i) { return SW == 1 ? lane % 32 : lane * (SW / 2) + i % (SW / 2); };
+    auto tile_of = [&](int i) { return SW == 1 ? lane / 32 : i / (SW / 2); };
+    const uint32_t vmask = word_of(0) >= D / 4 ? 0x7FFF7FFFu : 0u;  // this lane's words are value scales
+    const f16x8 off_even = as_h8(0x80208020u, 0x80208020u, 0x80208020u, 0x80208020u);  // -8 as the subnormals the
+    const f16x8 off_odd = as_h8(0x82008200u, 0x82008200u, 0x82008200u, 0x82008200u);   // two kinds of codes are
     f32x4 acc[ND] = {};
     float m = AT_NONE, l = 0.0f;
-    const int ptok = b.page_tokens, span = min(chunk, 63 * ptok & ~31);
-    for (int c0 = t0; c0 < t1; c0 += span) {
-        const int c1 = min(t1, c0 + span);
-        // this stretch's pages, one to a lane
-        const int page0 = c0 / ptok;
-        const int mine = c0 / ptok * ptok + lane * ptok < c1 ? page_of(b, ct.seq, (page0 + lane) * ptok) : 0;
-        auto load = [&](int st, KvStep<D> &k) {
+    float A = 0.0f;           // the same in all lanes of a wave
+    uint32_t below = 0u;      // pairs of halves: the largest scale that A allows for
+    auto work = [&](KvStep<D> &k, int step) {
+        const bool edge = step * 32 + 31 > all;  // some column does not see all of it
+        // scales to LDS as the tiles hold them; what no column sees is zero
+        uint32_t big = below;
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                int t = st * 32 + 16 * x;
-                t = t < c1 ? t : c0;  // behind the end: any tile, its tokens are masked
-                const int pg = __builtin_amdgcn_readlane(mine, t / ptok - page0);
-                k.bad[x] = pg < 0;
-                const uint8_t *p = b.pages + tile_at<D>(b, max(pg, 0), hk, (t % ptok) / 16);
-                load_words<NG>(p + lane * (NG * 4), k.k[x]);
-                load_words<NG>(p + 8 * D + lane * (NG * 4), &k.v[x][0][0]);
-                // lane's share of the scales: the step's 4 D bytes over 64 lanes
-                if (SW == 1) {
-                    if (lane / 32 == x) k.s[0] = reinterpret_cast<const uint32_t *>(p + 16 * D)[lane % 32];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < SW / 2; i++)
-                        k.s[x * (SW / 2) + i] = reinterpret_cast<const uint32_t *>(p + 16 * D)[lane * (SW / 2) + i];
-                }
-            }
-        };
-        const int s1 = (c1 + 31) / 32;
-        int st = c0 / 32 + wave;
-        KvStep<D> cur, nxt;
-        if (st < s1) load(st, nxt);
-        for (; st < s1; st += 4) {
-            cur = nxt;
-            if (st + 4 < s1) load(st + 4, nxt);
-            const bool edge = st * 32 + 31 > ct.len - ct.n + (ct.tile * 16) / G;  // some column does not see all of it
-            // scales to LDS as the tiles hold them; what no column sees is zero
-            bool oddv = false;
-#pragma unroll
-            for (int i = 0; i < SW; i++) {
-                const int w = SW == 1 ? lane % 32 : lane * (SW / 2) + i % (SW / 2);  // word of the tile's 2 D bytes
-                const int x = SW == 1 ? lane / 32 : i / (SW / 2);
-                uint32_t v = cur.s[i];
-                const bool isv = w >= D / 4;
-                if (edge) {
-                    const int t = st * 32 + 16 * x;
-                    if (!isv) {
-                        if (t + w / (NG / 2) >= seen) v = 0;
-                    } else {
-                        const int tp = t + (w - D / 4) / NG * 2;
-                        if (tp + 1 >= seen) v &= 0xFFFFu;
-                        if (tp >= seen) v = 0;
-                    }
-                }
-                oddv |= isv && odd_half(v);
-                sl[x * (D / 2) + w] = v;
-            }
-            const bool odd = __ballot(oddv) != 0 || cur.bad[0] || cur.bad[1];
-            wave_lds_sync();
-            float s[2][4];
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                uint32_t kd[2 * NG];  // halves [token i][block g]
-                load_words<2 * NG>(sl + x * (D / 2) + h * (2 * NG), kd);
-#pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    const uint32_t w = cur.k[x][g], w8 = w >> 8;
-                    const f16x8 kf = as_h8(w & 0x000F000Fu, w & 0x00F000F0u, w8 & 0x000F000Fu, w8 & 0x00F000F0u);
-                    const f32x4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[g], start[g], 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float d = (float)as_h2(kd[(i * NG + g) / 2])[g % 2];
-                        s[x][i] = g == 0 ? d * r[i] : __builtin_fmaf(d, r[i], s[x][i]);
-                    }
-                }
-            }
-            if (odd) {
-                // NaN for the tokens of a bad page and of value blocks that are not finite; those blocks become 0
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    uint32_t vd[2 * NG];
-                    load_words<2 * NG>(sl + x * (D / 2) + D / 4 + h * (2 * NG), vd);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        bool n = cur.bad[x];
-#pragma unroll
-                        for (int g = 0; g < NG; g++) n |= ((vd[(i / 2) * NG + g] >> (16 * (i % 2))) & 0x7C00u) == 0x7C00u;
-                        if (n) s[x][i] = __builtin_nanf("");
-                    }
-                }
-                wave_lds_sync();
-#pragma unroll
-                for (int i = 0; i < SW; i++) {
-                    const int w = SW == 1 ? lane % 32 : lane * (SW / 2) + i % (SW / 2);
-                    const int x = SW == 1 ? lane / 32 : i / (SW / 2);
-                    if (w >= D / 4) {
-                        uint32_t v = sl[x * (D / 2) + w];
-                        if ((v & 0x7C00u) == 0x7C00u) v &= 0xFFFF0000u;
-                        if ((v & 0x7C000000u) == 0x7C000000u) v &= 0xFFFFu;
-                        sl[x * (D / 2) + w] = v;
-                    }
-                }
-                wave_lds_sync();
-            }
+        for (int i = 0; i < SW; i++) {
+            const int w = word_of(i), x = tile_of(i);
+            uint32_t v = k.bad[SW == 1 ? 0 : x] ? 0x7E007E00u : k.s[i];  // a page that is none has NaN scales
             if (edge) {
-#pragma unroll
-                for (int x = 0; x < 2; x++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (st * 32 + 16 * x + 4 * h + i > pos) s[x][i] = -INFINITY;
+                const int t = step * 32 + 16 * x;
+                if (w < D / 4) {
+                    if (t + w / (NG / 2) >= seen) v = 0;
+                } else {
+                    const int tp = t + (w - D / 4) / NG * 2;
+                    if (tp + 1 >= seen) v &= 0xFFFFu;
+                    if (tp >= seen) v = 0;
+                }
             }
-            // cs > 0, so the largest s is the largest score
-            float top = s[0][0];
+            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+            big = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, big), __builtin_bit_cast(u16x2, v & vmask)));
+            sl[x * (D / 2) + w] = v;
+        }
+        bool odd = false;
+        if (__ballot(big != below)) {
+            // a scale at or above the bound: a new one, or a block that is not finite
+            uint32_t top = max(big & 0xFFFFu, big >> 16);
+            odd = __ballot(top >= 0x7C00u) != 0;
+            if (top >= 0x7C00u) top = 0;
 #pragma unroll
-            for (int i = 1; i < 8; i++) top = fmaxf(top, s[i / 4][i % 4]);
-            if (__ballot(top * cs > m + AT_ROOM)) {
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float m2 = fmaxf(m, top * cs), r = __builtin_amdgcn_exp2f(m - m2);
+            for (int i = 1; i < 64; i *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, i));
+            if (top > (below & 0xFFFFu)) {
+                const int e = min(16, max((int)(top >> 10), 1) - 15 + 2);  // below 2^(e - 1), one bit of room
+                below = e > 15 ? 0x7BFF7BFFu : e < -13 ? (uint32_t)((1 << (e + 24)) - 1) * 0x10001u : (uint32_t)(((e + 15) << 10) - 1) * 0x10001u;
+                const float r = ldexpf(1.0f, AT_TOP - e - (int)A);
+                A = (float)(AT_TOP - e);
                 l *= r;
 #pragma unroll
                 for (int j = 0; j < ND; j++) acc[j] *= r;
-                m = m2;
             }
-            const float off = AT_LIFT - m;
-            float p[2][4];
+        }
+        wave_lds_sync();
+        f32x4 r[2][NG];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                p[i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], cs, off));
-                l += p[i / 4][i % 4];
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const uint32_t w = k.k[x][g] << 2, w2 = k.k[x][g] >> 6;
+                const f16x8 kf = as_h8(w & AT_EVEN, w & AT_ODD, w2 & AT_EVEN, w2 & AT_ODD);
+                r[x][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[g], start[g], 0, 0, 0);
             }
-            const f16x8 pf = as_h8(pack_h2(p[0][0], p[0][1]), pack_h2(p[0][2], p[0][3]), pack_h2(p[1][0], p[1][1]),
-                                   pack_h2(p[1][2], p[1][3]));
-            // values: words [token pair][block] of each tile's scales
-            uint32_t vd[2][2 * NG];
+        if (D <= 128) __builtin_amdgcn_sched_barrier(0);  // all of them under way before the first is waited for
+        float s[2][4];
 #pragma unroll
-            for (int x = 0; x < 2; x++) load_words<2 * NG>(sl + x * (D / 2) + D / 4 + h * (2 * NG), vd[x]);
+        for (int x = 0; x < 2; x++) {
+            uint32_t kd[2 * NG];  // halves [token i][block g]
+            load_words<2 * NG>(sl + x * (D / 2) + h * (2 * NG), kd);
 #pragma unroll
-            for (int bq = 0; bq < NG / 2; bq++) {
+            for (int g = 0; g < NG; g++)
 #pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    uint32_t w[4];
+                for (int i = 0; i < 4; i++)
+                    s[x][i] = __builtin_fmaf((float)as_h2(kd[(i * NG + g) / 2])[g % 2], r[x][g][i], g == 0 ? 0.0f : s[x][i]);
+        }
+        if (odd) {
+            // NaN for the tokens of value blocks that are not finite; those blocks become 0
 #pragma unroll
-                    for (int y = 0; y < 4; y++) {
-                        const uint32_t raw = cur.v[y / 2][y % 2][bq], sh = n < 2 ? raw : raw >> 8;
-                        f16x2 t;
-                        if (n % 2 == 0) t = as_h2((sh & 0x000F000Fu) | 0x64006400u) - f16x2{(_Float16)1032.0f, (_Float16)1032.0f};
-                        else t = as_h2((sh & 0x00F000F0u) | 0x54005400u) - f16x2{(_Float16)72.0f, (_Float16)72.0f};
-                        w[y] = as_u(t * as_h2(vd[y / 2][(y % 2) * NG + 2 * bq + n / 2]));
-                    }
-                    acc[4 * bq + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(w[0], w[1], w[2], w[3]), pf, acc[4 * bq + n], 0, 0, 0);
+            for (int x = 0; x < 2; x++) {
+                uint32_t vd[2 * NG];
+                load_words<2 * NG>(sl + x * (D / 2) + D / 4 + h * (2 * NG), vd);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    bool n = false;
+#pragma unroll
+                    for (int g = 0; g < NG; g++) n |= ((vd[(i / 2) * NG + g] >> (16 * (i % 2))) & 0x7C00u) == 0x7C00u;
+                    if (n) s[x][i] = __builtin_nanf("");
+                }
+            }
+            wave_lds_sync();
+#pragma unroll
+            for (int i = 0; i < SW; i++) {
+                if (vmask) {
+                    uint32_t *at = sl + tile_of(i) * (D / 2) + word_of(i), v = *at;
+                    if ((v & 0x7C00u) == 0x7C00u) v &= 0xFFFF0000u;
+                    if ((v & 0x7C000000u) == 0x7C000000u) v &= 0xFFFFu;
+                    *at = v;
                 }
             }
             wave_lds_sync();
         }
+        if (edge) {
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (step * 32 + 16 * x + 4 * h + i > pos) s[x][i] = -INFINITY;
+        }
+        // cs > 0, so the largest s is the largest score
+        float top = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) top = fmaxf(top, s[i / 4][i % 4]);
+        if (__ballot(top * cs > m + AT_ROOM)) {
+            top = col_max(top);
+            const float m2 = fmaxf(m, top * cs), r = __builtin_amdgcn_exp2f(m - m2);
+            l *= r;
+#pragma unroll
+            for (int j = 0; j < ND; j++) acc[j] *= r;
+            m = m2;
+        }
+        const float off = A - m;
+        float p[2][4];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            p[i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], cs, off));
+            l += p[i / 4][i % 4];
+        }
+        // value scales: words [token pair][block] of each tile
+        uint32_t vd[2][2 * NG];
+#pragma unroll
+        for (int x = 0; x < 2; x++) load_words<2 * NG>(sl + x * (D / 2) + D / 4 + h * (2 * NG), vd[x]);
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            uint32_t w[4];
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const f16x2 d = as_h2(vd[y / 2][(y % 2) * NG + g]);
+                const f16x2 v = {(_Float16)__builtin_fmaf(p[y / 2][2 * (y % 2)], (float)d[0], 0.0f),
+                                 (_Float16)__builtin_fmaf(p[y / 2][2 * (y % 2) + 1], (float)d[1], 0.0f)};
+                w[y] = as_u(v);
+            }
+            const f16x8 pf = as_h8(w[0], w[1], w[2], w[3]);
+            uint32_t r[4];  // the block's two column tiles are nibbles 2 (g % 2) and 2 (g % 2) + 1
+#pragma unroll
+            for (int y = 0; y < 4; y++) r[y] = g % 2 ? k.v[y / 2][y % 2][g / 2] >> 6 : k.v[y / 2][y % 2][g / 2] << 2;
+            const f16x8 even = as_h8(r[0] & AT_EVEN, r[1] & AT_EVEN, r[2] & AT_EVEN, r[3] & AT_EVEN);
+            const f16x8 odd8 = as_h8(r[0] & AT_ODD, r[1] & AT_ODD, r[2] & AT_ODD, r[3] & AT_ODD);
+            acc[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pf, acc[2 * g], 0, 0, 0);
+            acc[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd8, pf, acc[2 * g + 1], 0, 0, 0);
+            acc[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(off_even, pf, acc[2 * g], 0, 0, 0);
+            acc[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(off_odd, pf, acc[2 * g + 1], 0, 0, 0);
+        }
+        wave_lds_sync();
+    };
+    while (c0 < t1) {
+        // loads ahead of the last step too (of a tile that is there): were they conditional, the wait for a
+        // step's bytes would have to take in those of the steps behind it
+        while (st < s1) {
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                load(k[(i + NB - 1) % NB], st + 4 * (NB - 1));
+                work(k[i], st);
+                st += 4;
+                if (st >= s1) break;
+            }
+        }
+        c0 += span;
+        if (c0 < t1) begin();
     }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    l = col_sum(l);
+    m -= A;  // weights were exp2(score - (m - A))
 
     // the waves' shares joined in order: O[wave][column][D], m and l [wave][column]
     __syncthreads();
     float *so = reinterpret_cast<float *>(sm) + wave * 16 * D, *sml = reinterpret_cast<float *>(sm + 4 * 16 * D * 4);
 #pragma unroll
-    for (int j = 0; j < ND; j++) *reinterpret_cast<f32x4 *>(so + c * D + 16 * j + 4 * h) = acc[j];
+    for (int j = 0; j < ND; j++) *reinterpret_cast<f32x4 *>(so + c * D + 16 * j + 4 * h) = acc[j] * (j % 2 ? 262144.0f : 4194304.0f);
     if (h == 0) sml[(wave * 16 + c) * 2] = m, sml[(wave * 16 + c) * 2 + 1] = l;
     __syncthreads();
-    const int active = (seen + chunk - 1) / chunk;
-    const bool whole = active <= 1 || nsplit == 1;
+    const bool whole = seen <= ct.per;
     for (int i = threadIdx.x; i < 16 * D / 4; i += 256) {
         const int cc = i / (D / 4), d = (i % (D / 4)) * 4, ff = ct.tile * 16 + cc;
         if (ff >= ct.n * G) break;
@@ -660,37 +846,80 @@ __global__ __launch_bounds__(256, 2) void k_attn_split(KvBatch b, KvRows q, int 
             const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
             store4<BF ? TG_T_BF16 : TG_T_F16>(o.p, (int64_t)(ct.lo + ff / G) * o.stride + (int64_t)(hk * G + ff % G) * D + d, v * inv);
         } else {
-            float *pp = o.part + ((((size_t)z * b.n_kv + hk) * nsplit + split) * 16 + cc) * (D + 2);
-            pp[d] = v[0], pp[d + 1] = v[1], pp[d + 2] = v[2], pp[d + 3] = v[3];
-            if (d == 0) pp[D] = mm, pp[D + 1] = ll;
+            float *pp = o.part + ((size_t)(ct.part + ct.split) * b.n_kv + hk) * AT_PART<D>;
+            *reinterpret_cast<f32x4 *>(pp + cc * D + d) = v;
+            if (d == 0) pp[16 * D + 2 * cc] = mm, pp[16 * D + 2 * cc + 1] = ll;
         }
     }
 }
 
-// The splits of one column tile, joined in order.
-template <int D, bool BF>
-__global__ __launch_bounds__(256) void k_attn_join(KvBatch b, int G, int chunk, int nsplit, AttnOut o) {
-    const int hk = blockIdx.y, z = blockIdx.x;
-    const ColTile ct = col_tile(b, G, 16, z, threadIdx.x % 64);
-    if (ct.seq < 0) return;
-    const int last = min(ct.n * G - 1, ct.tile * 16 + 15), seen = tokens_seen(b, ct, last / G);
-    const int active = min(nsplit, (seen + chunk - 1) / chunk);
-    if (active <= 1) return;
-    const float *part = o.part + ((size_t)z * b.n_kv + hk) * nsplit * 16 * (D + 2);
-    for (int i = threadIdx.x; i < 16 * D; i += 256) {
-        const int cc = i / D, d = i % D, ff = ct.tile * 16 + cc;
-        if (ff >= ct.n * G) break;
-        float mm = AT_NONE, ll = 0.0f, v = 0.0f;
-        for (int s = 0; s < active; s++) mm = fmaxf(mm, part[(s * 16 + cc) * (D + 2) + D]);
-        for (int s = 0; s < active; s++) {
-            const float *pp = part + (s * 16 + cc) * (D + 2);
-            const float r = __builtin_amdgcn_exp2f(pp[D] - mm);
-            ll += pp[D + 1] * r;
-            v += pp[d] * r;
-        }
-        v *= ll == 0.0f ? 0.0f : 1.0f / ll;
-        static_cast<uint16_t *>(o.p)[(int64_t)(ct.lo + ff / G) * o.stride + (int64_t)(hk * G + ff % G) * D + d] = BF ? f2bf(v) : f2h(v);
+// The splits of one column, joined in order: TC threads per column, D / 4
+// lanes side by side for one split, each group of them every GR-th split.  A
+// block per column where few tiles have many splits, four columns to a block otherwise.
+template <int D, bool BF, int TC>
+__global__ __launch_bounds__(256) void k_attn_join(KvBatch b, int G, AttnOut o) {
+    constexpr int L = D / 4, GR = TC / L > 0 ? TC / L : 1, NC = 256 / TC, W = TC / 64;
+    static_assert(TC >= L, "");
+    __shared__ float sm_m[4], sm_l[4], sw[256];
+    __shared__ __align__(16) f32x4 so[256];
+    const int hk = blockIdx.y, tid = threadIdx.x % TC, ci = threadIdx.x / TC, cc = blockIdx.z * NC + ci;
+    const JoinTile jt = o.join[(size_t)blockIdx.x * b.n_kv + hk];
+    if (!jt.splits || (int)blockIdx.z * NC >= jt.cols) return;
+    const size_t step = (size_t)b.n_kv * AT_PART<D>;
+    const float *part = o.part + ((size_t)jt.part * b.n_kv + hk) * AT_PART<D>;
+    // all of a thread's sums (those of the first 8 turns) and its (m, l) are asked for before the first is
+    // waited for; columns behind the last hold zeros
+    const float *mine = part + cc * D + 4 * (tid % L), *ml = part + 16 * D + 2 * cc;
+    f32x4 first[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const int i = tid / L + k * GR;
+        first[k] = f32x4{0, 0, 0, 0};
+        if (i < jt.splits && cc < jt.cols) first[k] = *reinterpret_cast<const f32x4 *>(mine + i * step);
     }
+    float mm = AT_NONE;
+    for (int s = tid; s < jt.splits && cc < jt.cols; s += TC) mm = fmaxf(mm, ml[s * step]);
+    mm = col_max(mm);
+#pragma unroll
+    for (int i = 1; i < 16; i *= 2) mm = fmaxf(mm, __shfl_xor(mm, i));
+    if (tid % 64 == 0) sm_m[threadIdx.x / 64] = mm;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; i++) mm = fmaxf(mm, sm_m[ci * W + i]);
+    float ll = 0.0f;
+    f32x4 v = {0, 0, 0, 0};
+    for (int s0 = 0; s0 < jt.splits; s0 += TC) {
+        float w = 0.0f;
+        if (s0 + tid < jt.splits && cc < jt.cols) {
+            const float *p = ml + (s0 + tid) * step;
+            w = __builtin_amdgcn_exp2f(p[0] - mm);
+            ll += p[1] * w;
+        }
+        __syncthreads();
+        sw[threadIdx.x] = w;
+        __syncthreads();
+        const int n = min(TC, jt.splits - s0);
+        int i = tid / L;
+        if (s0 == 0) {
+#pragma unroll
+            for (int k = 0; k < 8; k++, i += GR)
+                if (i < n) v += first[k] * sw[ci * TC + i];
+        }
+        for (; i < n && cc < jt.cols; i += GR) v += *reinterpret_cast<const f32x4 *>(mine + (s0 + i) * step) * sw[ci * TC + i];
+    }
+    ll = wave_sum(ll);
+    if (tid % 64 == 0) sm_l[threadIdx.x / 64] = ll;
+    so[threadIdx.x] = v;
+    __syncthreads();
+    if (tid >= L || cc >= jt.cols) return;
+    ll = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; i++) ll += sm_l[ci * W + i];
+#pragma unroll
+    for (int i = 1; i < GR; i++) v += so[ci * TC + i * L + tid];
+    const int f = jt.col + cc, row = f / G;
+    store4<BF ? TG_T_BF16 : TG_T_F16>(o.p, (int64_t)row * o.stride + (int64_t)(hk * G + f - row * G) * D + 4 * tid,
+                                      v * (ll == 0.0f ? 0.0f : 1.0f / ll));
 }
 
 // ================================================================ launchers
@@ -722,42 +951,56 @@ hipError_t launch_kv_read(const KvBatch &b, void *k, void *v, hipStream_t st) {
     return hipGetLastError();
 }
 
-// Splits of one launch: chunks of a power of two of 128 tokens or more, so
-// many that about 1024 blocks of the longest sequences share the device.
+// Blocks of one launch: `share` per key head for the splits, and one for each
+// column tile that the shares do not fill.  Where the tiles are at most
+// `share` their splits are at most that too, so half as many tiles can be
+// split (more than 64 sequences, whose share is not searched: 4 share / 3 splits); where they
+// are more, 4 share splits and 2 share tiles.
 struct AttnPlan {
     int64_t tiles;
-    int chunk, nsplit;
+    int share, joins;
 };
+#ifndef AT_BLOCKS
+#define AT_BLOCKS 512
+#endif
 static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len) {
-    const int G = n_heads / b.n_kv;
     AttnPlan p;
-    p.tiles = (int64_t)b.n_tokens * G / 16 + b.n_seqs;
-    p.chunk = 128;
-    while (p.chunk < 4096 && (int64_t)p.chunk * 2048 < (int64_t)max_len * p.tiles * b.n_kv) p.chunk *= 2;
-    while (max_len / p.chunk >= 4096) p.chunk *= 2;
-    p.nsplit = std::max(1, (max_len + p.chunk - 1) / p.chunk);
+    p.tiles = (int64_t)b.n_tokens * (n_heads / b.n_kv) / 16 + b.n_seqs;
+    // nothing to split where no sequence is over what one block takes at the least, or there are tiles enough
+    p.share = std::max(1, AT_BLOCKS / b.n_kv);
+    if (max_len <= 32 * AT_MIN || p.tiles > 4 * p.share) p.share = 0;
+    p.joins = (int)std::min<int64_t>(p.tiles, p.tiles > p.share ? 2 * p.share : p.share);
     return p;
+}
+
+static size_t attn_join_bytes(const KvBatch &b, const AttnPlan &p) {
+    return ((size_t)p.joins * b.n_kv * sizeof(JoinTile) + 255) / 256 * 256;
 }
 
 size_t attn_workspace(const KvBatch &b, int n_heads, int max_len) {
     const AttnPlan p = attn_plan(b, n_heads, max_len);
-    return p.nsplit == 1 ? 0 : (size_t)p.tiles * b.n_kv * p.nsplit * 16 * (b.D + 2) * sizeof(float);
+    return p.share ? attn_join_bytes(b, p) + (size_t)4 * p.share * b.n_kv * (16 * b.D + 32) * sizeof(float) : 0;
+}
+
+template <int D, bool BF>
+static void attn_split_launch(const KvBatch &b, KvRows q, int G, float scale, const AttnPlan &p, const AttnOut &o, hipStream_t st) {
+    const dim3 grid((unsigned)(p.tiles + 2 * p.share), (unsigned)b.n_kv);
+    TG_LAUNCH((k_attn_split<D, BF>), grid, dim3(256), 0, st, b, q, G, scale, p.share, make_fastdiv((uint32_t)(b.page_tokens / 16)), o);
+    if (!p.share) return;
+    if (p.joins * b.n_kv <= 64) TG_LAUNCH((k_attn_join<D, BF, 256>), dim3(p.joins, b.n_kv, 16), dim3(256), 0, st, b, G, o);
+    else TG_LAUNCH((k_attn_join<D, BF, 64>), dim3(p.joins, b.n_kv, 4), dim3(256), 0, st, b, G, o);
 }
 
 hipError_t launch_attn(const KvBatch &b, int type, KvRows q, int n_heads, float scale, void *out, int64_t out_stride,
                        int max_len, void *ws, hipStream_t st) {
     const AttnPlan p = attn_plan(b, n_heads, max_len);
-    if (p.tiles > INT32_MAX) return hipErrorInvalidValue;
+    if (p.tiles + 2 * p.share > INT32_MAX / 16) return hipErrorInvalidValue;
     const int G = n_heads / b.n_kv;
-    const AttnOut o{out, out_stride, static_cast<float *>(ws)};
-    const dim3 grid((unsigned)p.tiles, (unsigned)b.n_kv, (unsigned)p.nsplit), join((unsigned)p.tiles, (unsigned)b.n_kv);
+    const AttnOut o{out, out_stride, static_cast<JoinTile *>(ws), p.joins,
+                    reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + attn_join_bytes(b, p))};
     TG_BY_DIM(b.D, {
-        if (type == TG_T_F16) TG_LAUNCH((k_attn_split<DIM, false>), grid, dim3(256), 0, st, b, q, G, scale, p.chunk, p.nsplit, o);
-        else TG_LAUNCH((k_attn_split<DIM, true>), grid, dim3(256), 0, st, b, q, G, scale, p.chunk, p.nsplit, o);
-        if (p.nsplit > 1) {
-            if (type == TG_T_F16) TG_LAUNCH((k_attn_join<DIM, false>), join, dim3(256), 0, st, b, G, p.chunk, p.nsplit, o);
-            else TG_LAUNCH((k_attn_join<DIM, true>), join, dim3(256), 0, st, b, G, p.chunk, p.nsplit, o);
-        }
+        if (type == TG_T_F16) attn_split_launch<DIM, false>(b, q, G, scale, p, o, st);
+        else attn_split_launch<DIM, true>(b, q, G, scale, p, o, st);
     });
     return hipGetLastError();
 }
