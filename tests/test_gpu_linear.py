@@ -42,7 +42,8 @@ def check(out, x, w, ws, nw, r, eps=1e-6):
 
 SHAPES = [(1, 1, 16), (1, 5120, 2048), (2, 48, 64), (3, 200, 80), (7, 1000, 2048), (8, 256, 4096), (9, 130, 1040), (16, 512, 2048),
           (17, 333, 512), (31, 64, 96), (32, 96, 1008), (33, 2048, 1024), (64, 640, 768), (65, 129, 160), (100, 255, 2064), (128, 128, 128),
-          (200, 1111, 336), (257, 300, 2048), (511, 515, 272), (600, 1024, 4096)]
+          (200, 1111, 336), (257, 300, 2048), (511, 515, 272), (600, 1024, 4096),
+          (1, 64, 8208), (4, 4096, 8192), (3, 40, 16384), (5, 33000, 64), (20, 33010, 208), (50, 32768, 128), (70, 16, 16384), (4096, 4100, 144)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
