@@ -114,6 +114,10 @@ ATTEND = [
     (128, 1, 7, 16, [1], [300], "bf16"),
     (64, 8, 2, 16, [5 + i % 37 for i in range(80)] + [3000, 1700], [1] * 82, "f16"),  # more tiles than shares, two long ones
     (64, 1, 3, 32, [900 + 13 * i for i in range(10)], [1, 2, 3, 4, 5, 6, 7, 8, 9, 10], "bf16"),
+    (128, 2, 8, 16, [3000, 40], [64, 40], "bf16"),                                    # many columns, split over the tokens
+    (256, 2, 4, 32, [2000, 700, 3], [90, 1, 3], "f16"),
+    (64, 4, 4, 64, [5000], [33], "bf16"),
+    (128, 1, 16, 48, [777, 1300], [100, 300], "f16"),
     (128, 1, 4, 16, [i % 5 * 100 for i in range(130)], [1] * 130, "f16"),             # more sequences than lanes, some empty
     (64, 1, 8, 16, [0], [40], "f16"),
 ]

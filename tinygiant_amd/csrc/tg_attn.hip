@@ -12,6 +12,7 @@
 #include "../../include/tinygiant.h"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace tg {
@@ -337,6 +338,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float AT_NONE = -3.402823466e38f;  // m of a column that has seen nothing
 constexpr uint32_t AT_EVEN = 0x003C003Cu, AT_ODD = 0x03C003C0u;  // codes in bits 2..5, 6..9 of both halves
+constexpr float AT_LEAST = 1e-37f;           // of the factor on scores: times it -inf stays -inf, and finite sums vanish
 constexpr float AT_ROOM = 6.0f;
 constexpr int AT_TOP = 9;                    // A + e
 
@@ -372,6 +374,7 @@ TG_DEV float col_sum(float v) {
 struct SeqWork {
     int lo, n, len, tiles, steps;
 };
+template <int COLS>
 TG_DEV SeqWork seq_work(const KvBatch &b, int G, int j) {
     const bool in = j < b.n_seqs;
     const int jj = in ? j : 0;  // three loads side by side, not one behind the other
@@ -380,7 +383,7 @@ TG_DEV SeqWork seq_work(const KvBatch &b, int G, int j) {
     w.lo = min(max(c0, 0), b.n_tokens);
     w.n = in ? min(max(c1, w.lo), b.n_tokens) - w.lo : 0;
     w.len = max(cl, 0);
-    w.tiles = (int)(((int64_t)w.n * G + 15) / 16);
+    w.tiles = (int)(((int64_t)w.n * G + COLS - 1) / COLS);
     w.steps = max(1, (min(w.len, b.table_cols * b.page_tokens + 1) + 31) / 32);
     return w;
 }
@@ -424,12 +427,13 @@ struct ColTile {
 TG_DEV int splits_of(int steps, float inv) { return max(1, (int)ceilf((float)steps * inv)); }
 
 // 1 / (the most steps of one block)
+template <int COLS>
 TG_DEV float block_share(const KvBatch &b, int G, int share, int lane, const SeqWork &w0) {
     if (share == 0) return 0.0f;  // no splits
     float all = (float)w0.tiles * (float)w0.steps;
     int tiles = min(w0.tiles, 1 << 20);
     for (int j = lane + 64; j < (b.n_seqs + 63) / 64 * 64; j += 64) {
-        const SeqWork w = seq_work(b, G, j);
+        const SeqWork w = seq_work<COLS>(b, G, j);
         all += (float)w.tiles * (float)w.steps;
         tiles = min(tiles + w.tiles, 1 << 20);
     }
@@ -443,13 +447,14 @@ TG_DEV float block_share(const KvBatch &b, int G, int share, int lane, const Seq
 }
 
 // Block x of the launch; seq -1 where there is none.
+template <int COLS>
 TG_DEV ColTile col_tile(const KvBatch &b, int G, int share, int x, int lane) {
-    const SeqWork w0 = seq_work(b, G, lane);
-    const float inv = block_share(b, G, share, lane, w0);
+    const SeqWork w0 = seq_work<COLS>(b, G, lane);
+    const float inv = block_share<COLS>(b, G, share, lane, w0);
     ColTile r{-1, 0, 0, 0, 0, 0, 1, 0, 0, 0, 0};
     int before = 0, parts = 0, joins = 0;
     for (int j0 = 0; j0 < b.n_seqs; j0 += 64) {
-        const SeqWork w = j0 == 0 ? w0 : seq_work(b, G, j0 + lane);
+        const SeqWork w = j0 == 0 ? w0 : seq_work<COLS>(b, G, j0 + lane);
         const int splits = splits_of(w.steps, inv);
         const int mine = w.tiles * splits, mparts = splits > 1 ? mine : 0;
         const int items = wave_scan(mine), ps = wave_scan(mparts);
@@ -466,7 +471,7 @@ TG_DEV ColTile col_tile(const KvBatch &b, int G, int share, int x, int lane) {
             r.n = __builtin_amdgcn_readlane(w.n, k);
             r.len = __builtin_amdgcn_readlane(w.len, k);
             r.splits = sp;
-            r.per = (st + sp - 1) / sp * 32;
+            r.per = COLS == 16 ? (st + sp - 1) / sp * 32 : (st + 2 * sp - 1) / (2 * sp) * 64;
             r.part = parts + __builtin_amdgcn_readlane(ps, k) - __builtin_amdgcn_readlane(mparts, k) + r.tile * sp;
             r.join = joins + __builtin_amdgcn_readlane(js, k) - __builtin_amdgcn_readlane(mjoins, k) + r.tile;
         }
@@ -528,10 +533,10 @@ struct AttnOut {
     int64_t stride;
     JoinTile *join;  // [joins][key head]
     int joins;       // no more tiles than this are split
-    float *part;     // [split][key head] of 16 x D sums, then 16 pairs (m, l)
+    float *part;     // [split][key head] of COLS x D sums, then COLS pairs (m, l)
 };
-template <int D>
-constexpr int AT_PART = 16 * D + 32;  // floats of one split
+template <int D, int COLS>
+constexpr int AT_PART = COLS * (D + 2);  // floats of one split
 
 template <int D, bool BF>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_attn_split(KvBatch b, KvRows q, int G, float scale, int share,
@@ -542,7 +547,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_attn_split(KvBatch b, 
     const int lane = threadIdx.x % 64, wave = uni(threadIdx.x / 64);
     const int c = lane % 16, h = lane / 16;
     const int hk = blockIdx.y;
-    const ColTile ct = col_tile(b, G, share, blockIdx.x, lane);
+    const ColTile ct = col_tile<16>(b, G, share, blockIdx.x, lane);
     if ((int)blockIdx.x >= ct.joins && (int)blockIdx.x < o.joins && threadIdx.x == 0)
         o.join[(size_t)blockIdx.x * b.n_kv + hk] = JoinTile{0, 0, 0, 0};
     if (ct.seq < 0) return;
@@ -634,7 +639,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_attn_split(KvBatch b, 
         int e2 = 0;
         (void)frexpf(top, &e2);  // top = m 2^e2, m in [0.5, 1)
         const int a = top > 0.0f && top < INFINITY ? 11 - e2 : 0;
-        cs = ldexpf(scale * 1.44269504f, 18 - a);
+        cs = fmaxf(ldexpf(scale * 1.44269504f, 18 - a), AT_LEAST);
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             float sum = 0.0f;
@@ -846,9 +851,326 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_attn_split(KvBatch b, 
             const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
             store4<BF ? TG_T_BF16 : TG_T_F16>(o.p, (int64_t)(ct.lo + ff / G) * o.stride + (int64_t)(hk * G + ff % G) * D + d, v * inv);
         } else {
-            float *pp = o.part + ((size_t)(ct.part + ct.split) * b.n_kv + hk) * AT_PART<D>;
+            float *pp = o.part + ((size_t)(ct.part + ct.split) * b.n_kv + hk) * AT_PART<D, 16>;
             *reinterpret_cast<f32x4 *>(pp + cc * D + d) = v;
             if (d == 0) pp[16 * D + 2 * cc] = mm, pp[16 * D + 2 * cc + 1] = ll;
+        }
+    }
+}
+
+// Many columns: a block of 8 waves holds 256 columns of one key head, 32 to a
+// wave, and goes through the tokens in steps of 64, which it dequantises to
+// fp16 once for all of them: half the waves take a tile's keys, half its
+// values, ahead of their use (the packed bytes a phase before that), and leave
+// them in LDS as whole operands of the matrix instructions, 16 bytes to a
+// lane, which every wave then reads without conflict.
+//
+// The two waves of a SIMD (w and w + 4) take turns: a step is a matrix phase
+// (the output of step t - 1, the scores of step t) and a vector phase (the
+// weights of step t, dequantising a later one) with a barrier behind each,
+// and the second four waves run one phase behind, so that one wave's vector work
+// hides under the other's matrix work.  In intervals between barriers: waves
+// 0..3 have M(t) in 2 t and V(t) in 2 t + 1, where they write step t + 1;
+// waves 4..7 have M(t) in 2 t + 1 and V(t) in 2 t + 2, where they write step t +
+// 2.  K(t) is read in 2 t and 2 t + 1, V(t) in 2 t + 2 and 2 t + 3: two places for
+// keys and three for values keep every write behind the last reading.
+//
+// The roundings (keys and values 2^-11 each, weights as before) buy scores and
+// weights without a scale to apply.  The weights' sum is a matrix product with
+// ones.  Scores and bounds as in k_attn_split, A = 9 throughout.
+//
+// Bound: at D = 128 a phase of a wave is 66 matrix instructions (1056 clocks)
+// behind 32 KB of operands from LDS (1024 for the four waves that read), about 1750
+// together, against 32 exponentials and what surrounds them (1200) and the
+// dequantising of a sixteenth of the step (900).  Three prompts of 4096, 4046 and
+// 2482 tokens, 32 heads over 4: 391 us, 0.83 PFLOP/s; all waves in step, one
+// barrier to a step: 422; heads one after the other instead of side by side: 455, since
+// the longest blocks of the last head start late.  Heads of 256 leave 16 columns to a wave, which
+// reads as much for each: 1.2 to 2 times as long as k_attn_split, so they have only that.
+constexpr int AT_COLS = 256;
+
+template <int D, bool BF>
+__global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G, float scale, int share, FastDiv tpp, AttnOut o) {
+    constexpr int NG = D / 32, ND = D / 16, NC = 2, COLS = AT_COLS, BUF = 64 * D * 2;  // keys or values of a step
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = threadIdx.x % 64, wave = uni(threadIdx.x / 64), c16 = lane % 16, h = lane / 16;
+    // all heads of a tile side by side, and the late tiles of a sequence, which see the most tokens, first
+    const int x = blockIdx.x / (unsigned)b.n_kv, hk = blockIdx.x - x * b.n_kv;
+    const ColTile ct = col_tile<COLS>(b, G, share, gridDim.x / (unsigned)b.n_kv - 1 - x, lane);
+    if (x >= ct.joins && x < o.joins && threadIdx.x == 0)
+        o.join[(size_t)x * b.n_kv + hk] = JoinTile{0, 0, 0, 0};
+    if (ct.seq < 0) return;
+    const int ncol = ct.n * G, col0 = ct.tile * COLS, last = min(ncol - 1, col0 + COLS - 1);
+    const int seen = uni(tokens_seen(b, ct, last / G));
+    const int t0 = ct.split * ct.per, t1 = min(seen, t0 + ct.per);
+    if (ct.splits > 1 && ct.split == 0 && threadIdx.x == 0)
+        o.join[(size_t)ct.join * b.n_kv + hk] = JoinTile{ct.lo * G + col0, last - col0 + 1, ct.part, seen <= ct.per ? 0 : (seen + ct.per - 1) / ct.per};
+    if (t0 >= t1 && ct.split > 0) return;
+
+    // this lane's columns, one of each column tile of the wave
+    const int f0 = col0 + wave * 16 * NC;
+    int pos[NC];
+    uint32_t qw[NC][NG][4];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int f = f0 + 16 * c + c16;
+        const bool col = f < ncol;
+        pos[c] = col ? ct.len - ct.n + f / G : -1;
+        const uint16_t *qp = static_cast<const uint16_t *>(q.p) + (int64_t)(ct.lo + (col ? f / G : 0)) * q.stride +
+                             (int64_t)(hk * G + (col ? f % G : 0)) * D;
+#pragma unroll
+        for (int g = 0; g < NG; g++) load_words<4>(qp + 32 * g + 8 * h, qw[c][g]);
+    }
+    const int first = uni(ct.len - ct.n + min(f0, last) / G);  // position of the wave's first column
+
+    // this wave's share of a step: the keys (even) or values (odd) of its tile wave / 2
+    const int ntile = (int)tpp.d, span = min(ct.per, 63 * 16 * ntile & ~63);
+    const size_t head_bytes = (size_t)ntile * (18 * D), page_bytes = head_bytes * b.n_kv;
+    const uint8_t *base = b.pages + hk * head_bytes;
+    const bool is_v = wave % 2;
+    const int xt = wave / 2;
+    int mine = 0, page0 = 0, from = t0 - span;
+    // codes; scales.  Values: words [token pair][block].  Keys: those of token c16 (and what follows them), then
+    // the value scales of it and its neighbour.  The same loads for either, so that no branch waits for one.
+    uint32_t raw[NG], sc[2 * NG];
+    const uint32_t code_at = (is_v ? 8 * D : 0) + lane * (NG * 4), scale_at = is_v ? 17 * D + h * (8 * NG) : 16 * D + c16 * (2 * NG);
+    const uint32_t more_at = is_v ? scale_at + 4 * NG : 17 * D + c16 / 2 * (4 * NG);
+    bool bad = false;
+    auto pages = [&](int step) {  // those of the stretch that holds it
+        const int t = t0 + 64 * step;
+        if (t >= from + span && t < t1) {
+            from = t;
+            page0 = uni(from / 16 / ntile);
+            mine = (page0 + lane) * 16 * ntile < t1 ? page_of(b, ct.seq, (page0 + lane) * 16 * ntile) : 0;
+        }
+    };
+    auto fetch = [&](int step) {  // tile xt of it, or any behind the end, whose scales become 0
+        int t = t0 + 64 * step + 16 * xt;
+        t = t < t1 ? t : from;
+        const int tt = t / 16 - page0 * ntile, pi = (int)fdiv((uint32_t)tt, tpp), pg = __builtin_amdgcn_readlane(mine, pi);
+        bad = pg < 0;
+        const uint8_t *p = base + (size_t)max(pg, 0) * page_bytes + (size_t)(tt - pi * ntile) * (18 * D);
+        load_words<NG>(p + code_at, raw);
+        load_words<NG>(p + scale_at, sc);
+        load_words<NG>(p + more_at, sc + NG);
+    };
+    // codes n of the four-code halfwords of w, less 8, times d; one of the two constants in a scalar register
+    // and one in a vector register make a single instruction of the mask and what makes a number of it
+    uint32_t lo = 0x000F000Fu, hi = 0x00F000F0u, k1024 = 0x64006400u, k64 = 0x54005400u;
+    asm("" : "+s"(lo), "+s"(hi), "+v"(k1024), "+v"(k64));
+    auto unpack = [&](uint32_t w, int n, f16x2 d) {
+        const uint32_t v = n < 2 ? w : w >> 8;
+        const f16x2 t = n % 2 == 0 ? as_h2((v & lo) | k1024) - f16x2{(_Float16)1032.0f, (_Float16)1032.0f}
+                                   : as_h2((v & hi) | k64) - f16x2{(_Float16)72.0f, (_Float16)72.0f};
+        return as_u(t * d);
+    };
+    auto spread = [&](int step) {  // what fetch(step) brought, to LDS
+        const int t = t0 + 64 * step + 16 * xt;
+        uint8_t *buf = lds + (is_v ? 2 + step % 3 : step % 2) * BUF + lane * 16;
+        // an infinity or NaN among the value scales makes the sum of products with 0 a NaN
+        f16x2 odd = {0, 0};
+#pragma unroll
+        for (int i = 0; i < NG; i++) {
+            if (is_v) odd = __builtin_elementwise_fma(as_h2(sc[i]), f16x2{0, 0}, odd);
+            odd = __builtin_elementwise_fma(as_h2(sc[NG + i]), f16x2{0, 0}, odd);
+        }
+        const bool plain = !bad && t + 16 <= seen && !__ballot(as_u(odd) & 0x7C007C00u);
+        if (!is_v) {
+            if (!plain) {
+                uint32_t inf = 0;
+#pragma unroll
+                for (int g = 0; g < NG; g++) inf |= ((sc[NG + g] >> (16 * (c16 % 2))) & 0x7C00u) == 0x7C00u;
+                const bool poison = bad || inf, none = t + c16 >= seen;
+#pragma unroll
+                for (int g = 0; g < NG / 2; g++) sc[g] = none ? 0u : poison ? 0x7E007E00u : sc[g];
+            }
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const _Float16 d = as_h2(sc[g / 2])[g % 2];
+                const f16x2 dd = {d, d};
+                *reinterpret_cast<u32x4 *>(buf + (xt * NG + g) * 1024) =
+                    u32x4{unpack(raw[g], 0, dd), unpack(raw[g], 1, dd), unpack(raw[g], 2, dd), unpack(raw[g], 3, dd)};
+            }
+        } else {
+            if (!plain) {
+#pragma unroll
+                for (int i = 0; i < 2 * NG; i++) {
+                    const int tp = t + 4 * h + 2 * (i / NG);
+                    uint32_t d = bad ? 0u : sc[i];
+                    if ((d & 0x7C00u) == 0x7C00u || tp >= seen) d &= 0xFFFF0000u;
+                    if ((d & 0x7C000000u) == 0x7C000000u || tp + 1 >= seen) d &= 0xFFFFu;
+                    sc[i] = d;
+                }
+            }
+#pragma unroll
+            for (int bq = 0; bq < NG / 2; bq++)
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+                    *reinterpret_cast<u32x2 *>(buf + (xt / 2 * ND + 4 * bq + n) * 1024 + xt % 2 * 8) =
+                        u32x2{unpack(raw[bq], n, as_h2(sc[2 * bq + n / 2])), unpack(raw[NG / 2 + bq], n, as_h2(sc[NG + 2 * bq + n / 2]))};
+        }
+    };
+
+    const int steps = (t1 - t0 + 63) / 64;
+    if (steps > 0) {
+        pages(0);
+        fetch(0);  // before the conversions that follow
+    }
+    f16x8 qf[NC][NG];
+    float cs[NC];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        uint32_t mag = 0;
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (pos[c] < 0) qw[c][g][e] = 0;
+                mag = max(mag, max(qw[c][g][e] & 0x7FFFu, (qw[c][g][e] >> 16) & 0x7FFFu));
+            }
+        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 16));
+        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
+        const float top = BF ? bf2f((uint16_t)mag) : h2f((uint16_t)mag);
+        int e2 = 0;
+        (void)frexpf(top, &e2);
+        const int a = top > 0.0f && top < INFINITY ? 14 - e2 : 0;  // the row's largest value to 2^13 .. 2^14
+        cs[c] = fmaxf(ldexpf(scale * 1.44269504f, -a), AT_LEAST);
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint16_t u = (uint16_t)(qw[c][g][e / 2] >> (16 * (e % 2)));
+                qf[c][g][e] = (_Float16)ldexpf(BF ? bf2f(u) : h2f(u), a);
+            }
+    }
+
+    f32x4 acc[NC][ND] = {}, sum[NC] = {};
+    float m[NC];
+#pragma unroll
+    for (int c = 0; c < NC; c++) m[c] = AT_NONE;
+    const f16x8 ones = as_h8(0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u);
+    f32x4 s[NC][4];
+    f16x8 pf[NC][2];
+    const bool late = wave >= 4;
+    auto matrix = [&](int step, auto with_pv, auto with_qk) {
+        constexpr bool PV = decltype(with_pv)::value, QK = decltype(with_qk)::value;
+        const int next = step + (late ? 2 : 1);
+        if (QK) pages(next);
+        if (QK) fetch(next);
+        if (PV) {
+            const uint8_t *vb = lds + (2 + (step - 1) % 3) * BUF + lane * 16;
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+#pragma unroll
+                for (int c = 0; c < NC; c++) sum[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[c][p], sum[c], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < ND; j++) {
+                    const f16x8 vf = *reinterpret_cast<const f16x8 *>(vb + (p * ND + j) * 1024);
+#pragma unroll
+                    for (int c = 0; c < NC; c++) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[c][p], acc[c][j], 0, 0, 0);
+                }
+            }
+        }
+        if (QK) {
+            const uint8_t *kb = lds + step % 2 * BUF + lane * 16;
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const f16x8 kf = *reinterpret_cast<const f16x8 *>(kb + (x * NG + g) * 1024);
+#pragma unroll
+                    for (int c = 0; c < NC; c++)
+                        s[c][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[c][g], g == 0 ? f32x4{0, 0, 0, 0} : s[c][x], 0, 0, 0);
+                }
+        }
+    };
+    auto vector = [&](int step) {
+        const int t = t0 + 64 * step;
+        if (t + 63 > first) {
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (t + 16 * x + 4 * h + i > pos[c]) s[c][x][i] = -INFINITY;
+        }
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            float top = s[c][0][0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) top = __builtin_elementwise_maximum(top, s[c][i / 4][i % 4]);  // a NaN stays one
+            if (__ballot(top * cs[c] > m[c] + AT_ROOM)) {
+                const float m2 = fmaxf(m[c], col_max(top) * cs[c]), r = __builtin_amdgcn_exp2f(m[c] - m2);
+                sum[c] *= r;
+#pragma unroll
+                for (int j = 0; j < ND; j++) acc[c][j] *= r;
+                m[c] = m2;
+            }
+            const float off = (float)AT_TOP - m[c];
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                w[i] = pack_h2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[c][i / 2][i % 2 * 2], cs[c], off)),
+                               __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][i / 2][i % 2 * 2 + 1], cs[c], off)));
+            pf[c][0] = as_h8(w[0], w[1], w[2], w[3]);
+            pf[c][1] = as_h8(w[4], w[5], w[6], w[7]);
+        }
+        const int ahead = step + (late ? 2 : 1);
+        if (ahead < steps) spread(ahead);
+    };
+    if (steps > 0) {
+        using std::true_type, std::false_type;
+        spread(0);
+        lds_barrier();
+        if (late) {
+            if (steps > 1) {
+                pages(1);
+                fetch(1);
+                spread(1);
+            }
+            lds_barrier();
+        }
+        matrix(0, false_type{}, true_type{});
+        lds_barrier();
+        vector(0);
+        lds_barrier();
+        for (int i = 1; i < steps; i++) {
+            matrix(i, true_type{}, true_type{});
+            lds_barrier();
+            vector(i);
+            lds_barrier();
+        }
+        matrix(steps, true_type{}, false_type{});
+        if (!late) lds_barrier();
+        lds_barrier();
+    }
+    const bool whole = seen <= ct.per;
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int f = f0 + 16 * c + c16;
+        if (whole) {
+            // through LDS, 16 columns of the wave at a time, so that a head leaves as whole lines
+            uint16_t *so = reinterpret_cast<uint16_t *>(lds) + wave * 16 * (D + 8);
+            const float inv = sum[c][0] == 0.0f ? 0.0f : 1.0f / sum[c][0];
+#pragma unroll
+            for (int j = 0; j < ND; j++) store4<BF ? TG_T_BF16 : TG_T_F16>(so, c16 * (D + 8) + 16 * j + 4 * h, acc[c][j] * inv);
+            wave_lds_sync();
+            constexpr int L = D / 8;  // lanes of one head
+#pragma unroll
+            for (int i = 0; i < 16 * L / 64; i++) {
+                const int cc = i * (64 / L) + lane / L, ff = f0 + 16 * c + cc;
+                const u32x4 v = *reinterpret_cast<const u32x4 *>(so + cc * (D + 8) + 8 * (lane % L));
+                if (ff < ncol)
+                    *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(o.p) + (int64_t)(ct.lo + ff / G) * o.stride + (int64_t)(hk * G + ff % G) * D + 8 * (lane % L)) = v;
+            }
+            wave_lds_sync();
+        } else if (f < ncol) {
+            float *pp = o.part + ((size_t)(ct.part + ct.split) * b.n_kv + hk) * AT_PART<D, COLS>;
+            const int cc = f - col0;
+#pragma unroll
+            for (int j = 0; j < ND; j++) *reinterpret_cast<f32x4 *>(pp + (size_t)cc * D + 16 * j + 4 * h) = acc[c][j];
+            if (h == 0) pp[COLS * D + 2 * cc] = m[c], pp[COLS * D + 2 * cc + 1] = sum[c][0];
         }
     }
 }
@@ -865,8 +1187,8 @@ __global__ __launch_bounds__(256) void k_attn_join(KvBatch b, int G, AttnOut o) 
     const int hk = blockIdx.y, tid = threadIdx.x % TC, ci = threadIdx.x / TC, cc = blockIdx.z * NC + ci;
     const JoinTile jt = o.join[(size_t)blockIdx.x * b.n_kv + hk];
     if (!jt.splits || (int)blockIdx.z * NC >= jt.cols) return;
-    const size_t step = (size_t)b.n_kv * AT_PART<D>;
-    const float *part = o.part + ((size_t)jt.part * b.n_kv + hk) * AT_PART<D>;
+    const size_t step = (size_t)b.n_kv * AT_PART<D, 16>;
+    const float *part = o.part + ((size_t)jt.part * b.n_kv + hk) * AT_PART<D, 16>;
     // all of a thread's sums (those of the first 8 turns) and its (m, l) are asked for before the first is
     // waited for; columns behind the last hold zeros
     const float *mine = part + cc * D + 4 * (tid % L), *ml = part + 16 * D + 2 * cc;
@@ -922,7 +1244,45 @@ __global__ __launch_bounds__(256) void k_attn_join(KvBatch b, int G, AttnOut o) 
                                       v * (ll == 0.0f ? 0.0f : 1.0f / ll));
 }
 
+// The same for the wide column tiles, which have few splits: a thread to four
+// dims of a column, which goes through them alone.
+template <int D, bool BF, int COLS>
+__global__ __launch_bounds__(256) void k_attn_join_wide(KvBatch b, int G, AttnOut o) {
+    constexpr int L = D / 4, NC = 256 / L;
+    const int hk = blockIdx.y, d = threadIdx.x % L * 4, cc = blockIdx.z * NC + threadIdx.x / L;
+    const JoinTile jt = o.join[(size_t)blockIdx.x * b.n_kv + hk];
+    if (!jt.splits || cc >= jt.cols) return;
+    const size_t step = (size_t)b.n_kv * AT_PART<D, COLS>;
+    const float *part = o.part + ((size_t)jt.part * b.n_kv + hk) * AT_PART<D, COLS>, *ml = part + COLS * D + 2 * cc, *mine = part + (size_t)cc * D + d;
+    float mm = AT_NONE, ll = 0.0f;
+    f32x4 v = {0, 0, 0, 0};
+    for (int s = 0; s < jt.splits; s++) mm = fmaxf(mm, ml[s * step]);
+#pragma unroll 4
+    for (int s = 0; s < jt.splits; s++) {
+        const float w = __builtin_amdgcn_exp2f(ml[s * step] - mm);
+        ll += ml[s * step + 1] * w;
+        v += *reinterpret_cast<const f32x4 *>(mine + s * step) * w;
+    }
+    const int f = jt.col + cc, row = f / G;
+    store4<BF ? TG_T_BF16 : TG_T_F16>(o.p, (int64_t)row * o.stride + (int64_t)(hk * G + f - row * G) * D + d,
+                                      v * (ll == 0.0f ? 0.0f : 1.0f / ll));
+}
+
 // ================================================================ launchers
+// The dynamic-LDS limit of kernel fn raised to `bytes` (above 64 KB) on the
+// current device, once per (kernel, device): `done` holds a bit per device.
+static hipError_t attn_lds(const void *fn, size_t bytes, std::atomic<uint64_t> &done) {
+    if (bytes <= 65536) return hipSuccess;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (bit && (done.load(std::memory_order_relaxed) & bit)) return hipSuccess;
+    e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == hipSuccess && bit) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
 #define TG_BY_DIM(D, ...)                                                     \
     do {                                                                      \
         if ((D) == 64) { constexpr int DIM = 64; __VA_ARGS__; }               \
@@ -958,16 +1318,20 @@ hipError_t launch_kv_read(const KvBatch &b, void *k, void *v, hipStream_t st) {
 // are more, 4 share splits and 2 share tiles.
 struct AttnPlan {
     int64_t tiles;
-    int share, joins;
+    int cols, share, joins;
 };
-#ifndef AT_BLOCKS
-#define AT_BLOCKS 512
-#endif
 static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len) {
+    const int64_t all = (int64_t)b.n_tokens * (n_heads / b.n_kv);
     AttnPlan p;
-    p.tiles = (int64_t)b.n_tokens * (n_heads / b.n_kv) / 16 + b.n_seqs;
+    // The mean number of columns of a sequence says which kernel takes all of them.  16 sequences of up to 4096
+    // tokens, D = 128, few against many: 64 columns 42 and 50 us, 96 51 and 52, 128 53 and 54, 256 88 and 59; one of
+    // 16000: 128 43 and 56, 256 51 and 61; 200 of up to 1000: 128 117 and 129, 256 203 and 127; D = 64, 16 of up to
+    // 8192: 64 72 and 88, 128 87 and 89.
+    const bool many = b.D < 256 && all >= 128 * (int64_t)b.n_seqs;
+    p.cols = many ? AT_COLS : 16;
+    p.tiles = all / p.cols + b.n_seqs;
     // nothing to split where no sequence is over what one block takes at the least, or there are tiles enough
-    p.share = std::max(1, AT_BLOCKS / b.n_kv);
+    p.share = std::max(1, (many ? 256 : 512) / b.n_kv);
     if (max_len <= 32 * AT_MIN || p.tiles > 4 * p.share) p.share = 0;
     p.joins = (int)std::min<int64_t>(p.tiles, p.tiles > p.share ? 2 * p.share : p.share);
     return p;
@@ -979,30 +1343,45 @@ static size_t attn_join_bytes(const KvBatch &b, const AttnPlan &p) {
 
 size_t attn_workspace(const KvBatch &b, int n_heads, int max_len) {
     const AttnPlan p = attn_plan(b, n_heads, max_len);
-    return p.share ? attn_join_bytes(b, p) + (size_t)4 * p.share * b.n_kv * (16 * b.D + 32) * sizeof(float) : 0;
+    return p.share ? attn_join_bytes(b, p) + (size_t)(p.tiles > p.share ? 4 : 2) * p.share * b.n_kv * (p.cols * (b.D + 2)) * sizeof(float) : 0;
 }
 
 template <int D, bool BF>
-static void attn_split_launch(const KvBatch &b, KvRows q, int G, float scale, const AttnPlan &p, const AttnOut &o, hipStream_t st) {
+static hipError_t attn_launch(const KvBatch &b, KvRows q, int G, float scale, const AttnPlan &p, const AttnOut &o, hipStream_t st) {
+    static std::atomic<uint64_t> done{0};
     const dim3 grid((unsigned)(p.tiles + 2 * p.share), (unsigned)b.n_kv);
-    TG_LAUNCH((k_attn_split<D, BF>), grid, dim3(256), 0, st, b, q, G, scale, p.share, make_fastdiv((uint32_t)(b.page_tokens / 16)), o);
-    if (!p.share) return;
+    const FastDiv tpp = make_fastdiv((uint32_t)(b.page_tokens / 16));
+    if constexpr (D < 256) {
+        if (p.cols == AT_COLS) {
+            constexpr size_t LDS = 5 * 64 * D * 2;
+            const hipError_t e = attn_lds((const void *)k_attn_tile<D, BF>, LDS, done);
+            if (e != hipSuccess) return e;
+            TG_LAUNCH((k_attn_tile<D, BF>), dim3(grid.x * grid.y), dim3(512), LDS, st, b, q, G, scale, p.share, tpp, o);
+            if (p.share) TG_LAUNCH((k_attn_join_wide<D, BF, AT_COLS>), dim3(p.joins, b.n_kv, AT_COLS * D / 1024), dim3(256), 0, st, b, G, o);
+            return hipSuccess;
+        }
+    }
+    TG_LAUNCH((k_attn_split<D, BF>), grid, dim3(256), 0, st, b, q, G, scale, p.share, tpp, o);
+    if (!p.share) return hipSuccess;
     if (p.joins * b.n_kv <= 64) TG_LAUNCH((k_attn_join<D, BF, 256>), dim3(p.joins, b.n_kv, 16), dim3(256), 0, st, b, G, o);
     else TG_LAUNCH((k_attn_join<D, BF, 64>), dim3(p.joins, b.n_kv, 4), dim3(256), 0, st, b, G, o);
+    return hipSuccess;
 }
 
 hipError_t launch_attn(const KvBatch &b, int type, KvRows q, int n_heads, float scale, void *out, int64_t out_stride,
                        int max_len, void *ws, hipStream_t st) {
     const AttnPlan p = attn_plan(b, n_heads, max_len);
-    if (p.tiles + 2 * p.share > INT32_MAX / 16) return hipErrorInvalidValue;
+    // threads of the launch's first dimension
+    if ((p.tiles + 2 * p.share) * (p.cols == AT_COLS ? 512 * b.n_kv : 256) > UINT32_MAX) return hipErrorInvalidValue;
     const int G = n_heads / b.n_kv;
     const AttnOut o{out, out_stride, static_cast<JoinTile *>(ws), p.joins,
                     reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + attn_join_bytes(b, p))};
+    hipError_t e = hipSuccess;
     TG_BY_DIM(b.D, {
-        if (type == TG_T_F16) attn_split_launch<DIM, false>(b, q, G, scale, p, o, st);
-        else attn_split_launch<DIM, true>(b, q, G, scale, p, o, st);
+        if (type == TG_T_F16) e = attn_launch<DIM, false>(b, q, G, scale, p, o, st);
+        else e = attn_launch<DIM, true>(b, q, G, scale, p, o, st);
     });
-    return hipGetLastError();
+    return e != hipSuccess ? e : hipGetLastError();
 }
 
 }  // namespace tg
