@@ -875,23 +875,29 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_attn_split(KvBatch b, 
 // 2.  K(t) is read in 2 t and 2 t + 1, V(t) in 2 t + 2 and 2 t + 3: two places for
 // keys and three for values keep every write behind the last reading.
 //
-// The roundings (keys and values 2^-11 each, weights as before) buy scores and
-// weights without a scale to apply.  The weights' sum is a matrix product with
+// Keys and values rounded to fp16 (2^-11 of each at the most) buy scores and
+// weights without a scale to apply.  For bf16 rows that stays under the rounding
+// of the result, 2^-9; fp16 rows, whose results show it (2.1 times the error of one
+// rounding), take the roundings' remainders, which fp16 holds exactly, as a second
+// operand of every product.  The weights' sum is a matrix product with
 // ones.  Scores and bounds as in k_attn_split, A = 9 throughout.
 //
-// Bound: at D = 128 a phase of a wave is 66 matrix instructions (1056 clocks)
+// Bound: at D = 128, bf16, a phase of a wave is 66 matrix instructions (1056 clocks)
 // behind 32 KB of operands from LDS (1024 for the four waves that read), about 1750
 // together, against 32 exponentials and what surrounds them (1200) and the
 // dequantising of a sixteenth of the step (900).  Three prompts of 4096, 4046 and
-// 2482 tokens, 32 heads over 4: 391 us, 0.83 PFLOP/s; all waves in step, one
+// 2482 tokens, 32 heads over 4: 390 us, 0.83 PFLOP/s; all waves in step, one
 // barrier to a step: 422; heads one after the other instead of side by side: 455, since
-// the longest blocks of the last head start late.  Heads of 256 leave 16 columns to a wave, which
+// the longest blocks of the last head start late.  fp16, D = 64, 500 tokens each of two prompts of
+// 16001, 32 heads over 8: 250 us, without the remainders 186, with those of the keys and of the weights
+// (more vector work, less of LDS) 284.  Heads of 256 leave 16 columns to a wave, which
 // reads as much for each: 1.2 to 2 times as long as k_attn_split, so they have only that.
 constexpr int AT_COLS = 256;
 
 template <int D, bool BF>
 __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G, float scale, int share, FastDiv tpp, AttnOut o) {
     constexpr int NG = D / 32, ND = D / 16, NC = 2, COLS = AT_COLS, BUF = 64 * D * 2;  // keys or values of a step
+    constexpr int REST = BF ? 0 : 5 * BUF;  // where the roundings' remainders are
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x % 64, wave = uni(threadIdx.x / 64), c16 = lane % 16, h = lane / 16;
     // all heads of a tile side by side, and the late tiles of a sequence, which see the most tokens, first
@@ -954,27 +960,60 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
         load_words<NG>(p + scale_at, sc);
         load_words<NG>(p + more_at, sc + NG);
     };
-    // codes n of the four-code halfwords of w, less 8, times d; one of the two constants in a scalar register
+    // codes n of the four-code halfwords of w, less 8, times d, and the rounding's remainder; one of the two constants in a scalar register
     // and one in a vector register make a single instruction of the mask and what makes a number of it
     uint32_t lo = 0x000F000Fu, hi = 0x00F000F0u, k1024 = 0x64006400u, k64 = 0x54005400u;
     asm("" : "+s"(lo), "+s"(hi), "+v"(k1024), "+v"(k64));
-    auto unpack = [&](uint32_t w, int n, f16x2 d) {
+    auto unpack = [&](uint32_t w, int n, f16x2 d, uint32_t &rest) {
         const uint32_t v = n < 2 ? w : w >> 8;
         const f16x2 t = n % 2 == 0 ? as_h2((v & lo) | k1024) - f16x2{(_Float16)1032.0f, (_Float16)1032.0f}
                                    : as_h2((v & hi) | k64) - f16x2{(_Float16)72.0f, (_Float16)72.0f};
-        return as_u(t * d);
+        const f16x2 v16 = t * d;
+        rest = as_u(__builtin_elementwise_fma(t, d, -v16));
+        return as_u(v16);
     };
-    auto spread = [&](int step) {  // what fetch(step) brought, to LDS
+    auto spread = [&](int step) __attribute__((always_inline)) {  // what fetch(step) brought, to LDS
         const int t = t0 + 64 * step + 16 * xt;
         uint8_t *buf = lds + (is_v ? 2 + step % 3 : step % 2) * BUF + lane * 16;
-        // an infinity or NaN among the value scales makes the sum of products with 0 a NaN
-        f16x2 odd = {0, 0};
+        // an infinity or NaN among the value scales makes the sum of products with 0 a NaN; so does, for the
+        // remainders, a scale whose values fp16 does not hold
+        f16x2 odd = {0, 0}, over = {0, 0};
 #pragma unroll
         for (int i = 0; i < NG; i++) {
             if (is_v) odd = __builtin_elementwise_fma(as_h2(sc[i]), f16x2{0, 0}, odd);
             odd = __builtin_elementwise_fma(as_h2(sc[NG + i]), f16x2{0, 0}, odd);
+            if (REST && (is_v || i < NG / 2)) over = __builtin_elementwise_fma(as_h2(sc[i]) * (_Float16)8.0f, f16x2{0, 0}, over);
+            if (REST && is_v) over = __builtin_elementwise_fma(as_h2(sc[NG + i]) * (_Float16)8.0f, f16x2{0, 0}, over);
         }
         const bool plain = !bad && t + 16 <= seen && !__ballot(as_u(odd) & 0x7C007C00u);
+        const bool rests = REST && !__ballot(as_u(over) & 0x7C007C00u);
+        auto keys = [&](auto with) __attribute__((always_inline)) {
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const _Float16 d = as_h2(sc[g / 2])[g % 2];
+                u32x4 v, r;
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    uint32_t lo2 = 0;
+                    v[n] = unpack(raw[g], n, f16x2{d, d}, lo2);
+                    r[n] = decltype(with)::value ? lo2 : 0;
+                }
+                *reinterpret_cast<u32x4 *>(buf + (xt * NG + g) * 1024) = v;
+                if (REST) *reinterpret_cast<u32x4 *>(buf + REST + (xt * NG + g) * 1024) = r;
+            }
+        };
+        auto values = [&](auto with) __attribute__((always_inline)) {
+#pragma unroll
+            for (int bq = 0; bq < NG / 2; bq++)
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    uint32_t r0, r1;
+                    const u32x2 v = {unpack(raw[bq], n, as_h2(sc[2 * bq + n / 2]), r0), unpack(raw[NG / 2 + bq], n, as_h2(sc[NG + 2 * bq + n / 2]), r1)};
+                    uint8_t *p = buf + (xt / 2 * ND + 4 * bq + n) * 1024 + xt % 2 * 8;
+                    *reinterpret_cast<u32x2 *>(p) = v;
+                    if (REST) *reinterpret_cast<u32x2 *>(p + REST) = decltype(with)::value ? u32x2{r0, r1} : u32x2{0, 0};
+                }
+        };
         if (!is_v) {
             if (!plain) {
                 uint32_t inf = 0;
@@ -984,13 +1023,8 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
 #pragma unroll
                 for (int g = 0; g < NG / 2; g++) sc[g] = none ? 0u : poison ? 0x7E007E00u : sc[g];
             }
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const _Float16 d = as_h2(sc[g / 2])[g % 2];
-                const f16x2 dd = {d, d};
-                *reinterpret_cast<u32x4 *>(buf + (xt * NG + g) * 1024) =
-                    u32x4{unpack(raw[g], 0, dd), unpack(raw[g], 1, dd), unpack(raw[g], 2, dd), unpack(raw[g], 3, dd)};
-            }
+            if (rests) keys(std::true_type{});
+            else keys(std::false_type{});
         } else {
             if (!plain) {
 #pragma unroll
@@ -1002,12 +1036,8 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
                     sc[i] = d;
                 }
             }
-#pragma unroll
-            for (int bq = 0; bq < NG / 2; bq++)
-#pragma unroll
-                for (int n = 0; n < 4; n++)
-                    *reinterpret_cast<u32x2 *>(buf + (xt / 2 * ND + 4 * bq + n) * 1024 + xt % 2 * 8) =
-                        u32x2{unpack(raw[bq], n, as_h2(sc[2 * bq + n / 2])), unpack(raw[NG / 2 + bq], n, as_h2(sc[NG + 2 * bq + n / 2]))};
+            if (rests) values(std::true_type{});
+            else values(std::false_type{});
         }
     };
 
@@ -1052,7 +1082,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
     f32x4 s[NC][4];
     f16x8 pf[NC][2];
     const bool late = wave >= 4;
-    auto matrix = [&](int step, auto with_pv, auto with_qk) {
+    auto matrix = [&](int step, auto with_pv, auto with_qk) __attribute__((always_inline)) {
         constexpr bool PV = decltype(with_pv)::value, QK = decltype(with_qk)::value;
         const int next = step + (late ? 2 : 1);
         if (QK) pages(next);
@@ -1068,6 +1098,11 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
                     const f16x8 vf = *reinterpret_cast<const f16x8 *>(vb + (p * ND + j) * 1024);
 #pragma unroll
                     for (int c = 0; c < NC; c++) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[c][p], acc[c][j], 0, 0, 0);
+                    if (REST) {
+                        const f16x8 vr = *reinterpret_cast<const f16x8 *>(vb + REST + (p * ND + j) * 1024);
+#pragma unroll
+                        for (int c = 0; c < NC; c++) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vr, pf[c][p], acc[c][j], 0, 0, 0);
+                    }
                 }
             }
         }
@@ -1081,10 +1116,15 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
 #pragma unroll
                     for (int c = 0; c < NC; c++)
                         s[c][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[c][g], g == 0 ? f32x4{0, 0, 0, 0} : s[c][x], 0, 0, 0);
+                    if (REST) {
+                        const f16x8 kr = *reinterpret_cast<const f16x8 *>(kb + REST + (x * NG + g) * 1024);
+#pragma unroll
+                        for (int c = 0; c < NC; c++) s[c][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kr, qf[c][g], s[c][x], 0, 0, 0);
+                    }
                 }
         }
     };
-    auto vector = [&](int step) {
+    auto vector = [&](int step) __attribute__((always_inline)) {
         const int t = t0 + 64 * step;
         if (t + 63 > first) {
 #pragma unroll
@@ -1320,14 +1360,15 @@ struct AttnPlan {
     int64_t tiles;
     int cols, share, joins;
 };
-static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len) {
+static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len, bool bf16) {
     const int64_t all = (int64_t)b.n_tokens * (n_heads / b.n_kv);
     AttnPlan p;
     // The mean number of columns of a sequence says which kernel takes all of them.  16 sequences of up to 4096
     // tokens, D = 128, few against many: 64 columns 42 and 50 us, 96 51 and 52, 128 53 and 54, 256 88 and 59; one of
     // 16000: 128 43 and 56, 256 51 and 61; 200 of up to 1000: 128 117 and 129, 256 203 and 127; D = 64, 16 of up to
-    // 8192: 64 72 and 88, 128 87 and 89.
-    const bool many = b.D < 256 && all >= 128 * (int64_t)b.n_seqs;
+    // 8192: 64 72 and 88, 128 87 and 89.  fp16, whose many take longer: D = 128, 128 columns 56 and 74, 192 73 and 74,
+    // 256 88 and 76; D = 64 128 88 and 109, 192 114 and 111, 256 137 and 114.
+    const bool many = b.D < 256 && all >= (bf16 ? 128 : 192) * (int64_t)b.n_seqs;
     p.cols = many ? AT_COLS : 16;
     p.tiles = all / p.cols + b.n_seqs;
     // nothing to split where no sequence is over what one block takes at the least, or there are tiles enough
@@ -1341,9 +1382,15 @@ static size_t attn_join_bytes(const KvBatch &b, const AttnPlan &p) {
     return ((size_t)p.joins * b.n_kv * sizeof(JoinTile) + 255) / 256 * 256;
 }
 
+// Enough for rows of either type.
 size_t attn_workspace(const KvBatch &b, int n_heads, int max_len) {
-    const AttnPlan p = attn_plan(b, n_heads, max_len);
-    return p.share ? attn_join_bytes(b, p) + (size_t)(p.tiles > p.share ? 4 : 2) * p.share * b.n_kv * (p.cols * (b.D + 2)) * sizeof(float) : 0;
+    size_t most = 0;
+    for (const bool bf16 : {false, true}) {
+        const AttnPlan p = attn_plan(b, n_heads, max_len, bf16);
+        if (p.share)
+            most = std::max(most, attn_join_bytes(b, p) + (size_t)(p.tiles > p.share ? 4 : 2) * p.share * b.n_kv * (p.cols * (b.D + 2)) * sizeof(float));
+    }
+    return most;
 }
 
 template <int D, bool BF>
@@ -1353,7 +1400,7 @@ static hipError_t attn_launch(const KvBatch &b, KvRows q, int G, float scale, co
     const FastDiv tpp = make_fastdiv((uint32_t)(b.page_tokens / 16));
     if constexpr (D < 256) {
         if (p.cols == AT_COLS) {
-            constexpr size_t LDS = 5 * 64 * D * 2;
+            constexpr size_t LDS = (BF ? 5 : 10) * 64 * D * 2;
             const hipError_t e = attn_lds((const void *)k_attn_tile<D, BF>, LDS, done);
             if (e != hipSuccess) return e;
             TG_LAUNCH((k_attn_tile<D, BF>), dim3(grid.x * grid.y), dim3(512), LDS, st, b, q, G, scale, p.share, tpp, o);
@@ -1370,7 +1417,7 @@ static hipError_t attn_launch(const KvBatch &b, KvRows q, int G, float scale, co
 
 hipError_t launch_attn(const KvBatch &b, int type, KvRows q, int n_heads, float scale, void *out, int64_t out_stride,
                        int max_len, void *ws, hipStream_t st) {
-    const AttnPlan p = attn_plan(b, n_heads, max_len);
+    const AttnPlan p = attn_plan(b, n_heads, max_len, type == TG_T_BF16);
     // threads of the launch's first dimension
     if ((p.tiles + 2 * p.share) * (p.cols == AT_COLS ? 512 * b.n_kv : 256) > UINT32_MAX) return hipErrorInvalidValue;
     const int G = n_heads / b.n_kv;
