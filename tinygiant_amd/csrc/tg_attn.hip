@@ -409,8 +409,8 @@ TG_DEV T wave_scan(T v) {
 template <class T>
 TG_DEV T wave_sum(T v) { return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(v)), 63)); }
 
-// How the launch is cut.  Sequence s has `tiles` column tiles of `steps` steps
-// of 32 tokens.  A block takes at most `each` steps of one tile, the fewest
+// How a launch of wide column tiles is cut.  Sequence s has `tiles` of them of
+// `steps` steps of 32 tokens.  A block takes at most `each` steps of one tile, the fewest
 // (from an even share on, an eighth more at a time) with which all the pieces of a key head are
 // `share` blocks or less, so that one round of the device's CUs does them
 // all and the longest block is as short as that allows; where there are more tiles than that anyway, an
@@ -471,7 +471,7 @@ TG_DEV ColTile col_tile(const KvBatch &b, int G, int share, int x, int lane) {
             r.n = __builtin_amdgcn_readlane(w.n, k);
             r.len = __builtin_amdgcn_readlane(w.len, k);
             r.splits = sp;
-            r.per = COLS == 16 ? (st + sp - 1) / sp * 32 : (st + 2 * sp - 1) / (2 * sp) * 64;
+            r.per = (st + 2 * sp - 1) / (2 * sp) * 64;
             r.part = parts + __builtin_amdgcn_readlane(ps, k) - __builtin_amdgcn_readlane(mparts, k) + r.tile * sp;
             r.join = joins + __builtin_amdgcn_readlane(js, k) - __builtin_amdgcn_readlane(mjoins, k) + r.tile;
         }
@@ -486,9 +486,69 @@ TG_DEV ColTile col_tile(const KvBatch &b, int G, int share, int x, int lane) {
     return r;
 }
 
+// How a launch of narrow column tiles is cut.  The column tiles of a key head
+// stand in a row, each as long as its steps of 32 tokens (in units of `unit`)
+// and AT_OVER units more for what beginning it costs, and the row is cut into `share`
+// equal lengths (fewer where there are fewer units), one to a block, which does the
+// pieces of tiles that it holds one after the other.  share 0: a tile is one
+// unit, a block one tile.  64 sequences of up to 8192 tokens, 32 heads of 128 over 4: 40 us
+// (AT_OVER 3 .. 6; 8: 41), with tiles cut into even parts of their own, a block to a part: 45.
+constexpr uint32_t AT_OVER = 4;
+struct Spot {
+    int seq, tile, lo, n, len;
+    int place;           // the tile's among all
+    uint32_t at, units;  // units into the tile, and its length
+};
+struct Cut {
+    SeqWork w;  // of the lane's sequence among the first 64
+    uint32_t mine, upto, total, share, each, more;  // the first `more` blocks have each + 1 units
+    int unit, tiles;
+    TG_DEV uint32_t length(const SeqWork &s) const { return share ? ((uint32_t)s.steps + unit - 1) / unit + AT_OVER : 1; }
+    TG_DEV Cut(const KvBatch &b, int G, int share_, int unit_, int lane) : w(seq_work<16>(b, G, lane)), share(share_), unit(unit_) {
+        mine = (uint32_t)w.tiles * length(w), upto = wave_scan(mine);
+        total = __builtin_amdgcn_readlane(upto, 63), tiles = wave_sum(w.tiles);
+        if (!share) return;
+        for (int j = lane + 64; j < (b.n_seqs + 63) / 64 * 64; j += 64) {
+            const SeqWork s = seq_work<16>(b, G, j);
+            total += wave_sum((uint32_t)s.tiles * length(s)), tiles += wave_sum(s.tiles);
+        }
+        total = uni(total), tiles = uni(tiles);
+        share = min(share, max(total, 1u));
+        each = total / share, more = total - each * share;
+    }
+    TG_DEV uint32_t begin(uint32_t x) const { return share ? x * each + min(x, more) : x; }
+    TG_DEV uint32_t block_of(uint32_t u) const {  // share only
+        const uint32_t w = more * (each + 1);
+        return u < w ? u / (each + 1) : more + (u - w) / max(each, 1u);
+    }
+    TG_DEV Spot at(const KvBatch &b, int G, uint32_t u, int lane) const {
+        uint32_t before = 0;
+        int tiles_before = 0;
+        for (int j0 = 0; j0 < b.n_seqs; j0 += 64) {
+            const SeqWork s = j0 == 0 ? w : seq_work<16>(b, G, j0 + lane);
+            const uint32_t m = j0 == 0 ? mine : (uint32_t)s.tiles * length(s), up = j0 == 0 ? upto : wave_scan(m);
+            const uint64_t found = __ballot(before + up > u);
+            if (found) {
+                const int k = __builtin_ctzll(found);
+                Spot r;
+                r.units = __builtin_amdgcn_readlane(length(s), k);
+                const uint32_t local = u - before - __builtin_amdgcn_readlane(up, k) + __builtin_amdgcn_readlane(m, k);
+                r.seq = j0 + k, r.tile = uni(local / r.units), r.at = local - r.tile * r.units;
+                r.place = tiles_before + wave_sum(lane < k ? s.tiles : 0) + r.tile;
+                r.lo = __builtin_amdgcn_readlane(s.lo, k), r.n = __builtin_amdgcn_readlane(s.n, k), r.len = __builtin_amdgcn_readlane(s.len, k);
+                if ((uint32_t)r.tile >= (uint32_t)__builtin_amdgcn_readlane(s.tiles, k)) r.seq = -1;  // rows counted twice, sums that wrapped
+                return r;
+            }
+            before += __builtin_amdgcn_readlane(up, 63), tiles_before += wave_sum(s.tiles);
+        }
+        return Spot{-1, 0, 0, 0, 0, 0, 0, 0};
+    }
+};
+
 // How many tokens row i of the sequence sees.  One beyond the table is
 // enough to make NaN of it, so a length that no table holds costs no more.
-TG_DEV int tokens_seen(const KvBatch &b, const ColTile &ct, int i) {
+template <class T>
+TG_DEV int tokens_seen(const KvBatch &b, const T &ct, int i) {
     return max(0, min(ct.len - ct.n + i + 1, b.table_cols * b.page_tokens + 1));
 }
 
@@ -515,16 +575,16 @@ TG_DEV void load_words(const void *p, uint32_t *w) {
     }
 }
 
-// Few columns: split over the tokens.  A block holds one column tile of one
-// key head and a chunk of tokens, its four waves every fourth step of 32; the
+// Few columns: split over the tokens.  A block goes through pieces of column
+// tiles (as Cut says), its four waves every fourth step of 32 tokens; the
 // packed bytes go from memory to registers one step ahead and are unpacked
 // there (each is used by one wave, so LDS would only add a trip), the scales
-// through a wave's corner of LDS because 16 lanes need the same ones.  Chunks
+// through a wave's corner of LDS because 16 lanes need the same ones.  The pieces
 // of one column tile are joined by k_attn_join, or written out at once where
-// one chunk is all.
+// one is all.
 // What k_attn_join needs of one column tile that is split: its first column
-// (row * G + head of the key head's), how many, its first partial result, and
-// how many to join (0: the first holds all that the tile sees).
+// (row * G + head of the key head's), how many, its first partial result (of
+// narrow tiles: the block that began it), and how many to join (0: none is split).
 struct JoinTile {
     int col, cols, part, splits;
 };
@@ -533,44 +593,59 @@ struct AttnOut {
     int64_t stride;
     JoinTile *join;  // [joins][key head]
     int joins;       // no more tiles than this are split
-    float *part;     // [split][key head] of COLS x D sums, then COLS pairs (m, l)
+    float *part;     // [split][key head] of COLS x D sums, then COLS pairs (m, l); narrow tiles: two to a block, that of the
+                     // tile it goes on with and that of the tile it leaves
 };
 template <int D, int COLS>
 constexpr int AT_PART = COLS * (D + 2);  // floats of one split
 
 template <int D, bool BF>
-__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_attn_split(KvBatch b, KvRows q, int G, float scale, int share,
-                                                                      FastDiv tpp, AttnOut o) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_split(KvBatch b, KvRows q, int G, float scale, int share,
+                                                                      int unit, FastDiv tpp, AttnOut o) {
     constexpr int NG = D / 32, ND = D / 16, SW = D / 64;
     constexpr int NB = D == 256 ? 2 : 3;  // steps held: one at work, the others on their way
     __shared__ __align__(16) uint8_t sm[4 * 16 * D * 4 + 4 * 16 * 8];
     const int lane = threadIdx.x % 64, wave = uni(threadIdx.x / 64);
     const int c = lane % 16, h = lane / 16;
     const int hk = blockIdx.y;
-    const ColTile ct = col_tile<16>(b, G, share, blockIdx.x, lane);
-    if ((int)blockIdx.x >= ct.joins && (int)blockIdx.x < o.joins && threadIdx.x == 0)
-        o.join[(size_t)blockIdx.x * b.n_kv + hk] = JoinTile{0, 0, 0, 0};
-    if (ct.seq < 0) return;
+    const Cut cut(b, G, share, unit, lane);
+    // what is to be joined stands at the tile's place where places are few, at that of the block that begins it otherwise
+    const bool by_tile = o.joins < share;
+    JoinTile left{0, 0, 0, 0};  // the tile that the block begins and does not end
+    uint32_t u = cut.begin(blockIdx.x);
+    const uint32_t u1 = cut.share && blockIdx.x >= cut.share ? u : cut.begin(blockIdx.x + 1);
+    while (u < u1) {
+    const Spot ct = cut.at(b, G, u, lane);
+    if (ct.seq < 0) break;
+    const uint32_t over = cut.share ? AT_OVER : 0, end = min(ct.at + (u1 - u), ct.units);
+    const uint32_t tile_u = u - ct.at;
+    u = tile_u + end;
+    if (end <= over && end < ct.units) break;  // the block ends before the tile's first step
     // this lane's column
     const int f = ct.tile * 16 + c, last = min(ct.n * G - 1, ct.tile * 16 + 15);
     const bool col = f < ct.n * G;
     const int row = ct.lo + (col ? f / G : 0), head = hk * G + (col ? f % G : 0);
     const int pos = col ? ct.len - ct.n + f / G : -1;
     const int seen = uni(tokens_seen(b, ct, last / G)), all = uni(ct.len - ct.n + (ct.tile * 16) / G);  // first column's position
-    const int t0 = ct.split * ct.per, t1 = min(seen, t0 + ct.per);
-    if (ct.splits > 1 && ct.split == 0 && threadIdx.x == 0)
-        o.join[(size_t)ct.join * b.n_kv + hk] =
-            JoinTile{ct.lo * G + ct.tile * 16, last - ct.tile * 16 + 1, ct.part, seen <= ct.per ? 0 : (seen + ct.per - 1) / ct.per};
+    const bool first = ct.at <= over;
+    const int t0 = first ? 0 : (int)(ct.at - over) * cut.unit * 32;
+    const int t1 = end == ct.units ? seen : min(seen, (int)(end - over) * cut.unit * 32);
+    const bool whole = first && t1 == seen;
+    if (first && !whole) {
+        const uint32_t last_u = tile_u + over + ((uint32_t)seen + 32 * cut.unit - 1) / (32 * cut.unit) - 1;
+        left = JoinTile{ct.lo * G + ct.tile * 16, last - ct.tile * 16 + 1, (int)blockIdx.x, (int)(cut.block_of(last_u) - blockIdx.x) + 1};
+    }
+    if (first && by_tile && ct.place < o.joins && threadIdx.x == 0) o.join[(size_t)ct.place * b.n_kv + hk] = left;
     if (t0 >= t1) {
-        // nothing to see here; a column tile that sees nothing at all is split 0's to write
-        if (ct.split == 0) {
+        // nothing to see here; a column tile that sees nothing at all is its first piece's to write
+        if (first) {
             for (int i = threadIdx.x; i < 16 * D / 4; i += 256) {
                 const int ff = ct.tile * 16 + i / (D / 4);
                 if (ff >= ct.n * G) break;
                 store4<BF ? TG_T_BF16 : TG_T_F16>(o.p, (int64_t)(ct.lo + ff / G) * o.stride + (int64_t)(hk * G + ff % G) * D + i % (D / 4) * 4, f32x4{0, 0, 0, 0});
             }
         }
-        return;
+        continue;
     }
 
     uint32_t qw[NG][4];
@@ -581,7 +656,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_attn_split(KvBatch b, 
     }
 
     // a stretch of tokens c0 .. c1 - 1 whose pages the lanes hold, one each
-    const int ntile = (int)tpp.d, span = min(ct.per, 63 * 16 * ntile & ~31);
+    const int ntile = (int)tpp.d, span = 63 * 16 * ntile & ~31;
     const size_t head_bytes = (size_t)ntile * (18 * D), page_bytes = head_bytes * b.n_kv;
     const uint8_t *base = b.pages + hk * head_bytes;
     int c0 = t0, c1 = 0, page0 = 0, mine = 0, st = 0, s1 = 0;
@@ -765,7 +840,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_attn_split(KvBatch b, 
         // cs > 0, so the largest s is the largest score
         float top = s[0][0];
 #pragma unroll
-        for (int i = 1; i < 8; i++) top = fmaxf(top, s[i / 4][i % 4]);
+        for (int i = 1; i < 8; i++) top = __builtin_elementwise_maximum(top, s[i / 4][i % 4]);  // a NaN stays one
         if (__ballot(top * cs > m + AT_ROOM)) {
             top = col_max(top);
             const float m2 = fmaxf(m, top * cs), r = __builtin_amdgcn_exp2f(m - m2);
@@ -833,7 +908,6 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_attn_split(KvBatch b, 
     for (int j = 0; j < ND; j++) *reinterpret_cast<f32x4 *>(so + c * D + 16 * j + 4 * h) = acc[j] * (j % 2 ? 262144.0f : 4194304.0f);
     if (h == 0) sml[(wave * 16 + c) * 2] = m, sml[(wave * 16 + c) * 2 + 1] = l;
     __syncthreads();
-    const bool whole = seen <= ct.per;
     for (int i = threadIdx.x; i < 16 * D / 4; i += 256) {
         const int cc = i / (D / 4), d = (i % (D / 4)) * 4, ff = ct.tile * 16 + cc;
         if (ff >= ct.n * G) break;
@@ -851,10 +925,16 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_attn_split(KvBatch b, 
             const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
             store4<BF ? TG_T_BF16 : TG_T_F16>(o.p, (int64_t)(ct.lo + ff / G) * o.stride + (int64_t)(hk * G + ff % G) * D + d, v * inv);
         } else {
-            float *pp = o.part + ((size_t)(ct.part + ct.split) * b.n_kv + hk) * AT_PART<D, 16>;
+            float *pp = o.part + ((size_t)(2 * blockIdx.x + first) * b.n_kv + hk) * AT_PART<D, 16>;
             *reinterpret_cast<f32x4 *>(pp + cc * D + d) = v;
             if (d == 0) pp[16 * D + 2 * cc] = mm, pp[16 * D + 2 * cc + 1] = ll;
         }
+    }
+    if (u < u1) __syncthreads();  // before the next piece's scales go where the sums were
+    }
+    if (share && threadIdx.x == 0) {
+        if (!by_tile) o.join[(size_t)blockIdx.x * b.n_kv + hk] = left;
+        else for (int i = cut.tiles + blockIdx.x; i < o.joins; i += gridDim.x) o.join[(size_t)i * b.n_kv + hk] = JoinTile{0, 0, 0, 0};
     }
 }
 
@@ -1228,7 +1308,8 @@ __global__ __launch_bounds__(256) void k_attn_join(KvBatch b, int G, AttnOut o) 
     const JoinTile jt = o.join[(size_t)blockIdx.x * b.n_kv + hk];
     if (!jt.splits || (int)blockIdx.z * NC >= jt.cols) return;
     const size_t step = (size_t)b.n_kv * AT_PART<D, 16>;
-    const float *part = o.part + ((size_t)jt.part * b.n_kv + hk) * AT_PART<D, 16>;
+    const float *part = o.part + ((size_t)(2 * jt.part) * b.n_kv + hk) * AT_PART<D, 16>;
+    auto piece = [&](int i) { return i == 0 ? step : 2 * i * step; };  // from there
     // all of a thread's sums (those of the first 8 turns) and its (m, l) are asked for before the first is
     // waited for; columns behind the last hold zeros
     const float *mine = part + cc * D + 4 * (tid % L), *ml = part + 16 * D + 2 * cc;
@@ -1237,10 +1318,10 @@ __global__ __launch_bounds__(256) void k_attn_join(KvBatch b, int G, AttnOut o) 
     for (int k = 0; k < 8; k++) {
         const int i = tid / L + k * GR;
         first[k] = f32x4{0, 0, 0, 0};
-        if (i < jt.splits && cc < jt.cols) first[k] = *reinterpret_cast<const f32x4 *>(mine + i * step);
+        if (i < jt.splits && cc < jt.cols) first[k] = *reinterpret_cast<const f32x4 *>(mine + piece(i));
     }
     float mm = AT_NONE;
-    for (int s = tid; s < jt.splits && cc < jt.cols; s += TC) mm = fmaxf(mm, ml[s * step]);
+    for (int s = tid; s < jt.splits && cc < jt.cols; s += TC) mm = fmaxf(mm, ml[piece(s)]);
     mm = col_max(mm);
 #pragma unroll
     for (int i = 1; i < 16; i *= 2) mm = fmaxf(mm, __shfl_xor(mm, i));
@@ -1253,7 +1334,7 @@ __global__ __launch_bounds__(256) void k_attn_join(KvBatch b, int G, AttnOut o) 
     for (int s0 = 0; s0 < jt.splits; s0 += TC) {
         float w = 0.0f;
         if (s0 + tid < jt.splits && cc < jt.cols) {
-            const float *p = ml + (s0 + tid) * step;
+            const float *p = ml + piece(s0 + tid);
             w = __builtin_amdgcn_exp2f(p[0] - mm);
             ll += p[1] * w;
         }
@@ -1267,7 +1348,7 @@ __global__ __launch_bounds__(256) void k_attn_join(KvBatch b, int G, AttnOut o) 
             for (int k = 0; k < 8; k++, i += GR)
                 if (i < n) v += first[k] * sw[ci * TC + i];
         }
-        for (; i < n && cc < jt.cols; i += GR) v += *reinterpret_cast<const f32x4 *>(mine + (s0 + i) * step) * sw[ci * TC + i];
+        for (; i < n && cc < jt.cols; i += GR) v += *reinterpret_cast<const f32x4 *>(mine + piece(s0 + i)) * sw[ci * TC + i];
     }
     ll = wave_sum(ll);
     if (tid % 64 == 0) sm_l[threadIdx.x / 64] = ll;
@@ -1351,14 +1432,15 @@ hipError_t launch_kv_read(const KvBatch &b, void *k, void *v, hipStream_t st) {
     return hipGetLastError();
 }
 
-// Blocks of one launch: `share` per key head for the splits, and one for each
-// column tile that the shares do not fill.  Where the tiles are at most
+// Blocks of one launch.  Narrow column tiles: `share` per key head, or one for each tile.  Wide ones:
+// `share` per key head for the splits, and one for each column tile that the shares do not fill; where the tiles are at most
 // `share` their splits are at most that too, so half as many tiles can be
 // split (more than 64 sequences, whose share is not searched: 4 share / 3 splits); where they
 // are more, 4 share splits and 2 share tiles.
 struct AttnPlan {
     int64_t tiles;
-    int cols, share, joins;
+    int cols, share, joins, unit;
+    int64_t blocks, parts;  // of a key head
 };
 static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len, bool bf16) {
     const int64_t all = (int64_t)b.n_tokens * (n_heads / b.n_kv);
@@ -1374,7 +1456,15 @@ static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len, bool bf16)
     // nothing to split where no sequence is over what one block takes at the least, or there are tiles enough
     p.share = std::max(1, (many ? 256 : 512) / b.n_kv);
     if (max_len <= 32 * AT_MIN || p.tiles > 4 * p.share) p.share = 0;
-    p.joins = (int)std::min<int64_t>(p.tiles, p.tiles > p.share ? 2 * p.share : p.share);
+    p.unit = 4;  // a step for each wave; more only where their number would not stay below 2^30
+    if (many) {
+        p.joins = (int)std::min<int64_t>(p.tiles, p.tiles > p.share ? 2 * p.share : p.share);
+        p.blocks = p.tiles + 2 * p.share, p.parts = (p.tiles > p.share ? 4 : 2) * p.share;
+    } else {
+        p.joins = (int)std::min<int64_t>(p.tiles, p.share), p.blocks = p.share ? p.share : p.tiles, p.parts = 2 * p.share;
+        const int64_t steps = (int64_t)b.table_cols * b.page_tokens / 32 + 1;
+        while (p.share && p.tiles * (steps / p.unit + 1 + AT_OVER) >= 1 << 30) p.unit *= 2;
+    }
     return p;
 }
 
@@ -1387,8 +1477,7 @@ size_t attn_workspace(const KvBatch &b, int n_heads, int max_len) {
     size_t most = 0;
     for (const bool bf16 : {false, true}) {
         const AttnPlan p = attn_plan(b, n_heads, max_len, bf16);
-        if (p.share)
-            most = std::max(most, attn_join_bytes(b, p) + (size_t)(p.tiles > p.share ? 4 : 2) * p.share * b.n_kv * (p.cols * (b.D + 2)) * sizeof(float));
+        if (p.share) most = std::max(most, attn_join_bytes(b, p) + (size_t)p.parts * b.n_kv * (p.cols * (b.D + 2)) * sizeof(float));
     }
     return most;
 }
@@ -1396,7 +1485,7 @@ size_t attn_workspace(const KvBatch &b, int n_heads, int max_len) {
 template <int D, bool BF>
 static hipError_t attn_launch(const KvBatch &b, KvRows q, int G, float scale, const AttnPlan &p, const AttnOut &o, hipStream_t st) {
     static std::atomic<uint64_t> done{0};
-    const dim3 grid((unsigned)(p.tiles + 2 * p.share), (unsigned)b.n_kv);
+    const dim3 grid((unsigned)p.blocks, (unsigned)b.n_kv);
     const FastDiv tpp = make_fastdiv((uint32_t)(b.page_tokens / 16));
     if constexpr (D < 256) {
         if (p.cols == AT_COLS) {
@@ -1408,7 +1497,7 @@ static hipError_t attn_launch(const KvBatch &b, KvRows q, int G, float scale, co
             return hipSuccess;
         }
     }
-    TG_LAUNCH((k_attn_split<D, BF>), grid, dim3(256), 0, st, b, q, G, scale, p.share, tpp, o);
+    TG_LAUNCH((k_attn_split<D, BF>), grid, dim3(256), 0, st, b, q, G, scale, p.share, p.unit, tpp, o);
     if (!p.share) return hipSuccess;
     if (p.joins * b.n_kv <= 64) TG_LAUNCH((k_attn_join<D, BF, 256>), dim3(p.joins, b.n_kv, 16), dim3(256), 0, st, b, G, o);
     else TG_LAUNCH((k_attn_join<D, BF, 64>), dim3(p.joins, b.n_kv, 4), dim3(256), 0, st, b, G, o);
@@ -1419,7 +1508,7 @@ hipError_t launch_attn(const KvBatch &b, int type, KvRows q, int n_heads, float 
                        int max_len, void *ws, hipStream_t st) {
     const AttnPlan p = attn_plan(b, n_heads, max_len, type == TG_T_BF16);
     // threads of the launch's first dimension
-    if ((p.tiles + 2 * p.share) * (p.cols == AT_COLS ? 512 * b.n_kv : 256) > UINT32_MAX) return hipErrorInvalidValue;
+    if (p.blocks * (p.cols == AT_COLS ? 512 * b.n_kv : 256) > UINT32_MAX) return hipErrorInvalidValue;
     const int G = n_heads / b.n_kv;
     const AttnOut o{out, out_stride, static_cast<JoinTile *>(ws), p.joins,
                     reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + attn_join_bytes(b, p))};
