@@ -600,10 +600,12 @@ template <int D, int COLS>
 constexpr int AT_PART = COLS * (D + 2);  // floats of one split
 
 template <int D, bool BF>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_split(KvBatch b, KvRows q, int G, float scale, int share,
+__global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_split(KvBatch b, KvRows q, int G, float scale, int share,
                                                                       int unit, FastDiv tpp, AttnOut o) {
     constexpr int NG = D / 32, ND = D / 16, SW = D / 64;
-    constexpr int NB = D == 256 ? 2 : 3;  // steps held: one at work, the others on their way
+    // Steps held: one at work, the others on their way.  Heads of 256 take all of a CU's registers for a block; in
+    // half of them, 120 a lane spilled: 64 sequences of up to 4096 tokens, 32 heads over 4: 58 us, 113 so.
+    constexpr int NB = D == 256 ? 2 : 3;
     __shared__ __align__(16) uint8_t sm[4 * 16 * D * 4 + 4 * 16 * 8];
     const int lane = threadIdx.x % 64, wave = uni(threadIdx.x / 64);
     const int c = lane % 16, h = lane / 16;
@@ -971,7 +973,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_split(KvBatch b, 
 // the longest blocks of the last head start late.  fp16, D = 64, 500 tokens each of two prompts of
 // 16001, 32 heads over 8: 250 us, without the remainders 186, with those of the keys and of the weights
 // (more vector work, less of LDS) 284.  Heads of 256 leave 16 columns to a wave, which
-// reads as much for each: 1.2 to 2 times as long as k_attn_split, so they have only that.
+// reads as much for each: 2 to 3 times as long as k_attn_split, so they have only that.
 constexpr int AT_COLS = 256;
 
 template <int D, bool BF>
@@ -1454,7 +1456,8 @@ static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len, bool bf16)
     p.cols = many ? AT_COLS : 16;
     p.tiles = all / p.cols + b.n_seqs;
     // nothing to split where no sequence is over what one block takes at the least, or there are tiles enough
-    p.share = std::max(1, (many ? 256 : 512) / b.n_kv);
+    // one block of wide tiles or of heads of 256 fits a CU, two of the others
+    p.share = std::max(1, (many || b.D == 256 ? 256 : 512) / b.n_kv);
     if (max_len <= 32 * AT_MIN || p.tiles > 4 * p.share) p.share = 0;
     p.unit = 4;  // a step for each wave; more only where their number would not stay below 2^30
     if (many) {
