@@ -43,7 +43,8 @@ def check(out, x, w, ws, nw, r, eps=1e-6):
 SHAPES = [(1, 1, 16), (1, 5120, 2048), (2, 48, 64), (3, 200, 80), (7, 1000, 2048), (8, 256, 4096), (9, 130, 1040), (16, 512, 2048),
           (17, 333, 512), (31, 64, 96), (32, 96, 1008), (33, 2048, 1024), (64, 640, 768), (65, 129, 160), (100, 255, 2064), (128, 128, 128),
           (200, 1111, 336), (257, 300, 2048), (511, 515, 272), (600, 1024, 4096),
-          (1, 64, 8208), (4, 4096, 8192), (3, 40, 16384), (5, 33000, 64), (20, 33010, 208), (50, 32768, 128), (70, 16, 16384), (4096, 4100, 144)]
+          (1, 64, 8208), (4, 4096, 8192), (3, 40, 16384), (5, 33000, 64), (20, 33010, 208), (50, 32768, 128), (70, 16, 16384), (4096, 4100, 144),
+          (222, 130, 2576), (300, 515, 4112), (129, 1922, 2704), (66, 1, 5008), (2000, 4098, 160)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -123,6 +124,23 @@ def test_matmul_strides_shapes_and_aliases():
     assert out.shape == (2, 3, 4, 40) and out.dtype == torch.float16
     check(out.view(24, 40), x, w, ws, None, None)
     assert matmul_i8(x.cuda()[:0], w.cuda(), ws.cuda()).shape == (0, 40)
+
+
+def test_matmul_split_columns_in_place():
+    """Few tiles, many columns (split): strided rows, the residual in out's place, the bytes around it untouched, twice the same."""
+    from tinygiant_amd.linear import matmul_i8
+    gpu_note("matmul_i8 split columns in place")
+    x, w, ws, nw, r = problem(3, 150, 90, 4112, "f16", True, True, "bf16")
+    for width, at in ((101, 3), (128, 16)):
+        outs = []
+        for _ in range(2):
+            acc = torch.full((150, width), 9.0, dtype=torch.bfloat16, device="cuda")
+            acc[:, at:at + 90] = r.cuda()
+            o = matmul_i8(x.cuda(), w.cuda(), ws.cuda(), norm=nw.cuda(), residual=acc[:, at:at + 90], out=acc[:, at:at + 90])
+            check(o, x, w, ws, nw, r)
+            assert (acc[:, :at] == 9).all() and (acc[:, at + 90:] == 9).all()
+            outs.append(o.clone())
+        assert torch.equal(*outs)
 
 
 def test_matmul_refuses_on_device():

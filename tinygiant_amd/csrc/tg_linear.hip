@@ -25,21 +25,21 @@ TG_DEV float lin_get(const void *p, int64_t i) {
     return TYPE == TG_T_F16 ? h2f(v) : lin_bf(v);
 }
 
-// four values from element i on; wide where `vec` says that the address allows it
+// Four elements of memory that is aligned to one: still one access.
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x4_u __attribute__((ext_vector_type(4), aligned(2)));
+
 template <int TYPE>
-TG_DEV f32x4 lin_get4(const void *p, int64_t i, bool vec) {
-    f32x4 r;
-    if (!vec) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) r[e] = lin_get<TYPE>(p, i + e);
-    } else if constexpr (TYPE == TG_T_F32) {
-        r = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + i);
+TG_DEV f32x4 lin_get4(const void *p, int64_t i) {
+    if constexpr (TYPE == TG_T_F32) {
+        return *reinterpret_cast<const f32x4_u *>(static_cast<const float *>(p) + i);
     } else {
-        const u16x4 v = *reinterpret_cast<const u16x4 *>(static_cast<const uint16_t *>(p) + i);
+        const u16x4 v = *reinterpret_cast<const u16x4_u *>(static_cast<const uint16_t *>(p) + i);
+        f32x4 r;
 #pragma unroll
         for (int e = 0; e < 4; e++) r[e] = TYPE == TG_T_F16 ? h2f(v[e]) : lin_bf(v[e]);
+        return r;
     }
-    return r;
 }
 
 template <int TYPE>
@@ -51,31 +51,39 @@ TG_DEV void lin_put(void *p, int64_t i, float v) {
 template <int TYPE>
 TG_DEV void lin_put4(void *p, int64_t i, f32x4 v) {
     if constexpr (TYPE == TG_T_F32) {
-        *reinterpret_cast<f32x4 *>(static_cast<float *>(p) + i) = v;
+        *reinterpret_cast<f32x4_u *>(static_cast<float *>(p) + i) = v;
     } else {
         u16x4 r;
 #pragma unroll
         for (int e = 0; e < 4; e++) r[e] = TYPE == TG_T_F16 ? f2h(v[e]) : __builtin_bit_cast(uint16_t, (__bf16)v[e]);
-        *reinterpret_cast<u16x4 *>(static_cast<uint16_t *>(p) + i) = r;
+        *reinterpret_cast<u16x4_u *>(static_cast<uint16_t *>(p) + i) = r;
     }
 }
 
-// Channels n .. n + 3 of row m: sums times the row's scale to the output; sw: their scales where vec and all four are there.
+TG_DEV int lin_fours(int N) { return (N + 3) / 4 * 4; }
+
+// Channel n of row m.
 template <int OT>
-TG_DEV void lin_out(const MatmulI8Args &a, bool vec, int m, int n, f32x4 v, f32x4 sw) {
-    if (vec && n + 4 <= a.N) {
+TG_DEV void lin_out1(const MatmulI8Args &a, int m, int n, float v) {
+    float y = v * a.w_scale[n];
+    if (a.res) y += lin_get<OT>(a.res, (int64_t)m * a.res_stride + n);
+    lin_put<OT>(a.out, (int64_t)m * a.out_stride + n, y);
+}
+
+// Channels n .. n + 3 of row m: sums times the row's scale to the output; sw: their scales where all four are there.
+template <int OT>
+TG_DEV void lin_out(const MatmulI8Args &a, int m, int n, f32x4 v, f32x4 sw) {
+    if (n + 4 <= a.N) {
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = v[e] * sw[e];
-        if (a.res) v += lin_get4<OT>(a.res, (int64_t)m * a.res_stride + n, true);
+        if (a.res) v += lin_get4<OT>(a.res, (int64_t)m * a.res_stride + n);
         lin_put4<OT>(a.out, (int64_t)m * a.out_stride + n, v);
         return;
     }
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         if (n + e >= a.N) return;
-        float y = v[e] * a.w_scale[n + e];
-        if (a.res) y += lin_get<OT>(a.res, (int64_t)m * a.res_stride + n + e);
-        lin_put<OT>(a.out, (int64_t)m * a.out_stride + n + e, y);
+        lin_out1<OT>(a, m, n + e, v[e]);
     }
 }
 
@@ -134,14 +142,13 @@ struct QuantLds {
 // shows.  put(k, four codes) for every k below Kp.  A barrier at least lies between the last look at
 // `l` and the return, none behind a second row's first write to it: callers with two rows put one there.
 template <int TYPE, int TPR, int NV, class P>
-TG_DEV float quant_row(const MatmulI8Args &a, int Kp, bool vec, int row, QuantLds &l, P put) {
+TG_DEV float quant_row(const MatmulI8Args &a, int Kp, int row, QuantLds &l, P put) {
     const int tid = threadIdx.x % TPR;
     const int64_t x0 = (int64_t)row * a.x_stride;
     constexpr int NH = NV ? NV : 1;
     f32x4 h[NH], g[NH];
-    const bool wv = reinterpret_cast<uintptr_t>(a.norm_w) % 16 == 0;
-    auto load = [&](int k) { return k < a.K ? lin_get4<TYPE>(a.x, x0 + k, vec) : f32x4{0, 0, 0, 0}; };
-    auto weight = [&](int k) { return a.norm_w && k < a.K ? lin_get4<TG_T_F32>(a.norm_w, k, wv) : f32x4{1, 1, 1, 1}; };
+    auto load = [&](int k) { return k < a.K ? lin_get4<TYPE>(a.x, x0 + k) : f32x4{0, 0, 0, 0}; };
+    auto weight = [&](int k) { return a.norm_w && k < a.K ? lin_get4<TG_T_F32>(a.norm_w, k) : f32x4{1, 1, 1, 1}; };
     if constexpr (NV > 0) {
 #pragma unroll
         for (int i = 0; i < NV; i++) h[i] = load(4 * (tid + i * TPR));
@@ -226,11 +233,11 @@ TG_DEV float quant_row(const MatmulI8Args &a, int Kp, bool vec, int row, QuantLd
 
 // A launch of its own for the codes, bound by bytes.
 template <int TYPE, int TPR, int NV>
-__global__ __launch_bounds__(256) void k_lin_quant(MatmulI8Args a, int Kp, bool vec, int8_t *xq, float *xs) {
+__global__ __launch_bounds__(256) void k_lin_quant(MatmulI8Args a, int Kp, int8_t *xq, float *xs) {
     __shared__ QuantLds l;
     const int row = blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
     if (row >= a.M) return;  // whole waves
-    const float s = quant_row<TYPE, TPR, NV>(a, Kp, vec, row, l, [&](int k, uint32_t q) {
+    const float s = quant_row<TYPE, TPR, NV>(a, Kp, row, l, [&](int k, uint32_t q) {
         *reinterpret_cast<uint32_t *>(xq + (size_t)row * Kp + k) = q;
     });
     if (threadIdx.x % TPR == 0) xs[row] = s;
@@ -246,7 +253,7 @@ __global__ __launch_bounds__(256) void k_lin_quant(MatmulI8Args a, int Kp, bool 
 constexpr int LIN_FUSE_M = 4, LIN_FUSE = 4096;
 
 template <int MT, int R, int U, int OT, int XT>
-__global__ __launch_bounds__(256) void k_lin_few(MatmulI8Args a, int Kp, const int8_t *xq, const float *xs, bool vec, bool xvec) {
+__global__ __launch_bounds__(256) void k_lin_few(MatmulI8Args a, int Kp, const int8_t *xq, const float *xs) {
     constexpr bool FUSE = XT >= 0;
     __shared__ __align__(16) i32x4 part[4][R * MT][64];
     __shared__ float scale[LIN_FUSE_M];
@@ -287,8 +294,8 @@ __global__ __launch_bounds__(256) void k_lin_few(MatmulI8Args a, int Kp, const i
         for (int m = 0; m < a.M; m++) {
             const auto put = [&](int k, uint32_t q) { *reinterpret_cast<uint32_t *>(codes + (size_t)m * Kp + k) = q; };
             float s;
-            if (Kp <= 2048) s = quant_row<XT, 256, 2>(a, Kp, xvec, m, ql, put);
-            else s = quant_row<XT, 256, 4>(a, Kp, xvec, m, ql, put);
+            if (Kp <= 2048) s = quant_row<XT, 256, 2>(a, Kp, m, ql, put);
+            else s = quant_row<XT, 256, 4>(a, Kp, m, ql, put);
             if (threadIdx.x == 0) scale[m] = s;
             __syncthreads();
         }
@@ -323,10 +330,10 @@ __global__ __launch_bounds__(256) void k_lin_few(MatmulI8Args a, int Kp, const i
         if (m >= a.M) continue;
         const float s = FUSE ? scale[m & 3] : xs[m];
         f32x4 y, sw = {0, 0, 0, 0};
-        if (vec && n + 4 <= a.N) sw = *reinterpret_cast<const f32x4 *>(a.w_scale + n);
+        if (n + 4 <= a.N) sw = *reinterpret_cast<const f32x4_u *>(a.w_scale + n);
 #pragma unroll
         for (int e = 0; e < 4; e++) y[e] = (float)v[e] * s;
-        lin_out<OT>(a, vec, m, n, y, sw);
+        lin_out<OT>(a, m, n, y, sw);
     }
 }
 
@@ -341,16 +348,22 @@ __global__ __launch_bounds__(256) void k_lin_few(MatmulI8Args a, int Kp, const i
 // barrier per stage, in its middle: behind it every wave holds the rest of
 // stage k in registers, so k's place is loaded with stage k + ST, and stage k
 // + 1 has landed for every wave.
+//
+// Where the tiles are too few for the device's CUs the columns are split: a block takes `stages` of
+// them and leaves its int32 sums in part [split][row][N in fours] (OT LIN_PART), which
+// k_lin_sum adds.
+constexpr int LIN_PART = -1;
+
 template <int BN, int BM, int WN, int WM, int ST, int OT>
 __global__ __launch_bounds__(64 * WN * WM, 2) void k_lin_tile(MatmulI8Args a, int Kp, const int8_t *xq, const float *xs, int tiles_n,
-                                                              int tiles_m, bool vec) {
+                                                              int tiles_m, int stages, int32_t *part) {
     constexpr int NW = WN * WM, PER = (BN + BM) / 8 / NW, TN = BN / WN / 16, TM = BM / WM / 16;
     constexpr int STAGE = (BN + BM) * 128;
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     // blocks of one XCD (every eighth) take neighbouring tiles, in bands of 8 tiles of channels
-    const int total = tiles_n * tiles_m, id = blockIdx.x, q8 = total / 8, r8 = total % 8, xcd = id % 8;
-    const int t = xcd * q8 + min(xcd, r8) + id / 8;
+    const int total = tiles_n * tiles_m, id = blockIdx.x, q8 = gridDim.x / 8, r8 = gridDim.x % 8, xcd = id % 8;
+    const int item = xcd * q8 + min(xcd, r8) + id / 8, split = OT == LIN_PART ? item / total : 0, t = item - split * total;
     constexpr int BAND = 8;
     const int band = t / (BAND * tiles_m), wide = min(BAND, tiles_n - band * BAND), in = t - band * BAND * tiles_m;
     const int n0 = (band * BAND + in % wide) * BN, m0 = in / wide * BM;
@@ -363,9 +376,9 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_lin_tile(MatmulI8Args a, in
         const int r0 = (wave * PER + i) * 8, r = r0 + lane / 8;
         at[i] = r0 < BN ? (uint32_t)min(r, a.N - 1 - n0) * a.K : (uint32_t)min(r - BN, a.M - 1 - m0) * Kp;
     }
-    const int nk = Kp / 128;
+    const int last = Kp / 128 - 1, from = split * stages, nk = OT == LIN_PART ? min(stages, last + 1 - from) : last + 1;
     auto load = [&](int k) {
-        const uint32_t kx = min(k, nk - 1) * 128 + chunk, kw = kx < (uint32_t)a.K ? kx : 0;  // columns of w behind its last meet zeros: any
+        const uint32_t kx = min(from + k, last) * 128 + chunk, kw = kx < (uint32_t)a.K ? kx : 0;  // columns of w behind its last meet zeros: any
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const bool w = (wave * PER + i) * 8 < BN;
@@ -417,7 +430,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_lin_tile(MatmulI8Args a, in
     float *so = reinterpret_cast<float *>(lds) + wave * 16 * LD;
     const int n = n0 + wn + 4 * (lane % L);
     f32x4 sw = {0, 0, 0, 0};
-    if (vec && n + 4 <= a.N) sw = *reinterpret_cast<const f32x4 *>(a.w_scale + n);
+    if (OT != LIN_PART && n + 4 <= a.N) sw = *reinterpret_cast<const f32x4_u *>(a.w_scale + n);
 #pragma unroll
     for (int j = 0; j < TM; j++) {
         const int mj = m0 + wm + 16 * j;
@@ -426,17 +439,38 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_lin_tile(MatmulI8Args a, in
         for (int i = 0; i < TN; i++) {
             f32x4 v;
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = (float)acc[i][j][e] * s;
+            for (int e = 0; e < 4; e++) v[e] = OT == LIN_PART ? __int_as_float(acc[i][j][e]) : (float)acc[i][j][e] * s;
             *reinterpret_cast<f32x4 *>(so + r16 * LD + 16 * i + 4 * (lane / 16)) = v;
         }
         wave_lds_sync();
 #pragma unroll
         for (int q = 0; q < 16 / RW; q++) {
             const int r = q * RW + lane / L, m = mj + r;
-            if (m < a.M) lin_out<OT>(a, vec, m, n, *reinterpret_cast<const f32x4 *>(so + r * LD + 4 * (lane % L)), sw);
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(so + r * LD + 4 * (lane % L));
+            if constexpr (OT == LIN_PART) {
+                if (m < a.M && n < a.N) *reinterpret_cast<f32x4 *>(part + ((size_t)split * a.M + m) * lin_fours(a.N) + n) = v;
+            } else {
+                if (m < a.M) lin_out<OT>(a, m, n, v, sw);
+            }
         }
         wave_lds_sync();
     }
+}
+
+// Four channels of a row: the splits' sums, exact, and what follows them.
+template <int OT>
+__global__ __launch_bounds__(256) void k_lin_sum(MatmulI8Args a, const float *xs, const int32_t *part, int splits) {
+    const int ld = lin_fours(a.N), m = blockIdx.y, n = 4 * (blockIdx.x * 256 + threadIdx.x);
+    if (n >= a.N) return;
+    const int32_t *p = part + (size_t)m * ld + n;
+    i32x4 v = *reinterpret_cast<const i32x4 *>(p);
+    for (int i = 1; i < splits; i++) v += *reinterpret_cast<const i32x4 *>(p + (size_t)i * a.M * ld);
+    const float s = xs[m];
+    f32x4 y, sw = {0, 0, 0, 0};
+    if (n + 4 <= a.N) sw = *reinterpret_cast<const f32x4_u *>(a.w_scale + n);
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = (float)v[e] * s;
+    lin_out<OT>(a, m, n, y, sw);
 }
 
 // ================================================================ launchers
@@ -462,21 +496,38 @@ static hipError_t lin_lds(const void *fn, size_t bytes, std::atomic<uint64_t> &d
 static bool lin_wide_n(int N) { return N >= 32768; }
 static bool lin_fused(int M, int N, int Kp) { return !lin_wide_n(N) && M <= LIN_FUSE_M && M * Kp <= LIN_FUSE; }
 
-size_t matmul_i8_workspace(int M, int N, int K) {
-    return lin_fused(M, N, lin_kp(K)) ? 0 : (size_t)M * lin_kp(K) + 4 * (size_t)M + 16;
+// Which kernel, and how many stages of 128 columns a block takes (0: all).
+struct LinPlan {
+    bool few, big;
+    int stages, splits;
+};
+static LinPlan lin_plan(int M, int N, int Kp) {
+    const int64_t tiles = (int64_t)((N + 127) / 128) * ((M + 127) / 128);
+    LinPlan p{M <= 64, (int64_t)((N + 255) / 256) * ((M + 255) / 256) >= 256, 0, 1};
+    const int nk = Kp / 128;
+    // Tiles for half the CUs or fewer: a block to a CU by splitting the columns, 8 stages to a block at the least
+    // (4: 30 us for 200 x 130 x 16384, 28 with 8, 68 as few rows; 300 x 2048 x 4096 25, 21 and 28), where there are more than
+    // 2560 of them (300 x 256 x 2048: 16 us split, 13 as few rows).
+    if (!p.few && tiles <= 128 && nk > 20) {
+        p.stages = std::max(8, (int)((nk * tiles + 255) / 256));
+        p.splits = (nk + p.stages - 1) / p.stages;
+    }
+    // Short columns and next to no tiles: the few rows' kernel, 16 channels to a block (500 x 1024 x 1024: 12 us, 14 by tiles).
+    if (p.splits == 1 && tiles <= 40) p.few = true;
+    return p;
 }
+static size_t lin_codes(int M, int Kp) { return ((size_t)M * Kp + 4 * (size_t)M + 15) / 16 * 16; }
 
-static size_t lin_size(int type) { return type == TG_T_F32 ? 4 : 2; }
-
-// four elements at a time from every row
-static bool lin_wide(const void *p, int64_t stride, int type) {
-    return reinterpret_cast<uintptr_t>(p) % (4 * lin_size(type)) == 0 && stride % 4 == 0;
+size_t matmul_i8_workspace(int M, int N, int K) {
+    const int Kp = lin_kp(K);
+    if (lin_fused(M, N, Kp)) return 0;
+    const LinPlan p = lin_plan(M, N, Kp);
+    return lin_codes(M, Kp) + (p.splits > 1 ? (size_t)p.splits * M * ((N + 3) / 4 * 4) * 4 : 0) + 16;
 }
 
 template <int TYPE>
 static void quant_launch(const MatmulI8Args &a, int Kp, int8_t *xq, float *xs, hipStream_t st) {
-    const bool vec = lin_wide(a.x, a.x_stride, a.x_type);
-#define TG_QUANT(TPR, NV) TG_LAUNCH((k_lin_quant<TYPE, TPR, NV>), dim3((unsigned)((a.M + 256 / TPR - 1) / (256 / TPR))), dim3(256), 0, st, a, Kp, vec, xq, xs)
+#define TG_QUANT(TPR, NV) TG_LAUNCH((k_lin_quant<TYPE, TPR, NV>), dim3((unsigned)((a.M + 256 / TPR - 1) / (256 / TPR))), dim3(256), 0, st, a, Kp, xq, xs)
     if (Kp <= 256) TG_QUANT(64, 1);
     else if (Kp <= 512) TG_QUANT(64, 2);
     else if (Kp <= 1024) TG_QUANT(256, 1);
@@ -488,26 +539,25 @@ static void quant_launch(const MatmulI8Args &a, int Kp, int8_t *xq, float *xs, h
 }
 
 template <int BN, int BM, int WN, int WM, int ST, int OT>
-static hipError_t tile_launch(const MatmulI8Args &a, int Kp, const int8_t *xq, const float *xs, bool vec, hipStream_t st) {
+static hipError_t tile_launch(const MatmulI8Args &a, int Kp, const int8_t *xq, const float *xs, const LinPlan &p, int32_t *part, hipStream_t st) {
     static std::atomic<uint64_t> done{0};
     constexpr size_t bytes = (size_t)ST * (BN + BM) * 128;
     const hipError_t e = lin_lds((const void *)k_lin_tile<BN, BM, WN, WM, ST, OT>, bytes, done);
     if (e != hipSuccess) return e;
     const int tn = (a.N + BN - 1) / BN, tm = (a.M + BM - 1) / BM;
-    if ((int64_t)tn * tm > INT32_MAX) return hipErrorInvalidValue;
-    TG_LAUNCH((k_lin_tile<BN, BM, WN, WM, ST, OT>), dim3((unsigned)(tn * tm)), dim3(64 * WN * WM), bytes, st, a, Kp, xq, xs, tn, tm, vec);
+    if ((int64_t)tn * tm > INT32_MAX / 64) return hipErrorInvalidValue;
+    TG_LAUNCH((k_lin_tile<BN, BM, WN, WM, ST, OT>), dim3((unsigned)(tn * tm * p.splits)), dim3(64 * WN * WM), bytes, st, a, Kp, xq, xs, tn, tm, p.stages, part);
     return hipSuccess;
 }
 
 template <int MT, int R, int U, int OT>
-static void few_launch(const MatmulI8Args &a, int Kp, const int8_t *xq, const float *xs, bool vec, hipStream_t st) {
+static void few_launch(const MatmulI8Args &a, int Kp, const int8_t *xq, const float *xs, hipStream_t st) {
     const dim3 grid((unsigned)((a.N + 16 * R - 1) / (16 * R)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
     if (MT == 1 && lin_fused(a.M, a.N, Kp)) {
-        const bool xvec = lin_wide(a.x, a.x_stride, a.x_type);
         if constexpr (MT == 1)
-            TG_BY_TYPE(a.x_type, XT, TG_LAUNCH((k_lin_few<MT, R, U, OT, XT>), grid, dim3(256), (size_t)a.M * Kp, st, a, Kp, xq, xs, vec, xvec));
+            TG_BY_TYPE(a.x_type, XT, TG_LAUNCH((k_lin_few<MT, R, U, OT, XT>), grid, dim3(256), (size_t)a.M * Kp, st, a, Kp, xq, xs));
     } else {
-        TG_LAUNCH((k_lin_few<MT, R, U, OT, -1>), grid, dim3(256), 0, st, a, Kp, xq, xs, vec, false);
+        TG_LAUNCH((k_lin_few<MT, R, U, OT, -1>), grid, dim3(256), 0, st, a, Kp, xq, xs);
     }
 }
 
@@ -516,21 +566,24 @@ hipError_t launch_matmul_i8(const MatmulI8Args &a, void *ws, hipStream_t st) {
     int8_t *xq = static_cast<int8_t *>(ws);
     float *xs = reinterpret_cast<float *>(xq + (size_t)a.M * Kp);
     if (!lin_fused(a.M, a.N, Kp)) TG_BY_TYPE(a.x_type, XT, quant_launch<XT>(a, Kp, xq, xs, st));
-    const bool vec = lin_wide(a.out, a.out_stride, a.out_type) && (!a.res || lin_wide(a.res, a.res_stride, a.out_type)) &&
-                     reinterpret_cast<uintptr_t>(a.w_scale) % 16 == 0;
-    const bool wide = lin_wide_n(a.N), few = a.M <= 64 || (int64_t)((a.N + 127) / 128) * ((a.M + 127) / 128) <= 40;
+    const bool wide = lin_wide_n(a.N);
+    const LinPlan p = lin_plan(a.M, a.N, Kp);
+    int32_t *part = reinterpret_cast<int32_t *>(xq + lin_codes(a.M, Kp));
     hipError_t e = hipSuccess;
-    const int64_t big = (int64_t)((a.N + 255) / 256) * ((a.M + 255) / 256);
+    if (p.splits > 1) e = tile_launch<128, 128, 2, 2, 4, LIN_PART>(a, Kp, xq, xs, p, part, st);
+    if (e != hipSuccess) return e;
     TG_BY_TYPE(a.out_type, OT, {
-        if (few) {
-            if (a.M <= 16 && wide) few_launch<1, 4, 2, OT>(a, Kp, xq, xs, vec, st);
-            else if (a.M <= 16) few_launch<1, 1, 8, OT>(a, Kp, xq, xs, vec, st);
-            else if (a.M <= 32 && wide) few_launch<2, 4, 2, OT>(a, Kp, xq, xs, vec, st);
-            else if (a.M <= 32) few_launch<2, 1, 4, OT>(a, Kp, xq, xs, vec, st);
-            else if (wide) few_launch<4, 4, 1, OT>(a, Kp, xq, xs, vec, st);
-            else few_launch<4, 1, 2, OT>(a, Kp, xq, xs, vec, st);
-        } else if (big >= 256) e = tile_launch<256, 256, 2, 4, 2, OT>(a, Kp, xq, xs, vec, st);
-        else e = tile_launch<128, 128, 2, 2, 4, OT>(a, Kp, xq, xs, vec, st);
+        if (p.splits > 1) {
+            TG_LAUNCH((k_lin_sum<OT>), dim3((unsigned)((a.N + 1023) / 1024), (unsigned)a.M), dim3(256), 0, st, a, xs, part, p.splits);
+        } else if (p.few) {
+            if (a.M <= 16 && wide) few_launch<1, 4, 2, OT>(a, Kp, xq, xs, st);
+            else if (a.M <= 16) few_launch<1, 1, 8, OT>(a, Kp, xq, xs, st);
+            else if (a.M <= 32 && wide) few_launch<2, 4, 2, OT>(a, Kp, xq, xs, st);
+            else if (a.M <= 32) few_launch<2, 1, 4, OT>(a, Kp, xq, xs, st);
+            else if (wide) few_launch<4, 4, 1, OT>(a, Kp, xq, xs, st);
+            else few_launch<4, 1, 2, OT>(a, Kp, xq, xs, st);
+        } else if (p.big) e = tile_launch<256, 256, 2, 4, 2, OT>(a, Kp, xq, xs, p, part, st);
+        else e = tile_launch<128, 128, 2, 2, 4, OT>(a, Kp, xq, xs, p, part, st);
     });
     return e != hipSuccess ? e : hipGetLastError();
 }
