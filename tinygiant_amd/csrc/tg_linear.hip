@@ -231,7 +231,7 @@ TG_DEV float quant_row(const MatmulI8Args &a, int Kp, int row, QuantLds &l, P pu
     return bad ? __builtin_nanf("") : (float)(top / 127.0);
 }
 
-// A launch of its own for the codes, bound by bytes.
+// A launch of its own for the codes, bound by bytes: 8192 x 4096 fp32 with norm 42 us, 4.0 TB/s; 1999 x 4096 bf16 11 us, its latency.
 template <int TYPE, int TPR, int NV>
 __global__ __launch_bounds__(256) void k_lin_quant(MatmulI8Args a, int Kp, int8_t *xq, float *xs) {
     __shared__ QuantLds l;
@@ -247,9 +247,10 @@ __global__ __launch_bounds__(256) void k_lin_quant(MatmulI8Args a, int Kp, int8_
 // Up to 16 MT rows: bound by the weights' bytes, each read once, 16 bytes of
 // a channel per lane straight into the matrix instruction's operand.  A block takes 16 R channels, its
 // four waves every fourth step of 64 columns, two batches of U steps under
-// way in each; the waves' int32 sums meet in LDS.  XT >= 0: up to 4 rows (of at most 8192 columns) are
+// way in each; the waves' int32 sums meet in LDS.  XT >= 0: up to 4 rows (4096 columns together) are
 // quantised by every block for itself, the codes in LDS, while its first
-// weights are on their way, which saves a launch.
+// weights are on their way, which saves a launch.  7 rows by 151936 x 2048: 66 us, 4.7 TB/s of the 6
+// that reading reaches; 1 by 5120 x 2048: 8.1, its latency.
 constexpr int LIN_FUSE_M = 4, LIN_FUSE = 4096;
 
 template <int MT, int R, int U, int OT, int XT>
@@ -348,6 +349,9 @@ __global__ __launch_bounds__(256) void k_lin_few(MatmulI8Args a, int Kp, const i
 // barrier per stage, in its middle: behind it every wave holds the rest of
 // stage k in registers, so k's place is loaded with stage k + ST, and stage k
 // + 1 has landed for every wave.
+//
+// Bound by the tiles' bytes from the caches to LDS, 7.5 TB/s over the device: 8192 x 9216 x 4096 in
+// tiles of 256 x 256 310 us, 2.0 POP/s; 1999 x 2048 x 4096 in tiles of 128 x 128 32 us, 1.0.
 //
 // Where the tiles are too few for the device's CUs the columns are split: a block takes `stages` of
 // them and leaves its int32 sums in part [split][row][N in fours] (OT LIN_PART), which
@@ -493,7 +497,9 @@ static hipError_t lin_lds(const void *fn, size_t bytes, std::atomic<uint64_t> &d
         else { constexpr int NAME = TG_T_BF16; __VA_ARGS__; }                           \
     } while (0)
 
+// 64 channels to a block, not 16: 4 rows by 151936 x 2048 58 us (16: 72), 32768 x 2048 18 (21), 9216 x 4096 22 (19).
 static bool lin_wide_n(int N) { return N >= 32768; }
+// One launch, not two: 1 row by 5120 x 2048 8.7 us (12.4), by 2048 x 4096 8.7 (12.2); 2 rows by 5120 x 2048 7.9 (11.6).
 static bool lin_fused(int M, int N, int Kp) { return !lin_wide_n(N) && M <= LIN_FUSE_M && M * Kp <= LIN_FUSE; }
 
 // Which kernel, and how many stages of 128 columns a block takes (0: all).
@@ -503,7 +509,11 @@ struct LinPlan {
 };
 static LinPlan lin_plan(int M, int N, int Kp) {
     const int64_t tiles = (int64_t)((N + 127) / 128) * ((M + 127) / 128);
-    LinPlan p{M <= 64, (int64_t)((N + 255) / 256) * ((M + 255) / 256) >= 256, 0, 1};
+    // Up to 32 rows the weights' bytes count, above them the operands' way through LDS (64 rows: 2048 x 4096 16.4 us by
+    // tiles, 20.6 as few rows; 9216 x 4096 29 and 37; 33 rows: 27 and 30).  The large tiles halve that way, where they are
+    // enough for the CUs and rows fill them (8192 x 9216 x 4096: 310 us; 4096 rows 201, 234 by the small ones; 128 rows by
+    // 151936 x 2048: 121 and 99).
+    LinPlan p{M <= 32, M > 128 && (int64_t)((N + 255) / 256) * ((M + 255) / 256) >= 256, 0, 1};
     const int nk = Kp / 128;
     // Tiles for half the CUs or fewer: a block to a CU by splitting the columns, 8 stages to a block at the least
     // (4: 30 us for 200 x 130 x 16384, 28 with 8, 68 as few rows; 300 x 2048 x 4096 25, 21 and 28), where there are more than
@@ -580,7 +590,6 @@ hipError_t launch_matmul_i8(const MatmulI8Args &a, void *ws, hipStream_t st) {
             else if (a.M <= 16) few_launch<1, 1, 8, OT>(a, Kp, xq, xs, st);
             else if (a.M <= 32 && wide) few_launch<2, 4, 2, OT>(a, Kp, xq, xs, st);
             else if (a.M <= 32) few_launch<2, 1, 4, OT>(a, Kp, xq, xs, st);
-            else if (wide) few_launch<4, 4, 1, OT>(a, Kp, xq, xs, st);
             else few_launch<4, 1, 2, OT>(a, Kp, xq, xs, st);
         } else if (p.big) e = tile_launch<256, 256, 2, 4, 2, OT>(a, Kp, xq, xs, p, part, st);
         else e = tile_launch<128, 128, 2, 2, 4, OT>(a, Kp, xq, xs, p, part, st);
