@@ -118,6 +118,8 @@ ATTEND = [
     (256, 2, 4, 32, [2000, 700, 3], [90, 1, 3], "f16"),
     (64, 4, 4, 64, [5000], [33], "bf16"),
     (128, 1, 16, 48, [777, 1300], [100, 300], "f16"),
+    (64, 1, 16, 16, [8 + i % 30 for i in range(64)] + [3000, 2500], [8] * 66, "bf16"),     # wide column tiles of more sequences than lanes
+    (128, 1, 16, 32, [40 + i for i in range(70)] + [4000], [16] * 71, "f16"),
     (128, 1, 4, 16, [i % 5 * 100 for i in range(130)], [1] * 130, "f16"),             # more sequences than lanes, some empty
     (64, 1, 8, 16, [0], [40], "f16"),
 ]

@@ -417,10 +417,11 @@ TG_DEV T wave_sum(T v) { return __builtin_bit_cast(T, __builtin_amdgcn_readlane(
 // `steps` steps of 32 tokens.  A block takes at most `each` steps of one tile, the fewest
 // (from an even share on, an eighth more at a time) with which all the pieces of a key head are
 // `share` blocks or less, so that one round of the device's CUs does them
-// all and the longest block is as short as that allows; where there are more tiles than that anyway, an
-// even share of two rounds.  Every block works this out for itself from cu and kv_len (a wave's
+// all and the longest block is as short as that allows, and AT_WIDE at the least: what a piece costs
+// beside its steps (its start, 128 KB of partial sums written and read) is as long as 16.
+// Every block works this out for itself from cu and kv_len (a wave's
 // scan), so a launch follows lengths that only the device knows.
-constexpr int AT_MIN = 4;
+constexpr int AT_WIDE = 32;
 struct ColTile {
     int seq, tile, lo, n, len;
     int split, splits, per;  // this split of the tile's, tokens of one split
@@ -435,16 +436,11 @@ template <int COLS>
 TG_DEV float block_share(const KvBatch &b, int G, int share, int lane, const SeqWork &w0) {
     if (share == 0) return 0.0f;  // no splits
     float all = (float)w0.tiles * (float)w0.steps;
-    int tiles = min(w0.tiles, 1 << 20);
     for (int j = lane + 64; j < (b.n_seqs + 63) / 64 * 64; j += 64) {
         const SeqWork w = seq_work<COLS>(b, G, j);
         all += (float)w.tiles * (float)w.steps;
-        tiles = min(tiles + w.tiles, 1 << 20);
     }
-    all = wave_sum(all);
-    const float even = all / (float)share;
-    if (wave_sum(tiles) > share) return 1.0f / fmaxf((float)AT_MIN, even * 0.5f);
-    float each = fmaxf((float)AT_MIN, even);
+    float each = fmaxf((float)AT_WIDE, wave_sum(all) / (float)share);
     if (b.n_seqs > 64) return 1.0f / (each * 1.5f);
     for (int i = 0; i < 16 && wave_sum(w0.tiles * splits_of(w0.steps, 1.0f / each)) > share; i++) each *= 1.125f;
     return 1.0f / each;
@@ -523,7 +519,7 @@ struct Cut {
     TG_DEV uint32_t begin(uint32_t x) const { return share ? x * each + min(x, more) : x; }
     TG_DEV uint32_t block_of(uint32_t u) const {  // share only
         const uint32_t w = more * (each + 1);
-        return u < w ? u / (each + 1) : more + (u - w) / max(each, 1u);
+        return min(u < w ? u / (each + 1) : more + (u - w) / max(each, 1u), share - 1);
     }
     TG_DEV Spot at(const KvBatch &b, int G, uint32_t u, int lane) const {
         uint32_t before = 0;
@@ -1438,11 +1434,9 @@ hipError_t launch_kv_read(const KvBatch &b, void *k, void *v, hipStream_t st) {
     return hipGetLastError();
 }
 
-// Blocks of one launch.  Narrow column tiles: `share` per key head, or one for each tile.  Wide ones:
-// `share` per key head for the splits, and one for each column tile that the shares do not fill; where the tiles are at most
-// `share` their splits are at most that too, so half as many tiles can be
-// split (more than 64 sequences, whose share is not searched: 4 share / 3 splits); where they
-// are more, 4 share splits and 2 share tiles.
+// Blocks of one launch.  Narrow column tiles: `share` per key head, or one for each tile.  Wide ones: one
+// for each tile and `share` per key head more for their pieces, of which there are 2 share at most (share, where it is searched for;
+// 5 / 3 share with more than 64 sequences).
 struct AttnPlan {
     int64_t tiles;
     int cols, share, joins, unit;
@@ -1459,14 +1453,16 @@ static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len, bool bf16)
     const bool many = b.D < 256 && all >= (bf16 ? 128 : 192) * (int64_t)b.n_seqs;
     p.cols = many ? AT_COLS : 16;
     p.tiles = all / p.cols + b.n_seqs;
-    // nothing to split where no sequence is over what one block takes at the least, or there are tiles enough
     // one block of wide tiles or of heads of 256 fits a CU, two of the others
     p.share = std::max(1, (many || b.D == 256 ? 256 : 512) / b.n_kv);
-    if (max_len <= 32 * AT_MIN || p.tiles > 4 * p.share) p.share = 0;
+    // Nothing to split where no sequence is longer than a block should take, or there are tiles enough: narrow ones
+    // for four rounds; wide ones for one (4 prompts of 447 tokens, 64 heads of 128 over 8: 51 us, split over two rounds 85;
+    // one of 2000, 32 heads over 4: 77, split 84).
+    if (max_len <= 32 * (many ? 2 * AT_WIDE : 4) || p.tiles > (many ? 1 : 4) * p.share) p.share = 0;
     p.unit = 4;  // a step for each wave; more only where their number would not stay below 2^30
     if (many) {
-        p.joins = (int)std::min<int64_t>(p.tiles, p.tiles > p.share ? 2 * p.share : p.share);
-        p.blocks = p.tiles + 2 * p.share, p.parts = (p.tiles > p.share ? 4 : 2) * p.share;
+        p.joins = p.share ? (int)p.tiles : 0;
+        p.blocks = p.tiles + p.share, p.parts = 2 * p.share;
     } else {
         p.joins = (int)std::min<int64_t>(p.tiles, p.share), p.blocks = p.share ? p.share : p.tiles, p.parts = 2 * p.share;
         const int64_t steps = (int64_t)b.table_cols * b.page_tokens / 32 + 1;
