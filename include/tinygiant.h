@@ -487,8 +487,11 @@ int tg_kv_read_q4_dev(const tg_kv_batch *b, void *k, void *v, void *stream);
  * position p sees positions 0..p; out = softmax(scale * q . k) v, q and out
  * [n_tokens][n_heads][head_dim] fp16 or bf16, rows *_stride elements apart
  * (multiples of 8, pointers 16-byte aligned), out not overlapping q.  A row
- * at a position below 0 sees nothing and is zero.  n_heads is a multiple of
- * n_kv_heads.  max_len: about the longest kv_len (0: table_cols *
+ * at a position below 0 sees nothing and is zero.  scale is above 0 and
+ * finite; n_heads is a multiple of n_kv_heads.  Sums are fp32; weights, and the
+ * keys and values of many rows, are rounded to fp16 on the way (for fp16 rows
+ * keys and values are taken whole).  Scales above 8188, which append never
+ * writes, may count as infinite.  max_len: about the longest kv_len (0: table_cols *
  * page_tokens); it sets how the work is split, results hold for any.
  * workspace: at least tg_attn_q4_workspace bytes, 16-byte aligned, free
  * again when the call's work is done. */

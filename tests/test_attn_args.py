@@ -142,3 +142,8 @@ def test_python_refuses_host_tensors_and_shapes():
         PagedKV(1, 2, 16, 1, 64, pages=torch.zeros(1, 2, 1, 1, 18 * 64, dtype=torch.uint8))
     with pytest.raises(TypeError, match="x must be"):
         matmul_i8(torch.zeros(2, 64), torch.zeros(32, 64, dtype=torch.int8), torch.zeros(32))
+
+
+def test_results_in_the_place_of_their_operands_are_refused(lib):
+    assert attend(lib, batch()) == INVALID and "out is q" in said(lib)
+    assert product(lib) == INVALID and "out is x" in said(lib)

@@ -191,7 +191,7 @@ class PagedKV:
 
     def attend(self, layer: int, q, batch: KVBatch, scale: float | None = None, out=None):
         """softmax(scale q . k) v for q [T, heads, D] float16 or bfloat16
-        (scale: 1 / sqrt(D) by default), each row over the positions up to
+        (scale: above 0, 1 / sqrt(D) by default), each row over the positions up to
         its own; rows at positions below 0 are zero.  out: default a new
         tensor; must not overlap q."""
         heads, D = self._heads(q), self.head_dim

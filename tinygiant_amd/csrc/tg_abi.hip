@@ -2578,6 +2578,7 @@ extern "C" int tg_attn_q4_dev(const tg_kv_batch *b, int type, const void *q, int
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return set_err(TG_E_INVALID, "%s: workspace of %zu bytes, %zu and 16-byte alignment needed", fn,
                        workspace ? workspace_bytes : (size_t)0, need);
+    if (out == q) return set_err(TG_E_INVALID, "%s: out is q", fn);
     DeviceOf dev(as_stream(stream));
     if (dev.rc) return dev.rc;
     PROFILED("attn", as_stream(stream), tg::launch_attn(kb, type, {q, q_stride}, n_heads, scale, out, out_stride,
@@ -2613,6 +2614,7 @@ extern "C" int tg_matmul_i8_dev(const void *x, int x_type, int64_t x_stride, con
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return set_err(TG_E_INVALID, "%s: workspace of %zu bytes, %zu and 16-byte alignment needed", fn,
                        workspace ? workspace_bytes : (size_t)0, need);
+    if (out == x) return set_err(TG_E_INVALID, "%s: out is x", fn);
     DeviceOf dev(as_stream(stream));
     if (dev.rc) return dev.rc;
     const tg::MatmulI8Args a{x, x_type, x_stride, norm_w, eps, w, w_scale, residual, residual_stride,
