@@ -967,7 +967,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
 // Bound: at D = 128, bf16, a phase of a wave is 66 matrix instructions (1056 clocks)
 // behind 32 KB of operands from LDS (1024 for the four waves that read), about 1750
 // together, against 32 exponentials and what surrounds them (1200) and the
-// dequantising of a sixteenth of the step (900).  Three prompts of 4096, 4046 and
+// dequantising of a sixteenth of the step (900); the two overlap in part (the longer of two such
+// streams alone takes 290 us, both at once 406).  Three prompts of 4096, 4046 and
 // 2482 tokens, 32 heads over 4: 390 us, 0.83 PFLOP/s; all waves in step, one
 // barrier to a step: 422; heads one after the other instead of side by side: 455, since
 // the longest blocks of the last head start late.  fp16, D = 64, 500 tokens each of two prompts of
