@@ -575,13 +575,6 @@ TG_DEV void load_words(const void *p, uint32_t *w) {
     }
 }
 
-// Few columns: split over the tokens.  A block goes through pieces of column
-// tiles (as Cut says), its four waves every fourth step of 32 tokens; the
-// packed bytes go from memory to registers one step ahead and are unpacked
-// there (each is used by one wave, so LDS would only add a trip), the scales
-// through a wave's corner of LDS because 16 lanes need the same ones.  The pieces
-// of one column tile are joined by k_attn_join, or written out at once where
-// one is all.
 // What k_attn_join needs of one column tile that is split: its first column
 // (row * G + head of the key head's), how many, its first partial result (of
 // narrow tiles: the block that began it), and how many to join (0: none is split).
@@ -599,6 +592,15 @@ struct AttnOut {
 template <int D, int COLS>
 constexpr int AT_PART = COLS * (D + 2);  // floats of one split
 
+// Few columns: split over the tokens.  A block goes through pieces of column
+// tiles (as Cut says), its four waves every fourth step of 32 tokens; the
+// packed bytes go from memory to registers one step ahead and are unpacked
+// there (each is used by one wave, so LDS would only add a trip), the scales
+// through a wave's corner of LDS because 16 lanes need the same ones.  The pieces
+// of one column tile are joined by k_attn_join, or written out at once where
+// one is all.  Bound by the vector instructions that unpack codes
+// and weigh scores (40 to 46% of a SIMD's clocks) and by how far the loads run ahead: 64 sequences of up
+// to 8192 tokens, 32 heads of 128 over 4: 40 us, 3.8 TB/s; two of up to 200003, 64 heads over 4: 52 us, 4.4.
 template <int D, bool BF>
 __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_split(KvBatch b, KvRows q, int G, float scale, int share,
                                                                       int unit, FastDiv tpp, AttnOut o) {
@@ -617,322 +619,322 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
     uint32_t u = cut.begin(blockIdx.x);
     const uint32_t u1 = cut.share && blockIdx.x >= cut.share ? u : cut.begin(blockIdx.x + 1);
     while (u < u1) {
-    const Spot ct = cut.at(b, G, u, lane);
-    if (ct.seq < 0) break;
-    const uint32_t over = cut.share ? AT_OVER : 0, end = min(ct.at + (u1 - u), ct.units);
-    const uint32_t tile_u = u - ct.at;
-    u = tile_u + end;
-    if (end <= over && end < ct.units) break;  // the block ends before the tile's first step
-    // this lane's column
-    const int f = ct.tile * 16 + c, last = min(ct.n * G - 1, ct.tile * 16 + 15);
-    const bool col = f < ct.n * G;
-    const int row = ct.lo + (col ? f / G : 0), head = hk * G + (col ? f % G : 0);
-    const int pos = col ? ct.len - ct.n + f / G : -1;
-    const int seen = uni(tokens_seen(b, ct, last / G)), all = uni(ct.len - ct.n + (ct.tile * 16) / G);  // first column's position
-    const bool first = ct.at <= over;
-    const int t0 = first ? 0 : (int)(ct.at - over) * cut.unit * 32;
-    const int t1 = end == ct.units ? seen : min(seen, (int)(end - over) * cut.unit * 32);
-    const bool whole = first && t1 == seen;
-    if (first && !whole) {
-        const uint32_t last_u = tile_u + over + ((uint32_t)seen + 32 * cut.unit - 1) / (32 * cut.unit) - 1;
-        left = JoinTile{ct.lo * G + ct.tile * 16, last - ct.tile * 16 + 1, (int)blockIdx.x, (int)(cut.block_of(last_u) - blockIdx.x) + 1};
-    }
-    if (first && by_tile && ct.place < o.joins && threadIdx.x == 0) o.join[(size_t)ct.place * b.n_kv + hk] = left;
-    if (t0 >= t1) {
-        // nothing to see here; a column tile that sees nothing at all is its first piece's to write
-        if (first) {
-            for (int i = threadIdx.x; i < 16 * D / 4; i += 256) {
-                const int ff = ct.tile * 16 + i / (D / 4);
-                if (ff >= ct.n * G) break;
-                store4<BF ? TG_T_BF16 : TG_T_F16>(o.p, (int64_t)(ct.lo + ff / G) * o.stride + (int64_t)(hk * G + ff % G) * D + i % (D / 4) * 4, f32x4{0, 0, 0, 0});
-            }
+        const Spot ct = cut.at(b, G, u, lane);
+        if (ct.seq < 0) break;
+        const uint32_t over = cut.share ? AT_OVER : 0, end = min(ct.at + (u1 - u), ct.units);
+        const uint32_t tile_u = u - ct.at;
+        u = tile_u + end;
+        if (end <= over && end < ct.units) break;  // the block ends before the tile's first step
+        // this lane's column
+        const int f = ct.tile * 16 + c, last = min(ct.n * G - 1, ct.tile * 16 + 15);
+        const bool col = f < ct.n * G;
+        const int row = ct.lo + (col ? f / G : 0), head = hk * G + (col ? f % G : 0);
+        const int pos = col ? ct.len - ct.n + f / G : -1;
+        const int seen = uni(tokens_seen(b, ct, last / G)), all = uni(ct.len - ct.n + (ct.tile * 16) / G);  // first column's position
+        const bool first = ct.at <= over;
+        const int t0 = first ? 0 : (int)(ct.at - over) * cut.unit * 32;
+        const int t1 = end == ct.units ? seen : min(seen, (int)(end - over) * cut.unit * 32);
+        const bool whole = first && t1 == seen;
+        if (first && !whole) {
+            const uint32_t last_u = tile_u + over + ((uint32_t)seen + 32 * cut.unit - 1) / (32 * cut.unit) - 1;
+            left = JoinTile{ct.lo * G + ct.tile * 16, last - ct.tile * 16 + 1, (int)blockIdx.x, (int)(cut.block_of(last_u) - blockIdx.x) + 1};
         }
-        continue;
-    }
-
-    uint32_t qw[NG][4];
-    {
-        const uint16_t *qp = static_cast<const uint16_t *>(q.p) + (int64_t)row * q.stride + (int64_t)head * D;
-#pragma unroll
-        for (int g = 0; g < NG; g++) load_words<4>(qp + 32 * g + 8 * h, qw[g]);
-    }
-
-    // a stretch of tokens c0 .. c1 - 1 whose pages the lanes hold, one each
-    const int ntile = (int)tpp.d, span = 63 * 16 * ntile & ~31;
-    const size_t head_bytes = (size_t)ntile * (18 * D), page_bytes = head_bytes * b.n_kv;
-    const uint8_t *base = b.pages + hk * head_bytes;
-    int c0 = t0, c1 = 0, page0 = 0, mine = 0, st = 0, s1 = 0;
-    KvStep<D> k[NB];
-    auto load = [&](KvStep<D> &k, int step) {
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            int t = step * 2 + x;
-            t = (t * 16 < c1 ? t : c0 / 16) - page0 * ntile;  // behind the end: any tile, its tokens are masked
-            const int pi = (int)fdiv((uint32_t)t, tpp), pg = __builtin_amdgcn_readlane(mine, pi);
-            const uint8_t *p = base + (size_t)max(pg, 0) * page_bytes + (size_t)(t - pi * ntile) * (18 * D);
-            load_words<NG>(p + lane * (NG * 4), k.k[x]);
-            load_words<NG>(p + 8 * D + lane * (NG * 4), &k.v[x][0][0]);
-            // lane's share of the scales: the step's 4 D bytes over 64 lanes; a page that is none has NaN ones
-            const uint32_t *sp = reinterpret_cast<const uint32_t *>(p + 16 * D);
-            if (SW == 1) {
-                const uint32_t v = sp[lane % 32];
-                if (lane / 32 == x) k.s[0] = v, k.bad[0] = pg < 0;
-            } else {
-                k.bad[x] = pg < 0;
-#pragma unroll
-                for (int i = 0; i < SW / 2; i++) k.s[x * (SW / 2) + i] = sp[lane * (SW / 2) + i];
-            }
-        }
-        // loads leave in the order of their steps, so that the wait for one step leaves those behind it under way
-        asm volatile("" ::: "memory");
-    };
-    auto begin = [&]() {
-        c1 = min(t1, c0 + span);
-        page0 = uni(c0 / 16 / ntile);
-        mine = (page0 + lane) * 16 * ntile < c1 ? page_of(b, ct.seq, (page0 + lane) * 16 * ntile) : 0;
-        s1 = (c1 + 31) / 32;
-        st = c0 / 32 + wave;
-#pragma unroll
-        for (int i = 0; i < NB - 1; i++) load(k[i], st + 4 * i);
-    };
-    begin();
-
-    // queries: operand slots 8 h .. 8 h + 7 of each block, and the start of the sums
-    f16x8 qf[NG];
-    f32x4 start[NG];
-    float cs;
-    {
-        uint32_t mag = 0;  // magnitudes order as the integers they are stored as
-#pragma unroll
-        for (int g = 0; g < NG; g++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (!col) qw[g][e] = 0;
-                mag = max(mag, max(qw[g][e] & 0x7FFFu, (qw[g][e] >> 16) & 0x7FFFu));
-            }
-        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 16));
-        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
-        const float top = BF ? bf2f((uint16_t)mag) : h2f((uint16_t)mag);
-        int e2 = 0;
-        (void)frexpf(top, &e2);  // top = m 2^e2, m in [0.5, 1)
-        const int a = top > 0.0f && top < INFINITY ? 11 - e2 : 0;
-        cs = fmaxf(ldexpf(scale * 1.44269504f, 18 - a), AT_LEAST);
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint16_t u = (uint16_t)(qw[g][e / 2] >> (16 * (e % 2)));
-                const _Float16 v = (_Float16)ldexpf(BF ? bf2f(u) : h2f(u), a + ((e / 2) % 2 ? 0 : 4));
-                qf[g][e] = v;
-                sum += (e / 2) % 2 ? (float)v * 16.0f : (float)v;
-            }
-            sum = col_sum(sum);
-            const float s0 = sum * (-8.0f / 4194304.0f);
-            start[g] = f32x4{s0, s0, s0, s0};
-        }
-    }
-
-    uint32_t *sl = reinterpret_cast<uint32_t *>(sm) + wave * (16 * D);  // this wave's corner
-    // word w of a tile's 2 D bytes of scales that this lane's i-th word is, and its tile
-    auto word_of = [&](int i) { return SW == 1 ? lane % 32 : lane * (SW / 2) + i % (SW / 2); };
-    auto tile_of = [&](int i) { return SW == 1 ? lane / 32 : i / (SW / 2); };
-    const uint32_t vmask = word_of(0) >= D / 4 ? 0x7FFF7FFFu : 0u;  // this lane's words are value scales
-    const f16x8 off_even = as_h8(0x80208020u, 0x80208020u, 0x80208020u, 0x80208020u);  // -8 as the subnormals the
-    const f16x8 off_odd = as_h8(0x82008200u, 0x82008200u, 0x82008200u, 0x82008200u);   // two kinds of codes are
-    f32x4 acc[ND] = {};
-    float m = AT_NONE, l = 0.0f;
-    float A = 0.0f;           // the same in all lanes of a wave
-    uint32_t below = 0u;      // pairs of halves: the largest scale that A allows for
-    auto work = [&](KvStep<D> &k, int step) {
-        const bool edge = step * 32 + 31 > all;  // some column does not see all of it
-        // scales to LDS as the tiles hold them; what no column sees is zero
-        uint32_t big = below;
-#pragma unroll
-        for (int i = 0; i < SW; i++) {
-            const int w = word_of(i), x = tile_of(i);
-            uint32_t v = k.bad[SW == 1 ? 0 : x] ? 0x7E007E00u : k.s[i];  // a page that is none has NaN scales
-            if (edge) {
-                const int t = step * 32 + 16 * x;
-                if (w < D / 4) {
-                    if (t + w / (NG / 2) >= seen) v = 0;
-                } else {
-                    const int tp = t + (w - D / 4) / NG * 2;
-                    if (tp + 1 >= seen) v &= 0xFFFFu;
-                    if (tp >= seen) v = 0;
+        if (first && by_tile && ct.place < o.joins && threadIdx.x == 0) o.join[(size_t)ct.place * b.n_kv + hk] = left;
+        if (t0 >= t1) {
+            // nothing to see here; a column tile that sees nothing at all is its first piece's to write
+            if (first) {
+                for (int i = threadIdx.x; i < 16 * D / 4; i += 256) {
+                    const int ff = ct.tile * 16 + i / (D / 4);
+                    if (ff >= ct.n * G) break;
+                    store4<BF ? TG_T_BF16 : TG_T_F16>(o.p, (int64_t)(ct.lo + ff / G) * o.stride + (int64_t)(hk * G + ff % G) * D + i % (D / 4) * 4, f32x4{0, 0, 0, 0});
                 }
             }
-            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-            big = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, big), __builtin_bit_cast(u16x2, v & vmask)));
-            sl[x * (D / 2) + w] = v;
+            continue;
         }
-        bool odd = false;
-        if (__ballot(big != below)) {
-            // a scale at or above the bound: a new one, or a block that is not finite
-            uint32_t top = max(big & 0xFFFFu, big >> 16);
-            odd = __ballot(top >= 0x7C00u) != 0;
-            if (top >= 0x7C00u) top = 0;
+
+        uint32_t qw[NG][4];
+        {
+            const uint16_t *qp = static_cast<const uint16_t *>(q.p) + (int64_t)row * q.stride + (int64_t)head * D;
 #pragma unroll
-            for (int i = 1; i < 64; i *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, i));
-            if (top > (below & 0xFFFFu)) {
-                const int e = min(16, max((int)(top >> 10), 1) - 15 + 2);  // below 2^(e - 1), one bit of room
-                below = e > 15 ? 0x7BFF7BFFu : e < -13 ? (uint32_t)((1 << (e + 24)) - 1) * 0x10001u : (uint32_t)(((e + 15) << 10) - 1) * 0x10001u;
-                const float r = ldexpf(1.0f, AT_TOP - e - (int)A);
-                A = (float)(AT_TOP - e);
-                l *= r;
-#pragma unroll
-                for (int j = 0; j < ND; j++) acc[j] *= r;
-            }
+            for (int g = 0; g < NG; g++) load_words<4>(qp + 32 * g + 8 * h, qw[g]);
         }
-        wave_lds_sync();
-        f32x4 r[2][NG];
+
+        // a stretch of tokens c0 .. c1 - 1 whose pages the lanes hold, one each
+        const int ntile = (int)tpp.d, span = 63 * 16 * ntile & ~31;
+        const size_t head_bytes = (size_t)ntile * (18 * D), page_bytes = head_bytes * b.n_kv;
+        const uint8_t *base = b.pages + hk * head_bytes;
+        int c0 = t0, c1 = 0, page0 = 0, mine = 0, st = 0, s1 = 0;
+        KvStep<D> k[NB];
+        auto load = [&](KvStep<D> &k, int step) {
 #pragma unroll
-        for (int x = 0; x < 2; x++)
+            for (int x = 0; x < 2; x++) {
+                int t = step * 2 + x;
+                t = (t * 16 < c1 ? t : c0 / 16) - page0 * ntile;  // behind the end: any tile, its tokens are masked
+                const int pi = (int)fdiv((uint32_t)t, tpp), pg = __builtin_amdgcn_readlane(mine, pi);
+                const uint8_t *p = base + (size_t)max(pg, 0) * page_bytes + (size_t)(t - pi * ntile) * (18 * D);
+                load_words<NG>(p + lane * (NG * 4), k.k[x]);
+                load_words<NG>(p + 8 * D + lane * (NG * 4), &k.v[x][0][0]);
+                // lane's share of the scales: the step's 4 D bytes over 64 lanes; a page that is none has NaN ones
+                const uint32_t *sp = reinterpret_cast<const uint32_t *>(p + 16 * D);
+                if (SW == 1) {
+                    const uint32_t v = sp[lane % 32];
+                    if (lane / 32 == x) k.s[0] = v, k.bad[0] = pg < 0;
+                } else {
+                    k.bad[x] = pg < 0;
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const uint32_t w = k.k[x][g] << 2, w2 = k.k[x][g] >> 6;
-                const f16x8 kf = as_h8(w & AT_EVEN, w & AT_ODD, w2 & AT_EVEN, w2 & AT_ODD);
-                r[x][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[g], start[g], 0, 0, 0);
+                    for (int i = 0; i < SW / 2; i++) k.s[x * (SW / 2) + i] = sp[lane * (SW / 2) + i];
+                }
             }
-        if (D <= 128) __builtin_amdgcn_sched_barrier(0);  // all of them under way before the first is waited for
-        float s[2][4];
+            // loads leave in the order of their steps, so that the wait for one step leaves those behind it under way
+            asm volatile("" ::: "memory");
+        };
+        auto begin = [&]() {
+            c1 = min(t1, c0 + span);
+            page0 = uni(c0 / 16 / ntile);
+            mine = (page0 + lane) * 16 * ntile < c1 ? page_of(b, ct.seq, (page0 + lane) * 16 * ntile) : 0;
+            s1 = (c1 + 31) / 32;
+            st = c0 / 32 + wave;
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-            uint32_t kd[2 * NG];  // halves [token i][block g]
-            load_words<2 * NG>(sl + x * (D / 2) + h * (2 * NG), kd);
+            for (int i = 0; i < NB - 1; i++) load(k[i], st + 4 * i);
+        };
+        begin();
+
+        // queries: operand slots 8 h .. 8 h + 7 of each block, and the start of the sums
+        f16x8 qf[NG];
+        f32x4 start[NG];
+        float cs;
+        {
+            uint32_t mag = 0;  // magnitudes order as the integers they are stored as
 #pragma unroll
             for (int g = 0; g < NG; g++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    s[x][i] = __builtin_fmaf((float)as_h2(kd[(i * NG + g) / 2])[g % 2], r[x][g][i], g == 0 ? 0.0f : s[x][i]);
-        }
-        if (odd) {
-            // NaN for the tokens of value blocks that are not finite; those blocks become 0
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                uint32_t vd[2 * NG];
-                load_words<2 * NG>(sl + x * (D / 2) + D / 4 + h * (2 * NG), vd);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    bool n = false;
-#pragma unroll
-                    for (int g = 0; g < NG; g++) n |= ((vd[(i / 2) * NG + g] >> (16 * (i % 2))) & 0x7C00u) == 0x7C00u;
-                    if (n) s[x][i] = __builtin_nanf("");
+                for (int e = 0; e < 4; e++) {
+                    if (!col) qw[g][e] = 0;
+                    mag = max(mag, max(qw[g][e] & 0x7FFFu, (qw[g][e] >> 16) & 0x7FFFu));
                 }
+            mag = max(mag, (uint32_t)__shfl_xor((int)mag, 16));
+            mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
+            const float top = BF ? bf2f((uint16_t)mag) : h2f((uint16_t)mag);
+            int e2 = 0;
+            (void)frexpf(top, &e2);  // top = m 2^e2, m in [0.5, 1)
+            const int a = top > 0.0f && top < INFINITY ? 11 - e2 : 0;
+            cs = fmaxf(ldexpf(scale * 1.44269504f, 18 - a), AT_LEAST);
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint16_t u = (uint16_t)(qw[g][e / 2] >> (16 * (e % 2)));
+                    const _Float16 v = (_Float16)ldexpf(BF ? bf2f(u) : h2f(u), a + ((e / 2) % 2 ? 0 : 4));
+                    qf[g][e] = v;
+                    sum += (e / 2) % 2 ? (float)v * 16.0f : (float)v;
+                }
+                sum = col_sum(sum);
+                const float s0 = sum * (-8.0f / 4194304.0f);
+                start[g] = f32x4{s0, s0, s0, s0};
             }
-            wave_lds_sync();
+        }
+
+        uint32_t *sl = reinterpret_cast<uint32_t *>(sm) + wave * (16 * D);  // this wave's corner
+        // word w of a tile's 2 D bytes of scales that this lane's i-th word is, and its tile
+        auto word_of = [&](int i) { return SW == 1 ? lane % 32 : lane * (SW / 2) + i % (SW / 2); };
+        auto tile_of = [&](int i) { return SW == 1 ? lane / 32 : i / (SW / 2); };
+        const uint32_t vmask = word_of(0) >= D / 4 ? 0x7FFF7FFFu : 0u;  // this lane's words are value scales
+        const f16x8 off_even = as_h8(0x80208020u, 0x80208020u, 0x80208020u, 0x80208020u);  // -8 as the subnormals the
+        const f16x8 off_odd = as_h8(0x82008200u, 0x82008200u, 0x82008200u, 0x82008200u);   // two kinds of codes are
+        f32x4 acc[ND] = {};
+        float m = AT_NONE, l = 0.0f;
+        float A = 0.0f;           // the same in all lanes of a wave
+        uint32_t below = 0u;      // pairs of halves: the largest scale that A allows for
+        auto work = [&](KvStep<D> &k, int step) {
+            const bool edge = step * 32 + 31 > all;  // some column does not see all of it
+            // scales to LDS as the tiles hold them; what no column sees is zero
+            uint32_t big = below;
 #pragma unroll
             for (int i = 0; i < SW; i++) {
-                if (vmask) {
-                    uint32_t *at = sl + tile_of(i) * (D / 2) + word_of(i), v = *at;
-                    if ((v & 0x7C00u) == 0x7C00u) v &= 0xFFFF0000u;
-                    if ((v & 0x7C000000u) == 0x7C000000u) v &= 0xFFFFu;
-                    *at = v;
+                const int w = word_of(i), x = tile_of(i);
+                uint32_t v = k.bad[SW == 1 ? 0 : x] ? 0x7E007E00u : k.s[i];  // a page that is none has NaN scales
+                if (edge) {
+                    const int t = step * 32 + 16 * x;
+                    if (w < D / 4) {
+                        if (t + w / (NG / 2) >= seen) v = 0;
+                    } else {
+                        const int tp = t + (w - D / 4) / NG * 2;
+                        if (tp + 1 >= seen) v &= 0xFFFFu;
+                        if (tp >= seen) v = 0;
+                    }
+                }
+                typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+                big = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, big), __builtin_bit_cast(u16x2, v & vmask)));
+                sl[x * (D / 2) + w] = v;
+            }
+            bool odd = false;
+            if (__ballot(big != below)) {
+                // a scale at or above the bound: a new one, or a block that is not finite
+                uint32_t top = max(big & 0xFFFFu, big >> 16);
+                odd = __ballot(top >= 0x7C00u) != 0;
+                if (top >= 0x7C00u) top = 0;
+#pragma unroll
+                for (int i = 1; i < 64; i *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, i));
+                if (top > (below & 0xFFFFu)) {
+                    const int e = min(16, max((int)(top >> 10), 1) - 15 + 2);  // below 2^(e - 1), one bit of room
+                    below = e > 15 ? 0x7BFF7BFFu : e < -13 ? (uint32_t)((1 << (e + 24)) - 1) * 0x10001u : (uint32_t)(((e + 15) << 10) - 1) * 0x10001u;
+                    const float r = ldexpf(1.0f, AT_TOP - e - (int)A);
+                    A = (float)(AT_TOP - e);
+                    l *= r;
+#pragma unroll
+                    for (int j = 0; j < ND; j++) acc[j] *= r;
                 }
             }
             wave_lds_sync();
-        }
-        if (edge) {
+            f32x4 r[2][NG];
 #pragma unroll
             for (int x = 0; x < 2; x++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (step * 32 + 16 * x + 4 * h + i > pos) s[x][i] = -INFINITY;
-        }
-        // cs > 0, so the largest s is the largest score
-        float top = s[0][0];
+                for (int g = 0; g < NG; g++) {
+                    const uint32_t w = k.k[x][g] << 2, w2 = k.k[x][g] >> 6;
+                    const f16x8 kf = as_h8(w & AT_EVEN, w & AT_ODD, w2 & AT_EVEN, w2 & AT_ODD);
+                    r[x][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[g], start[g], 0, 0, 0);
+                }
+            if (D <= 128) __builtin_amdgcn_sched_barrier(0);  // all of them under way before the first is waited for
+            float s[2][4];
 #pragma unroll
-        for (int i = 1; i < 8; i++) top = __builtin_elementwise_maximum(top, s[i / 4][i % 4]);  // a NaN stays one
-        if (__ballot(top * cs > m + AT_ROOM)) {
-            top = col_max(top);
-            const float m2 = fmaxf(m, top * cs), r = __builtin_amdgcn_exp2f(m - m2);
-            l *= r;
+            for (int x = 0; x < 2; x++) {
+                uint32_t kd[2 * NG];  // halves [token i][block g]
+                load_words<2 * NG>(sl + x * (D / 2) + h * (2 * NG), kd);
 #pragma unroll
-            for (int j = 0; j < ND; j++) acc[j] *= r;
-            m = m2;
-        }
-        const float off = A - m;
-        float p[2][4];
+                for (int g = 0; g < NG; g++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            p[i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], cs, off));
-            l += p[i / 4][i % 4];
-        }
-        // value scales: words [token pair][block] of each tile
-        uint32_t vd[2][2 * NG];
-#pragma unroll
-        for (int x = 0; x < 2; x++) load_words<2 * NG>(sl + x * (D / 2) + D / 4 + h * (2 * NG), vd[x]);
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            uint32_t w[4];
-#pragma unroll
-            for (int y = 0; y < 4; y++) {
-                const f16x2 d = as_h2(vd[y / 2][(y % 2) * NG + g]);
-                const f16x2 v = {(_Float16)__builtin_fmaf(p[y / 2][2 * (y % 2)], (float)d[0], 0.0f),
-                                 (_Float16)__builtin_fmaf(p[y / 2][2 * (y % 2) + 1], (float)d[1], 0.0f)};
-                w[y] = as_u(v);
+                    for (int i = 0; i < 4; i++)
+                        s[x][i] = __builtin_fmaf((float)as_h2(kd[(i * NG + g) / 2])[g % 2], r[x][g][i], g == 0 ? 0.0f : s[x][i]);
             }
-            const f16x8 pf = as_h8(w[0], w[1], w[2], w[3]);
-            uint32_t r[4];  // the block's two column tiles are nibbles 2 (g % 2) and 2 (g % 2) + 1
+            if (odd) {
+                // NaN for the tokens of value blocks that are not finite; those blocks become 0
 #pragma unroll
-            for (int y = 0; y < 4; y++) r[y] = g % 2 ? k.v[y / 2][y % 2][g / 2] >> 6 : k.v[y / 2][y % 2][g / 2] << 2;
-            const f16x8 even = as_h8(r[0] & AT_EVEN, r[1] & AT_EVEN, r[2] & AT_EVEN, r[3] & AT_EVEN);
-            const f16x8 odd8 = as_h8(r[0] & AT_ODD, r[1] & AT_ODD, r[2] & AT_ODD, r[3] & AT_ODD);
-            acc[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pf, acc[2 * g], 0, 0, 0);
-            acc[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd8, pf, acc[2 * g + 1], 0, 0, 0);
-            acc[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(off_even, pf, acc[2 * g], 0, 0, 0);
-            acc[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(off_odd, pf, acc[2 * g + 1], 0, 0, 0);
-        }
-        wave_lds_sync();
-    };
-    while (c0 < t1) {
-        // loads ahead of the last step too (of a tile that is there): were they conditional, the wait for a
-        // step's bytes would have to take in those of the steps behind it
-        while (st < s1) {
+                for (int x = 0; x < 2; x++) {
+                    uint32_t vd[2 * NG];
+                    load_words<2 * NG>(sl + x * (D / 2) + D / 4 + h * (2 * NG), vd);
 #pragma unroll
-            for (int i = 0; i < NB; i++) {
-                load(k[(i + NB - 1) % NB], st + 4 * (NB - 1));
-                work(k[i], st);
-                st += 4;
-                if (st >= s1) break;
+                    for (int i = 0; i < 4; i++) {
+                        bool n = false;
+#pragma unroll
+                        for (int g = 0; g < NG; g++) n |= ((vd[(i / 2) * NG + g] >> (16 * (i % 2))) & 0x7C00u) == 0x7C00u;
+                        if (n) s[x][i] = __builtin_nanf("");
+                    }
+                }
+                wave_lds_sync();
+#pragma unroll
+                for (int i = 0; i < SW; i++) {
+                    if (vmask) {
+                        uint32_t *at = sl + tile_of(i) * (D / 2) + word_of(i), v = *at;
+                        if ((v & 0x7C00u) == 0x7C00u) v &= 0xFFFF0000u;
+                        if ((v & 0x7C000000u) == 0x7C000000u) v &= 0xFFFFu;
+                        *at = v;
+                    }
+                }
+                wave_lds_sync();
             }
+            if (edge) {
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (step * 32 + 16 * x + 4 * h + i > pos) s[x][i] = -INFINITY;
+            }
+            // cs > 0, so the largest s is the largest score
+            float top = s[0][0];
+#pragma unroll
+            for (int i = 1; i < 8; i++) top = __builtin_elementwise_maximum(top, s[i / 4][i % 4]);  // a NaN stays one
+            if (__ballot(top * cs > m + AT_ROOM)) {
+                top = col_max(top);
+                const float m2 = fmaxf(m, top * cs), r = __builtin_amdgcn_exp2f(m - m2);
+                l *= r;
+#pragma unroll
+                for (int j = 0; j < ND; j++) acc[j] *= r;
+                m = m2;
+            }
+            const float off = A - m;
+            float p[2][4];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                p[i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], cs, off));
+                l += p[i / 4][i % 4];
+            }
+            // value scales: words [token pair][block] of each tile
+            uint32_t vd[2][2 * NG];
+#pragma unroll
+            for (int x = 0; x < 2; x++) load_words<2 * NG>(sl + x * (D / 2) + D / 4 + h * (2 * NG), vd[x]);
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                uint32_t w[4];
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    const f16x2 d = as_h2(vd[y / 2][(y % 2) * NG + g]);
+                    const f16x2 v = {(_Float16)__builtin_fmaf(p[y / 2][2 * (y % 2)], (float)d[0], 0.0f),
+                                     (_Float16)__builtin_fmaf(p[y / 2][2 * (y % 2) + 1], (float)d[1], 0.0f)};
+                    w[y] = as_u(v);
+                }
+                const f16x8 pf = as_h8(w[0], w[1], w[2], w[3]);
+                uint32_t r[4];  // the block's two column tiles are nibbles 2 (g % 2) and 2 (g % 2) + 1
+#pragma unroll
+                for (int y = 0; y < 4; y++) r[y] = g % 2 ? k.v[y / 2][y % 2][g / 2] >> 6 : k.v[y / 2][y % 2][g / 2] << 2;
+                const f16x8 even = as_h8(r[0] & AT_EVEN, r[1] & AT_EVEN, r[2] & AT_EVEN, r[3] & AT_EVEN);
+                const f16x8 odd8 = as_h8(r[0] & AT_ODD, r[1] & AT_ODD, r[2] & AT_ODD, r[3] & AT_ODD);
+                acc[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pf, acc[2 * g], 0, 0, 0);
+                acc[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd8, pf, acc[2 * g + 1], 0, 0, 0);
+                acc[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(off_even, pf, acc[2 * g], 0, 0, 0);
+                acc[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(off_odd, pf, acc[2 * g + 1], 0, 0, 0);
+            }
+            wave_lds_sync();
+        };
+        while (c0 < t1) {
+            // loads ahead of the last step too (of a tile that is there): were they conditional, the wait for a
+            // step's bytes would have to take in those of the steps behind it
+            while (st < s1) {
+#pragma unroll
+                for (int i = 0; i < NB; i++) {
+                    load(k[(i + NB - 1) % NB], st + 4 * (NB - 1));
+                    work(k[i], st);
+                    st += 4;
+                    if (st >= s1) break;
+                }
+            }
+            c0 += span;
+            if (c0 < t1) begin();
         }
-        c0 += span;
-        if (c0 < t1) begin();
-    }
-    l = col_sum(l);
-    m -= A;  // weights were exp2(score - (m - A))
+        l = col_sum(l);
+        m -= A;  // weights were exp2(score - (m - A))
 
-    // the waves' shares joined in order: O[wave][column][D], m and l [wave][column]
-    __syncthreads();
-    float *so = reinterpret_cast<float *>(sm) + wave * 16 * D, *sml = reinterpret_cast<float *>(sm + 4 * 16 * D * 4);
+        // the waves' shares joined in order: O[wave][column][D], m and l [wave][column]
+        __syncthreads();
+        float *so = reinterpret_cast<float *>(sm) + wave * 16 * D, *sml = reinterpret_cast<float *>(sm + 4 * 16 * D * 4);
 #pragma unroll
-    for (int j = 0; j < ND; j++) *reinterpret_cast<f32x4 *>(so + c * D + 16 * j + 4 * h) = acc[j] * (j % 2 ? 262144.0f : 4194304.0f);
-    if (h == 0) sml[(wave * 16 + c) * 2] = m, sml[(wave * 16 + c) * 2 + 1] = l;
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * D / 4; i += 256) {
-        const int cc = i / (D / 4), d = (i % (D / 4)) * 4, ff = ct.tile * 16 + cc;
-        if (ff >= ct.n * G) break;
-        float mm = AT_NONE, ll = 0.0f;
-        f32x4 v = {0, 0, 0, 0};
+        for (int j = 0; j < ND; j++) *reinterpret_cast<f32x4 *>(so + c * D + 16 * j + 4 * h) = acc[j] * (j % 2 ? 262144.0f : 4194304.0f);
+        if (h == 0) sml[(wave * 16 + c) * 2] = m, sml[(wave * 16 + c) * 2 + 1] = l;
+        __syncthreads();
+        for (int i = threadIdx.x; i < 16 * D / 4; i += 256) {
+            const int cc = i / (D / 4), d = (i % (D / 4)) * 4, ff = ct.tile * 16 + cc;
+            if (ff >= ct.n * G) break;
+            float mm = AT_NONE, ll = 0.0f;
+            f32x4 v = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < 4; w++) mm = fmaxf(mm, sml[(w * 16 + cc) * 2]);
+            for (int w = 0; w < 4; w++) mm = fmaxf(mm, sml[(w * 16 + cc) * 2]);
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float r = __builtin_amdgcn_exp2f(sml[(w * 16 + cc) * 2] - mm);
-            ll += sml[(w * 16 + cc) * 2 + 1] * r;
-            v += *reinterpret_cast<const f32x4 *>(reinterpret_cast<float *>(sm) + (w * 16 + cc) * D + d) * r;
+            for (int w = 0; w < 4; w++) {
+                const float r = __builtin_amdgcn_exp2f(sml[(w * 16 + cc) * 2] - mm);
+                ll += sml[(w * 16 + cc) * 2 + 1] * r;
+                v += *reinterpret_cast<const f32x4 *>(reinterpret_cast<float *>(sm) + (w * 16 + cc) * D + d) * r;
+            }
+            if (whole) {
+                const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+                store4<BF ? TG_T_BF16 : TG_T_F16>(o.p, (int64_t)(ct.lo + ff / G) * o.stride + (int64_t)(hk * G + ff % G) * D + d, v * inv);
+            } else {
+                float *pp = o.part + ((size_t)(2 * blockIdx.x + first) * b.n_kv + hk) * AT_PART<D, 16>;
+                *reinterpret_cast<f32x4 *>(pp + cc * D + d) = v;
+                if (d == 0) pp[16 * D + 2 * cc] = mm, pp[16 * D + 2 * cc + 1] = ll;
+            }
         }
-        if (whole) {
-            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-            store4<BF ? TG_T_BF16 : TG_T_F16>(o.p, (int64_t)(ct.lo + ff / G) * o.stride + (int64_t)(hk * G + ff % G) * D + d, v * inv);
-        } else {
-            float *pp = o.part + ((size_t)(2 * blockIdx.x + first) * b.n_kv + hk) * AT_PART<D, 16>;
-            *reinterpret_cast<f32x4 *>(pp + cc * D + d) = v;
-            if (d == 0) pp[16 * D + 2 * cc] = mm, pp[16 * D + 2 * cc + 1] = ll;
-        }
-    }
-    if (u < u1) __syncthreads();  // before the next piece's scales go where the sums were
+        if (u < u1) __syncthreads();  // before the next piece's scales go where the sums were
     }
     if (share && threadIdx.x == 0) {
         if (!by_tile) o.join[(size_t)blockIdx.x * b.n_kv + hk] = left;
