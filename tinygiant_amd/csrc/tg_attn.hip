@@ -942,7 +942,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
     }
 }
 
-// Many columns: a block of 8 waves holds 256 columns of one key head, 32 to a
+// Many columns: a block of 8 waves holds 256 columns of one key head (heads of 256: 128), 32 to a
 // wave, and goes through the tokens in steps of 64, which it dequantises to
 // fp16 once for all of them: half the waves take a tile's keys, half its
 // values, ahead of their use (the packed bytes a phase before that), and leave
@@ -975,13 +975,18 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
 // barrier to a step: 422; heads one after the other instead of side by side: 455, since
 // the longest blocks of the last head start late.  fp16, D = 64, 500 tokens each of two prompts of
 // 16001, 32 heads over 8: 250 us, without the remainders 186, with those of the keys and of the weights
-// (more vector work, less of LDS) 284.  Heads of 256 leave 16 columns to a wave, which
-// reads as much for each: 2 to 3 times as long as k_attn_split, so they have only that.
-constexpr int AT_COLS = 256;
+// (more vector work, less of LDS) 284.
+//
+// Heads of 256: 128 columns to a block, and both waves of a SIMD hold the same 32, each with half of the output's dims; the
+// scores and weights they form twice, which keeps them from having to meet.  A prompt of 4096, bf16, 32 heads
+// over 8: 445 us, 0.62 PFLOP/s (by few columns 1133).
+template <int D>
+constexpr int AT_COLS = D == 256 ? 128 : 256;
 
 template <int D, bool BF>
 __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G, float scale, int share, FastDiv tpp, AttnOut o) {
-    constexpr int NG = D / 32, ND = D / 16, NC = 2, COLS = AT_COLS, BUF = 64 * D * 2;  // keys or values of a step
+    constexpr int NG = D / 32, ND = D / 16, NC = 2, COLS = AT_COLS<D>, BUF = 64 * D * 2;  // keys or values of a step
+    constexpr int DW = COLS * D / 256, NJ = DW / 16;  // dims of the output that are a wave's
     constexpr int REST = BF ? 0 : 5 * BUF;  // where the roundings' remainders are
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x % 64, wave = uni(threadIdx.x / 64), c16 = lane % 16, h = lane / 16;
@@ -999,7 +1004,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
     if (t0 >= t1 && ct.split > 0) return;
 
     // this lane's columns, one of each column tile of the wave
-    const int f0 = col0 + wave * 16 * NC;
+    const int f0 = col0 + wave % (COLS / (16 * NC)) * 16 * NC, dim0 = wave / (COLS / (16 * NC)) * DW;
     int pos[NC];
     uint32_t qw[NC][NG][4];
 #pragma unroll
@@ -1159,7 +1164,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
             }
     }
 
-    f32x4 acc[NC][ND] = {}, sum[NC] = {};
+    f32x4 acc[NC][NJ] = {}, sum[NC] = {};
     float m[NC];
 #pragma unroll
     for (int c = 0; c < NC; c++) m[c] = AT_NONE;
@@ -1173,13 +1178,13 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
         if (QK) pages(next);
         if (QK) fetch(next);
         if (PV) {
-            const uint8_t *vb = lds + (2 + (step - 1) % 3) * BUF + lane * 16;
+            const uint8_t *vb = lds + (2 + (step - 1) % 3) * BUF + dim0 * 64 + lane * 16;
 #pragma unroll
             for (int p = 0; p < 2; p++) {
 #pragma unroll
                 for (int c = 0; c < NC; c++) sum[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[c][p], sum[c], 0, 0, 0);
 #pragma unroll
-                for (int j = 0; j < ND; j++) {
+                for (int j = 0; j < NJ; j++) {
                     const f16x8 vf = *reinterpret_cast<const f16x8 *>(vb + (p * ND + j) * 1024);
 #pragma unroll
                     for (int c = 0; c < NC; c++) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[c][p], acc[c][j], 0, 0, 0);
@@ -1229,7 +1234,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
                 const float m2 = fmaxf(m[c], col_max(top) * cs[c]), r = __builtin_amdgcn_exp2f(m[c] - m2);
                 sum[c] *= r;
 #pragma unroll
-                for (int j = 0; j < ND; j++) acc[c][j] *= r;
+                for (int j = 0; j < NJ; j++) acc[c][j] *= r;
                 m[c] = m2;
             }
             const float off = (float)AT_TOP - m[c];
@@ -1276,26 +1281,26 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
         const int f = f0 + 16 * c + c16;
         if (whole) {
             // through LDS, 16 columns of the wave at a time, so that a head leaves as whole lines
-            uint16_t *so = reinterpret_cast<uint16_t *>(lds) + wave * 16 * (D + 8);
+            uint16_t *so = reinterpret_cast<uint16_t *>(lds) + wave * 16 * (DW + 8);
             const float inv = sum[c][0] == 0.0f ? 0.0f : 1.0f / sum[c][0];
 #pragma unroll
-            for (int j = 0; j < ND; j++) store4<BF ? TG_T_BF16 : TG_T_F16>(so, c16 * (D + 8) + 16 * j + 4 * h, acc[c][j] * inv);
+            for (int j = 0; j < NJ; j++) store4<BF ? TG_T_BF16 : TG_T_F16>(so, c16 * (DW + 8) + 16 * j + 4 * h, acc[c][j] * inv);
             wave_lds_sync();
-            constexpr int L = D / 8;  // lanes of one head
+            constexpr int L = DW / 8;  // lanes of one head
 #pragma unroll
             for (int i = 0; i < 16 * L / 64; i++) {
                 const int cc = i * (64 / L) + lane / L, ff = f0 + 16 * c + cc;
-                const u32x4 v = *reinterpret_cast<const u32x4 *>(so + cc * (D + 8) + 8 * (lane % L));
+                const u32x4 v = *reinterpret_cast<const u32x4 *>(so + cc * (DW + 8) + 8 * (lane % L));
                 if (ff < ncol)
-                    *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(o.p) + (int64_t)(ct.lo + ff / G) * o.stride + (int64_t)(hk * G + ff % G) * D + 8 * (lane % L)) = v;
+                    *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(o.p) + (int64_t)(ct.lo + ff / G) * o.stride + (int64_t)(hk * G + ff % G) * D + dim0 + 8 * (lane % L)) = v;
             }
             wave_lds_sync();
         } else if (f < ncol) {
             float *pp = o.part + ((size_t)(ct.part + ct.split) * b.n_kv + hk) * AT_PART<D, COLS>;
             const int cc = f - col0;
 #pragma unroll
-            for (int j = 0; j < ND; j++) *reinterpret_cast<f32x4 *>(pp + (size_t)cc * D + 16 * j + 4 * h) = acc[c][j];
-            if (h == 0) pp[COLS * D + 2 * cc] = m[c], pp[COLS * D + 2 * cc + 1] = sum[c][0];
+            for (int j = 0; j < NJ; j++) *reinterpret_cast<f32x4 *>(pp + (size_t)cc * D + dim0 + 16 * j + 4 * h) = acc[c][j];
+            if (h == 0 && dim0 == 0) pp[COLS * D + 2 * cc] = m[c], pp[COLS * D + 2 * cc + 1] = sum[c][0];
         }
     }
 }
@@ -1452,9 +1457,10 @@ static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len, bool bf16)
     // tokens, D = 128, few against many: 64 columns 42 and 50 us, 96 51 and 52, 128 53 and 54, 256 88 and 59; one of
     // 16000: 128 43 and 56, 256 51 and 61; 200 of up to 1000: 128 117 and 129, 256 203 and 127; D = 64, 16 of up to
     // 8192: 64 72 and 88, 128 87 and 89.  fp16, whose many take longer: D = 128, 128 columns 56 and 74, 192 73 and 74,
-    // 256 88 and 76; D = 64 128 88 and 109, 192 114 and 111, 256 137 and 114.
-    const bool many = b.D < 256 && all >= (bf16 ? 128 : 192) * (int64_t)b.n_seqs;
-    p.cols = many ? AT_COLS : 16;
+    // 256 88 and 76; D = 64 128 88 and 109, 192 114 and 111, 256 137 and 114.  D = 256, bf16, 16 of up to 4096: 64 columns 55
+    // and 72, 128 78 and 78, 192 103 and 83; fp16 has no wide tiles, its remainders do not fit LDS.
+    const bool many = (b.D < 256 || bf16) && all >= (bf16 ? 128 : 192) * (int64_t)b.n_seqs;
+    p.cols = !many ? 16 : b.D == 256 ? AT_COLS<256> : AT_COLS<128>;
     p.tiles = all / p.cols + b.n_seqs;
     // one block of wide tiles or of heads of 256 fits a CU, two of the others
     p.share = std::max(1, (many || b.D == 256 ? 256 : 512) / b.n_kv);
@@ -1493,13 +1499,14 @@ static hipError_t attn_launch(const KvBatch &b, KvRows q, int G, float scale, co
     static std::atomic<uint64_t> done{0};
     const dim3 grid((unsigned)p.blocks, (unsigned)b.n_kv);
     const FastDiv tpp = make_fastdiv((uint32_t)(b.page_tokens / 16));
-    if constexpr (D < 256) {
-        if (p.cols == AT_COLS) {
+    if constexpr (D < 256 || BF) {
+        if (p.cols != 16) {
             constexpr size_t LDS = (BF ? 5 : 10) * 64 * D * 2;
             const hipError_t e = attn_lds((const void *)k_attn_tile<D, BF>, LDS, done);
             if (e != hipSuccess) return e;
             TG_LAUNCH((k_attn_tile<D, BF>), dim3(grid.x * grid.y), dim3(512), LDS, st, b, q, G, scale, p.share, tpp, o);
-            if (p.share) TG_LAUNCH((k_attn_join_wide<D, BF, AT_COLS>), dim3(p.joins, b.n_kv, AT_COLS * D / 1024), dim3(256), 0, st, b, G, o);
+            if (p.share)
+                TG_LAUNCH((k_attn_join_wide<D, BF, AT_COLS<D>>), dim3(p.joins, b.n_kv, AT_COLS<D> * D / 1024), dim3(256), 0, st, b, G, o);
             return hipSuccess;
         }
     }
@@ -1514,7 +1521,7 @@ hipError_t launch_attn(const KvBatch &b, int type, KvRows q, int n_heads, float 
                        int max_len, void *ws, hipStream_t st) {
     const AttnPlan p = attn_plan(b, n_heads, max_len, type == TG_T_BF16);
     // threads of the launch's first dimension
-    if (p.blocks * (p.cols == AT_COLS ? 512 * b.n_kv : 256) > UINT32_MAX) return hipErrorInvalidValue;
+    if (p.blocks * (p.cols != 16 ? 512 * b.n_kv : 256) > UINT32_MAX) return hipErrorInvalidValue;
     const int G = n_heads / b.n_kv;
     const AttnOut o{out, out_stride, static_cast<JoinTile *>(ws), p.joins,
                     reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + attn_join_bytes(b, p))};
