@@ -119,6 +119,9 @@ ATTEND = [
     (64, 4, 4, 64, [5000], [33], "bf16"),
     (256, 2, 4, 32, [2500, 700, 3], [200, 90, 3], "bf16"),                            # heads of 256: two waves to a column
     (256, 1, 7, 16, [310, 77], [310, 77], "bf16"),
+    (256, 2, 4, 32, [2500, 700, 3], [250, 90, 3], "f16"),
+    (256, 1, 7, 16, [310, 77, 20], [310, 77, 20], "f16"),
+    (256, 1, 16, 48, [33], [33], "f16"),
     (128, 1, 16, 48, [777, 1300], [100, 300], "f16"),
     (64, 1, 16, 16, [8 + i % 30 for i in range(64)] + [3000, 2500], [8] * 66, "bf16"),     # wide column tiles of more sequences than lanes
     (128, 1, 16, 32, [40 + i for i in range(70)] + [4000], [16] * 71, "f16"),
