@@ -119,6 +119,9 @@ ATTEND = [
     (64, 4, 4, 64, [5000], [33], "bf16"),
     (256, 2, 4, 32, [2500, 700, 3], [200, 90, 3], "bf16"),                            # heads of 256: two waves to a column
     (256, 1, 7, 16, [310, 77], [310, 77], "bf16"),
+    (128, 2, 8, 32, [900, 700, 33, 0, 1500, 64, 5, 6, 7, 8], [600, 1, 33, 0, 1, 2, 1, 1, 1, 1], "bf16"),  # chunks and single tokens: two launches
+    (64, 1, 4, 16, [2600, 1, 40, 3000] + [20 + i for i in range(70)], [2600, 1, 7, 900] + [1] * 70, "f16"),
+    (256, 1, 4, 16, [600, 500, 7] + [31] * 7, [500, 3, 1] + [1] * 7, "bf16"),
     (256, 2, 4, 32, [2500, 700, 3], [250, 90, 3], "f16"),
     (256, 1, 7, 16, [310, 77, 20], [310, 77, 20], "f16"),
     (256, 1, 16, 48, [33], [33], "f16"),

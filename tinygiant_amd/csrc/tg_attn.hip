@@ -387,7 +387,8 @@ TG_DEV SeqWork seq_work(const KvBatch &b, int G, int j) {
     w.lo = min(max(c0, 0), b.n_tokens);
     w.n = in ? min(max(c1, w.lo), b.n_tokens) - w.lo : 0;
     w.len = max(cl, 0);
-    w.tiles = (int)(((int64_t)w.n * G + COLS - 1) / COLS);
+    const int64_t cols = (int64_t)w.n * G;
+    w.tiles = cols >= b.cols_from && cols < b.cols_to ? (int)((cols + COLS - 1) / COLS) : 0;
     w.steps = max(1, (min(w.len, b.table_cols * b.page_tokens + 1) + 31) / 32);
     return w;
 }
@@ -1449,19 +1450,15 @@ struct AttnPlan {
     int64_t tiles;
     int cols, share, joins, unit;
     int64_t blocks, parts;  // of a key head
+    int from, to;           // columns of the sequences that it is for
 };
-static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len, bool bf16) {
+static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len, bool many, int from, int to) {
     const int64_t all = (int64_t)b.n_tokens * (n_heads / b.n_kv);
     AttnPlan p;
-    // The mean number of columns of a sequence says which kernel takes all of them.  16 sequences of up to 4096
-    // tokens, D = 128, few against many: 64 columns 42 and 50 us, 96 51 and 52, 128 53 and 54, 256 88 and 59; one of
-    // 16000: 128 43 and 56, 256 51 and 61; 200 of up to 1000: 128 117 and 129, 256 203 and 127; D = 64, 16 of up to
-    // 8192: 64 72 and 88, 128 87 and 89.  fp16, whose many take longer: D = 128, 128 columns 56 and 74, 192 73 and 74,
-    // 256 88 and 76; D = 64 128 88 and 109, 192 114 and 111, 256 137 and 114.  D = 256, bf16, 16 of up to 4096: 64 columns 55
-    // and 72, 128 78 and 78, 192 103 and 83; fp16 has no wide tiles, its remainders do not fit LDS.
-    const bool many = (b.D < 256 || bf16) && all >= (bf16 ? 128 : 192) * (int64_t)b.n_seqs;
+    p.from = from, p.to = to;
     p.cols = !many ? 16 : b.D == 256 ? AT_COLS<256> : AT_COLS<128>;
-    p.tiles = all / p.cols + b.n_seqs;
+    p.tiles = all / p.cols + std::min<int64_t>(b.n_seqs, from ? all / from : b.n_seqs);
+    if (to != INT32_MAX) p.tiles = std::min(p.tiles, (int64_t)b.n_seqs * ((to + p.cols - 2) / p.cols));
     // one block of wide tiles or of heads of 256 fits a CU, two of the others
     p.share = std::max(1, (many || b.D == 256 ? 256 : 512) / b.n_kv);
     // Nothing to split where no sequence is longer than a block should take, or there are tiles enough: narrow ones
@@ -1480,16 +1477,39 @@ static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len, bool bf16)
     return p;
 }
 
+// The launches of a call, one or two.  The mean number of columns of a sequence says which kernel takes all of
+// them.  16 sequences of up to 4096
+// tokens, D = 128, few against many: 64 columns 42 and 50 us, 96 51 and 52, 128 53 and 54, 256 88 and 59; one of
+// 16000: 128 43 and 56, 256 51 and 61; 200 of up to 1000: 128 117 and 129, 256 203 and 127; D = 64, 16 of up to
+// 8192: 64 72 and 88, 128 87 and 89.  fp16, whose many take longer: D = 128, 128 columns 56 and 74, 192 73 and 74,
+// 256 88 and 76; D = 64 128 88 and 109, 192 114 and 111, 256 137 and 114.  D = 256, bf16, 16 of up to 4096: 64 columns 55
+// and 72, 128 78 and 78, 192 103 and 83; fp16 has no wide tiles, its remainders do not fit LDS.
+//
+// Where that is many, and the rows are so few next to the lengths that not all of more than 8 sequences can be prompts, single
+// tokens may be among them, to which a wide tile is a waste: each kernel takes those that are its.  A prompt of 2000 and 32
+// single tokens after 8192, 32 heads over 4: 133 us, 274 in one launch; after 4000 122 and 147; 8 chunks of 128, where
+// the second launch finds nothing to do: 84 and 79.
+static int attn_plans(const KvBatch &b, int n_heads, int max_len, bool bf16, AttnPlan p[2]) {
+    const int64_t all = (int64_t)b.n_tokens * (n_heads / b.n_kv);
+    const int few = bf16 ? 128 : 192;
+    const bool many = (b.D < 256 || bf16) && all >= few * (int64_t)b.n_seqs;
+    const bool both = many && b.n_seqs > 8 && 2 * (int64_t)b.n_tokens < (int64_t)b.n_seqs * max_len;
+    p[0] = attn_plan(b, n_heads, max_len, many, both ? few : 0, INT32_MAX);
+    if (both) p[1] = attn_plan(b, n_heads, max_len, false, 0, few);
+    return both ? 2 : 1;
+}
+
 static size_t attn_join_bytes(const KvBatch &b, const AttnPlan &p) {
     return ((size_t)p.joins * b.n_kv * sizeof(JoinTile) + 255) / 256 * 256;
 }
 
-// Enough for rows of either type.
+// Enough for rows of either type; a call's launches use it one after the other.
 size_t attn_workspace(const KvBatch &b, int n_heads, int max_len) {
     size_t most = 0;
     for (const bool bf16 : {false, true}) {
-        const AttnPlan p = attn_plan(b, n_heads, max_len, bf16);
-        if (p.share) most = std::max(most, attn_join_bytes(b, p) + (size_t)p.parts * b.n_kv * (p.cols * (b.D + 2)) * sizeof(float));
+        AttnPlan p[2];
+        for (int i = attn_plans(b, n_heads, max_len, bf16, p) - 1; i >= 0; i--)
+            if (p[i].share) most = std::max(most, attn_join_bytes(b, p[i]) + (size_t)p[i].parts * b.n_kv * (p[i].cols * (b.D + 2)) * sizeof(float));
     }
     return most;
 }
@@ -1519,17 +1539,22 @@ static hipError_t attn_launch(const KvBatch &b, KvRows q, int G, float scale, co
 
 hipError_t launch_attn(const KvBatch &b, int type, KvRows q, int n_heads, float scale, void *out, int64_t out_stride,
                        int max_len, void *ws, hipStream_t st) {
-    const AttnPlan p = attn_plan(b, n_heads, max_len, type == TG_T_BF16);
-    // threads of the launch's first dimension
-    if (p.blocks * (p.cols != 16 ? 512 * b.n_kv : 256) > UINT32_MAX) return hipErrorInvalidValue;
-    const int G = n_heads / b.n_kv;
-    const AttnOut o{out, out_stride, static_cast<JoinTile *>(ws), p.joins,
-                    reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + attn_join_bytes(b, p))};
+    AttnPlan plans[2];
+    const int n = attn_plans(b, n_heads, max_len, type == TG_T_BF16, plans), G = n_heads / b.n_kv;
     hipError_t e = hipSuccess;
-    TG_BY_DIM(b.D, {
-        if (type == TG_T_F16) e = attn_launch<DIM, false>(b, q, G, scale, p, o, st);
-        else e = attn_launch<DIM, true>(b, q, G, scale, p, o, st);
-    });
+    for (int i = 0; i < n && e == hipSuccess; i++) {
+        const AttnPlan &p = plans[i];
+        // threads of the launch's first dimension
+        if (p.blocks * (p.cols != 16 ? 512 * b.n_kv : 256) > UINT32_MAX) return hipErrorInvalidValue;
+        KvBatch kb = b;
+        kb.cols_from = p.from, kb.cols_to = p.to;
+        const AttnOut o{out, out_stride, static_cast<JoinTile *>(ws), p.joins,
+                        reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + attn_join_bytes(b, p))};
+        TG_BY_DIM(b.D, {
+            if (type == TG_T_F16) e = attn_launch<DIM, false>(kb, q, G, scale, p, o, st);
+            else e = attn_launch<DIM, true>(kb, q, G, scale, p, o, st);
+        });
+    }
     return e != hipSuccess ? e : hipGetLastError();
 }
 

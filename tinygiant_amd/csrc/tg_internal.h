@@ -390,6 +390,7 @@ struct KvBatch {
     int page_tokens, n_kv, D;
     int table_cols, table_stride;
     int n_seqs, n_tokens;
+    int cols_from = 0, cols_to = INT32_MAX;  // attention: the launch is for sequences with so many rows x heads of a key head
 };
 // strided rows of heads: element (t, h, d) at p[t * stride + h * D + d]
 struct KvRows {
