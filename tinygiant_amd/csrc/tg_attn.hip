@@ -304,9 +304,8 @@ __global__ __launch_bounds__(256) void k_kv_read(KvBatch b, _Float16 *k, _Float1
 // ================================================================ attention
 // Columns.  A sequence's rows and the G query heads of one key head are laid
 // out as columns f = row * G + head, 16 of which make a column tile, the
-// width of v_mfma_f32_16x16x32_f16.  Column tiles of all sequences are
-// numbered so that a launch needs no look at cu: sequence s starts at
-// cu[s] * G / 16 + s, at or behind the last tile of the sequence before it.
+// width of v_mfma_f32_16x16x32_f16.  Which blocks do which tiles and tokens is worked out on the
+// device from cu and kv_len (Cut and col_tile, below); the launch knows only how many there can be.
 //
 // Scores.  S^T = K Q^T with keys as the A operand: lane (c = lane % 16, h =
 // lane / 16) supplies key token c (16 bytes of a tile: its codes 8 h .. 8 h +
@@ -328,10 +327,10 @@ __global__ __launch_bounds__(256) void k_kv_read(KvBatch b, _Float16 *k, _Float1
 // exp2(s - m + A) d, one rounding to fp16, once for its two column tiles, and
 // the codes stay the integers they are, again as subnormals; a constant operand of -8
 // takes the codes' offset off within the same step, so no sum grows with it.
-// A = 11 - e where every scale so far is below 2^e, and m is raised (and the sums rescaled)
-// only where a score passes m + 4: p' stays below 2^15, and with the largest weight
-// at 2^5 or more it is a normal fp16 down to 2^-19 of that, the smallest
-// subnormal at 2^-29.  Sums, maxima and outputs are fp32.
+// A = 9 - e where every scale so far is below 2^(e - 1), and m is raised (and the sums rescaled)
+// only where a score passes m + 6: p' stays below 2^14, and next to the largest weight on the largest
+// scale, 2^7 or more, it is a normal fp16 down to 2^-21, the smallest
+// subnormal at 2^-31.  Sums, maxima and outputs are fp32.
 //
 // A value block that is not finite makes the token's scores NaN and its values 0, so
 // that rows which see the token are NaN and rows which do not are as ever.
@@ -344,7 +343,7 @@ constexpr float AT_NONE = -3.402823466e38f;  // m of a column that has seen noth
 constexpr uint32_t AT_EVEN = 0x003C003Cu, AT_ODD = 0x03C003C0u;  // codes in bits 2..5, 6..9 of both halves
 constexpr float AT_LEAST = 1e-37f;           // of the factor on scores: times it -inf stays -inf, and finite sums vanish
 constexpr float AT_ROOM = 6.0f;
-constexpr int AT_TOP = 9;                    // A + e
+constexpr int AT_TOP = 9;                    // A + e, and A of the wide tiles
 
 TG_DEV f16x2 as_h2(uint32_t v) { return __builtin_bit_cast(f16x2, v); }
 TG_DEV uint32_t as_u(f16x2 v) { return __builtin_bit_cast(uint32_t, v); }
