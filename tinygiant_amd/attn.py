@@ -78,7 +78,7 @@ class KVBatch:
         if max_len < 0:
             raise ValueError(f"max_len {max_len}")
         self.cu, self.kv_len, self.table, self.max_len = cu, kv_len, table, int(max_len)
-        self.n_seqs = n
+        self.n_seqs, self.device = n, cu.device
 
 
 class PagedKV:
@@ -101,7 +101,7 @@ class PagedKV:
         elif (not isinstance(pages, torch.Tensor) or not pages.is_cuda or pages.dtype != torch.uint8
               or tuple(pages.shape) != shape or not pages.is_contiguous()):
             raise TypeError(f"pages must be a contiguous uint8 CUDA (HIP) tensor of shape {shape}")
-        self.pages = pages
+        self.pages, self.device = pages, pages.device
         self.n_layers, self.n_pages, self.page_tokens = n_layers, n_pages, page_tokens
         self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
         self.layer_bytes = pages.stride(0)
@@ -109,8 +109,8 @@ class PagedKV:
     def _batch(self, layer: int, batch: KVBatch, n_tokens: int) -> _Batch:
         if not 0 <= layer < self.n_layers:
             raise ValueError(f"layer {layer} of {self.n_layers}")
-        if batch.cu.device != self.pages.device:
-            raise ValueError(f"batch on {batch.cu.device}, pages on {self.pages.device}")
+        if batch.device != self.device:
+            raise ValueError(f"batch on {batch.device}, pages on {self.device}")
         t = batch.table
         cols = t.shape[1]
         return _Batch(self.pages.data_ptr() + layer * self.layer_bytes, t.data_ptr(), batch.cu.data_ptr(),
@@ -119,8 +119,8 @@ class PagedKV:
 
     def _rows(self, t, name, heads, dtype, n_tokens):
         """A [T, heads, D] (or [T, heads * D]) tensor with packed heads: its row stride."""
-        if not isinstance(t, torch.Tensor) or t.device != self.pages.device or t.dtype != dtype:
-            raise TypeError(f"{name} must be a {dtype} tensor on {self.pages.device}")
+        if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != dtype:
+            raise TypeError(f"{name} must be a {dtype} tensor on {self.device}")
         D, shape, stride = self.head_dim, t.shape, t.stride()
         if len(shape) == 3:
             ok = shape[1] == heads and shape[2] == D and stride[2] == 1 and (heads == 1 or stride[1] == D)
@@ -138,9 +138,9 @@ class PagedKV:
         return q.shape[1] if q.dim() == 3 else q.shape[1] // D
 
     def _floats(self, t, name, shape):
-        if (not isinstance(t, torch.Tensor) or t.device != self.pages.device or t.dtype != torch.float32
+        if (not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != torch.float32
                 or t.shape != shape or not t.is_contiguous()):
-            raise TypeError(f"{name} must be a contiguous float32 tensor of shape {shape} on {self.pages.device}")
+            raise TypeError(f"{name} must be a contiguous float32 tensor of shape {shape} on {self.device}")
         return t.data_ptr()
 
     def append(self, layer: int, q, k, v, batch: KVBatch, cos=None, sin=None, q_norm=None, k_norm=None,
@@ -160,8 +160,9 @@ class PagedKV:
         if q is not None:
             qs = self._rows(q, "q", heads, dt, T)
             if out is None:
-                out = q.new_empty((T, heads, D))
-            os_ = self._rows(out, "out", heads, dt, T)
+                out, os_ = q.new_empty((T, heads, D)), heads * D
+            else:
+                os_ = self._rows(out, "out", heads, dt, T)
             qp, op = q.data_ptr(), out.data_ptr()
         if (cos is None) != (sin is None):
             raise ValueError("cos and sin are given together")
@@ -182,7 +183,7 @@ class PagedKV:
         n_kv_heads, D] float16."""
         if n_tokens < 0:
             raise ValueError(f"n_tokens {n_tokens}")
-        k = torch.empty((n_tokens, self.n_kv_heads, self.head_dim), dtype=torch.float16, device=self.pages.device)
+        k = torch.empty((n_tokens, self.n_kv_heads, self.head_dim), dtype=torch.float16, device=self.device)
         v = torch.empty_like(k)
         b = self._batch(layer, batch, n_tokens)
         if n_tokens and batch.n_seqs:
@@ -200,8 +201,9 @@ class PagedKV:
             raise TypeError(f"q of type {dt}: float16 or bfloat16 needed")
         qs = self._rows(q, "q", heads, dt, T)
         if out is None:
-            out = q.new_empty((T, heads, D))
-        os_ = self._rows(out, "out", heads, dt, T)
+            out, os_ = q.new_empty((T, heads, D)), heads * D
+        else:
+            os_ = self._rows(out, "out", heads, dt, T)
         b = self._batch(layer, batch, T)
         if not T or not batch.n_seqs:
             return out
