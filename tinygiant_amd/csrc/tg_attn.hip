@@ -1050,8 +1050,9 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
         load_words<NG>(p + scale_at, sc);
         load_words<NG>(p + more_at, sc + NG);
     };
-    // codes n of the four-code halfwords of w, less 8, times d, and the rounding's remainder; one of the two constants in a scalar register
-    // and one in a vector register make a single instruction of the mask and what makes a number of it
+    // codes n of the four-code halfwords of w, less 8, times d, and the rounding's remainder; one of the two
+    // constants in a scalar register and one in a vector register make a single instruction of the mask and what
+    // makes a number of it
     uint32_t lo = 0x000F000Fu, hi = 0x00F000F0u, k1024 = 0x64006400u, k64 = 0x54005400u;
     asm("" : "+s"(lo), "+s"(hi), "+v"(k1024), "+v"(k64));
     auto unpack = [&](uint32_t w, int n, f16x2 d, uint32_t &rest) {
@@ -1443,8 +1444,8 @@ hipError_t launch_kv_read(const KvBatch &b, void *k, void *v, hipStream_t st) {
 }
 
 // Blocks of one launch.  Narrow column tiles: `share` per key head, or one for each tile.  Wide ones: one
-// for each tile and `share` per key head more for their pieces, of which there are 2 share at most (share, where it is searched for;
-// 5 / 3 share with more than 64 sequences).
+// for each tile and `share` per key head more for their pieces, of which there are 2 share at most (share,
+// where it is searched for; 5 / 3 share with more than 64 sequences).
 struct AttnPlan {
     int64_t tiles;
     int cols, share, joins, unit;

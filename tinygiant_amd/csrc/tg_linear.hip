@@ -231,7 +231,8 @@ TG_DEV float quant_row(const MatmulI8Args &a, int Kp, int row, QuantLds &l, P pu
     return bad ? __builtin_nanf("") : (float)(top / 127.0);
 }
 
-// A launch of its own for the codes, bound by bytes: 8192 x 4096 fp32 with norm 42 us, 4.0 TB/s; 1999 x 4096 bf16 11 us, its latency.
+// A launch of its own for the codes, bound by bytes: 8192 x 4096 fp32 with norm 42 us, 4.0 TB/s; 1999 x 4096
+// bf16 11 us, its latency.
 template <int TYPE, int TPR, int NV>
 __global__ __launch_bounds__(256) void k_lin_quant(MatmulI8Args a, int Kp, int8_t *xq, float *xs) {
     __shared__ QuantLds l;
