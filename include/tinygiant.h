@@ -452,7 +452,7 @@ int tg_head_sample(tg_head *h, const float *x, float eps, float temperature, dou
  * memory outside the arguments is touched. */
 typedef struct {
     void *pages;
-    const int32_t *table;   /* [n_seqs][table_cols], rows table_stride apart */
+    const int32_t *table;   /* [n_seqs][table_cols], rows table_stride apart (0: one row for all) */
     const int32_t *cu;      /* [n_seqs + 1], from 0, not decreasing */
     const int32_t *kv_len;  /* [n_seqs] */
     int64_t n_pages;

@@ -1,0 +1,59 @@
+"""How the attention block's Python side hands its tensors to the C ABI.  No call reaches a kernel, so these run without
+a GPU; objects are made of host tensors around the constructors, which take only the device's."""
+import ctypes
+
+import pytest
+import torch
+
+from tinygiant_amd import _lib
+from tinygiant_amd.attn import KVBatch, PagedKV, table_stride
+
+
+def cache(head_dim=64, n_kv=2, page=16, n_pages=4):
+    kv = PagedKV.__new__(PagedKV)
+    kv.pages = torch.zeros(1, n_pages, n_kv, page // 16, 18 * head_dim, dtype=torch.uint8)
+    kv.device, kv.n_layers, kv.n_pages, kv.page_tokens, kv.n_kv_heads, kv.head_dim = kv.pages.device, 1, n_pages, page, n_kv, head_dim
+    kv.layer_bytes = kv.pages.stride(0)
+    return kv
+
+
+def batch_over(table):
+    b = KVBatch.__new__(KVBatch)
+    n = table.shape[0]
+    b.cu, b.kv_len, b.table = torch.arange(n + 1, dtype=torch.int32), torch.ones(n, dtype=torch.int32), table
+    b.max_len, b.n_seqs, b.device = 0, n, table.device
+    return b
+
+
+WIDE = torch.arange(60, dtype=torch.int32).view(5, 12)
+
+
+@pytest.mark.parametrize("table", [
+    WIDE, WIDE[:, :4], WIDE[::2, 3:7], WIDE[1:2], WIDE[0].expand(3, 12), WIDE[0, :4].expand(5, 4), WIDE[2:3, :4].expand(1, 4),
+    WIDE[:, :1], WIDE[0, :1].expand(7, 1)], ids=lambda t: f"{tuple(t.shape)}x{t.stride()}")
+def test_every_entry_of_the_table_is_where_the_kernels_look(table):
+    """Entry (s, c) at table + s * table_stride + c, whatever view the table is."""
+    b = cache()._batch(0, batch_over(table), 3)
+    flat = torch.as_strided(table, (table.untyped_storage().nbytes() // 4 - table.storage_offset(),), (1,))
+    assert b.table == table.data_ptr() and b.table_cols == table.shape[1]
+    for s in range(table.shape[0]):
+        for c in range(table.shape[1]):
+            at = s * b.table_stride + c
+            assert at < len(flat) and flat[at] == table[s, c], (s, c, b.table_stride)
+
+
+def test_a_table_whose_rows_overlap_is_refused():
+    for rows in (2, 3):
+        t = torch.as_strided(WIDE, (rows, 4), (2, 1))
+        with pytest.raises(ValueError, match="overlap"):
+            table_stride(t)
+    assert table_stride(torch.as_strided(WIDE, (1, 4), (2, 1))) >= 4  # one row overlaps nothing
+
+
+def test_one_row_for_every_sequence_is_taken_by_the_c_side():
+    lib = _lib.require_lib()
+    b = cache()._batch(0, batch_over(WIDE[0].expand(3, 12)), 0)  # no rows: checked, nothing launched
+    P = 1 << 20
+    assert b.table_stride == 0 and lib.tg_kv_read_q4_dev(ctypes.byref(b), P, P, None) == 0
+    b.table_stride = 5
+    assert lib.tg_kv_read_q4_dev(ctypes.byref(b), P, P, None) == -1 and "5 apart" in lib.tg_last_error().decode()

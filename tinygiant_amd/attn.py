@@ -56,12 +56,24 @@ def _index(t, name, dims):
         raise TypeError(f"{name} must be a {dims}-dimensional int32 CUDA (HIP) tensor")
 
 
+def table_stride(table) -> int:
+    """Entries from one sequence's row of a page table to the next's; 0 where
+    all of them have the same row (an expanded one).  Of one row there is no
+    next, and torch gives its stride any value."""
+    n, cols = table.shape
+    stride = table.stride(0) if n > 1 else cols
+    if 0 < stride < cols:
+        raise ValueError(f"rows of table overlap: {cols} entries, {stride} apart")
+    return stride
+
+
 class KVBatch:
     """A ragged batch: rows cu[s]..cu[s+1]-1 are the last tokens of sequence
     s, which has kv_len[s] tokens in the pages table[s].  cu [n_seqs + 1],
     kv_len [n_seqs], table [n_seqs, pages] are int32 CUDA tensors that the
     kernels read at each call, so they may be rewritten in place between
-    calls (and graph replays).  max_len: about the longest kv_len; it only
+    calls (and graph replays).  table may be a view: columns of a wider one,
+    or one row expanded, whose pages the sequences then share.  max_len: about the longest kv_len; it only
     sets how attention's work is split (default: what the table can hold)."""
 
     def __init__(self, cu, kv_len, table, max_len: int = 0):
@@ -73,6 +85,7 @@ class KVBatch:
             raise ValueError(f"{n} sequences, {cu.numel()} row bounds, {table.shape[0]} table rows")
         if not cu.is_contiguous() or not kv_len.is_contiguous() or (table.numel() and table.stride(1) != 1):
             raise TypeError("cu, kv_len and the rows of table must be contiguous")
+        table_stride(table)
         if not cu.device == kv_len.device == table.device:
             raise ValueError(f"cu on {cu.device}, kv_len on {kv_len.device}, table on {table.device}")
         if max_len < 0:
@@ -112,10 +125,9 @@ class PagedKV:
         if batch.device != self.device:
             raise ValueError(f"batch on {batch.device}, pages on {self.device}")
         t = batch.table
-        cols = t.shape[1]
         return _Batch(self.pages.data_ptr() + layer * self.layer_bytes, t.data_ptr(), batch.cu.data_ptr(),
-                      batch.kv_len.data_ptr(), self.n_pages, self.page_tokens, self.n_kv_heads, self.head_dim, cols,
-                      max(t.stride(0), cols), batch.n_seqs, n_tokens)
+                      batch.kv_len.data_ptr(), self.n_pages, self.page_tokens, self.n_kv_heads, self.head_dim, t.shape[1],
+                      table_stride(t), batch.n_seqs, n_tokens)
 
     def _rows(self, t, name, heads, dtype, n_tokens):
         """A [T, heads, D] (or [T, heads * D]) tensor with packed heads: its row stride."""

@@ -2479,7 +2479,7 @@ static int kv_batch(const char *fn, const tg_kv_batch *b, tg::KvBatch *k) {
         return set_err(TG_E_INVALID, "%s: page_tokens %d is not a multiple of 16 up to 65536", fn, b->page_tokens);
     if (b->n_kv_heads < 1 || b->n_kv_heads > 1024 || b->n_pages < 1 || b->n_pages > INT32_MAX)
         return set_err(TG_E_INVALID, "%s: n_kv_heads %d, n_pages %lld", fn, b->n_kv_heads, (long long)b->n_pages);
-    if (b->table_cols < 1 || b->table_stride < b->table_cols || (int64_t)b->table_cols * b->page_tokens > 1 << 30)
+    if (b->table_cols < 1 || (b->table_stride && b->table_stride < b->table_cols) || (int64_t)b->table_cols * b->page_tokens > 1 << 30)
         return set_err(TG_E_INVALID, "%s: table_cols %d (rows %d apart) of %d tokens", fn, b->table_cols,
                        b->table_stride, b->page_tokens);
     if (!b->pages || !b->table || !b->cu || !b->kv_len) return set_err(TG_E_INVALID, "%s: a NULL pointer in the batch", fn);
