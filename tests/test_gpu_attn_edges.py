@@ -50,3 +50,77 @@ def test_overlapping_rows_of_a_page_table_are_refused():
     s = Setup(52, 64, 1, 16, [40, 40], [1, 1])
     with pytest.raises(ValueError, match="overlap"):
         KVBatch(s.batch.cu, s.batch.kv_len, torch.as_strided(s.batch.table, (2, 3), (1, 1)))
+
+
+# ---------------------------------------------------------------- blocks that are not finite
+def value_scales(s, i, t):
+    """The value scales of token t of sequence i as bits [n_kv, D / 32], to be written in place."""
+    tiles = s.cache.pages[s.table[i, t // s.page], :, t % s.page // 16].view(np.uint16)
+    at = s.cache._places(t % 16)[5]
+    return tiles, at
+
+
+def set_scales(s, i, t, f):
+    """Token t's value scales multiplied by f, or set to it where it is not finite."""
+    tiles, at = value_scales(s, i, t)
+    old = tiles[:, at].view(np.float16)
+    tiles[:, at] = (old * np.float16(f) if np.isfinite(f) else np.full_like(old, f)).view(np.uint16)
+
+
+class Prefix:
+    """Sequence 0 of s without its tokens from n on, and its first rows."""
+
+    def __init__(self, s, n, new):
+        self.lens, self.news, self.cu, self.table, self.cache, self.D = [n], [new], [0, new], s.table, s.cache, s.D
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("what", ["page", "nan pair", "inf pair", "nan other tile"])
+@pytest.mark.parametrize("factor", [16, 256, 2048])
+@pytest.mark.parametrize("G,after,dt", [(2, 4, "f16"), (1, 16, "bf16"), (5, 1, "f16")])
+def test_a_block_that_is_not_finite_stays_in_the_rows_that_see_it(D, what, factor, G, after, dt):
+    """Rows before it are as exact as ever, also where the largest value scales so far stand next to it: in the other
+    tile of its 32 tokens, or in the other half of its pair."""
+    from tinygiant_amd.attn import KVBatch
+    gpu_note(f"attend not finite {D} {what} {factor} {G} {after}")
+    bad = {"page": 144, "nan pair": 137, "inf pair": 137, "nan other tile": 148}[what]  # the token that is not finite
+    large = {"page": [128, 129], "nan pair": [136], "inf pair": [136], "nan other tile": [132]}[what]
+    before = 3 if bad == 137 else 6  # rows that do not see it; the last one does see the large scales
+    s = Setup(60 + D, D, 2, 16, [bad + after], [before + after])
+    for t in large:
+        set_scales(s, 0, t, factor)
+    table = s.table.copy()
+    if what == "page":
+        table[0, bad // 16] = -1
+    else:
+        set_scales(s, 0, bad, np.inf if what == "inf pair" else np.nan)
+    s.kv.pages.copy_(dev(s.all))
+    q, qn = s.rows(2 * G, dt)
+    for hint in (1, 0):  # the tile whole, and split
+        out = s.kv.attend(0, q, KVBatch(s.batch.cu, s.batch.kv_len, dev(table), max_len=hint))
+        check_attend(Prefix(s, bad, before), None, qn[:before], out[:before])
+        assert torch.isnan(out[before:]).all()
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [1, 90, 1]])
+def test_rows_beside_bad_pages_are_as_exact_as_ever(news):
+    """A page outside the pool in one of three sequences: the rows that do not see it, and the other sequences."""
+    from tinygiant_amd.attn import KVBatch
+    gpu_note(f"attend beside bad pages {news}")
+    s = Setup(14, 128, 2, 16, [100, 100, 100], news)
+    q, qn = s.rows(8, "f16")
+    q[0, 3] = float("nan")
+    for page in (len(s.cache.pages), -1):
+        table = s.table.copy()
+        table[1, 3] = page  # tokens 48..63 of sequence 1
+        out = s.kv.attend(0, q, KVBatch(s.batch.cu, s.batch.kv_len, dev(table), max_len=100))
+        assert torch.isnan(out[0, 3]).all() and torch.isfinite(out[0, :3]).all() and torch.isfinite(out[0, 4:]).all()
+        qn[0, 3] = 0  # a query of zeros weighs all values alike: key head 0's mean takes the place of the NaN row
+        out[0, 3] = dev(s.cache.rows(s.table[0], 100)[1].mean(axis=1)[0], torch.float16)
+        check_attend(s, q, qn, out, bad=(1,))
+        before = max(0, 48 - (100 - news[1]))
+        if before:
+            at = s.cu[1]
+            p = Prefix(s, 48, before)
+            p.table = s.table[1:]
+            check_attend(p, None, qn[at:at + before], out[at:at + before])

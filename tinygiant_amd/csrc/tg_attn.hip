@@ -770,10 +770,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
             }
             bool odd = false;
             if (__ballot(big != below)) {
-                // a scale at or above the bound: a new one, or a block that is not finite
-                uint32_t top = max(big & 0xFFFFu, big >> 16);
-                odd = __ballot(top >= 0x7C00u) != 0;
-                if (top >= 0x7C00u) top = 0;
+                // a scale at or above the bound: a new one, or a block that is not finite, which is left out by itself
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < SW; i++) {
+                    const uint32_t v = sl[tile_of(i) * (D / 2) + word_of(i)] & vmask;  // as this lane has just put it there
+                    const uint32_t lo = v & 0xFFFFu, hi = v >> 16;
+                    odd = odd || max(lo, hi) >= 0x7C00u;
+                    top = max(top, max(lo < 0x7C00u ? lo : 0u, hi < 0x7C00u ? hi : 0u));
+                }
+                odd = __ballot(odd) != 0;
 #pragma unroll
                 for (int i = 1; i < 64; i *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, i));
                 if (top > (below & 0xFFFFu)) {
