@@ -444,8 +444,9 @@ int tg_head_sample(tg_head *h, const float *x, float eps, float temperature, dou
  * Sequence s has kv_len[s] cached tokens, the batch's own among them; token
  * p of it sits in page table[s * table_stride + p / page_tokens].  Rows
  * cu[s] .. cu[s + 1] - 1 of the row tensors are its last tokens, the last
- * one at position kv_len[s] - 1; rows from cu[n_seqs] on (padding) are
- * neither read nor written.  Two sequences may share pages that the call
+ * one at position kv_len[s] - 1; rows from cu[n_seqs] on (padding) count for
+ * nothing and are not written.  Where cu counts more rows than n_tokens, the
+ * call does those that there are, at the positions they have in the batch.  Two sequences may share pages that the call
  * only reads.  table, cu and kv_len are read on the device: a page outside
  * 0..n_pages-1, or a position at or beyond table_cols * page_tokens, that a
  * call needs makes NaN of the rows that need it (and is not written); no

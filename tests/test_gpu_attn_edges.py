@@ -124,3 +124,47 @@ def test_rows_beside_bad_pages_are_as_exact_as_ever(news):
             p = Prefix(s, 48, before)
             p.table = s.table[1:]
             check_attend(p, None, qn[at:at + before], out[at:at + before])
+
+
+# ---------------------------------------------------------------- fewer rows than the batch counts
+@pytest.mark.parametrize("T", [1, 7, 30, 44])
+def test_rows_that_are_not_there(T):
+    """Row tensors that end before cu[n_seqs] does: the rows they hold are those rows, at their own positions."""
+    from tinygiant_amd.attn import KVBatch
+    gpu_note(f"fewer rows than the batch {T}")
+    lens, news = [60, 45, 9], [5, 40, 4]
+    s = Setup(71, 64, 2, 16, lens, news)
+    pos = np.concatenate([np.arange(n - new, n) for n, new in zip(lens, news)])[:T]
+    seq = np.repeat(np.arange(3), news)[:T]
+    k, v = s.kv.read(0, s.batch, T)
+    for got, at in ((k, 0), (v, 1)):
+        ref = np.stack([s.cache.rows(s.table[i], p + 1)[at][:, p] for i, p in zip(seq, pos)])
+        assert np.array_equal(got.cpu().numpy(), ref.astype(np.float16))
+    (q, qh), (k, kh), (v, vh) = s.rows(4, "f32"), s.rows(2, "f32"), s.rows(2, "f32")
+    ang = s.rng.uniform(0, 9, (60, 32))
+    cos, sin = np.cos(ang).astype(np.float32), np.sin(ang).astype(np.float32)
+    out = s.kv.append(0, q[:T], k[:T], v[:T], s.batch, dev(cos), dev(sin))
+    rq, rk = (A.rotate(x[:T], cos[pos][:, None], sin[pos][:, None]) for x in (qh, kh))
+    assert torch.equal(out, dev(rq))
+    for t, (i, p) in enumerate(zip(seq, pos)):
+        for h in range(2):
+            s.cache.put(s.table[i, p // 16], h, p % 16, rk[t, h], vh[t, h])
+    assert np.array_equal(s.kv.pages.cpu().numpy()[0], s.cache.pages)
+
+
+@pytest.mark.parametrize("news,T,G,dt", [([3, 40, 2], 20, 2, "f16"), ([300, 700], 900, 1, "bf16"), ([300, 700], 200, 4, "f16"),
+                                         ([1] * 9 + [600], 300, 2, "bf16")])
+def test_attention_of_rows_that_are_not_there(news, T, G, dt):
+    gpu_note(f"attend fewer rows {news} {T}")
+    lens = [n + 50 for n in news]
+    s = Setup(72, 64, 1, 16, lens, news)
+    q, qn = s.rows(G, dt)
+    out = s.kv.attend(0, q[:T], s.batch)
+    assert len(out) == T
+    for i, (n, new) in enumerate(zip(lens, news)):
+        there = min(max(T - int(s.cu[i]), 0), new)
+        if there:
+            p = Prefix(s, n - new + there, there)
+            p.table = s.table[i:]
+            at = s.cu[i]
+            check_attend(p, None, qn[at:at + there], out[at:at + there])

@@ -24,18 +24,21 @@ TG_DEV size_t tile_at(const KvBatch &b, int page, int head, int tile) {
     return (((size_t)page * b.n_kv + head) * (b.page_tokens / 16) + tile) * (size_t)(18 * D);
 }
 
-// rows [lo, hi) of sequence s, kept inside the row tensors whatever cu holds
+// Rows [lo, hi) of a sequence, kept inside the row tensors whatever cu holds,
+// and the tokens up to row hi - 1: its length less the rows behind the
+// tensors' end (so below 0 where those are more than its tokens).
 struct SeqRows {
     int lo, hi, len;
 };
-TG_DEV SeqRows seq_rows(const KvBatch &b, int s) {
+TG_DEV SeqRows seq_rows(const KvBatch &b, int c0, int c1, int len) {
     SeqRows r;
-    const int lo = b.cu[s], hi = b.cu[s + 1], len = b.kv_len[s];
-    r.lo = min(max(lo, 0), b.n_tokens);
-    r.hi = min(max(hi, r.lo), b.n_tokens);
-    r.len = max(len, 0);
+    r.lo = min(max(c0, 0), b.n_tokens);
+    const int end = max(c1, r.lo);
+    r.hi = min(end, b.n_tokens);
+    r.len = max(len, 0) - (end - r.hi);
     return r;
 }
+TG_DEV SeqRows seq_rows(const KvBatch &b, int s) { return seq_rows(b, b.cu[s], b.cu[s + 1], b.kv_len[s]); }
 
 // the page of position p of sequence s, or -1
 TG_DEV int page_of(const KvBatch &b, int s, int p) {
@@ -382,10 +385,11 @@ TG_DEV SeqWork seq_work(const KvBatch &b, int G, int j) {
     const bool in = j < b.n_seqs;
     const int jj = in ? j : 0;  // three loads side by side, not one behind the other
     const int c0 = b.cu[jj], c1 = b.cu[jj + 1], cl = b.kv_len[jj];
+    const SeqRows r = seq_rows(b, c0, c1, cl);
     SeqWork w;
-    w.lo = min(max(c0, 0), b.n_tokens);
-    w.n = in ? min(max(c1, w.lo), b.n_tokens) - w.lo : 0;
-    w.len = max(cl, 0);
+    w.lo = r.lo;
+    w.n = in ? r.hi - r.lo : 0;
+    w.len = r.len;
     const int64_t cols = (int64_t)w.n * G;
     w.tiles = cols >= b.cols_from && cols < b.cols_to ? (int)((cols + COLS - 1) / COLS) : 0;
     w.steps = max(1, (min(w.len, b.table_cols * b.page_tokens + 1) + 31) / 32);
