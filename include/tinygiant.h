@@ -489,7 +489,8 @@ int tg_kv_read_q4_dev(const tg_kv_batch *b, void *k, void *v, void *stream);
  * [n_tokens][n_heads][head_dim] fp16 or bf16, rows *_stride elements apart
  * (multiples of 8, pointers 16-byte aligned), out not overlapping q.  A row
  * at a position below 0 sees nothing and is zero.  scale is above 0 and
- * finite; n_heads is a multiple of n_kv_heads.  Sums are fp32; weights, and the
+ * finite; n_heads is a multiple of n_kv_heads.  Scores may be as large as
+ * fp32 holds (larger ones count as infinite).  Sums are fp32; weights, and the
  * keys and values of many rows, are rounded to fp16 on the way (for fp16 rows
  * keys and values are taken whole).  Scales above 8188, which append never
  * writes, may count as infinite.  max_len: about the longest kv_len (0: table_cols *

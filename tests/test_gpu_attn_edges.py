@@ -168,3 +168,73 @@ def test_attention_of_rows_that_are_not_there(news, T, G, dt):
             p.table = s.table[i:]
             at = s.cu[i]
             check_attend(p, None, qn[at:at + there], out[at:at + there])
+
+
+# ---------------------------------------------------------------- scores of any size
+def check_weights(s, qn, out, ref_of):
+    """out against sums of values whose weights are known: off by the weights' and values' roundings alone."""
+    half, u = torch.finfo(out.dtype).eps / 2, 2.0 ** -11
+    got = out.double().cpu().numpy()
+    v, step = s.cache.rows(s.table[0], s.lens[0])[1], s.cache.rows(s.table[0], s.lens[0], steps=True)[1]
+    G = got.shape[1] // s.n_kv
+    for i in range(s.news[0]):
+        w = ref_of(i)  # [tokens]
+        for h in range(got.shape[1]):
+            ref, size, vstep = w @ v[h // G], w @ np.abs(v[h // G]), w @ np.abs(step[h // G])
+            tol = size * (2.0 ** -16 + 2 * u) + 2.0 ** -10 * vstep + half * np.abs(ref) * (1 + 1e-3) + 2.0 ** -24
+            assert (np.abs(got[i, h] - ref) <= tol).all(), (i, h, got[i, h][:4], ref[:4])
+
+
+# of the query (times the key) and of the keys, and the scale; in the last three the one or the other of their factors passes fp32's range on the way
+LARGE = [(1.0, 1.0, 0.1), (1.0, 1.0, 1e3), (1.0, 1.0, 3e5), (1.0, 1.0, 1e6), (1.0, 1.0, 1e7), (1.0, 1.0, 1e8), (1.0, 1.0, 1e12),
+         (1.0, 1.0, 1e30), (1e20, 1.0, 0.1), (1e34, 1.0, 0.1), (1e40, 1e-3, 0.1), (1e-36, 1.0, 3e38), (1e40, 1e-3, 1e-3)]
+
+
+@pytest.mark.parametrize("D,G,news", [(128, 4, 1), (128, 4, 3), (64, 2, 300), (256, 2, 2), (128, 2, 200), (256, 1, 200)])
+@pytest.mark.parametrize("size,small,scale", LARGE)
+def test_a_key_that_outweighs_all_others(D, G, news, size, small, scale):
+    """Queries along one token's key: its value is the result, however large the scores are."""
+    gpu_note(f"attend large scores {D} {G} {news} {size} {small} {scale}")
+    s = Setup(81, D, 1, 16, [600], [news])
+    winner = 200
+    s.cache.pages[..., 16 * D:17 * D].view(np.float16)[...] *= np.float16(small)
+    s.cache.pages[s.table[0, winner // 16], :, 0].view(np.uint16)[:, s.cache._places(winner % 16)[4]] = np.float16(small).view(np.uint16)
+    s.kv.pages.copy_(dev(s.all))
+    k = s.cache.rows(s.table[0], 600)[0][0]  # the other keys' steps are 0.15 of the winner's
+    q = dev(np.broadcast_to(k[winner] * size, (news, G, D)).astype(np.float32), torch.bfloat16)
+    score = q[0, 0].double().cpu().numpy() @ k.T * scale
+    assert score.argmax() == winner and np.sort(score)[-2] < 0.5 * score.max() < 1e38
+    if score.max() < 100:
+        return check_attend(s, q, q.float().cpu().numpy(), s.kv.attend(0, q, s.batch, scale=scale), scale=scale)
+    one = np.zeros(600)
+    one[winner] = 1
+    for b in (s.batch, type(s.batch)(s.batch.cu, s.batch.kv_len, s.batch.table, max_len=1)):
+        check_weights(s, None, s.kv.attend(0, q, b, scale=scale), lambda i: one)
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("D,G,news", [(128, 4, 1), (64, 2, 3), (256, 2, 2), (128, 2, 200)])
+@pytest.mark.parametrize("scale", [0.1, 3e5, 1e7, 1e9, 1e12, 1e30])
+def test_equal_scores_of_any_size(D, G, news, scale, sign):
+    """The same key in every place: all values weigh alike, whatever the score and however the values' sizes differ."""
+    gpu_note(f"attend equal scores {D} {G} {news} {scale} {sign}")
+    s = Setup(82, D, 1, 16, [500], [news])
+    pages, rng = s.cache.pages.view(np.uint16), np.random.default_rng(5)
+    code, step = rng.integers(0, 16, D), np.float16(rng.uniform(0.1, 0.2, D // 32))
+    for r in range(16):
+        ka, kn, _, _, ks, _ = s.cache._places(r)
+        half = np.zeros(pages.shape[-1], np.int64)
+        np.add.at(half, ka, code << (4 * kn))
+        pages[..., ka] = half[ka].astype(np.uint16)
+        pages[..., ks] = step.view(np.uint16)
+    for t in range(0, 500):
+        set_scales(s, 0, t, [1.0, 30.0, 0.01, 900.0][t // 32 % 4])  # each of a block's waves its own size
+    s.kv.pages.copy_(dev(s.all))
+    k = s.cache.rows(s.table[0], 500)[0][0]
+    assert (k == k[0]).all()
+    q = dev(np.broadcast_to(k[0] * sign, (news, G, D)).astype(np.float32), torch.bfloat16)
+    def weights(i):
+        n = 500 - news + i + 1
+        return np.where(np.arange(500) < n, 1 / n, 0)
+    for b in (s.batch, type(s.batch)(s.batch.cu, s.batch.kv_len, s.batch.table, max_len=1)):
+        check_weights(s, None, s.kv.attend(0, q, b, scale=scale), weights)

@@ -345,7 +345,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr float AT_NONE = -3.402823466e38f;  // m of a column that has seen nothing
 constexpr uint32_t AT_EVEN = 0x003C003Cu, AT_ODD = 0x03C003C0u;  // codes in bits 2..5, 6..9 of both halves
 constexpr float AT_LEAST = 1e-37f;           // of the factor on scores: times it -inf stays -inf, and finite sums vanish
+constexpr float AT_MOST = 3.402823466e38f;   // ... and +-0 stays 0
 constexpr float AT_ROOM = 6.0f;
+constexpr float AT_FINE = 4194304.0f;        // up to this m (2^22) a score's product, m and A fit one multiply-add
 constexpr int AT_TOP = 9;                    // A + e, and A of the wide tiles
 
 TG_DEV f16x2 as_h2(uint32_t v) { return __builtin_bit_cast(f16x2, v); }
@@ -375,6 +377,19 @@ TG_DEV float col_sum(float v) {
     const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
+
+// What a score's fp32 sum is multiplied by, scale log2(e) 2^e.  Between its bounds: beyond them, scores that fp32 holds
+// differ by so much, or so little, that the weights are the same.
+TG_DEV float score_factor(float scale, int e) {
+    return fminf(fmaxf(ldexpf(scale, e) * 1.44269504f, AT_LEAST), AT_MOST);
+}
+
+// Is some m so large that exponents have to be formed in two steps?  exp2(s cs + (A - m)) as one multiply-add is exact
+// in s cs, but m and A - m are rounded, together by 2^(k - 24) where m is below 2^k: a factor on all of a column's
+// weights, which falls out in the end if fp16 holds them.  Up to 2^22 it is below 2^0.25, and p' below 2^15.25;
+// beyond 2^26 it could be 2^8.  In two steps, s cs - m and then A, the largest weight is 2^A again, and a score is
+// off by the rounding of its product.
+TG_DEV bool coarse(float m) { return __ballot(fabsf(m) > AT_FINE && m != AT_NONE) != 0; }
 
 // One sequence as a lane of the planning scan holds it
 struct SeqWork {
@@ -722,7 +737,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
             int e2 = 0;
             (void)frexpf(top, &e2);  // top = m 2^e2, m in [0.5, 1)
             const int a = top > 0.0f && top < INFINITY ? 11 - e2 : 0;
-            cs = fmaxf(ldexpf(scale * 1.44269504f, 18 - a), AT_LEAST);
+            cs = score_factor(scale, 18 - a);
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 float sum = 0.0f;
@@ -750,6 +765,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
         float m = AT_NONE, l = 0.0f;
         float A = 0.0f;           // the same in all lanes of a wave
         uint32_t below = 0u;      // pairs of halves: the largest scale that A allows for
+        bool rough = false;       // as coarse(m) says
         auto work = [&](KvStep<D> &k, int step) {
             const bool edge = step * 32 + 31 > all;  // some column does not see all of it
             // scales to LDS as the tiles hold them; what no column sees is zero
@@ -862,12 +878,18 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
 #pragma unroll
                 for (int j = 0; j < ND; j++) acc[j] *= r;
                 m = m2;
+                rough = coarse(m);
             }
-            const float off = A - m;
+            float by = cs, off = A - m;
+            if (rough) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) s[i / 4][i % 4] = s[i / 4][i % 4] * cs - m;
+                by = 1.0f, off = A;
+            }
             float p[2][4];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                p[i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], cs, off));
+                p[i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], by, off));
                 l += p[i / 4][i % 4];
             }
             // value scales: words [token pair][block] of each tile
@@ -912,14 +934,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
             c0 += span;
             if (c0 < t1) begin();
         }
-        l = col_sum(l);
-        m -= A;  // weights were exp2(score - (m - A))
+        // weights were exp2(score - m + A), and m may be too large to take A up
+        const float unit = ldexpf(1.0f, -(int)A);
+        l = col_sum(l) * unit;
 
         // the waves' shares joined in order: O[wave][column][D], m and l [wave][column]
         __syncthreads();
         float *so = reinterpret_cast<float *>(sm) + wave * 16 * D, *sml = reinterpret_cast<float *>(sm + 4 * 16 * D * 4);
 #pragma unroll
-        for (int j = 0; j < ND; j++) *reinterpret_cast<f32x4 *>(so + c * D + 16 * j + 4 * h) = acc[j] * (j % 2 ? 262144.0f : 4194304.0f);
+        for (int j = 0; j < ND; j++) *reinterpret_cast<f32x4 *>(so + c * D + 16 * j + 4 * h) = acc[j] * (unit * (j % 2 ? 262144.0f : 4194304.0f));
         if (h == 0) sml[(wave * 16 + c) * 2] = m, sml[(wave * 16 + c) * 2 + 1] = l;
         __syncthreads();
         for (int i = threadIdx.x; i < 16 * D / 4; i += 256) {
@@ -1165,7 +1188,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
         int e2 = 0;
         (void)frexpf(top, &e2);
         const int a = top > 0.0f && top < INFINITY ? 14 - e2 : 0;  // the row's largest value to 2^13 .. 2^14
-        cs[c] = fmaxf(ldexpf(scale * 1.44269504f, -a), AT_LEAST);
+        cs[c] = score_factor(scale, -a);
 #pragma unroll
         for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -1177,8 +1200,9 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
 
     f32x4 acc[NC][NJ] = {}, sum[NC] = {};
     float m[NC];
+    bool rough[NC];  // as coarse(m) says
 #pragma unroll
-    for (int c = 0; c < NC; c++) m[c] = AT_NONE;
+    for (int c = 0; c < NC; c++) m[c] = AT_NONE, rough[c] = false;
     const f16x8 ones = as_h8(0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u);
     f32x4 s[NC][4];
     f16x8 pf[NC][2];
@@ -1247,13 +1271,19 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
 #pragma unroll
                 for (int j = 0; j < NJ; j++) acc[c][j] *= r;
                 m[c] = m2;
+                rough[c] = coarse(m2);
             }
-            const float off = (float)AT_TOP - m[c];
+            float by = cs[c], off = (float)AT_TOP - m[c];
+            if (rough[c]) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[c][i / 4][i % 4] = s[c][i / 4][i % 4] * cs[c] - m[c];
+                by = 1.0f, off = (float)AT_TOP;
+            }
             uint32_t w[8];
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                w[i] = pack_h2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[c][i / 2][i % 2 * 2], cs[c], off)),
-                               __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][i / 2][i % 2 * 2 + 1], cs[c], off)));
+                w[i] = pack_h2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[c][i / 2][i % 2 * 2], by, off)),
+                               __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][i / 2][i % 2 * 2 + 1], by, off)));
             pf[c][0] = as_h8(w[0], w[1], w[2], w[3]);
             pf[c][1] = as_h8(w[4], w[5], w[6], w[7]);
         }
