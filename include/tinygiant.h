@@ -509,7 +509,9 @@ int tg_attn_q4_dev(const tg_kv_batch *b, int type, const void *q,
  * residual (NULL: none; of out's type, may be out).  The int32 sums are
  * exact.  A row that holds NaN or inf is NaN.  x and out of any element
  * type, rows *_stride elements apart; out overlaps neither x nor w.  w
- * 16-byte aligned, K a multiple of 16 up to 131072.  workspace as above. */
+ * 16-byte aligned, K a multiple of 16 up to 131072, M and N up to 2^30 (and
+ * to what a launch of 2^32 threads takes, 2^24 rows where K is above 512).
+ * workspace as above. */
 size_t tg_matmul_i8_workspace(int M, int N, int K);
 int tg_matmul_i8_dev(const void *x, int x_type, int64_t x_stride,
                      const float *norm_w, float eps, const int8_t *w,

@@ -57,3 +57,19 @@ def test_one_row_for_every_sequence_is_taken_by_the_c_side():
     assert b.table_stride == 0 and lib.tg_kv_read_q4_dev(ctypes.byref(b), P, P, None) == 0
     b.table_stride = 5
     assert lib.tg_kv_read_q4_dev(ctypes.byref(b), P, P, None) == -1 and "5 apart" in lib.tg_last_error().decode()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, (1 << 31) - 1, 16), ((1 << 31) - 1, 1, 16), ((1 << 30) + 1, 16, 16), (7, (1 << 30) + 1, 128),
+                                   (1 << 27, 16, 16), (1 << 24, 16, 1024), (1 << 20, 1 << 21, 64)])
+def test_products_that_no_launch_takes_are_refused(M, N, K):
+    """Before a device is looked for: rows or channels beyond 32-bit indexes, or beyond a launch's threads."""
+    lib = _lib.require_lib()
+    P = 1 << 20
+    assert lib.tg_matmul_i8_workspace(M, N, K) == 0
+    assert lib.tg_matmul_i8_dev(P, 1, K, None, 1e-6, P, P, None, 0, 2 * P, 1, N, M, N, K, P, 1 << 60, None) == -1
+    assert "than a launch takes" in lib.tg_last_error().decode()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1 << 29, 16), ((1 << 26) - 4, 16, 512), ((1 << 24) - 1, 16, 1024), (0, 1 << 30, 16), (1 << 15, 1 << 15, 4096)])
+def test_the_largest_products_are_taken(M, N, K):
+    assert _lib.require_lib().tg_matmul_i8_workspace(M, N, K) >= M * K

@@ -2589,6 +2589,8 @@ extern "C" int tg_attn_q4_dev(const tg_kv_batch *b, int type, const void *q, int
 static int matmul_shape(const char *fn, int M, int N, int K) {
     if (M < 0 || N < 1 || K < 16 || K % 16 || K > 131072)
         return set_err(TG_E_INVALID, "%s: M %d, N %d, K %d (a multiple of 16 up to 131072)", fn, M, N, K);
+    if (!tg::matmul_i8_fits(M, N, K))
+        return set_err(TG_E_INVALID, "%s: M %d, N %d, K %d: more rows or channels than a launch takes", fn, M, N, K);
     return TG_OK;
 }
 

@@ -427,6 +427,7 @@ struct MatmulI8Args {
     int64_t out_stride;
     int M, N, K;
 };
+bool matmul_i8_fits(int M, int N, int K);  // in the threads of a launch, and in 32-bit indexes
 size_t matmul_i8_workspace(int M, int N, int K);
 hipError_t launch_matmul_i8(const MatmulI8Args &a, void *ws, hipStream_t st);
 

@@ -527,7 +527,20 @@ static LinPlan lin_plan(int M, int N, int Kp) {
     if (p.splits == 1 && tiles <= 40) p.few = true;
     return p;
 }
+static int lin_quant_threads(int Kp) { return Kp <= 512 ? 64 : 256; }  // of a row
 static size_t lin_codes(int M, int Kp) { return ((size_t)M * Kp + 4 * (size_t)M + 15) / 16 * 16; }
+
+// A launch has fewer than 2^32 threads.  Rows and channels up to 2^30, so that indexes of tiles that pass the last one
+// stay within 32 bits.
+bool matmul_i8_fits(int M, int N, int K) {
+    if (M > 1 << 30 || N > 1 << 30) return false;
+    const int Kp = lin_kp(K), few_n = M <= 32 && lin_wide_n(N) ? 64 : 16;
+    const LinPlan p = lin_plan(M, N, Kp);
+    const int64_t codes = lin_fused(M, N, Kp) ? 0 : ((int64_t)M * lin_quant_threads(Kp) + 255) / 256;
+    const int64_t tiles = p.big ? 2 * (int64_t)((N + 255) / 256) * ((M + 255) / 256)  // of 512 threads
+                                : (int64_t)((N + 127) / 128) * ((M + 127) / 128) * p.splits;
+    return std::max(codes, p.few ? (int64_t)(N + few_n - 1) / few_n : tiles) * 256 <= UINT32_MAX;
+}
 
 size_t matmul_i8_workspace(int M, int N, int K) {
     const int Kp = lin_kp(K);
@@ -556,7 +569,6 @@ static hipError_t tile_launch(const MatmulI8Args &a, int Kp, const int8_t *xq, c
     const hipError_t e = lin_lds((const void *)k_lin_tile<BN, BM, WN, WM, ST, OT>, bytes, done);
     if (e != hipSuccess) return e;
     const int tn = (a.N + BN - 1) / BN, tm = (a.M + BM - 1) / BM;
-    if ((int64_t)tn * tm > INT32_MAX / 64) return hipErrorInvalidValue;
     TG_LAUNCH((k_lin_tile<BN, BM, WN, WM, ST, OT>), dim3((unsigned)(tn * tm * p.splits)), dim3(64 * WN * WM), bytes, st, a, Kp, xq, xs, tn, tm, p.stages, part);
     return hipSuccess;
 }

@@ -49,6 +49,8 @@ def matmul_i8(x, w, w_scale, *, norm=None, eps: float = RMS_EPS, residual=None, 
     N = w.shape[0]
     if w.shape[1] != K:
         raise ValueError(f"x has {K} columns, w {w.shape[1]}")
+    if max(M, N) > 1 << 30:  # before they become C ints
+        raise ValueError(f"{M} rows, {N} channels: at most 2^30 of either")
     if w_scale.dtype != torch.float32 or w_scale.device != dev or w_scale.shape != (N,) or not w_scale.is_contiguous():
         raise TypeError(f"w_scale must be {N} contiguous float32 values on {dev}")
     if norm is not None and (norm.dtype != torch.float32 or norm.device != dev or norm.shape != (K,)
