@@ -73,3 +73,20 @@ def test_products_that_no_launch_takes_are_refused(M, N, K):
 @pytest.mark.parametrize("M,N,K", [(1, 1 << 29, 16), ((1 << 26) - 4, 16, 512), ((1 << 24) - 1, 16, 1024), (0, 1 << 30, 16), (1 << 15, 1 << 15, 4096)])
 def test_the_largest_products_are_taken(M, N, K):
     assert _lib.require_lib().tg_matmul_i8_workspace(M, N, K) >= M * K
+
+
+def test_gradients_are_refused_where_torch_records_them():
+    """And only there: without them the calls go on, here to the layer that there is not."""
+    kv, b = cache(), batch_over(WIDE[:1])
+    z = lambda *shape: torch.zeros(*shape)
+    attend = dict(q=z(1, 2, 64).half(), out=z(1, 2, 64).half())
+    append = dict(q=z(1, 2, 64), k=z(1, 2, 64), v=z(1, 2, 64), cos=z(9, 32), sin=z(9, 32), q_norm=z(64), k_norm=z(64), out=z(1, 2, 64))
+    for args, name in ((attend, "attend"), (append, "append")):
+        for one in args:
+            leaf = dict(args, **{one: args[one].clone().requires_grad_()})
+            with pytest.raises(RuntimeError, match=f"{name} has no gradients"):
+                getattr(kv, name)(7, batch=b, **leaf)
+            with torch.no_grad(), pytest.raises(ValueError, match="layer 7"):
+                getattr(kv, name)(7, batch=b, **leaf)
+        with pytest.raises(ValueError, match="layer 7"):
+            getattr(kv, name)(7, batch=b, **args)

@@ -238,3 +238,25 @@ def test_equal_scores_of_any_size(D, G, news, scale, sign):
         return np.where(np.arange(500) < n, 1 / n, 0)
     for b in (s.batch, type(s.batch)(s.batch.cu, s.batch.kv_len, s.batch.table, max_len=1)):
         check_weights(s, None, s.kv.attend(0, q, b, scale=scale), weights)
+
+
+# ---------------------------------------------------------------- gradients
+def test_parameters_without_gradients():
+    """Tensors that require gradients are operands as any where torch does not record them, and refused where it does."""
+    from tinygiant_amd.linear import matmul_i8
+    gpu_note("parameters")
+    s = Setup(91, 64, 2, 16, [30], [3])
+    q, qn = s.rows(4, "f16")
+    k, v = s.rows(2, "f16")[0], s.rows(2, "f16")[0]
+    norm = torch.ones(64, device="cuda")
+    w, ws, x = torch.ones(8, 64, dtype=torch.int8, device="cuda"), torch.ones(8, device="cuda"), torch.ones(3, 64, device="cuda")
+    plain = s.kv.append(0, q, k, v, s.batch, q_norm=norm), s.kv.attend(0, q, s.batch), matmul_i8(x, w, ws, norm=norm)
+    p, xp, qp = torch.nn.Parameter(norm), torch.nn.Parameter(x), q.clone().requires_grad_()
+    for call in (lambda: s.kv.append(0, q, k, v, s.batch, q_norm=p), lambda: s.kv.attend(0, qp, s.batch),
+                 lambda: matmul_i8(xp, w, ws), lambda: matmul_i8(x, w, ws, norm=p)):
+        with pytest.raises(RuntimeError, match="no_grad"):
+            call()
+    for off in (torch.no_grad, torch.inference_mode):
+        with off():
+            got = s.kv.append(0, qp, k, v, s.batch, q_norm=p), s.kv.attend(0, qp, s.batch), matmul_i8(xp, w, ws, norm=p)
+        assert all(torch.equal(a, b) and not b.requires_grad for a, b in zip(plain, got))

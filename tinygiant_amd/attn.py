@@ -12,6 +12,8 @@ PagedKV holds the pages of every layer; KVBatch says which rows belong to
 which sequence and which pages hold its tokens.  The projections before and
 after are linear.matmul_i8.  Every step runs in libtinygiant.so's gfx950
 kernels; torch is used only to hold device buffers and name the stream.
+There are no gradients: where torch records them, calls refuse tensors that
+require one.
 
     kv = PagedKV(n_layers=48, n_pages=4096, page_tokens=64, n_kv_heads=4, head_dim=128)
     batch = KVBatch(cu, kv_len, table)             # int32 CUDA tensors
@@ -49,6 +51,17 @@ def run_on(t, name, *args):
     else:
         with torch.cuda.device(index):
             call(name, *args, stream)
+
+
+def records(a, b=None, c=None, d=None) -> bool:
+    """Would torch record gradients through one of these tensors?"""
+    return (a.requires_grad or (b is not None and b.requires_grad) or (c is not None and c.requires_grad)
+            or (d is not None and d.requires_grad)) and torch.is_grad_enabled()
+
+
+def no_gradients(name):
+    """The error of a call that would drop them, as torch's out= does."""
+    return RuntimeError(f"{name} has no gradients and a tensor requires one: call it under torch.no_grad()")
 
 
 def _index(t, name, dims):
@@ -184,6 +197,8 @@ class PagedKV:
         sp = None if sin is None else self._floats(sin, "sin", (max_pos, D // 2))
         qn = None if q_norm is None else self._floats(q_norm, "q_norm", (D,))
         kn = None if k_norm is None else self._floats(k_norm, "k_norm", (D,))
+        if records(k, v, q, out) or records(k, q_norm, k_norm, cos) or (sin is not None and records(sin)):
+            raise no_gradients("append")
         b = self._batch(layer, batch, T)
         if not T or not batch.n_seqs:
             return out
@@ -217,6 +232,8 @@ class PagedKV:
             out, os_ = q.new_empty((T, heads, D)), heads * D
         else:
             os_ = self._rows(out, "out", heads, dt, T)
+        if records(q, out):
+            raise no_gradients("attend")
         b = self._batch(layer, batch, T)
         if not T or not batch.n_seqs:
             return out

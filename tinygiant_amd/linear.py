@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import require_lib
-from .attn import TYPES, run_on
+from .attn import TYPES, no_gradients, records, run_on
 from .moe import RMS_EPS
 
 
@@ -40,7 +40,8 @@ def matmul_i8(x, w, w_scale, *, norm=None, eps: float = RMS_EPS, residual=None, 
     Per row xn = x / rms(x) * norm (norm [K] float32, else xn = x), a =
     max |xn|, codes rint(127 xn / a); the result is the exact int32 product
     times a / 127 and the channel's scale, plus residual (out's type; out may
-    be residual itself)."""
+    be residual itself).  There are no gradients: where torch records them,
+    tensors that require one are refused."""
     xm = _matrix(x, "x", None)
     M, K = xm.shape
     dev = xm.device
@@ -68,6 +69,8 @@ def matmul_i8(x, w, w_scale, *, norm=None, eps: float = RMS_EPS, residual=None, 
             raise TypeError(f"residual is {rm.dtype}, out {om.dtype}")
     if om.shape[0] != M or (rm is not None and rm.shape[0] != M):
         raise ValueError(f"{M} rows of x, {om.shape[0]} of out" + (f", {rm.shape[0]} of residual" if rm is not None else ""))
+    if records(xm, om, rm, norm) or records(w_scale):
+        raise no_gradients("matmul_i8")
     if not M:
         return out
     n = require_lib().tg_matmul_i8_workspace(M, N, K)
