@@ -90,3 +90,13 @@ def test_gradients_are_refused_where_torch_records_them():
                 getattr(kv, name)(7, batch=b, **leaf)
         with pytest.raises(ValueError, match="layer 7"):
             getattr(kv, name)(7, batch=b, **args)
+
+
+def test_one_row_has_no_row_stride():
+    """A row of a tensor of any width: there is no next one, so its stride is never what a call is refused for."""
+    kv = cache()
+    for width in (131, 130, 5 * 64):
+        x = torch.zeros(3, width)[1:2, :128]
+        for t in (x, x.view(1, 2, 64)):
+            assert kv._rows(t, "k", 2, torch.float32, 1) == 128
+    assert kv._rows(torch.zeros(3, 192)[:, :128], "k", 2, torch.float32, 3) == 192

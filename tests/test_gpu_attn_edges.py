@@ -260,3 +260,22 @@ def test_parameters_without_gradients():
         with off():
             got = s.kv.append(0, qp, k, v, s.batch, q_norm=p), s.kv.attend(0, qp, s.batch), matmul_i8(xp, w, ws, norm=p)
         assert all(torch.equal(a, b) and not b.requires_grad for a, b in zip(plain, got))
+
+
+# ---------------------------------------------------------------- one row, hints
+def test_one_row_of_a_tensor_of_odd_width():
+    """Aligned rows whose stride is no multiple of what a kernel loads at a time: with one of them it is not used."""
+    gpu_note("one row")
+    s = Setup(95, 64, 1, 16, [20], [1])
+    buf = torch.zeros(1, 64 * 4 + 3, device="cuda", dtype=torch.float16)
+    x, xn = s.rows(4, "f16")
+    buf[:, :256] = x.view(1, 256)
+    q, k, v = buf[:, :128], buf[:, 128:192], buf[:, 192:256]
+    out = torch.full((1, 131), 3.0, device="cuda", dtype=torch.float16)
+    got = s.kv.append(0, q, k, v, s.batch, out=out[:, :128])
+    assert torch.equal(got, q) and (out[:, 128:] == 3).all()
+    s.cache.put(s.table[0, 1], 0, 3, xn[0, 2], xn[0, 3])
+    assert np.array_equal(s.kv.pages.cpu().numpy()[0], s.cache.pages)
+    s.kv.attend(0, q, s.batch, out=out[:, :128])
+    check_attend(s, q, xn[:, :2], out[:, :128].view(1, 2, 64))
+    assert (out[:, 128:] == 3).all()

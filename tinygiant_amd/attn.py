@@ -155,7 +155,7 @@ class PagedKV:
         if not ok or shape[0] != n_tokens:
             raise ValueError(f"{name} of shape {tuple(shape)}, strides {stride}: "
                              f"[{n_tokens}, {heads}, {D}] with packed heads needed")
-        return max(stride[0], heads * D) if n_tokens == 1 else stride[0]
+        return heads * D if n_tokens == 1 else stride[0]  # of one row the stride is any
 
     def _heads(self, q):
         D = self.head_dim
