@@ -279,3 +279,14 @@ def test_one_row_of_a_tensor_of_odd_width():
     s.kv.attend(0, q, s.batch, out=out[:, :128])
     check_attend(s, q, xn[:, :2], out[:, :128].view(1, 2, 64))
     assert (out[:, 128:] == 3).all()
+
+
+@pytest.mark.parametrize("hint", [(1 << 31) - 1, 1 << 31, (1 << 32) + 1, 10 ** 15])
+def test_hints_beyond_32_bits(hint):
+    from tinygiant_amd.attn import KVBatch
+    gpu_note(f"attend hint {hint}")
+    s = Setup(96, 128, 1, 16, [300, 20], [1, 2])
+    q, qn = s.rows(4, "bf16")
+    whole = s.kv.attend(0, q, KVBatch(s.batch.cu, s.batch.kv_len, s.batch.table))  # 0: what the table holds
+    assert torch.equal(s.kv.attend(0, q, KVBatch(s.batch.cu, s.batch.kv_len, s.batch.table, max_len=hint)), whole)
+    check_attend(s, q, qn, whole)

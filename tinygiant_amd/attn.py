@@ -104,7 +104,7 @@ class KVBatch:
             raise ValueError(f"cu on {cu.device}, kv_len on {kv_len.device}, table on {table.device}")
         if max_len < 0:
             raise ValueError(f"max_len {max_len}")
-        self.cu, self.kv_len, self.table, self.max_len = cu, kv_len, table, int(max_len)
+        self.cu, self.kv_len, self.table, self.max_len = cu, kv_len, table, min(int(max_len), 1 << 30)  # no table holds more
         self.n_seqs, self.device = n, cu.device
 
 
