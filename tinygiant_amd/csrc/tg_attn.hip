@@ -803,8 +803,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
 #pragma unroll
                 for (int i = 1; i < 64; i *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, i));
                 if (top > (below & 0xFFFFu)) {
-                    const int e = min(16, max((int)(top >> 10), 1) - 15 + 2);  // below 2^(e - 1), one bit of room
-                    below = e > 15 ? 0x7BFF7BFFu : e < -13 ? (uint32_t)((1 << (e + 24)) - 1) * 0x10001u : (uint32_t)(((e + 15) << 10) - 1) * 0x10001u;
+                    const int e = min(16, max((int)(top >> 10), 1) - 15 + 2);  // top is below 2^(e - 1): one bit of room; e is -12 or more
+                    below = e > 15 ? 0x7BFF7BFFu : (uint32_t)(((e + 15) << 10) - 1) * 0x10001u;
                     const float r = ldexpf(1.0f, AT_TOP - e - (int)A);
                     A = (float)(AT_TOP - e);
                     l *= r;

@@ -576,12 +576,13 @@ static hipError_t tile_launch(const MatmulI8Args &a, int Kp, const int8_t *xq, c
 template <int MT, int R, int U, int OT>
 static void few_launch(const MatmulI8Args &a, int Kp, const int8_t *xq, const float *xs, hipStream_t st) {
     const dim3 grid((unsigned)((a.N + 16 * R - 1) / (16 * R)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
-    if (MT == 1 && lin_fused(a.M, a.N, Kp)) {
-        if constexpr (MT == 1)
+    if constexpr (MT == 1 && R == 1) {  // the only one that lin_fused's N and M come to
+        if (lin_fused(a.M, a.N, Kp)) {
             TG_BY_TYPE(a.x_type, XT, TG_LAUNCH((k_lin_few<MT, R, U, OT, XT>), grid, dim3(256), (size_t)a.M * Kp, st, a, Kp, xq, xs));
-    } else {
-        TG_LAUNCH((k_lin_few<MT, R, U, OT, -1>), grid, dim3(256), 0, st, a, Kp, xq, xs);
+            return;
+        }
     }
+    TG_LAUNCH((k_lin_few<MT, R, U, OT, -1>), grid, dim3(256), 0, st, a, Kp, xq, xs);
 }
 
 hipError_t launch_matmul_i8(const MatmulI8Args &a, void *ws, hipStream_t st) {
