@@ -102,6 +102,29 @@ def test_a_block_that_is_not_finite_stays_in_the_rows_that_see_it(D, what, facto
         assert torch.isnan(out[before:]).all()
 
 
+@pytest.mark.parametrize("what", ["page", "nan", "inf"])
+@pytest.mark.parametrize("D,G,dt,new", [(64, 4, "f16", 400), (64, 2, "bf16", 400), (128, 4, "f16", 400), (128, 1, "bf16", 700), (256, 2, "bf16", 400)])
+def test_many_rows_before_a_block_that_is_not_finite(D, G, dt, new, what):
+    """The same where rows are many; the row before the first that sees it shares its column tile."""
+    from tinygiant_amd.attn import KVBatch
+    gpu_note(f"attend many rows not finite {D} {G} {dt} {what}")
+    n, bad = 4000, 3850 if what != "page" else 3856
+    s = Setup(160 + D, D, 1, 16, [n], [new])
+    set_scales(s, 0, bad - 1, 256)
+    table = s.table.copy()
+    if what == "page":
+        table[0, bad // 16] = len(s.cache.pages)
+    else:
+        set_scales(s, 0, bad, {"nan": np.nan, "inf": np.inf}[what])
+    s.kv.pages.copy_(dev(s.all))
+    q, qn = s.rows(G, dt)
+    before = bad - (n - new)
+    for hint in (1, 0):
+        out = s.kv.attend(0, q, KVBatch(s.batch.cu, s.batch.kv_len, dev(table), max_len=hint))
+        check_attend(Prefix(s, bad, before), None, qn[:before], out[:before])
+        assert torch.isnan(out[before:]).all()
+
+
 @pytest.mark.parametrize("news", [[1, 1, 1], [1, 90, 1]])
 def test_rows_beside_bad_pages_are_as_exact_as_ever(news):
     """A page outside the pool in one of three sequences: the rows that do not see it, and the other sequences."""
@@ -290,3 +313,15 @@ def test_hints_beyond_32_bits(hint):
     whole = s.kv.attend(0, q, KVBatch(s.batch.cu, s.batch.kv_len, s.batch.table))  # 0: what the table holds
     assert torch.equal(s.kv.attend(0, q, KVBatch(s.batch.cu, s.batch.kv_len, s.batch.table, max_len=hint)), whole)
     check_attend(s, q, qn, whole)
+
+
+@pytest.mark.parametrize("D,G,lens,news,dt", [(128, 8, [2005], [1], "bf16"), (64, 4, [3000, 70], [300, 70], "f16"),
+                                              (256, 2, [2500, 700, 3], [200, 1, 3], "bf16"), (128, 4, [900] * 70, [1] * 70, "f16")])
+def test_the_same_call_gives_the_same_bits(D, G, lens, news, dt):
+    """Splits are joined in an order of their own: no result depends on which block was first."""
+    gpu_note(f"attend twice {D} {G} {dt}")
+    s = Setup(97, D, 2, 16, lens, news)
+    q, _ = s.rows(2 * G, dt)
+    first = s.kv.attend(0, q, s.batch)
+    for _ in range(5):
+        assert torch.equal(s.kv.attend(0, q, s.batch), first)
