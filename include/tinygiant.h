@@ -492,9 +492,12 @@ int tg_kv_read_q4_dev(const tg_kv_batch *b, void *k, void *v, void *stream);
  * finite; n_heads is a multiple of n_kv_heads.  Scores may be as large as
  * fp32 holds (larger ones count as infinite).  Sums are fp32; weights, and the
  * keys and values of many rows, are rounded to fp16 on the way (for fp16 rows
- * keys and values are taken whole).  Scales above 8188, which append never
- * writes, may count as infinite.  max_len: about the longest kv_len (0: table_cols *
- * page_tokens); it sets how the work is split, results hold for any.
+ * keys and values are taken whole).  Whether rows are many is decided for the
+ * call, by n_tokens, n_seqs and max_len, so a row may get the one or the
+ * other; the same call gives the same bits.  Scales above 8188, which append
+ * never writes, may count as infinite.  max_len: about the longest kv_len (0:
+ * table_cols * page_tokens); it sets how the work is split, results hold for
+ * any.
  * workspace: at least tg_attn_q4_workspace bytes, 16-byte aligned, free
  * again when the call's work is done. */
 size_t tg_attn_q4_workspace(const tg_kv_batch *b, int n_heads, int max_len);

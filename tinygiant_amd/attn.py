@@ -175,7 +175,8 @@ class PagedKV:
         one type (float32, float16, bfloat16; views of a projection's rows
         do) are normed (q_norm, k_norm [D]) and rotated (cos, sin [max_pos,
         D / 2]); k and v go into the cache, the rotated q into out (default:
-        a new tensor; may be q itself), which is returned."""
+        a new tensor; may be q itself), which is returned.  Rows behind the
+        last sequence are not written."""
         heads = 0 if q is None else self._heads(q)
         T, dt, D = k.shape[0], k.dtype, self.head_dim
         if dt not in TYPES:
@@ -208,7 +209,7 @@ class PagedKV:
 
     def read(self, layer: int, batch: KVBatch, n_tokens: int):
         """What the cache holds for the batch's rows: k, v [n_tokens,
-        n_kv_heads, D] float16."""
+        n_kv_heads, D] float16 (rows behind the last sequence: not written)."""
         if n_tokens < 0:
             raise ValueError(f"n_tokens {n_tokens}")
         k = torch.empty((n_tokens, self.n_kv_heads, self.head_dim), dtype=torch.float16, device=self.device)
@@ -221,8 +222,8 @@ class PagedKV:
     def attend(self, layer: int, q, batch: KVBatch, scale: float | None = None, out=None):
         """softmax(scale q . k) v for q [T, heads, D] float16 or bfloat16
         (scale: above 0, 1 / sqrt(D) by default), each row over the positions up to
-        its own; rows at positions below 0 are zero.  out: default a new
-        tensor; must not overlap q."""
+        its own; rows at positions below 0 are zero, those behind the last
+        sequence not written.  out: default a new tensor; must not overlap q."""
         heads, D = self._heads(q), self.head_dim
         T, dt = q.shape[0], q.dtype
         if dt not in (torch.float16, torch.bfloat16):

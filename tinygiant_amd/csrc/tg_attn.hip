@@ -330,13 +330,13 @@ __global__ __launch_bounds__(256) void k_kv_read(KvBatch b, _Float16 *k, _Float1
 // exp2(s - m + A) d, one rounding to fp16, once for its two column tiles, and
 // the codes stay the integers they are, again as subnormals; a constant operand of -8
 // takes the codes' offset off within the same step, so no sum grows with it.
-// A = 9 - e where every scale so far is below 2^(e - 1), and m is raised (and the sums rescaled)
-// only where a score passes m + 6: p' stays below 2^14, and next to the largest weight on the largest
-// scale, 2^7 or more, it is a normal fp16 down to 2^-21, the smallest
-// subnormal at 2^-31.  Sums, maxima and outputs are fp32.
+// A = 9 - e where every scale so far is below 2^e (2^(e - 1) when A was set: one bit of room), and m is raised
+// (and the sums rescaled) only where a score passes m + 6: p' stays below 2^15, 2^15.25 with m's own rounding
+// (coarse, below), and next to the largest weight on the largest scale, 2^7 or more when A was set, it is a normal
+// fp16 down to 2^-21, the smallest subnormal at 2^-31.  Sums, maxima and outputs are fp32.
 //
 // A value block that is not finite makes the token's scores NaN and its values 0, so
-// that rows which see the token are NaN and rows which do not are as ever.
+// that rows which see the token are NaN and rows which do not are as ever; its scales do not count for A.
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -434,10 +434,11 @@ TG_DEV T wave_sum(T v) { return __builtin_bit_cast(T, __builtin_amdgcn_readlane(
 
 // How a launch of wide column tiles is cut.  Sequence s has `tiles` of them of
 // `steps` steps of 32 tokens.  A block takes at most `each` steps of one tile, the fewest
-// (from an even share on, an eighth more at a time) with which all the pieces of a key head are
+// (from an even share on, an eighth more at a time, 16 times at the most) with which all the pieces of a key head are
 // `share` blocks or less, so that one round of the device's CUs does them
 // all and the longest block is as short as that allows, and AT_WIDE at the least: what a piece costs
-// beside its steps (its start, 128 KB of partial sums written and read) is as long as 16.
+// beside its steps (its start, 128 KB of partial sums written and read) is as long as 16.  A tile is one piece at the
+// least, so next to `share` short tiles a long one leaves up to share / 6.6 pieces for a second round.
 // Every block works this out for itself from cu and kv_len (a wave's
 // scan), so a launch follows lengths that only the device knows.
 constexpr int AT_WIDE = 32;
@@ -617,9 +618,10 @@ constexpr int AT_PART = COLS * (D + 2);  // floats of one split
 // there (each is used by one wave, so LDS would only add a trip), the scales
 // through a wave's corner of LDS because 16 lanes need the same ones.  The pieces
 // of one column tile are joined by k_attn_join, or written out at once where
-// one is all.  Bound by the vector instructions that unpack codes
-// and weigh scores (40 to 46% of a SIMD's clocks) and by how far the loads run ahead: 64 sequences of up
-// to 8192 tokens, 32 heads of 128 over 4: 40 us, 3.8 TB/s; two of up to 200003, 64 heads over 4: 52 us, 4.4.
+// one is all.  64 sequences of up to 8192 tokens, 32 heads of 128 over 4: 40 us, 3.8 TB/s; two of up to 200003,
+// 64 heads over 4: 52 us, 4.4.  No unit is busy throughout: vector instructions, which unpack codes and weigh scores, take
+// 40 to 46% of a SIMD's clocks, matrix ones 11 to 14%.  What is left is waiting: a step is a chain (scales to LDS and
+// back, matrix, exponents, matrix), and two waves to a SIMD are few to cover it.
 template <int D, bool BF>
 __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_split(KvBatch b, KvRows q, int G, float scale, int share,
                                                                       int unit, FastDiv tpp, AttnOut o) {
@@ -1483,9 +1485,10 @@ hipError_t launch_kv_read(const KvBatch &b, void *k, void *v, hipStream_t st) {
     return hipGetLastError();
 }
 
-// Blocks of one launch.  Narrow column tiles: `share` per key head, or one for each tile.  Wide ones: one
-// for each tile and `share` per key head more for their pieces, of which there are 2 share at most (share,
-// where it is searched for; 5 / 3 share with more than 64 sequences).
+// Blocks of one launch.  Narrow column tiles: `share` per key head, or one for each tile.  Wide ones, of which there are
+// `share` at most: one for each tile and `share` per key head more.  That is enough for their pieces: where an even
+// share is taken as it is there are as many at the most (a piece more than its part of them for each tile), and a
+// larger one makes fewer.  Of split tiles alone there are 2 share pieces at the most, which is what `parts` holds.
 struct AttnPlan {
     int64_t tiles;
     int cols, share, joins, unit;
@@ -1528,7 +1531,8 @@ static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len, bool many,
 // Where that is many, and the rows are so few next to the lengths that not all of more than 8 sequences can be prompts, single
 // tokens may be among them, to which a wide tile is a waste: each kernel takes those that are its.  A prompt of 2000 and 32
 // single tokens after 8192, 32 heads over 4: 133 us, 274 in one launch; after 4000 122 and 147; 8 chunks of 128, where
-// the second launch finds nothing to do: 84 and 79.
+// the second launch finds nothing to do: 84 and 79.  So a row's roundings are those of the kernel that its call's
+// numbers choose, not of the row alone.
 static int attn_plans(const KvBatch &b, int n_heads, int max_len, bool bf16, AttnPlan p[2]) {
     const int64_t all = (int64_t)b.n_tokens * (n_heads / b.n_kv);
     const int few = bf16 ? 128 : 192;

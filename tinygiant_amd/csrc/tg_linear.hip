@@ -231,8 +231,8 @@ TG_DEV float quant_row(const MatmulI8Args &a, int Kp, int row, QuantLds &l, P pu
     return bad ? __builtin_nanf("") : (float)(top / 127.0);
 }
 
-// A launch of its own for the codes, bound by bytes: 8192 x 4096 fp32 with norm 42 us, 4.0 TB/s; 1999 x 4096
-// bf16 11 us, its latency.
+// A launch of its own for the codes: 8192 x 4096 fp32 with norm 42 us, 4.0 TB/s, bound by bytes; 1999 x 4096
+// bf16 11 us, 2.2 TB/s, of which 5 are what 7 rows take too.
 template <int TYPE, int TPR, int NV>
 __global__ __launch_bounds__(256) void k_lin_quant(MatmulI8Args a, int Kp, int8_t *xq, float *xs) {
     __shared__ QuantLds l;
@@ -351,8 +351,9 @@ __global__ __launch_bounds__(256) void k_lin_few(MatmulI8Args a, int Kp, const i
 // stage k in registers, so k's place is loaded with stage k + ST, and stage k
 // + 1 has landed for every wave.
 //
-// Bound by the tiles' bytes from the caches to LDS, 7.5 TB/s over the device: 8192 x 9216 x 4096 in
-// tiles of 256 x 256 310 us, 2.0 POP/s; 1999 x 2048 x 4096 in tiles of 128 x 128 32 us, 1.0.
+// 8192 x 9216 x 4096 in tiles of 256 x 256: 310 us, 2.0 POP/s, matrix units busy 41%, vector instructions 20%; by
+// count, not by a counter, the tiles' bytes come to 2.4 GB, 7.8 TB/s out of the caches.  1999 x 2048 x 4096 in tiles of
+// 128 x 128: 32 us, 1.0; its 256 blocks, one to a CU, are one round, whose start and way out nothing covers.
 //
 // Where the tiles are too few for the device's CUs the columns are split: a block takes `stages` of
 // them and leaves its int32 sums in part [split][row][N in fours] (OT LIN_PART), which
