@@ -771,7 +771,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
         auto work = [&](KvStep<D> &k, int step) {
             const bool edge = step * 32 + 31 > all;  // some column does not see all of it
             // scales to LDS as the tiles hold them; what no column sees is zero
-            uint32_t big = below;
+            uint32_t big = below, vs[SW];  // value scales
 #pragma unroll
             for (int i = 0; i < SW; i++) {
                 const int w = word_of(i), x = tile_of(i);
@@ -787,7 +787,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
                     }
                 }
                 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-                big = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, big), __builtin_bit_cast(u16x2, v & vmask)));
+                vs[i] = v & vmask;
+                big = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, big), __builtin_bit_cast(u16x2, vs[i])));
                 sl[x * (D / 2) + w] = v;
             }
             bool odd = false;
@@ -796,8 +797,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
                 uint32_t top = 0;
 #pragma unroll
                 for (int i = 0; i < SW; i++) {
-                    const uint32_t v = sl[tile_of(i) * (D / 2) + word_of(i)] & vmask;  // as this lane has just put it there
-                    const uint32_t lo = v & 0xFFFFu, hi = v >> 16;
+                    const uint32_t lo = vs[i] & 0xFFFFu, hi = vs[i] >> 16;
                     odd = odd || max(lo, hi) >= 0x7C00u;
                     top = max(top, max(lo < 0x7C00u ? lo : 0u, hi < 0x7C00u ? hi : 0u));
                 }
