@@ -86,9 +86,11 @@ class KVBatch:
     kv_len [n_seqs], table [n_seqs, pages] are int32 CUDA tensors that the
     kernels read at each call, so they may be rewritten in place between
     calls (and graph replays).  table may be a view: columns of a wider one,
-    or one row expanded, whose pages the sequences then share.  Tensors of
-    fewer rows than cu counts are its first rows.  max_len: about the longest kv_len; it only
-    sets how attention's work is split (default: what the table can hold)."""
+    or one row expanded, whose pages the sequences then share (to read: a
+    token's place is one sequence's to append to).  Tensors of fewer rows
+    than cu counts are its first rows.  max_len: about the longest kv_len;
+    it only sets how attention's work is split (default: what the table can
+    hold)."""
 
     def __init__(self, cu, kv_len, table, max_len: int = 0):
         _index(cu, "cu", 1)
