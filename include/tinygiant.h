@@ -505,6 +505,58 @@ int tg_attn_q4_dev(const tg_kv_batch *b, int type, const void *q,
                    int64_t q_stride, int n_heads, float scale, void *out,
                    int64_t out_stride, int max_len, void *workspace,
                    size_t workspace_bytes, void *stream);
+/* Trees of drafted tokens, for steps that let one pass of a model answer
+ * several guesses at what follows (tinygiant/engine.py:317-409 generates one
+ * token a pass).  Node j of sequence s is row cu[s] + j of the batch's rows;
+ * node 0 is the last token that is decided (its entry is not in the cache
+ * yet), parent[row] < j the node that a node follows, -1 none.  parent NULL:
+ * each node follows the one before it (a chain).  A node whose parent is no
+ * node before it, one behind such a node, and nodes from max_nodes on are not
+ * part of the tree. */
+typedef struct {
+    const int32_t *cu;     /* [n_seqs + 1], the batch's */
+    const int32_t *parent; /* [n_tokens] */
+    int32_t n_seqs, n_tokens;
+    int32_t max_nodes;     /* of one sequence, 1 to 1024 */
+} tg_draft_trees;
+/* What each node sees of its tree, bit i of the words bits[row]
+ * [(max_nodes + 31) / 32] being set for itself and the nodes it follows, and
+ * how many of those there are, depth[row].  Rows that are no nodes of a tree:
+ * no bits, depth -1; rows behind the last sequence are not written. */
+int tg_draft_tree_dev(const tg_draft_trees *t, uint32_t *bits, int32_t *depth,
+                      void *stream);
+/* tg_kv_append_q4_dev for nodes: node j goes to the place of the sequence's
+ * j-th new token, rotated by the position of the first one plus depth[row]
+ * (places may be behind max_pos, positions not).  A row of depth below 0 is
+ * not written and its q_out row is NaN. */
+int tg_kv_append_tree_q4_dev(const tg_kv_batch *b, const int32_t *depth,
+                             int type, const void *q, int64_t q_stride,
+                             const void *k, int64_t k_stride, const void *v,
+                             int64_t v_stride, void *q_out,
+                             int64_t q_out_stride, int n_heads,
+                             const float *q_norm, const float *k_norm,
+                             float eps, const float *rope_cos,
+                             const float *rope_sin, int max_pos, void *stream);
+/* tg_attn_q4_dev for nodes: a row sees the tokens before the batch's, and of
+ * the batch's those whose bits are set among its words (1 to 32 a row) up to
+ * itself.  A row whose own bit is clear is NaN.  Everything else, the
+ * workspace too, as there; with the bits of a chain the results are its. */
+int tg_attn_tree_q4_dev(const tg_kv_batch *b, const uint32_t *bits, int words,
+                        int type, const void *q, int64_t q_stride, int n_heads,
+                        float scale, void *out, int64_t out_stride,
+                        int max_len, void *workspace, size_t workspace_bytes,
+                        void *stream);
+/* The cache after a step that kept the nodes path[s][0..count[s]) (rows
+ * path_stride apart): the i-th one's entry is moved, as it is, from its own
+ * place to that of node i, in n_layers layers from pages on, layer_bytes
+ * apart.  path[s][i] is at least i, as a walk from node 0 leaves it; an entry
+ * that is below i or no row of the sequence makes NaN of the token at place i.  kv_len (n_seqs, NULL: none; may be the
+ * batch's own, but overlap it in no other way) gets the sequences' lengths
+ * without the nodes that were not kept.  n_tokens counts for nothing; pages
+ * that a call moves tokens in or out of belong to one sequence. */
+int tg_kv_keep_q4_dev(const tg_kv_batch *b, int n_layers, int64_t layer_bytes,
+                      const int32_t *path, int64_t path_stride, int path_cols,
+                      const int32_t *count, int32_t *kv_len, void *stream);
 /* out [M][N] = x [M][K] times int8 weights w [N][K] (scale w_scale[n] per
  * channel), activations quantised per row on the way: xn = x / rms(x) *
  * norm_w (norm_w K floats, NULL: xn = x; eps), a = max |xn|, q = rint(127 xn /

@@ -102,9 +102,10 @@ class Cache:
         return out
 
 
-def attend(q, k, v, n_new, scale, steps=None):
+def attend(q, k, v, n_new, scale, steps=None, seen=None):
     """q [n_new, heads, D], the last rows of a sequence with k, v [n_kv, n,
-    D]: row i sees positions 0 .. n - n_new + i.  Returns in float64 out
+    D]: row i sees positions 0 .. n - n_new + i, and of the last n_new of them
+    (seen [n_new, n_new], for draft trees) those that seen[i] says.  Returns in float64 out
     [n_new, heads, D], sum p |v| of the same shape, and the largest scale *
     sum |q_i k_i| that each row sees [n_new, heads, 1] (for error bounds).
     steps (the scales of k's and v's blocks): two more for bounds, sum p
@@ -116,6 +117,8 @@ def attend(q, k, v, n_new, scale, steps=None):
     out, size, vstep = np.zeros((3, n_new, heads, D))
     top, kstep = np.zeros((2, n_new, heads, 1))
     hide = np.arange(n)[None, :] > np.arange(n - n_new, n)[:, None]
+    if seen is not None:
+        hide[:, max(0, n - n_new):] |= ~seen[:, max(0, n_new - n):]
     blind = hide.all(axis=1) if n else np.ones(n_new, bool)
     for h in range(heads if n else 0):
         x = q[:, h].astype(np.float64)

@@ -171,14 +171,21 @@ class PagedKV:
             raise TypeError(f"{name} must be a contiguous float32 tensor of shape {shape} on {self.device}")
         return t.data_ptr()
 
+    def _tree(self, tree, batch, n_tokens):
+        if tree.device != self.device or tree.n_seqs != batch.n_seqs or n_tokens > tree.n_tokens:
+            raise ValueError(f"tree of {tree.n_seqs} sequences and {tree.n_tokens} rows on {tree.device}: "
+                             f"{batch.n_seqs} and {n_tokens} on {self.device} needed")
+
     def append(self, layer: int, q, k, v, batch: KVBatch, cos=None, sin=None, q_norm=None, k_norm=None,
-               eps: float = RMS_EPS, out=None):
+               eps: float = RMS_EPS, out=None, tree=None):
         """New rows: q [T, heads, D] (or None), k and v [T, n_kv_heads, D] of
         one type (float32, float16, bfloat16; views of a projection's rows
         do) are normed (q_norm, k_norm [D]) and rotated (cos, sin [max_pos,
         D / 2]); k and v go into the cache, the rotated q into out (default:
         a new tensor; may be q itself), which is returned.  Rows behind the
-        last sequence are not written."""
+        last sequence are not written.  tree (draft.DraftTree): the rows are
+        nodes of draft trees, each at its own place in the cache but rotated by
+        the position of its tree's first node plus its depth."""
         heads = 0 if q is None else self._heads(q)
         T, dt, D = k.shape[0], k.dtype, self.head_dim
         if dt not in TYPES:
@@ -202,11 +209,16 @@ class PagedKV:
         kn = None if k_norm is None else self._floats(k_norm, "k_norm", (D,))
         if records(k, v, q, out) or records(k, q_norm, k_norm, cos) or (sin is not None and records(sin)):
             raise no_gradients("append")
+        if tree is not None:
+            self._tree(tree, batch, T)
         b = self._batch(layer, batch, T)
         if not T or not batch.n_seqs:
             return out
-        run_on(k, "tg_kv_append_q4_dev", ctypes.byref(b), TYPES[dt], qp, qs or 0, k.data_ptr(), ks, v.data_ptr(), vs,
-               op, os_ or 0, heads, qn, kn, float(eps), cp, sp, max_pos)
+        args = (TYPES[dt], qp, qs or 0, k.data_ptr(), ks, v.data_ptr(), vs, op, os_ or 0, heads, qn, kn, float(eps), cp, sp, max_pos)
+        if tree is None:
+            run_on(k, "tg_kv_append_q4_dev", ctypes.byref(b), *args)
+        else:
+            run_on(k, "tg_kv_append_tree_q4_dev", ctypes.byref(b), tree.depth.data_ptr(), *args)
         return out
 
     def read(self, layer: int, batch: KVBatch, n_tokens: int):
@@ -221,11 +233,13 @@ class PagedKV:
             run_on(k, "tg_kv_read_q4_dev", ctypes.byref(b), k.data_ptr(), v.data_ptr())
         return k, v
 
-    def attend(self, layer: int, q, batch: KVBatch, scale: float | None = None, out=None):
+    def attend(self, layer: int, q, batch: KVBatch, scale: float | None = None, out=None, tree=None):
         """softmax(scale q . k) v for q [T, heads, D] float16 or bfloat16
         (scale: above 0, 1 / sqrt(D) by default), each row over the positions up to
         its own; rows at positions below 0 are zero, those behind the last
-        sequence not written.  out: default a new tensor; must not overlap q."""
+        sequence not written.  out: default a new tensor; must not overlap q.
+        tree (draft.DraftTree): the rows are nodes of draft trees, and of the
+        batch's own tokens each sees itself and the nodes it follows."""
         heads, D = self._heads(q), self.head_dim
         T, dt = q.shape[0], q.dtype
         if dt not in (torch.float16, torch.bfloat16):
@@ -237,13 +251,55 @@ class PagedKV:
             os_ = self._rows(out, "out", heads, dt, T)
         if records(q, out):
             raise no_gradients("attend")
+        if tree is not None:
+            self._tree(tree, batch, T)
         b = self._batch(layer, batch, T)
         if not T or not batch.n_seqs:
             return out
         ref = ctypes.byref(b)
         n = require_lib().tg_attn_q4_workspace(ref, heads, batch.max_len)
         ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        run_on(q, "tg_attn_q4_dev", ref, TYPES[dt], q.data_ptr(), qs, heads,
-               D ** -0.5 if scale is None else float(scale), out.data_ptr(), os_, batch.max_len,
-               ws.data_ptr() if n else None, n)
+        args = (TYPES[dt], q.data_ptr(), qs, heads, D ** -0.5 if scale is None else float(scale), out.data_ptr(), os_,
+                batch.max_len, ws.data_ptr() if n else None, n)
+        if tree is None:
+            run_on(q, "tg_attn_q4_dev", ref, *args)
+        else:
+            run_on(q, "tg_attn_tree_q4_dev", ref, tree.bits.data_ptr(), tree.words, *args)
         return out
+
+    def keep(self, batch: KVBatch, path, count, kv_len=None, layer: int = 0, n_layers: int | None = None):
+        """After a step over draft trees: of each sequence s, whose nodes are the
+        batch's rows, the entries of the nodes path[s, :count[s]] (int32
+        [n_seqs, any], as draft.verify gives them) become those of its first
+        new tokens, in the layers from layer on (n_layers; default: all that
+        follow).  path[s, i] is at least i; an entry that is not, or is no row
+        of the sequence, makes NaN of the token at its place.  kv_len (int32
+        [n_seqs], may be the batch's own) then gets the lengths without the
+        nodes that were not kept, and is returned.  The pages that a sequence's
+        last tokens are in are its alone."""
+        n_layers = self.n_layers - layer if n_layers is None else n_layers
+        if layer < 0 or n_layers < 0 or layer + n_layers > self.n_layers:
+            raise ValueError(f"layers {layer} to {layer + n_layers} of {self.n_layers}")
+        _index(path, "path", 2)
+        _index(count, "count", 1)
+        n, cols = batch.n_seqs, path.shape[1]
+        if not path.device == count.device == batch.device == self.device:
+            raise ValueError(f"path on {path.device}, count on {count.device}, batch on {batch.device}, pages on {self.device}")
+        if path.shape[0] != n or count.numel() != n or not cols:
+            raise ValueError(f"{n} sequences, {count.numel()} counts, path of shape {tuple(path.shape)}")
+        if path.stride(1) != 1 or not count.is_contiguous():
+            raise TypeError("count and the rows of path must be contiguous")
+        stride = max(path.stride(0), cols) if n == 1 else path.stride(0)
+        if kv_len is not None:
+            _index(kv_len, "kv_len", 1)
+            if kv_len.device != self.device or kv_len.numel() != n or not kv_len.is_contiguous():
+                raise ValueError(f"kv_len must be {n} contiguous lengths on {self.device}")
+            at = kv_len.data_ptr()
+            for t, size in ((batch.kv_len, n), (batch.cu, n + 1), (count, n), (path, (n - 1) * stride + cols)):
+                if t.data_ptr() < at + 4 * n and at < t.data_ptr() + 4 * size and not (t is batch.kv_len and at == t.data_ptr()):
+                    raise ValueError("kv_len overlaps what the call reads")
+        if n:
+            b = self._batch(min(layer, self.n_layers - 1), batch, 0)
+            run_on(path, "tg_kv_keep_q4_dev", ctypes.byref(b), n_layers, self.layer_bytes, path.data_ptr(), stride, cols,
+                   count.data_ptr(), None if kv_len is None else kv_len.data_ptr())
+        return kv_len

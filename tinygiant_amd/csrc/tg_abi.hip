@@ -2498,12 +2498,10 @@ static int kv_rows(const char *fn, const char *name, const void *p, int64_t stri
     return TG_OK;
 }
 
-extern "C" int tg_kv_append_q4_dev(const tg_kv_batch *b, int type, const void *q, int64_t q_stride, const void *k,
-                                   int64_t k_stride, const void *v, int64_t v_stride, void *q_out,
-                                   int64_t q_out_stride, int n_heads, const float *q_norm, const float *k_norm,
-                                   float eps, const float *rope_cos, const float *rope_sin, int max_pos,
-                                   void *stream) {
-    const char *fn = "tg_kv_append_q4_dev";
+static int kv_append(const char *fn, const tg_kv_batch *b, const int32_t *depth, int type, const void *q,
+                     int64_t q_stride, const void *k, int64_t k_stride, const void *v, int64_t v_stride, void *q_out,
+                     int64_t q_out_stride, int n_heads, const float *q_norm, const float *k_norm, float eps,
+                     const float *rope_cos, const float *rope_sin, int max_pos, void *stream) {
     tg::KvBatch kb;
     int rc = kv_batch(fn, b, &kb);
     if (rc) return rc;
@@ -2524,8 +2522,53 @@ extern "C" int tg_kv_append_q4_dev(const tg_kv_batch *b, int type, const void *q
     DeviceOf dev(as_stream(stream));
     if (dev.rc) return dev.rc;
     const tg::AppendArgs a{{q, q_stride}, {k, k_stride}, {v, v_stride}, q_out, q_out_stride, n_heads, q_norm, k_norm,
-                           eps, rope_cos, rope_sin, rope_cos ? max_pos : INT32_MAX};
+                           eps, rope_cos, rope_sin, rope_cos ? max_pos : INT32_MAX, depth};
     PROFILED("kv_append", as_stream(stream), tg::launch_kv_append(kb, type, a, as_stream(stream)));
+    return TG_OK;
+}
+
+extern "C" int tg_kv_append_q4_dev(const tg_kv_batch *b, int type, const void *q, int64_t q_stride, const void *k,
+                                   int64_t k_stride, const void *v, int64_t v_stride, void *q_out,
+                                   int64_t q_out_stride, int n_heads, const float *q_norm, const float *k_norm,
+                                   float eps, const float *rope_cos, const float *rope_sin, int max_pos,
+                                   void *stream) {
+    return kv_append("tg_kv_append_q4_dev", b, nullptr, type, q, q_stride, k, k_stride, v, v_stride, q_out,
+                     q_out_stride, n_heads, q_norm, k_norm, eps, rope_cos, rope_sin, max_pos, stream);
+}
+
+extern "C" int tg_kv_append_tree_q4_dev(const tg_kv_batch *b, const int32_t *depth, int type, const void *q,
+                                        int64_t q_stride, const void *k, int64_t k_stride, const void *v,
+                                        int64_t v_stride, void *q_out, int64_t q_out_stride, int n_heads,
+                                        const float *q_norm, const float *k_norm, float eps, const float *rope_cos,
+                                        const float *rope_sin, int max_pos, void *stream) {
+    const char *fn = "tg_kv_append_tree_q4_dev";
+    if (!depth) return set_err(TG_E_INVALID, "%s: depth is NULL", fn);
+    return kv_append(fn, b, depth, type, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, n_heads, q_norm,
+                     k_norm, eps, rope_cos, rope_sin, max_pos, stream);
+}
+
+extern "C" int tg_kv_keep_q4_dev(const tg_kv_batch *b, int n_layers, int64_t layer_bytes, const int32_t *path,
+                                 int64_t path_stride, int path_cols, const int32_t *count, int32_t *kv_len,
+                                 void *stream) {
+    const char *fn = "tg_kv_keep_q4_dev";
+    tg::KvBatch kb;
+    int rc = kv_batch(fn, b, &kb);
+    if (rc) return rc;
+    const int64_t layer = kb.n_pages * kb.n_kv * (kb.page_tokens / 16) * 18 * kb.D;
+    if (n_layers < 0 || n_layers > 65536 || (n_layers > 1 && layer_bytes < layer) || layer_bytes % 16)
+        return set_err(TG_E_INVALID, "%s: %d layers %lld bytes apart, of %lld bytes each", fn, n_layers,
+                       (long long)layer_bytes, (long long)layer);
+    if (!path || !count) return set_err(TG_E_INVALID, "%s: path or count is NULL", fn);
+    if (path_cols < 1 || path_stride < path_cols)
+        return set_err(TG_E_INVALID, "%s: path of %d columns, rows %lld apart", fn, path_cols, (long long)path_stride);
+    if ((int64_t)kb.n_seqs * kb.n_kv * n_layers > 4ll * (UINT32_MAX / 256))
+        return set_err(TG_E_INVALID, "%s: %d sequences, %d heads and %d layers: more than a launch takes", fn,
+                       kb.n_seqs, kb.n_kv, n_layers);
+    if (!kb.n_seqs) return TG_OK;
+    DeviceOf dev(as_stream(stream));
+    if (dev.rc) return dev.rc;
+    const tg::KeepArgs a{path, count, path_stride, layer_bytes, path_cols, n_layers, kv_len};
+    PROFILED("kv_keep", as_stream(stream), tg::launch_kv_keep(kb, a, as_stream(stream)));
     return TG_OK;
 }
 
@@ -2561,13 +2604,13 @@ extern "C" size_t tg_attn_q4_workspace(const tg_kv_batch *b, int n_heads, int ma
     return tg::attn_workspace(kb, n_heads, max_len);
 }
 
-extern "C" int tg_attn_q4_dev(const tg_kv_batch *b, int type, const void *q, int64_t q_stride, int n_heads, float scale,
-                              void *out, int64_t out_stride, int max_len, void *workspace, size_t workspace_bytes,
-                              void *stream) {
-    const char *fn = "tg_attn_q4_dev";
+static int attn(const char *fn, const tg_kv_batch *b, const uint32_t *bits, int words, int type, const void *q,
+                int64_t q_stride, int n_heads, float scale, void *out, int64_t out_stride, int max_len,
+                void *workspace, size_t workspace_bytes, void *stream) {
     tg::KvBatch kb;
     int rc = attn_args(fn, b, n_heads, &max_len, &kb);
     if (rc) return rc;
+    kb.bits = bits, kb.words = words;
     if (type != TG_T_F16 && type != TG_T_BF16)
         return set_err(TG_E_INVALID, "%s: element type %d is not fp16 or bf16", fn, type);
     if ((rc = kv_rows(fn, "q", q, q_stride, n_heads, kb.D, type, 8))) return rc;
@@ -2583,6 +2626,48 @@ extern "C" int tg_attn_q4_dev(const tg_kv_batch *b, int type, const void *q, int
     if (dev.rc) return dev.rc;
     PROFILED("attn", as_stream(stream), tg::launch_attn(kb, type, {q, q_stride}, n_heads, scale, out, out_stride,
                                                         max_len, workspace, as_stream(stream)));
+    return TG_OK;
+}
+
+extern "C" int tg_attn_q4_dev(const tg_kv_batch *b, int type, const void *q, int64_t q_stride, int n_heads, float scale,
+                              void *out, int64_t out_stride, int max_len, void *workspace, size_t workspace_bytes,
+                              void *stream) {
+    return attn("tg_attn_q4_dev", b, nullptr, 0, type, q, q_stride, n_heads, scale, out, out_stride, max_len, workspace,
+                workspace_bytes, stream);
+}
+
+extern "C" int tg_attn_tree_q4_dev(const tg_kv_batch *b, const uint32_t *bits, int words, int type, const void *q,
+                                   int64_t q_stride, int n_heads, float scale, void *out, int64_t out_stride,
+                                   int max_len, void *workspace, size_t workspace_bytes, void *stream) {
+    const char *fn = "tg_attn_tree_q4_dev";
+    if (!bits) return set_err(TG_E_INVALID, "%s: bits is NULL", fn);
+    if (words < 1 || words > 32) return set_err(TG_E_INVALID, "%s: %d words a row, at most 32", fn, words);
+    return attn(fn, b, bits, words, type, q, q_stride, n_heads, scale, out, out_stride, max_len, workspace,
+                workspace_bytes, stream);
+}
+
+// ---------------------------------------------------------- drafted tokens
+static int draft_trees(const char *fn, const tg_draft_trees *t, tg::DraftTrees *d) {
+    if (!t) return set_err(TG_E_INVALID, "%s: trees is NULL", fn);
+    if (t->n_seqs < 0 || t->n_tokens < 0 || (int64_t)t->n_seqs > UINT32_MAX / 256)
+        return set_err(TG_E_INVALID, "%s: n_seqs %d, n_tokens %d", fn, t->n_seqs, t->n_tokens);
+    if (t->max_nodes < 1 || t->max_nodes > 1024)
+        return set_err(TG_E_INVALID, "%s: max_nodes %d is not 1 to 1024", fn, t->max_nodes);
+    if (!t->cu) return set_err(TG_E_INVALID, "%s: cu is NULL", fn);
+    *d = tg::DraftTrees{t->cu, t->parent, t->n_seqs, t->n_tokens, t->max_nodes};
+    return TG_OK;
+}
+
+extern "C" int tg_draft_tree_dev(const tg_draft_trees *t, uint32_t *bits, int32_t *depth, void *stream) {
+    const char *fn = "tg_draft_tree_dev";
+    tg::DraftTrees d;
+    int rc = draft_trees(fn, t, &d);
+    if (rc) return rc;
+    if (!bits || !depth) return set_err(TG_E_INVALID, "%s: bits or depth is NULL", fn);
+    if (!d.n_seqs || !d.n_tokens) return TG_OK;
+    DeviceOf dev(as_stream(stream));
+    if (dev.rc) return dev.rc;
+    PROFILED("draft_tree", as_stream(stream), tg::launch_draft_tree(d, bits, depth, as_stream(stream)));
     return TG_OK;
 }
 

@@ -48,6 +48,9 @@ TG_DEV int page_of(const KvBatch &b, int s, int p) {
     return page >= 0 && page < b.n_pages ? page : -1;
 }
 
+// a value that is the same in every lane, told to the compiler
+TG_DEV int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // The sequence of row t: the number of j with cu[j + 1] <= t, counted by L
 // neighbouring lanes (li: lane among them); n_seqs for padding rows.
 template <int L>
@@ -147,11 +150,16 @@ __global__ __launch_bounds__(256) void k_kv_append(KvBatch b, AppendArgs a) {
 
     const int s = seq_of<L>(b, t, li);
     const bool row = live && s < b.n_seqs;
-    int pos = -1, page = -1;
+    int pos = -1, page = -1, turn = -1;  // place, its page, the position that it is rotated by
     if (row) {
         const SeqRows r = seq_rows(b, s);
-        pos = r.len - r.hi + t;
-        if (pos >= a.max_pos) pos = -1;
+        pos = turn = r.len - r.hi + t;
+        // a node of a draft tree has its own place but stands as many steps behind the sequence as it is deep
+        if (a.depth) {
+            const int depth = a.depth[t];
+            turn = depth < 0 ? -1 : r.len - r.hi + r.lo + depth;
+        }
+        if (turn < 0 || turn >= a.max_pos) pos = -1;
         page = page_of(b, s, pos);
     }
 
@@ -173,8 +181,8 @@ __global__ __launch_bounds__(256) void k_kv_append(KvBatch b, AppendArgs a) {
         }
     }
     if (!is_v && a.cos && pos >= 0) {
-        const f32x4 c = *reinterpret_cast<const f32x4 *>(a.cos + (size_t)pos * (D / 2) + 4 * li);
-        const f32x4 sn = *reinterpret_cast<const f32x4 *>(a.sin + (size_t)pos * (D / 2) + 4 * li);
+        const f32x4 c = *reinterpret_cast<const f32x4 *>(a.cos + (size_t)turn * (D / 2) + 4 * li);
+        const f32x4 sn = *reinterpret_cast<const f32x4 *>(a.sin + (size_t)turn * (D / 2) + 4 * li);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const float x = lo[e] * c[e] - hi[e] * sn[e], y = hi[e] * c[e] + lo[e] * sn[e];
@@ -304,6 +312,68 @@ __global__ __launch_bounds__(256) void k_kv_read(KvBatch b, _Float16 *k, _Float1
     *reinterpret_cast<f16x8 *>(v + o) = vv;
 }
 
+// ================================================================ keep
+// The token that a walk through a draft tree kept as its i-th to place i of the tree, codes and scales as they are.  A
+// wave has one key head of one sequence and layer and goes through the places in order: entry i comes from path[i] >= i,
+// so no place is written before what it held is read.
+//
+// Bound by latency: cu and kv_len, path and count, the table, and the entries themselves, one after the other.
+template <int D>
+__global__ __launch_bounds__(256) void k_kv_keep(KvBatch b, KeepArgs a) {
+    constexpr int NG = D / 32, KW = D / 8, VH = D / 4, ITEMS = KW + VH + 2 * NG;  // K words, V halfwords, scales of a token
+    constexpr int PER = (ITEMS + 63) / 64;
+    const int lane = threadIdx.x % 64;
+    const uint32_t unit = blockIdx.x * 4 + uni(threadIdx.x / 64), pair = unit / b.n_kv;  // below 2^26, as the launch checks
+    const int hk = unit - pair * b.n_kv, layer = pair / b.n_seqs, s = pair - layer * b.n_seqs;
+    if (layer >= a.n_layers) return;
+    const int lo = max(b.cu[s], 0), n = max(b.cu[s + 1], lo) - lo, base = max(b.kv_len[s], 0) - n;
+    const int count = min(max(a.count[s], 0), min(n, a.path_cols));
+    uint8_t *pages = b.pages + layer * a.layer_bytes;
+    // bytes of this lane's items in token r's tile: V's as halfwords, K's as words
+    auto at = [&](int item, int r) {
+        if (item < KW) return ((item / NG * 16 + r) * NG + item % NG) * 4;
+        item -= KW;
+        if (item < VH) return 8 * D + ((((r / 4) * 16 + item / (NG / 2)) * 2 + r % 4 / 2) * NG + 2 * (item % (NG / 2)) + r % 2) * 2;
+        item -= VH;
+        if (item < NG) return 16 * D + (r * NG + item) * 2;
+        return 17 * D + ((r / 2 * NG + item - NG) * 2 + r % 2) * 2;
+    };
+    for (int i0 = 0; i0 < count; i0 += 64) {
+        // lane i finds entry i0 + i's places
+        const int i = i0 + lane, from = i < count ? a.path[(int64_t)s * a.path_stride + i] : i;
+        const int to_page = i < count && from != i ? page_of(b, s, base + i) : -1;
+        const int from_page = to_page >= 0 && from > i && from < n ? page_of(b, s, base + from) : -1;
+        for (uint64_t todo = __ballot(to_page >= 0); todo; todo &= todo - 1) {
+            const int e = __builtin_ctzll(todo);
+            const int tp = __builtin_amdgcn_readlane(to_page, e), fp = __builtin_amdgcn_readlane(from_page, e);
+            const int t = base + i0 + e, f = base + __builtin_amdgcn_readlane(from, e);
+            uint8_t *tt = pages + tile_at<D>(b, tp, hk, t % b.page_tokens / 16);
+            const uint8_t *ft = fp < 0 ? tt : pages + tile_at<D>(b, fp, hk, f % b.page_tokens / 16);
+#pragma unroll
+            for (int k = 0; k < PER; k++) {
+                const int item = lane + 64 * k;
+                if (item >= ITEMS) break;
+                const int to = at(item, t % 16), fr = at(item, (fp < 0 ? t : f) % 16);
+                if (item < KW) {
+                    *reinterpret_cast<uint32_t *>(tt + to) = *reinterpret_cast<const uint32_t *>(ft + fr);
+                } else {
+                    // an entry that is none: NaN for scales
+                    const uint16_t v = *reinterpret_cast<const uint16_t *>(ft + fr);
+                    *reinterpret_cast<uint16_t *>(tt + to) = fp < 0 && item >= KW + VH ? (uint16_t)0x7E00 : v;
+                }
+            }
+        }
+    }
+}
+
+// The lengths by themselves: they may stand where the ones before do.
+__global__ __launch_bounds__(256) void k_kv_keep_len(KvBatch b, KeepArgs a) {
+    const int s = blockIdx.x * 256 + threadIdx.x;
+    if (s >= b.n_seqs) return;
+    const int lo = max(b.cu[s], 0), n = max(b.cu[s + 1], lo) - lo;
+    a.kv_len[s] = max(max(b.kv_len[s], 0) - n + min(max(a.count[s], 0), min(n, a.path_cols)), 0);
+}
+
 // ================================================================ attention
 // Columns.  A sequence's rows and the G query heads of one key head are laid
 // out as columns f = row * G + head, 16 of which make a column tile, the
@@ -360,9 +430,6 @@ TG_DEV uint32_t pack_h2(float a, float b) {
     const f32x2 v = {a, b};
     return as_u(__builtin_convertvector(v, f16x2));
 }
-
-// a value that is the same in every lane, told to the compiler
-TG_DEV int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // The maximum of v over the four lanes that share a column (lane % 16)
 TG_DEV float col_max(float v) {
@@ -572,6 +639,22 @@ TG_DEV int tokens_seen(const KvBatch &b, const T &ct, int i) {
     return max(0, min(ct.len - ct.n + i + 1, b.table_cols * b.page_tokens + 1));
 }
 
+// Draft trees.  Behind the tokens that all rows of a sequence see, row i sees token base + j where bit j of its words
+// is set.  tree_window: those of 32 tokens from token base + j on (j may be below 0: those before the tree are seen).
+TG_DEV uint32_t tree_word(const uint32_t *bits, int words, int w) {
+    const uint32_t v = bits[min(max(w, 0), words - 1)];
+    return w < 0 ? ~0u : w < words ? v : 0u;
+}
+TG_DEV uint32_t tree_window(const uint32_t *bits, int words, int j) {
+    const int w = j >> 5;
+    return __builtin_amdgcn_alignbit(tree_word(bits, words, w + 1), tree_word(bits, words, w), j & 31);
+}
+// A token that a row of a tree does not see; the row's own place, where its own bit is clear, says that it is no node of
+// the tree, and makes NaN of it.
+TG_DEV float tree_hides(float s, bool seen, int t, int pos) {
+    return t > pos ? -INFINITY : seen ? s : t == pos ? __builtin_nanf("") : -INFINITY;
+}
+
 // One step of 32 tokens of one key head as a lane holds it: tiles x = 0, 1
 template <int D>
 struct KvStep {
@@ -622,7 +705,7 @@ constexpr int AT_PART = COLS * (D + 2);  // floats of one split
 // 64 heads over 4: 52 us, 4.4.  No unit is busy throughout: vector instructions, which unpack codes and weigh scores, take
 // 40 to 46% of a SIMD's clocks, matrix ones 11 to 14%.  What is left is waiting: a step is a chain (scales to LDS and
 // back, matrix, exponents, matrix), and two waves to a SIMD are few to cover it.
-template <int D, bool BF>
+template <int D, bool BF, bool TREE>
 __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_split(KvBatch b, KvRows q, int G, float scale, int share,
                                                                       int unit, FastDiv tpp, AttnOut o) {
     constexpr int NG = D / 32, ND = D / 16, SW = D / 64;
@@ -651,7 +734,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
         const bool col = f < ct.n * G;
         const int row = ct.lo + (col ? f / G : 0), head = hk * G + (col ? f % G : 0);
         const int pos = col ? ct.len - ct.n + f / G : -1;
-        const int seen = uni(tokens_seen(b, ct, last / G)), all = uni(ct.len - ct.n + (ct.tile * 16) / G);  // first column's position
+        // what every column sees ends at the first one's position, of trees before their first node
+        const int seen = uni(tokens_seen(b, ct, last / G)), all = uni(ct.len - ct.n + (TREE ? -1 : (ct.tile * 16) / G));
         const bool first = ct.at <= over;
         const int t0 = first ? 0 : (int)(ct.at - over) * cut.unit * 32;
         const int t1 = end == ct.units ? seen : min(seen, (int)(end - over) * cut.unit * 32);
@@ -863,11 +947,20 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
                 wave_lds_sync();
             }
             if (edge) {
+                if (TREE) {
+                    const uint32_t w = tree_window(b.bits + (size_t)row * b.words, b.words, step * 32 - all - 1) >> 4 * h;
 #pragma unroll
-                for (int x = 0; x < 2; x++)
+                    for (int x = 0; x < 2; x++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (step * 32 + 16 * x + 4 * h + i > pos) s[x][i] = -INFINITY;
+                        for (int i = 0; i < 4; i++)
+                            s[x][i] = tree_hides(s[x][i], w >> (16 * x + i) & 1, step * 32 + 16 * x + 4 * h + i, pos);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (step * 32 + 16 * x + 4 * h + i > pos) s[x][i] = -INFINITY;
+                }
             }
             // cs > 0, so the largest s is the largest score
             float top = s[0][0];
@@ -1018,7 +1111,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
 template <int D>
 constexpr int AT_COLS = D == 256 ? 128 : 256;
 
-template <int D, bool BF>
+template <int D, bool BF, bool TREE>
 __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G, float scale, int share, FastDiv tpp, AttnOut o) {
     constexpr int NG = D / 32, ND = D / 16, NC = 2, COLS = AT_COLS<D>, BUF = 64 * D * 2;  // keys or values of a step
     constexpr int DW = COLS * D / 256, NJ = DW / 16;  // dims of the output that are a wave's
@@ -1052,7 +1145,8 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
 #pragma unroll
         for (int g = 0; g < NG; g++) load_words<4>(qp + 32 * g + 8 * h, qw[c][g]);
     }
-    const int first = uni(ct.len - ct.n + min(f0, last) / G);  // position of the wave's first column
+    // position of the wave's first column; of trees the one before their first node
+    const int first = uni(ct.len - ct.n + (TREE ? -1 : min(f0, last) / G));
 
     // this wave's share of a step: the keys (even) or values (odd) of its tile wave / 2
     const int ntile = (int)tpp.d, span = min(ct.per, 63 * 16 * ntile & ~63);
@@ -1253,7 +1347,22 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
     };
     auto vector = [&](int step) __attribute__((always_inline)) {
         const int t = t0 + 64 * step;
-        if (t + 63 > first) {
+        if (TREE && t + 63 > first) {
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const int f = f0 + 16 * c + c16;
+                const uint32_t *bits = b.bits + (size_t)(ct.lo + (f < ncol ? f / G : 0)) * b.words;
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    const uint32_t w = tree_window(bits, b.words, t + 32 * y - first - 1) >> 4 * h;
+#pragma unroll
+                    for (int x = 2 * y; x < 2 * y + 2; x++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            s[c][x][i] = tree_hides(s[c][x][i], w >> (16 * (x % 2) + i) & 1, t + 16 * x + 4 * h + i, pos[c]);
+                }
+            }
+        } else if (!TREE && t + 63 > first) {
 #pragma unroll
             for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -1485,6 +1594,14 @@ hipError_t launch_kv_read(const KvBatch &b, void *k, void *v, hipStream_t st) {
     return hipGetLastError();
 }
 
+hipError_t launch_kv_keep(const KvBatch &b, const KeepArgs &a, hipStream_t st) {
+    const int64_t grid = ((int64_t)b.n_seqs * b.n_kv * a.n_layers + 3) / 4;
+    if (grid > UINT32_MAX / 256) return hipErrorInvalidValue;
+    if (a.n_layers) TG_BY_DIM(b.D, TG_LAUNCH(k_kv_keep<DIM>, dim3((unsigned)grid), dim3(256), 0, st, b, a));
+    if (a.kv_len) TG_LAUNCH(k_kv_keep_len, dim3((b.n_seqs + 255) / 256), dim3(256), 0, st, b, a);
+    return hipGetLastError();
+}
+
 // Blocks of one launch.  Narrow column tiles: `share` per key head, or one for each tile.  Wide ones, of which there are
 // `share` at most: one for each tile and `share` per key head more.  That is enough for their pieces: where an even
 // share is taken as it is there are as many at the most (a piece more than its part of them for each tile), and a
@@ -1558,7 +1675,7 @@ size_t attn_workspace(const KvBatch &b, int n_heads, int max_len) {
     return most;
 }
 
-template <int D, bool BF>
+template <int D, bool BF, bool TREE>
 static hipError_t attn_launch(const KvBatch &b, KvRows q, int G, float scale, const AttnPlan &p, const AttnOut &o, hipStream_t st) {
     static std::atomic<uint64_t> done{0};
     const dim3 grid((unsigned)p.blocks, (unsigned)b.n_kv);
@@ -1566,15 +1683,15 @@ static hipError_t attn_launch(const KvBatch &b, KvRows q, int G, float scale, co
     if constexpr (D < 256 || BF) {
         if (p.cols != 16) {
             constexpr size_t LDS = (BF ? 5 : 10) * 64 * D * 2;
-            const hipError_t e = attn_lds((const void *)k_attn_tile<D, BF>, LDS, done);
+            const hipError_t e = attn_lds((const void *)k_attn_tile<D, BF, TREE>, LDS, done);
             if (e != hipSuccess) return e;
-            TG_LAUNCH((k_attn_tile<D, BF>), dim3(grid.x * grid.y), dim3(512), LDS, st, b, q, G, scale, p.share, tpp, o);
+            TG_LAUNCH((k_attn_tile<D, BF, TREE>), dim3(grid.x * grid.y), dim3(512), LDS, st, b, q, G, scale, p.share, tpp, o);
             if (p.share)
                 TG_LAUNCH((k_attn_join_wide<D, BF, AT_COLS<D>>), dim3(p.joins, b.n_kv, AT_COLS<D> * D / 1024), dim3(256), 0, st, b, G, o);
             return hipSuccess;
         }
     }
-    TG_LAUNCH((k_attn_split<D, BF>), grid, dim3(256), 0, st, b, q, G, scale, p.share, p.unit, tpp, o);
+    TG_LAUNCH((k_attn_split<D, BF, TREE>), grid, dim3(256), 0, st, b, q, G, scale, p.share, p.unit, tpp, o);
     if (!p.share) return hipSuccess;
     if (p.joins * b.n_kv <= 64) TG_LAUNCH((k_attn_join<D, BF, 256>), dim3(p.joins, b.n_kv, 16), dim3(256), 0, st, b, G, o);
     else TG_LAUNCH((k_attn_join<D, BF, 64>), dim3(p.joins, b.n_kv, 4), dim3(256), 0, st, b, G, o);
@@ -1595,8 +1712,9 @@ hipError_t launch_attn(const KvBatch &b, int type, KvRows q, int n_heads, float 
         const AttnOut o{out, out_stride, static_cast<JoinTile *>(ws), p.joins,
                         reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + attn_join_bytes(b, p))};
         TG_BY_DIM(b.D, {
-            if (type == TG_T_F16) e = attn_launch<DIM, false>(kb, q, G, scale, p, o, st);
-            else e = attn_launch<DIM, true>(kb, q, G, scale, p, o, st);
+            const bool bf = type != TG_T_F16;
+            if (b.bits) e = bf ? attn_launch<DIM, true, true>(kb, q, G, scale, p, o, st) : attn_launch<DIM, false, true>(kb, q, G, scale, p, o, st);
+            else e = bf ? attn_launch<DIM, true, false>(kb, q, G, scale, p, o, st) : attn_launch<DIM, false, false>(kb, q, G, scale, p, o, st);
         });
     }
     return e != hipSuccess ? e : hipGetLastError();

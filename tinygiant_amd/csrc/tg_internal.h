@@ -391,6 +391,8 @@ struct KvBatch {
     int table_cols, table_stride;
     int n_seqs, n_tokens;
     int cols_from = 0, cols_to = INT32_MAX;  // attention: the launch is for sequences with so many rows x heads of a key head
+    const uint32_t *bits = nullptr;          // attention of draft trees: [n_tokens][words], the nodes that a row sees
+    int words = 0;
 };
 // strided rows of heads: element (t, h, d) at p[t * stride + h * D + d]
 struct KvRows {
@@ -406,12 +408,29 @@ struct AppendArgs {
     float eps;
     const float *cos, *sin;
     int max_pos;
+    const int32_t *depth = nullptr;  // of draft trees [n_tokens]: rows are rotated by it from their tree's first place on
 };
 hipError_t launch_kv_append(const KvBatch &b, int type, const AppendArgs &a, hipStream_t st);
 hipError_t launch_kv_read(const KvBatch &b, void *k, void *v, hipStream_t st);
 size_t attn_workspace(const KvBatch &b, int n_heads, int max_len);
 hipError_t launch_attn(const KvBatch &b, int type, KvRows q, int n_heads, float scale, void *out, int64_t out_stride,
                        int max_len, void *ws, hipStream_t st);
+// Entries of the tokens path[s][0 .. count[s]) of the sequences' last cu[s + 1] - cu[s] tokens to the first places of
+// those, in n_layers layers layer_bytes apart; kv_len (may be the batch's) then has the sequences' lengths.
+struct KeepArgs {
+    const int32_t *path, *count;
+    int64_t path_stride, layer_bytes;
+    int path_cols, n_layers;
+    int32_t *kv_len;
+};
+hipError_t launch_kv_keep(const KvBatch &b, const KeepArgs &a, hipStream_t st);
+// Trees of drafted tokens: node j of sequence s is row cu[s] + j, parent[row] < j the node it follows (-1 none); parent
+// NULL: each node follows the one before it.
+struct DraftTrees {
+    const int32_t *cu, *parent;
+    int n_seqs, n_tokens, max_nodes;
+};
+hipError_t launch_draft_tree(const DraftTrees &t, uint32_t *bits, int32_t *depth, hipStream_t st);
 struct MatmulI8Args {
     const void *x;
     int x_type;
