@@ -94,3 +94,46 @@ def test_python_refuses():
     for layer, n in ((-1, 1), (0, 2), (2, None), (1, -1)):
         with pytest.raises(ValueError, match="layers"):
             kv.keep(b, WIDE[:1], i[:1], layer=layer, n_layers=n)
+
+
+# ---------------------------------------------------------------- verify
+def verify_args(lib, t=None, **kw):
+    d = dict(type=0, logits=P, stride=100, draft=P, dstride=100, vocab=100, tokens=P, u=P, temp=1.0, temps=None, out=P, path=P,
+             count=P, ws=P, n=1 << 40)
+    d.update(kw)
+    return lib.tg_verify_dev(ctypes.byref(t if t is not None else trees()), *[d[n] for n in (
+        "type", "logits", "stride", "draft", "dstride", "vocab", "tokens", "u", "temp", "temps", "out", "path", "count", "ws", "n")], None)
+
+
+@pytest.mark.parametrize("kw,msg", BAD_TREES)
+def test_verify_refuses_trees(lib, kw, msg):
+    t = trees(**kw)
+    assert verify_args(lib, t) == INVALID and msg in said(lib)
+    assert lib.tg_verify_workspace(ctypes.byref(t), 100) == 0
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(type=3), "element type 3"), (dict(logits=None), "NULL"), (dict(tokens=None), "NULL"), (dict(u=None), "NULL"),
+    (dict(out=None), "NULL"), (dict(path=None), "NULL"), (dict(count=None), "NULL"), (dict(vocab=0), "vocab 0"),
+    (dict(vocab=(1 << 24) + 1, stride=1 << 25), "vocab 16777217"), (dict(stride=99), "overlap"), (dict(dstride=99), "overlap"),
+    (dict(logits=P + 2), "aligned"), (dict(draft=P + 1, type=1), "aligned"), (dict(temp=float("inf")), "temperature inf"),
+    (dict(ws=None), "workspace"), (dict(n=8), "workspace"), (dict(ws=P + 8), "workspace")])
+def test_verify_refuses(lib, kw, msg):
+    assert verify_args(lib, **kw) == INVALID and msg in said(lib)
+
+
+def test_verify_refuses_more_than_a_launch_takes(lib):
+    t = trees(n_tokens=1 << 20, n_seqs=1 << 14)
+    assert lib.tg_verify_workspace(ctypes.byref(t), 1 << 18) == 0
+    assert verify_args(lib, t, vocab=1 << 18, stride=1 << 18, draft=None) == INVALID and "than a launch takes" in said(lib)
+
+
+def test_verify_of_nothing(lib):
+    assert verify_args(lib, trees(n_seqs=0)) == 0
+
+
+def test_python_verify_refuses():
+    from tinygiant_amd.draft import verify
+
+    with pytest.raises(TypeError, match="logits must be"):
+        verify(torch.zeros(3, 9), None, None, None)

@@ -2671,6 +2671,53 @@ extern "C" int tg_draft_tree_dev(const tg_draft_trees *t, uint32_t *bits, int32_
     return TG_OK;
 }
 
+static int verify_shape(const char *fn, const tg_draft_trees *t, int vocab, tg::DraftTrees *d) {
+    int rc = draft_trees(fn, t, d);
+    if (rc) return rc;
+    if (vocab < 1 || vocab > 1 << 24) return set_err(TG_E_INVALID, "%s: vocab %d is not 1 to 2^24", fn, vocab);
+    if (!tg::verify_fits(*d, vocab))
+        return set_err(TG_E_INVALID, "%s: %d rows of %d: more than a launch takes", fn, d->n_tokens, vocab);
+    return TG_OK;
+}
+
+extern "C" size_t tg_verify_workspace(const tg_draft_trees *t, int vocab) {
+    tg::DraftTrees d;
+    return verify_shape("tg_verify_workspace", t, vocab, &d) ? 0 : tg::verify_workspace(d, vocab);
+}
+
+extern "C" int tg_verify_dev(const tg_draft_trees *t, int type, const void *logits, int64_t stride, const void *draft,
+                             int64_t draft_stride, int vocab, const int32_t *tokens, const double *u,
+                             float temperature, const float *temperatures, int32_t *out_tokens, int32_t *path,
+                             int32_t *count, void *workspace, size_t workspace_bytes, void *stream) {
+    const char *fn = "tg_verify_dev";
+    tg::DraftTrees d;
+    int rc = verify_shape(fn, t, vocab, &d);
+    if (rc) return rc;
+    if (type != TG_T_F32 && type != TG_T_F16 && type != TG_T_BF16)
+        return set_err(TG_E_INVALID, "%s: element type %d", fn, type);
+    if (!out_tokens || !path || !count || (d.n_tokens && (!logits || !tokens || !u)))
+        return set_err(TG_E_INVALID, "%s: a NULL pointer", fn);
+    if (stride < vocab || (draft && draft_stride < vocab))
+        return set_err(TG_E_INVALID, "%s: rows overlap (logits %lld, draft %lld apart)", fn, (long long)stride, (long long)draft_stride);
+    if (!aligned(logits, type_size(type)) || !aligned(draft, type_size(type)))
+        return set_err(TG_E_INVALID, "%s: logits or draft are not aligned to their type", fn);
+    if (!temperatures && temperature == INFINITY)
+        return set_err(TG_E_INVALID, "%s: temperature %g", fn, (double)temperature);
+    if (!d.n_seqs) return TG_OK;
+    const size_t need = tg::verify_workspace(d, vocab);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+        return set_err(TG_E_INVALID, "%s: workspace of %zu bytes, %zu and 16-byte alignment needed", fn,
+                       workspace ? workspace_bytes : (size_t)0, need);
+    DeviceOf dev(as_stream(stream));
+    if (dev.rc) return dev.rc;
+    tg::VerifyArgs a{};
+    a.t = d, a.logits = logits, a.stride = stride, a.draft = draft, a.draft_stride = draft_stride, a.vocab = vocab;
+    a.tokens = tokens, a.u = u, a.temps = temperatures, a.temp = temperature;
+    a.out = out_tokens, a.path = path, a.count = count;
+    PROFILED("verify", as_stream(stream), tg::launch_verify(a, type, workspace, as_stream(stream)));
+    return TG_OK;
+}
+
 static int matmul_shape(const char *fn, int M, int N, int K) {
     if (M < 0 || N < 1 || K < 16 || K % 16 || K > 131072)
         return set_err(TG_E_INVALID, "%s: M %d, N %d, K %d (a multiple of 16 up to 131072)", fn, M, N, K);

@@ -431,6 +431,33 @@ struct DraftTrees {
     int n_seqs, n_tokens, max_nodes;
 };
 hipError_t launch_draft_tree(const DraftTrees &t, uint32_t *bits, int32_t *depth, hipStream_t st);
+struct RowPart {
+    float m, s;  // largest value of a chunk of a row, sum of exp((v - m) / T)
+};
+struct PieceSums {
+    double m[2], z[2], rest;  // of the target's and the draft's row in 64 bits; of what is left
+};
+struct VerifyArgs {
+    DraftTrees t;
+    const void *logits;
+    int64_t stride;
+    const void *draft;
+    int64_t draft_stride;
+    int vocab;
+    const int32_t *tokens;
+    const double *u;
+    const float *temps;
+    float temp;
+    int32_t *out, *path, *count;
+    // the workspace
+    int chunks, pieces;
+    RowPart *rows;    // [n_tokens][target, draft][chunks]
+    int *arg;         // [n_tokens][chunks]
+    PieceSums *sums;  // [n_seqs][pieces]
+};
+bool verify_fits(const DraftTrees &t, int vocab);  // in the threads of a launch
+size_t verify_workspace(const DraftTrees &t, int vocab);
+hipError_t launch_verify(VerifyArgs a, int type, void *ws, hipStream_t st);
 struct MatmulI8Args {
     const void *x;
     int x_type;
