@@ -431,12 +431,6 @@ struct DraftTrees {
     int n_seqs, n_tokens, max_nodes;
 };
 hipError_t launch_draft_tree(const DraftTrees &t, uint32_t *bits, int32_t *depth, hipStream_t st);
-struct RowPart {
-    float m, s;  // largest value of a chunk of a row, sum of exp((v - m) / T)
-};
-struct PieceSums {
-    double m[2], z[2], rest;  // of the target's and the draft's row in 64 bits; of what is left
-};
 struct VerifyArgs {
     DraftTrees t;
     const void *logits;
@@ -449,11 +443,16 @@ struct VerifyArgs {
     const float *temps;
     float temp;
     int32_t *out, *path, *count;
+    int team;          // blocks of a walk
     // the workspace
     int chunks, pieces;
-    RowPart *rows;    // [n_tokens][target, draft][chunks]
-    int *arg;         // [n_tokens][chunks]
-    PieceSums *sums;  // [n_seqs][pieces]
+    double *sum;       // [n_tokens][target, draft][pieces]
+    float *top;        // [n_tokens][target, draft][chunks]
+    int *arg;          // [n_tokens][chunks]
+    double *swept_sum; // [n_seqs][pieces]
+    float *swept_top;
+    uint32_t *meet;    // [n_seqs] of Meeting
+    size_t meet_words;
 };
 bool verify_fits(const DraftTrees &t, int vocab);  // in the threads of a launch
 size_t verify_workspace(const DraftTrees &t, int vocab);
