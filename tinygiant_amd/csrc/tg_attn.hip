@@ -48,9 +48,6 @@ TG_DEV int page_of(const KvBatch &b, int s, int p) {
     return page >= 0 && page < b.n_pages ? page : -1;
 }
 
-// a value that is the same in every lane, told to the compiler
-TG_DEV int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
 // The sequence of row t: the number of j with cu[j + 1] <= t, counted by L
 // neighbouring lanes (li: lane among them); n_seqs for padding rows.
 template <int L>

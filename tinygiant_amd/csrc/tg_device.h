@@ -18,6 +18,9 @@ constexpr int Q40_BYTES = 18;   // {half d; u8 qs[16]}
 constexpr int Q80_BYTES = 34;   // {half d; i8 qs[32]}
 constexpr int WAVE = 64;
 
+// a value that is the same in every lane, told to the compiler
+TG_DEV int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // ---------------------------------------------------------------- halves
 TG_DEV float h2f(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
 

@@ -444,12 +444,14 @@ struct VerifyArgs {
     float temp;
     int32_t *out, *path, *count;
     int team;          // blocks of a walk
+    bool early;        // rows are loaded before it is known whether they are asked for
     // the workspace
     int chunks, pieces;
     double *sum;       // [n_tokens][target, draft][pieces]
+    double *whole;     // [n_tokens][target, draft][chunks]
     float *top;        // [n_tokens][target, draft][chunks]
     int *arg;          // [n_tokens][chunks]
-    double *swept_sum; // [n_seqs][pieces]
+    double *swept_sum, *own_sum;  // [n_seqs][pieces]
     float *swept_top;
     uint32_t *meet;    // [n_seqs] of Meeting
     size_t meet_words;
