@@ -115,7 +115,7 @@ def test_verify_refuses_trees(lib, kw, msg):
 @pytest.mark.parametrize("kw,msg", [
     (dict(type=3), "element type 3"), (dict(logits=None), "NULL"), (dict(tokens=None), "NULL"), (dict(u=None), "NULL"),
     (dict(out=None), "NULL"), (dict(path=None), "NULL"), (dict(count=None), "NULL"), (dict(vocab=0), "vocab 0"),
-    (dict(vocab=(1 << 24) + 1, stride=1 << 25), "vocab 16777217"), (dict(stride=99), "overlap"), (dict(dstride=99), "overlap"),
+    (dict(vocab=(1 << 20) + 1, stride=1 << 25), "vocab 1048577"), (dict(stride=99), "overlap"), (dict(dstride=99), "overlap"),
     (dict(logits=P + 2), "aligned"), (dict(draft=P + 1, type=1), "aligned"), (dict(temp=float("inf")), "temperature inf"),
     (dict(ws=None), "workspace"), (dict(n=8), "workspace"), (dict(ws=P + 8), "workspace")])
 def test_verify_refuses(lib, kw, msg):

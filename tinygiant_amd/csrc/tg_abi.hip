@@ -2674,7 +2674,7 @@ extern "C" int tg_draft_tree_dev(const tg_draft_trees *t, uint32_t *bits, int32_
 static int verify_shape(const char *fn, const tg_draft_trees *t, int vocab, tg::DraftTrees *d) {
     int rc = draft_trees(fn, t, d);
     if (rc) return rc;
-    if (vocab < 1 || vocab > 1 << 24) return set_err(TG_E_INVALID, "%s: vocab %d is not 1 to 2^24", fn, vocab);
+    if (vocab < 1 || vocab > 1 << 20) return set_err(TG_E_INVALID, "%s: vocab %d is not 1 to 2^20", fn, vocab);
     if (!tg::verify_fits(*d, vocab))
         return set_err(TG_E_INVALID, "%s: %d rows of %d: more than a launch takes", fn, d->n_tokens, vocab);
     return TG_OK;

@@ -90,30 +90,43 @@ TG_DEV float load1(const void *p, int64_t i) {
     const uint16_t v = static_cast<const uint16_t *>(p)[i];
     return TYPE == TG_T_F16 ? h2f(v) : __uint_as_float((uint32_t)v << 16);
 }
-// 8 values of a row from i on, -inf behind its end.  Rows of any alignment: global loads of 16 bytes need that of their elements.
+// 8 values of a row from i on: rows of any alignment, global loads of 16 bytes need that of their elements
 template <int TYPE>
-TG_DEV void load8(const void *row, int i, int V, float v[8]) {
-    if (i + 8 <= V) {
-        if constexpr (TYPE == TG_T_F32) {
+TG_DEV void load8(const void *row, int i, float v[8]) {
+    if constexpr (TYPE == TG_T_F32) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                f32x4 x;
-                __builtin_memcpy(&x, static_cast<const float *>(row) + i + 4 * h, 16);
+        for (int h = 0; h < 2; h++) {
+            f32x4 x;
+            __builtin_memcpy(&x, static_cast<const float *>(row) + i + 4 * h, 16);
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[4 * h + e] = x[e];
-            }
-        } else {
-            u32x4 x;
-            __builtin_memcpy(&x, static_cast<const uint16_t *>(row) + i, 16);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint16_t b = (uint16_t)(x[e / 2] >> (16 * (e % 2)));
-                v[e] = TYPE == TG_T_F16 ? h2f(b) : __uint_as_float((uint32_t)b << 16);
-            }
+            for (int e = 0; e < 4; e++) v[4 * h + e] = x[e];
         }
     } else {
+        u32x4 x;
+        __builtin_memcpy(&x, static_cast<const uint16_t *>(row) + i, 16);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = i + e < V ? load1<TYPE>(row, i + e) : -INFINITY;
+        for (int e = 0; e < 8; e++) {
+            const uint16_t b = (uint16_t)(x[e / 2] >> (16 * (e % 2)));
+            v[e] = TYPE == TG_T_F16 ? h2f(b) : __uint_as_float((uint32_t)b << 16);
+        }
+    }
+}
+// N times 8 values, STEP apart, of a stretch of the row that ends at `end`: one branch around all of the loads, and a value
+// at a time, -inf behind the row's end, where the stretch passes it
+template <int TYPE, int N, int STEP>
+TG_DEV void load_stretch(const void *row, int i, int end, int V, float v[N][8]) {
+    if (end <= V) {
+#pragma unroll
+        for (int k = 0; k < N; k++) load8<TYPE>(row, i + k * STEP, v[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int at = i + k * STEP + e;
+                const float x = load1<TYPE>(row, min(at, V - 1));
+                v[k][e] = at < V ? x : -INFINITY;
+            }
     }
 }
 template <int TYPE>
@@ -163,30 +176,53 @@ TG_DEV float uni(float v) { return __int_as_float(uni(__float_as_int(v))); }
 // what is true or not in all lanes of a wave, told to the compiler
 TG_DEV bool sure(bool c) { return __ballot(c) != 0; }
 
-template <class T>
-TG_DEV T wave_max(T v) {
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-        const T o = __shfl_xor(v, m);
-        v = v > o ? v : o;
-    }
-    return v;
+// What a lane gets from `CTRL` lanes further down (DPP: row_shr 1, 2, 4, 8, row_bcast 15, 31 for rows ROWS), or `none`
+template <int CTRL, int ROWS>
+TG_DEV float from_below(float v, float none) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, ROWS, 0xF, false));
 }
+template <int CTRL, int ROWS>
+TG_DEV double from_below(double v, double none) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v), o = __builtin_bit_cast(uint64_t, none);
+    const uint32_t lo = __builtin_amdgcn_update_dpp((int)o, (int)b, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp((int)(o >> 32), (int)(b >> 32), CTRL, ROWS, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// over the lanes up to each (half: of its half of the wave), in a fixed order
+template <class T, class F>
+TG_DEV T wave_upto(T v, T none, bool half, F f) {
+    v = f(v, from_below<0x111, 0xF>(v, none));
+    v = f(v, from_below<0x112, 0xF>(v, none));
+    v = f(v, from_below<0x114, 0xF>(v, none));
+    v = f(v, from_below<0x118, 0xF>(v, none));
+    v = f(v, from_below<0x142, 0xA>(v, none));
+    return half ? v : f(v, from_below<0x143, 0xC>(v, none));
+}
+TG_DEV double of_lane(double v, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+TG_DEV float of_lane(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
+constexpr auto v_plus = [](auto x, auto y) { return x + y; };
+constexpr auto v_most = [](float x, float y) { return fmaxf(x, y); };
+TG_DEV double sums_upto(double v) { return wave_upto(v, 0.0, false, v_plus); }
+TG_DEV double wave_add(double v) { return of_lane(sums_upto(v), 63); }
+TG_DEV float wave_max(float v) { return of_lane(wave_upto(v, -INFINITY, false, v_most), 63); }
+// of the half of the wave that a lane is in
 template <class T>
-TG_DEV T wave_add(T v) {
+TG_DEV T half_of(T v, int lane) {
+    const T a = of_lane(v, 31), b = of_lane(v, 63);
+    return lane < 32 ? a : b;
+}
+TG_DEV double half_add(double v, int lane) { return half_of(wave_upto(v, 0.0, true, v_plus), lane); }
+TG_DEV float half_max(float v, int lane) { return half_of(wave_upto(v, -INFINITY, true, v_most), lane); }
+TG_DEV int wave_count(int v) {
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) v += __shfl_xor(v, m);
-    return v;
+    return uni(v);
 }
-// inclusive sums over the lanes
-TG_DEV double wave_upto(double v, int lane) {
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-        const double o = __shfl_up(v, m);
-        if (lane >= m) v += o;
-    }
-    return v;
-}
+
 // over the four waves of a block, in order; `sm` is 4 values that nothing else uses until the next barrier
 TG_DEV double block_add(double v, double *sm) {
     v = wave_add(v);
@@ -216,8 +252,7 @@ __global__ __launch_bounds__(256) void k_verify_rows(VerifyArgs a) {
     const void *p = of ? row_of<TYPE>(a.draft, a.draft_stride, row) : row_of<TYPE>(a.logits, a.stride, row);
     float v[V_PER][8], m = -INFINITY;
     auto load = [&]() {
-#pragma unroll
-        for (int k = 0; k < V_PER; k++) load8<TYPE>(p, chunk * V_CHUNK + k * V_PIECE + threadIdx.x * 8, a.vocab, v[k]);
+        load_stretch<TYPE, V_PER, V_PIECE>(p, chunk * V_CHUNK + threadIdx.x * 8, (chunk + 1) * V_CHUNK, a.vocab, v);
     };
     if (a.early) load();
     if (!of)
@@ -225,7 +260,7 @@ __global__ __launch_bounds__(256) void k_verify_rows(VerifyArgs a) {
     if (threadIdx.x < V_TABLE) exp_table(two, threadIdx.x);
     int s = 0;
     for (int j = lane; j < a.t.n_seqs; j += 64) s += a.t.cu[j + 1] <= row;
-    s = uni(wave_add(s));
+    s = wave_count(s);
     if (s >= a.t.n_seqs) return;
     const TreeRows r = tree_rows(a.t, s);
     const float t = uni(temperature_of(a, s));
@@ -313,8 +348,9 @@ TG_DEV void shown() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt 0: this th
 
 template <int TYPE>
 struct Walk {
-    const VerifyArgs &a;
-    int helpers;
+    const void *logits, *draft;
+    int64_t stride, draft_stride;
+    int vocab, pieces, helpers;
     Exp64 exp64;
     Meeting *meet;
     float *top;   // of a sweep's pieces: the largest value of each
@@ -323,29 +359,33 @@ struct Walk {
     double *smd;
     uint32_t *smu;
 
+    TG_DEV const void *row_p(int row) const { return row_of<TYPE>(logits, stride, row); }
+    TG_DEV const void *row_q(int row) const { return row_of<TYPE>(draft, draft_stride, row); }
+    TG_DEV void load_piece(const void *row, int k, float v[1][8]) const {
+        load_stretch<TYPE, 1, 0>(row, k * V_PIECE + (int)threadIdx.x * 8, (k + 1) * V_PIECE, vocab, v);
+    }
     // piece k of a sweep, by one block
-    TG_DEV void piece(const Sweep &w, int k) {
+    TG_DEV void piece(const Sweep &w, int k) const {
         const int row = uni((int)(w.row >> 1));
-        const void *pr = row_of<TYPE>(a.logits, a.stride, row);
-        float v[8], q[8];
-        load8<TYPE>(pr, k * V_PIECE + threadIdx.x * 8, a.vocab, v);
+        float v[1][8], q[1][8];
+        load_piece(row_p(row), k, v);
         double z = 0.0;
         if (uni((int)w.row & 1)) {
-            load8<TYPE>(row_of<TYPE>(a.draft, a.draft_stride, row), k * V_PIECE + threadIdx.x * 8, a.vocab, q);
+            load_piece(row_q(row), k, q);
 #pragma unroll
-            for (int e = 0; e < 8; e++) z += rest(w, v[e], q[e]);
+            for (int e = 0; e < 8; e++) z += rest(w, v[0][e], q[0][e]);
         } else {
             float m = -INFINITY;
             bool bad = false;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                bad |= !(v[e] < INFINITY);
-                m = fmaxf(m, v[e]);
+                bad |= !(v[0][e] < INFINITY);
+                m = fmaxf(m, v[0][e]);
             }
             m = block_max(bad ? INFINITY : m, smf);
             if (m > -INFINITY && m < INFINITY)
 #pragma unroll
-                for (int e = 0; e < 8; e++) z += exp64((double)v[e] - m);
+                for (int e = 0; e < 8; e++) z += exp64((double)v[0][e] - m);
             if (threadIdx.x == 0) show(top + k, m);
         }
         z = block_add(z, smd);
@@ -354,44 +394,48 @@ struct Walk {
     TG_DEV double rest(const Sweep &w, float v, float q) const {
         return fmax(exp64((double)v - w.Mp) * w.ip - exp64((double)q - w.Mq) * w.iq, 0.0);
     }
-    // takes pieces of sweep `number` until there are none
-    TG_DEV void take(const Sweep &w, uint32_t number) {
-        uint32_t *taken = meet->taken_done + 2 * number;
+    TG_DEV void claim(uint32_t number) const {  // thread 0's
+        *smu = __hip_atomic_fetch_add(meet->taken_done + 2 * number, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    // takes pieces of sweep `number` until there are none; the first is claimed
+    TG_DEV void take(const Sweep &w, uint32_t number) const {
         for (;;) {
             __syncthreads();
-            if (threadIdx.x == 0) *smu = __hip_atomic_fetch_add(taken, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __syncthreads();
             const uint32_t k = uni((int)*smu);
-            if (k >= (uint32_t)a.pieces) return;
+            __syncthreads();
+            if (k >= (uint32_t)pieces) return;
             piece(w, (int)k);
             if (threadIdx.x == 0) {
-                shown();
-                __hip_atomic_fetch_add(taken + 1, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                shown();  // the piece's sum before it counts
+                __hip_atomic_fetch_add(meet->taken_done + 2 * number + 1, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                claim(number);
             }
         }
     }
-    TG_DEV void help() {
+    TG_DEV void help() const {
         for (uint32_t number = 0;;) {
             __syncthreads();
             if (threadIdx.x == 0) {
                 uint32_t now;
-                while ((now = seen_now(&meet->number)) == number) __builtin_amdgcn_s_sleep(4);
+                while ((now = seen_now(&meet->number)) == number) __builtin_amdgcn_s_sleep(2);
                 *smu = now;
             }
             __syncthreads();
             number = uni((int)*smu);
+            __syncthreads();
             if (number == V_END) return;
             // this sweep's as long as pieces of it can be taken: a later one's is not worked on
             const Sweep w{seen_now(&meet->sweep.row), seen_now(&meet->sweep.Mp), seen_now(&meet->sweep.ip), seen_now(&meet->sweep.Mq),
                           seen_now(&meet->sweep.iq)};
+            if (threadIdx.x == 0) claim(number);
             take(w, number);
         }
     }
     // the leader's: a whole sweep
-    TG_DEV void lead(const Sweep &w, uint32_t number) {
+    TG_DEV void lead(const Sweep &w, uint32_t number) const {
         __syncthreads();
         if (!helpers) {
-            for (int k = 0; k < a.pieces; k++) piece(w, k);
+            for (int k = 0; k < pieces; k++) piece(w, k);
             shown();
             __syncthreads();
             return;
@@ -401,29 +445,33 @@ struct Walk {
             show(&meet->sweep.Mq, w.Mq), show(&meet->sweep.iq, w.iq);
             shown();
             show(&meet->number, number);
+            claim(number);
         }
         take(w, number);
         if (threadIdx.x == 0)
-            while (seen_now(meet->taken_done + 2 * number + 1) != (uint32_t)a.pieces) __builtin_amdgcn_s_sleep(1);
+            while (seen_now(meet->taken_done + 2 * number + 1) != (uint32_t)pieces) __builtin_amdgcn_s_sleep(1);
         __syncthreads();
     }
 };
 
-// LDS of a walk, for `nodes` of them
+// LDS of a walk, for `nodes` of them and rows of `pieces`
 struct WalkNodes {
-    double *u, *sum[2];    // random numbers; the rows' sums of exponentials, target's and draft's
-    float *x[2], *top[2];  // the nodes' logits at their parents; the rows' largest values
+    double *u, *e, *inv;  // random numbers; exponentials of the nodes' logits at their parents; 1 / the rows' sums of those
+    double *weight;       // of the pieces of what is left
+    float *x, *top;       // the nodes' logits at their parents; the rows' largest values (e, inv, x, top: target's, then draft's)
     int *tok;
     int16_t *par, *way;
-    uint8_t *kids;
-    TG_DEV WalkNodes(uint8_t *lds, int nodes) {
-        u = reinterpret_cast<double *>(lds), sum[0] = u + nodes, sum[1] = sum[0] + nodes;
-        x[0] = reinterpret_cast<float *>(sum[1] + nodes), x[1] = x[0] + nodes, top[0] = x[1] + nodes, top[1] = top[0] + nodes;
-        tok = reinterpret_cast<int *>(top[1] + nodes);
+    uint8_t *again;       // an earlier sibling has the same token
+    uint16_t *list;       // pieces to be summed again
+    TG_DEV WalkNodes(uint8_t *lds, int nodes, int pieces) {
+        u = reinterpret_cast<double *>(lds), e = u + nodes, inv = e + 2 * nodes, weight = inv + 2 * nodes;
+        x = reinterpret_cast<float *>(weight + pieces), top = x + 2 * nodes;
+        tok = reinterpret_cast<int *>(top + 2 * nodes);
         par = reinterpret_cast<int16_t *>(tok + nodes), way = par + nodes;
-        kids = reinterpret_cast<uint8_t *>(way + nodes);
+        list = reinterpret_cast<uint16_t *>(way + nodes);
+        again = reinterpret_cast<uint8_t *>(list + pieces);
     }
-    static size_t bytes(int nodes) { return (size_t)nodes * (3 * 8 + 5 * 4 + 2 * 2 + 1); }
+    static size_t bytes(int nodes, int pieces) { return (size_t)nodes * (5 * 8 + 5 * 4 + 2 * 2 + 1) + (size_t)pieces * (8 + 2); }
 };
 
 // A sequence's walk: one block leads, the others help with sums over whole rows.  What decides where the leader goes is the
@@ -434,36 +482,93 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ double smd[4], two[V_TABLE];
     __shared__ float smf[4];
-    __shared__ uint32_t gone[4][V_PIECE / 32];  // a wave's: tokens of a piece that were rejected
+    __shared__ int hits[4], lasts[4];
     __shared__ uint32_t smu;
-    __shared__ int found;
+    __shared__ int listed;
     const int tid = threadIdx.x, lane = tid % 64, wave = uni(tid / 64), s = blockIdx.x % a.t.n_seqs, V = a.vocab;
+    Meeting *meet = reinterpret_cast<Meeting *>(a.meet + s * (a.meet_words / a.t.n_seqs));
+    if (a.team > 1 && tid == 0) smu = __hip_atomic_fetch_add(&meet->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const TreeRows r = tree_rows(a.t, s);
     const float t = uni(temperature_of(a, s));
     const bool greedy = !(t > 0.0f), with_q = a.draft && !greedy;
     if (tid < V_TABLE) exp_table(two, tid);
     const Exp64 exp64{factor_of(t), two};
-    Walk<TYPE> walk{a, a.team - 1, exp64, reinterpret_cast<Meeting *>(a.meet + s * (a.meet_words / a.t.n_seqs)),
-                    a.swept_top + (size_t)s * a.pieces, a.swept_sum + (size_t)s * a.pieces, smf, smd, &smu};
-    if (a.team > 1) {
-        if (tid == 0) smu = __hip_atomic_fetch_add(&walk.meet->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __syncthreads();
-        if (uni((int)smu)) {
-            walk.help();
-            return;
-        }
-    }
-    const TreeRows r = tree_rows(a.t, s);
-    const int n = uni(min(r.n, a.t.max_nodes)), lo = uni(r.lo);
-    const WalkNodes d(lds, a.t.max_nodes);
-    for (int j = tid; j < n; j += 256) d.kids[j] = 0;
+    const Walk<TYPE> walk{a.logits, a.draft, a.stride, a.draft_stride, V, a.pieces, a.team - 1, exp64, meet,
+                          a.swept_top + (size_t)s * a.pieces, a.swept_sum + (size_t)s * a.pieces, smf, smd, &smu};
     __syncthreads();
+    if (a.team > 1 && uni((int)smu)) {
+        walk.help();
+        return;
+    }
+    const int n = uni(min(r.n, a.t.max_nodes)), lo = uni(r.lo);
+    const int N = a.t.max_nodes;
+    const WalkNodes d(lds, N, a.pieces);
+
+    // Largest values and sums of the rows of nodes j0 .. j0 + 63, from those of their chunks: half a wave to a row, the
+    // next one's on their way.  Of rows that nothing follows they are whatever the memory holds, and not used.  For a
+    // greedy sequence the first of the largest stands in the place of the draft's logits.
+    const int l = lane % 32, each = with_q ? 2 : 1;
+    struct Part {
+        float m;
+        double z;
+    };
+    auto part = [&](int j0, int i) {
+        Part c{-INFINITY, 0.0};
+        const int j = j0 + i / each;
+        if (i < 64 * each && j < n && l < a.chunks) {
+            const size_t at = ((size_t)(lo + j) * 2 + i % each) * a.chunks + l;
+            c.m = a.top[at];
+            if (!greedy) c.z = a.whole[at];
+        }
+        return c;
+    };
+    auto join = [&](int j0, Part c) {
+        const int units = min(n - j0, 64) * each;
+        for (int i0 = 2 * wave; i0 < units; i0 += 8) {
+            const int i = i0 + lane / 32, j = j0 + i / each, of = i % each;
+            const bool live = i < units;
+            const Part next = part(j0, i + 8);
+            const size_t at = ((size_t)(lo + j) * 2 + of) * a.chunks;
+            float m = c.m;
+            for (int k = 32; k < a.chunks; k += 32)
+                if (live && k + l < a.chunks) m = fmaxf(m, a.top[at + k + l]);
+            m = half_max(m, lane);
+            if (live && l == 0) d.top[of * N + j] = m;
+            if (greedy) {
+                int best = INT32_MAX;
+                for (int k = 0; k < a.chunks; k += 32)
+                    if (live && k + l < a.chunks && a.top[at + k + l] == m) best = min(best, a.arg[(size_t)(lo + j) * a.chunks + k + l]);
+#pragma unroll
+                for (int k = 1; k < 32; k *= 2) best = min(best, __shfl_xor(best, k));
+                if (live && l == 0) d.x[N + j] = __int_as_float(best);
+            } else {
+                double z = c.z * exp64((double)c.m - m);
+                for (int k = 32; k < a.chunks; k += 32)
+                    if (live && k + l < a.chunks) z += a.whole[at + k + l] * exp64((double)a.top[at + k + l] - m);
+                z = half_add(z, lane);
+                if (live && l == 0) d.inv[of * N + j] = 1.0 / z;
+            }
+            c = next;
+        }
+        __syncthreads();
+        if (greedy) return;
+        for (int j = j0 + 1 + tid; j < n; j += 256) {
+            const int p = d.par[j];
+            if (p < j0 || p >= j0 + 64) continue;
+            d.e[j] = exp64((double)d.x[j] - d.top[p]);
+            if (with_q) d.e[N + j] = exp64((double)d.x[N + j] - d.top[N + p]);
+        }
+        __syncthreads();
+    };
+    Part first = part(0, 2 * wave + lane / 32);
     for (int j = tid; j < n; j += 256) {
         const int p = parent_of(a.t, lo, j), x = a.tokens[lo + j];
         const bool ok = p >= 0 && x >= 0 && x < V;
-        if (p >= 0) d.kids[p] = 1;
-        d.par[j] = (int16_t)p, d.tok[j] = x, d.u[j] = a.u[lo + j];
-        d.x[0][j] = ok ? load1<TYPE>(row_of<TYPE>(a.logits, a.stride, lo + p), x) : -INFINITY;
-        d.x[1][j] = ok && with_q ? load1<TYPE>(row_of<TYPE>(a.draft, a.draft_stride, lo + p), x) : -INFINITY;
+        d.par[j] = (int16_t)p, d.tok[j] = x, d.u[j] = a.u[lo + j], d.again[j] = 0;
+        if (!greedy) {
+            d.x[j] = ok ? load1<TYPE>(walk.row_p(lo + p), x) : -INFINITY;
+            if (with_q) d.x[N + j] = ok ? load1<TYPE>(walk.row_q(lo + p), x) : -INFINITY;
+        }
     }
     __syncthreads();
     // the next child of `node` behind j, or -1: the same in every wave, like all that follows
@@ -474,89 +579,62 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
         }
         return -1;
     };
-    // is there a child of `node` before j whose token `same` takes for j's
-    auto earlier = [&](int node, int j, auto same) {
+    // is there a child of `node` before j with its token
+    auto earlier = [&](int node, int j) {
+        const int x = uni(d.tok[j]);
         for (int k = node + 1; k < j; k += 64)
-            if (__ballot(k + lane < j && d.par[k + lane < j ? k + lane : 0] == node && same(d.tok[k + lane < j ? k + lane : 0]))) return true;
+            if (__ballot(k + lane < j && d.par[k + lane < j ? k + lane : 0] == node && d.tok[k + lane < j ? k + lane : 0] == x)) return true;
         return false;
     };
-    // Largest values and sums of the rows of nodes j0 .. j0 + 63, from those of their chunks: half a wave to a row.  For a
-    // greedy sequence the first of the largest stands in the place of the draft's logits.
-    auto join = [&](int j0) {
-        const int each = with_q ? 2 : 1, units = min(n - j0, 64) * each, l = lane % 32;
-        for (int i = tid / 32; i < units; i += 8) {
-            const int j = j0 + i / each, of = i % each;
-            if (!greedy && !d.kids[j]) continue;
-            const size_t at = ((size_t)(lo + j) * 2 + of) * a.chunks;
-            float m = -INFINITY;
-            for (int k = l; k < a.chunks; k += 32) m = fmaxf(m, a.top[at + k]);
-#pragma unroll
-            for (int k = 1; k < 32; k *= 2) m = fmaxf(m, __shfl_xor(m, k));
-            if (l == 0) d.top[of][j] = m;
-            if (m == INFINITY || m == -INFINITY) continue;
-            if (greedy) {
-                int best = INT32_MAX;
-                for (int k = l; k < a.chunks; k += 32)
-                    if (a.top[at + k] == m) best = min(best, a.arg[(size_t)(lo + j) * a.chunks + k]);
-#pragma unroll
-                for (int k = 1; k < 32; k *= 2) best = min(best, __shfl_xor(best, k));
-                if (l == 0) d.x[1][j] = __int_as_float(best);
-            } else {
-                double z = 0.0;
-                for (int k = l; k < a.chunks; k += 32) z += a.whole[at + k] * exp64((double)a.top[at + k] - m);
-#pragma unroll
-                for (int k = 1; k < 32; k *= 2) z += __shfl_xor(z, k);
-                if (l == 0) d.sum[of][j] = z;
-            }
-        }
-        __syncthreads();
-    };
-    auto swept = [&]() {  // the sum over a sweep's pieces
+    auto no_number = [](float m) { return m == INFINITY || m == -INFINITY; };
+    auto total_of = [&]() {  // of the pieces' weights
         double z = 0.0;
-        for (int k = lane; k < a.pieces; k += 64) z += seen_now(walk.sum + k);
+        for (int k = lane; k < a.pieces; k += 64) z += d.weight[k];
         return wave_add(z);
     };
-    auto no_number = [](float m) { return m == INFINITY || m == -INFINITY; };
 
     int at = 0, kept = 1, next = -1, joined = 0;
     uint32_t sweeps = 0;
     if (tid == 0) d.way[0] = 0;
     while (n) {
-        const int row = lo + at, kid = child(at, at);  // all of these are the same in every lane
+        const int row = lo + at, kid = child(at, at);
         int yes = -1;
         if (at >= joined) {
-            join(at);
+            join(at, at ? part(at, 2 * wave + lane / 32) : first);
             joined = at + 64;
         }
         if (greedy) {
-            if (no_number(uni(d.top[0][at]))) break;
-            const int best = uni(__float_as_int(d.x[1][at]));
+            if (no_number(uni(d.top[at]))) break;
+            const int best = uni(__float_as_int(d.x[N + at]));
             for (int k = kid; k >= 0 && yes < 0; k = child(at, k))
                 if (uni(d.tok[k]) == best) yes = k;
             if (yes < 0) next = best;
         } else {
-            double Mp = 0, Zp = 1, Mq = 0, Zq = 1, c = 0;
+            double Mp = 0, ip = 1, Mq = 0, iq = 1, c = 0;
             if (kid >= 0) {
-                Mp = d.top[0][at], Zp = d.sum[0][at];
-                if (with_q) Mq = d.top[1][at], Zq = d.sum[1][at];
+                Mp = d.top[at], ip = d.inv[at];
+                if (with_q) Mq = d.top[N + at], iq = d.inv[N + at];
                 if (no_number(uni((float)Mp)) || no_number(uni((float)Mq))) break;
                 double left = 1.0;
                 for (int k = kid, after; k >= 0; k = after) {
                     after = child(at, k);
-                    double px = exp64((double)d.x[0][k] - Mp) / Zp;
+                    const double px = d.e[k] * ip;
                     if (with_q) {
-                        const double qx = exp64((double)d.x[1][k] - Mq) / Zq;
+                        const double qx = d.e[N + k] * iq;
                         if (sure(d.u[k] * left * qx < px - c * qx)) {
                             yes = k;
                             break;
                         }
                         c += left;
                         if (after >= 0) {
-                            walk.lead({2 * (uint64_t)row + 1, Mp, 1.0 / Zp, Mq, c / Zq}, ++sweeps);
-                            left = swept();
+                            walk.lead({2 * (uint64_t)row + 1, Mp, ip, Mq, c * iq}, ++sweeps);
+                            double z = 0.0;
+                            for (int k0 = lane; k0 < a.pieces; k0 += 64) z += seen_now(walk.sum + k0);
+                            left = wave_add(z);
                         }
+                    } else if (earlier(at, k)) {  // rejected already
+                        if (tid == 0) d.again[k] = 1;
                     } else {
-                        if (earlier(at, k, [&](int x) { return x == d.tok[k]; })) px = 0.0;  // rejected already
                         if (sure(px > 0.0 && d.u[k] * left < px)) {
                             yes = k;
                             break;
@@ -567,114 +645,111 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
             }
             if (yes < 0) {
                 if (!sure(d.u[0] >= 0.0 && d.u[0] < 1.0)) break;
-                // weights of the pieces of what is left: a sweep's sums, or those times exp((largest - M) / T)
-                Sweep w{2 * (uint64_t)row, Mp, 1.0 / Zp, Mq, c / Zq};
-                bool of_rest = with_q && kid >= 0;
+                // what is left, by pieces: of the row of a leaf and of p - c q by a sweep, else by the row's own sums
+                Sweep w{2 * (uint64_t)row, Mp, ip, Mq, c * iq};
+                bool of_rest = with_q && kid >= 0, without = !with_q && kid >= 0;
+                auto own_weights = [&]() {
+                    __syncthreads();
+                    for (int k = tid; k < a.pieces; k += 256)
+                        d.weight[k] = a.sum[(size_t)row * 2 * a.pieces + k] * exp64((double)a.top[(size_t)row * 2 * a.chunks + k / V_PER] - Mp);
+                    __syncthreads();
+                };
                 if (of_rest) {
                     w.row++;
                     walk.lead(w, ++sweeps);
-                    of_rest = sure(swept() > 0.0);  // nothing: of all that there was
+                    for (int k = tid; k < a.pieces; k += 256) d.weight[k] = seen_now(walk.sum + k);
+                    __syncthreads();
                 } else if (kid < 0) {
                     walk.lead(w, ++sweeps);
                     float m = -INFINITY;
                     for (int k = lane; k < a.pieces; k += 64) m = fmaxf(m, seen_now(walk.top + k));
                     m = uni(wave_max(m));
                     if (no_number(m)) break;
-                    w.Mp = m;
-                }
-                // the row's own sums, and of pieces that hold rejected tokens those without them
-                const bool own = kid >= 0 && !of_rest;
-                const double *own_sum = a.sum + (size_t)row * 2 * a.pieces;
-                const float *own_top = a.top + (size_t)row * 2 * a.chunks;
-                double *less = a.own_sum + (size_t)s * a.pieces;
-                // piece k's rejected tokens as bits of the wave's `gone`
-                auto mark = [&](int k) {
-                    wave_lds_sync();
-                    gone[wave][lane] = 0;
-                    wave_lds_sync();
-                    for (int j = at + 1 + lane; j < n; j += 64) {
-                        const int x = d.tok[j] - k * V_PIECE;
-                        if (d.par[j] == at && x >= 0 && x < V_PIECE) atomicOr(&gone[wave][x / 32], 1u << (x % 32));
-                    }
-                    wave_lds_sync();
-                };
-                const void *pr = row_of<TYPE>(a.logits, a.stride, row);
-                bool without = !with_q && kid >= 0;
-                if (without) {
-                    for (int k = tid; k < a.pieces; k += 256) less[k] = own_sum[k];
+                    w.Mp = Mp = m;
+                    for (int k = tid; k < a.pieces; k += 256) d.weight[k] = seen_now(walk.sum + k) * exp64((double)seen_now(walk.top + k) - Mp);
                     __syncthreads();
-                    // pieces that hold rejected tokens again, without those: each of them by one wave
-                    int i = 0;
-                    for (int j = kid; j >= 0; j = child(at, j)) {
-                        const int x = uni(d.tok[j]), k = x / V_PIECE;
-                        if (x < 0 || x >= V || earlier(at, j, [&](int y) { return y >= 0 && y / V_PIECE == k; })) continue;
-                        if (i++ % 4 != wave) continue;
-                        float v[4][8];
-#pragma unroll
-                        for (int h = 0; h < 4; h++) load8<TYPE>(pr, k * V_PIECE + h * 512 + lane * 8, V, v[h]);
-                        mark(k);
-                        double z = 0.0;
-                        const double m = own_top[k / V_PER];
-#pragma unroll
-                        for (int h = 0; h < 4; h++) {
-                            const uint32_t o = gone[wave][h * 16 + lane / 4] >> (8 * (lane % 4));
-#pragma unroll
-                            for (int e = 0; e < 8; e++) z += o >> e & 1 ? 0.0 : exp64((double)v[h][e] - m);
+                } else {
+                    // without the rejected tokens, which are taken off.  A piece of which less than a 16th is left, so that
+                    // what is left could be off by more than 2^-48, is summed again without them, by one wave.
+                    own_weights();
+                    if (tid == 0) listed = 0;
+                    __syncthreads();
+                    for (int k0 = 0; k0 < a.pieces; k0 += 256) {
+                        const int k = min(k0 + tid, a.pieces - 1);
+                        const double z = d.weight[k];
+                        double y = z;
+                        for (int j = kid; j >= 0; j = child(at, j))
+                            y -= d.tok[j] >= 0 && d.tok[j] < V && d.tok[j] / V_PIECE == k && !d.again[j] ? d.e[j] : 0.0;
+                        if (k0 + tid < a.pieces) {
+                            d.weight[k] = y;
+                            if (y < z / 16) d.list[atomicAdd(&listed, 1)] = (uint16_t)k;
                         }
+                    }
+                    __syncthreads();
+                    const int lists = uni(listed);
+                    for (int i = wave; i < lists; i += 4) {
+                        const int k = uni(d.list[i]);
+                        float v[4][8];
+                        load_stretch<TYPE, 4, 512>(walk.row_p(row), k * V_PIECE + lane * 8, (k + 1) * V_PIECE, V, v);
+                        uint32_t o[4] = {0, 0, 0, 0};
+                        for (int j = kid; j >= 0; j = child(at, j)) {
+                            const int x = d.tok[j] - k * V_PIECE;
+#pragma unroll
+                            for (int h = 0; h < 4; h++) o[h] |= x >= 0 && x >> 3 == h * 64 + lane ? 1u << (x & 7) : 0u;
+                        }
+                        double z = 0.0;
+#pragma unroll
+                        for (int h = 0; h < 4; h++)
+#pragma unroll
+                            for (int e = 0; e < 8; e++) z += o[h] >> e & 1 ? 0.0 : exp64((double)v[h][e] - Mp);
                         z = wave_add(z);
-                        if (lane == 0) less[k] = z;
+                        if (lane == 0) d.weight[k] = z;
                     }
                     __syncthreads();
                 }
-                auto weight_of = [&](int k) {
-                    if (own) return (without ? less : own_sum)[k] * exp64((double)own_top[k / V_PER] - w.Mp);
-                    const double z = seen_now(walk.sum + k);
-                    return of_rest ? z : z * exp64((double)seen_now(walk.top + k) - w.Mp);
-                };
-                auto all = [&]() {
-                    double z = 0.0;
-                    for (int k = lane; k < a.pieces; k += 64) z += weight_of(k);
-                    return wave_add(z);
-                };
-                double total = all();
-                if (without && !sure(total > 0.0)) {  // nothing left: of all that there was
-                    without = false;
-                    total = all();
+                double total = total_of();
+                if (kid >= 0 && !sure(total > 0.0)) {  // nothing left: of all that there was
+                    of_rest = without = false;
+                    own_weights();
+                    total = total_of();
                 }
                 // the piece in which the running sum passes the target, and the sum before it
                 const double target = d.u[0] * total;
                 double before = 0.0, start = 0.0;
                 int piece = -1, last = 0;
                 for (int k0 = 0; k0 < a.pieces && piece < 0; k0 += 64) {
-                    const double z = k0 + lane < a.pieces ? weight_of(k0 + lane) : 0.0, up = wave_upto(z, lane);
+                    const double z = k0 + lane < a.pieces ? d.weight[k0 + lane] : 0.0, up = sums_upto(z);
                     const uint64_t past = __ballot(before + up > target && z > 0.0), some = __ballot(z > 0.0);
                     if (some) last = k0 + 63 - __builtin_clzll(some);
                     if (past) {
                         const int k = __builtin_ctzll(past);
-                        piece = k0 + k, start = before + __shfl(up - z, k);
+                        piece = k0 + k, start = before + of_lane(up - z, k);
                     }
-                    before += __shfl(up, 63);
+                    before += of_lane(up, 63);
                 }
                 const bool behind = piece < 0;  // by a rounding: the last token there is
                 if (behind) piece = last;
-                float v[8], q[8];
+                float v[1][8], q[1][8];
                 double z[8], mine = 0.0;
-                load8<TYPE>(pr, piece * V_PIECE + tid * 8, V, v);
-                if (of_rest) load8<TYPE>(row_of<TYPE>(a.draft, a.draft_stride, row), piece * V_PIECE + tid * 8, V, q);
+                walk.load_piece(walk.row_p(row), piece, v);
+                if (of_rest) walk.load_piece(walk.row_q(row), piece, q);
                 uint32_t o = 0;
-                if (without) {
-                    mark(piece);
-                    o = gone[wave][tid / 4] >> (8 * (tid % 4));
+                if (without)
+                    for (int j = kid; j >= 0; j = child(at, j)) {
+                        const int x = d.tok[j] - piece * V_PIECE;
+                        o |= x >= 0 && x >> 3 == tid ? 1u << (x & 7) : 0u;
+                    }
+                if (of_rest) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) z[e] = walk.rest(w, v[0][e], q[0][e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) z[e] = o >> e & 1 ? 0.0 : exp64((double)v[0][e] - Mp);
                 }
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    z[e] = o >> e & 1 ? 0.0 : of_rest ? walk.rest(w, v[e], q[e]) : exp64((double)v[e] - w.Mp);
-                    mine += z[e];
-                }
-                const double up = wave_upto(mine, lane);
-                __syncthreads();
+                for (int e = 0; e < 8; e++) mine += z[e];
+                const double up = sums_upto(mine);
                 if (lane == 63) smd[wave] = up;
-                if (tid == 0) found = INT32_MAX;
                 __syncthreads();
                 double sum = start + (up - mine);
                 for (int k = 0; k < wave; k++) sum += smd[k];
@@ -687,17 +762,15 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
                         if (sum > target && hit == INT32_MAX) hit = most;
                     }
                 }
-                if (hit != INT32_MAX && !behind) atomicMin(&found, hit);
-                __syncthreads();
-                next = uni(found);
-                if (next == INT32_MAX) {
-                    __syncthreads();
-                    if (tid == 0) found = -1;
-                    __syncthreads();
-                    if (most >= 0) atomicMax(&found, most);
-                    __syncthreads();
-                    next = uni(found);
+                const uint64_t past = __ballot(hit != INT32_MAX), some = __ballot(most >= 0);
+                if (lane == 0) {
+                    hits[wave] = past ? __builtin_amdgcn_readlane(hit, __builtin_ctzll(past)) : INT32_MAX;
+                    lasts[wave] = some ? __builtin_amdgcn_readlane(most, 63 - __builtin_clzll(some)) : -1;
                 }
+                __syncthreads();
+                next = min(min(hits[0], hits[1]), min(hits[2], hits[3]));
+                if (behind || next == INT32_MAX) next = max(max(lasts[0], lasts[1]), max(lasts[2], lasts[3]));
+                next = uni(next);
             }
         }
         if (yes < 0) break;
@@ -706,7 +779,7 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
         kept++;
     }
     __syncthreads();
-    if (a.team > 1 && tid == 0) show(&walk.meet->number, V_END);
+    if (a.team > 1 && tid == 0) show(&meet->number, V_END);
     if (!n) kept = 0;
     int32_t *out = a.out + (size_t)s * a.t.max_nodes, *path = a.path + (size_t)s * a.t.max_nodes;
     for (int j = tid; j < a.t.max_nodes; j += 256) {
@@ -733,7 +806,6 @@ static size_t verify_layout(VerifyArgs &a, uint8_t *ws) {
     part(a.top, (size_t)a.t.n_tokens * 2 * a.chunks);
     part(a.arg, (size_t)a.t.n_tokens * a.chunks);
     part(a.swept_sum, (size_t)a.t.n_seqs * a.pieces);
-    part(a.own_sum, (size_t)a.t.n_seqs * a.pieces);
     part(a.swept_top, (size_t)a.t.n_seqs * a.pieces);
     part(a.meet, a.meet_words);
     return n;
@@ -759,7 +831,7 @@ hipError_t launch_verify(VerifyArgs a, int type, void *ws, hipStream_t st) {
     auto launch = [&](auto T) {
         constexpr int TYPE = decltype(T)::value;
         if (grid.x) TG_LAUNCH(k_verify_rows<TYPE>, grid, dim3(256), 0, st, a);
-        TG_LAUNCH(k_verify_walk<TYPE>, dim3((unsigned)(a.t.n_seqs * a.team)), dim3(256), WalkNodes::bytes(a.t.max_nodes), st, a);
+        TG_LAUNCH(k_verify_walk<TYPE>, dim3((unsigned)(a.t.n_seqs * a.team)), dim3(256), WalkNodes::bytes(a.t.max_nodes, a.pieces), st, a);
     };
     if (type == TG_T_F32) launch(std::integral_constant<int, TG_T_F32>{});
     else if (type == TG_T_F16) launch(std::integral_constant<int, TG_T_F16>{});

@@ -451,7 +451,7 @@ struct VerifyArgs {
     double *whole;     // [n_tokens][target, draft][chunks]
     float *top;        // [n_tokens][target, draft][chunks]
     int *arg;          // [n_tokens][chunks]
-    double *swept_sum, *own_sum;  // [n_seqs][pieces]
+    double *swept_sum; // [n_seqs][pieces]
     float *swept_top;
     uint32_t *meet;    // [n_seqs] of Meeting
     size_t meet_words;
