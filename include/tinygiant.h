@@ -521,10 +521,12 @@ typedef struct {
 } tg_draft_trees;
 /* What each node sees of its tree, bit i of the words bits[row]
  * [(max_nodes + 31) / 32] being set for itself and the nodes it follows, and
- * how many of those there are, depth[row].  Rows that are no nodes of a tree:
- * no bits, depth -1; rows behind the last sequence are not written. */
+ * how many of those there are, depth[row]; links[row] is twice the sequence,
+ * plus 1 where another node follows this one.  Rows that are no nodes of a
+ * tree: no bits, depth and links -1; of rows behind the last sequence links
+ * are written alone. */
 int tg_draft_tree_dev(const tg_draft_trees *t, uint32_t *bits, int32_t *depth,
-                      void *stream);
+                      int32_t *links, void *stream);
 /* tg_kv_append_q4_dev for nodes: node j goes to the place of the sequence's
  * j-th new token, rotated by the position of the first one plus depth[row]
  * (places may be behind max_pos, positions not).  A row of depth below 0 is
@@ -557,7 +559,8 @@ int tg_attn_tree_q4_dev(const tg_kv_batch *b, const uint32_t *bits, int words,
 int tg_kv_keep_q4_dev(const tg_kv_batch *b, int n_layers, int64_t layer_bytes,
                       const int32_t *path, int64_t path_stride, int path_cols,
                       const int32_t *count, int32_t *kv_len, void *stream);
-/* Which drafted tokens a target keeps.  logits [n_tokens][vocab] (any element
+/* Which drafted tokens a target keeps.  links are tg_draft_tree_dev's of the
+ * same trees.  logits [n_tokens][vocab] (any element
  * type, rows stride elements apart) are the target's after each row, draft
  * (NULL, or the same type and shape) those of the model that the tokens were
  * drawn from, tokens[row] the drafts, u[row] random numbers in [0, 1).  With p
@@ -580,9 +583,9 @@ int tg_kv_keep_q4_dev(const tg_kv_batch *b, int n_layers, int64_t layer_bytes,
  * temperature is below infinity.  workspace: at least tg_verify_workspace
  * bytes, 16-byte aligned, free again when the call's work is done. */
 size_t tg_verify_workspace(const tg_draft_trees *t, int vocab);
-int tg_verify_dev(const tg_draft_trees *t, int type, const void *logits,
-                  int64_t stride, const void *draft, int64_t draft_stride,
-                  int vocab, const int32_t *tokens, const double *u,
+int tg_verify_dev(const tg_draft_trees *t, const int32_t *links, int type,
+                  const void *logits, int64_t stride, const void *draft,
+                  int64_t draft_stride, int vocab, const int32_t *tokens, const double *u,
                   float temperature, const float *temperatures,
                   int32_t *out_tokens, int32_t *path, int32_t *count,
                   void *workspace, size_t workspace_bytes, void *stream);

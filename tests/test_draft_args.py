@@ -28,16 +28,17 @@ BAD_TREES = [(dict(cu=None), "cu is NULL"), (dict(n_seqs=-1), "n_seqs -1"), (dic
 
 @pytest.mark.parametrize("kw,msg", BAD_TREES)
 def test_trees_are_refused(lib, kw, msg):
-    assert lib.tg_draft_tree_dev(ctypes.byref(trees(**kw)), P, P, None) == INVALID and msg in said(lib)
+    assert lib.tg_draft_tree_dev(ctypes.byref(trees(**kw)), P, P, P, None) == INVALID and msg in said(lib)
 
 
 def test_tree_refuses(lib):
     t = trees()
-    assert lib.tg_draft_tree_dev(None, P, P, None) == INVALID and "trees is NULL" in said(lib)
-    assert lib.tg_draft_tree_dev(ctypes.byref(t), None, P, None) == INVALID
-    assert lib.tg_draft_tree_dev(ctypes.byref(t), P, None, None) == INVALID
+    assert lib.tg_draft_tree_dev(None, P, P, P, None) == INVALID and "trees is NULL" in said(lib)
+    assert lib.tg_draft_tree_dev(ctypes.byref(t), None, P, P, None) == INVALID
+    assert lib.tg_draft_tree_dev(ctypes.byref(t), P, None, P, None) == INVALID
+    assert lib.tg_draft_tree_dev(ctypes.byref(t), P, P, None, None) == INVALID and "links is NULL" in said(lib)
     for kw in (dict(n_seqs=0), dict(n_tokens=0)):
-        assert lib.tg_draft_tree_dev(ctypes.byref(trees(**kw)), P, P, None) == 0
+        assert lib.tg_draft_tree_dev(ctypes.byref(trees(**kw)), P, P, P, None) == 0
 
 
 def test_append_and_attend_of_trees_refuse(lib):
@@ -98,11 +99,11 @@ def test_python_refuses():
 
 # ---------------------------------------------------------------- verify
 def verify_args(lib, t=None, **kw):
-    d = dict(type=0, logits=P, stride=100, draft=P, dstride=100, vocab=100, tokens=P, u=P, temp=1.0, temps=None, out=P, path=P,
+    d = dict(links=P, type=0, logits=P, stride=100, draft=P, dstride=100, vocab=100, tokens=P, u=P, temp=1.0, temps=None, out=P, path=P,
              count=P, ws=P, n=1 << 40)
     d.update(kw)
     return lib.tg_verify_dev(ctypes.byref(t if t is not None else trees()), *[d[n] for n in (
-        "type", "logits", "stride", "draft", "dstride", "vocab", "tokens", "u", "temp", "temps", "out", "path", "count", "ws", "n")], None)
+        "links", "type", "logits", "stride", "draft", "dstride", "vocab", "tokens", "u", "temp", "temps", "out", "path", "count", "ws", "n")], None)
 
 
 @pytest.mark.parametrize("kw,msg", BAD_TREES)
@@ -113,7 +114,7 @@ def test_verify_refuses_trees(lib, kw, msg):
 
 
 @pytest.mark.parametrize("kw,msg", [
-    (dict(type=3), "element type 3"), (dict(logits=None), "NULL"), (dict(tokens=None), "NULL"), (dict(u=None), "NULL"),
+    (dict(type=3), "element type 3"), (dict(links=None), "NULL"), (dict(logits=None), "NULL"), (dict(tokens=None), "NULL"), (dict(u=None), "NULL"),
     (dict(out=None), "NULL"), (dict(path=None), "NULL"), (dict(count=None), "NULL"), (dict(vocab=0), "vocab 0"),
     (dict(vocab=(1 << 20) + 1, stride=1 << 25), "vocab 1048577"), (dict(stride=99), "overlap"), (dict(dstride=99), "overlap"),
     (dict(logits=P + 2), "aligned"), (dict(draft=P + 1, type=1), "aligned"), (dict(temp=float("inf")), "temperature inf"),

@@ -79,13 +79,17 @@ def test_trees(sizes, max_nodes):
         tree = DraftTree(dev(cu), T, None if kind == "none" else dev(flat), max_nodes=max_nodes)
         tree.bits.fill_(77)
         tree.depth.fill_(77)
+        tree.links.fill_(77)
         tree.build()
+        links = tree.links.cpu().numpy()
         bits, depth = tree.bits.cpu().numpy().view(np.uint32), tree.depth.cpu().numpy()
         for i, p in enumerate(parents):
             want = R.words(p, max_nodes)
             assert np.array_equal(bits[cu[i]:cu[i + 1]], want[0]), (kind, i)
             assert np.array_equal(depth[cu[i]:cu[i + 1]], want[1]), (kind, i)
-        assert (bits[cu[-1]:] == 77).all() and (depth[cu[-1]:] == 77).all()
+            follow = [j in [q for k, q in enumerate(p[:max_nodes]) if 0 <= q < k] for j in range(len(p))]
+            assert links[cu[i]:cu[i + 1]].tolist() == [-1 if want[1][j] < 0 else 2 * i + follow[j] for j in range(len(p))], (kind, i)
+        assert (bits[cu[-1]:] == 77).all() and (depth[cu[-1]:] == 77).all() and (links[cu[-1]:] == -1).all()
 
 
 def test_trees_of_fewer_rows_than_counted():

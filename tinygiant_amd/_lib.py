@@ -106,12 +106,12 @@ NEW_SYMBOLS = [
     ("tg_kv_read_q4_dev", CI, [VP, VP, VP, VP]),
     ("tg_attn_q4_workspace", SZ, [VP, CI, CI]),
     ("tg_attn_q4_dev", CI, [VP, CI, VP, I64, CI, CF, VP, I64, CI, VP, SZ, VP]),
-    ("tg_draft_tree_dev", CI, [VP, VP, VP, VP]),
+    ("tg_draft_tree_dev", CI, [VP, VP, VP, VP, VP]),
     ("tg_kv_append_tree_q4_dev", CI, [VP, VP, CI, VP, I64, VP, I64, VP, I64, VP, I64, CI, VP, VP, CF, VP, VP, CI, VP]),
     ("tg_attn_tree_q4_dev", CI, [VP, VP, CI, CI, VP, I64, CI, CF, VP, I64, CI, VP, SZ, VP]),
     ("tg_kv_keep_q4_dev", CI, [VP, CI, I64, VP, I64, CI, VP, VP, VP]),
     ("tg_verify_workspace", SZ, [VP, CI]),
-    ("tg_verify_dev", CI, [VP, CI, VP, I64, VP, I64, CI, VP, VP, CF, VP, VP, VP, VP, VP, SZ, VP]),
+    ("tg_verify_dev", CI, [VP, VP, CI, VP, I64, VP, I64, CI, VP, VP, CF, VP, VP, VP, VP, VP, SZ, VP]),
     ("tg_matmul_i8_workspace", SZ, [CI, CI, CI]),
     ("tg_matmul_i8_dev", CI, [VP, CI, I64, VP, CF, VP, VP, VP, I64, VP, CI, I64, CI, CI, CI, VP, SZ, VP]),
 ]

@@ -2658,16 +2658,17 @@ static int draft_trees(const char *fn, const tg_draft_trees *t, tg::DraftTrees *
     return TG_OK;
 }
 
-extern "C" int tg_draft_tree_dev(const tg_draft_trees *t, uint32_t *bits, int32_t *depth, void *stream) {
+extern "C" int tg_draft_tree_dev(const tg_draft_trees *t, uint32_t *bits, int32_t *depth, int32_t *links,
+                                 void *stream) {
     const char *fn = "tg_draft_tree_dev";
     tg::DraftTrees d;
     int rc = draft_trees(fn, t, &d);
     if (rc) return rc;
-    if (!bits || !depth) return set_err(TG_E_INVALID, "%s: bits or depth is NULL", fn);
+    if (!bits || !depth || !links) return set_err(TG_E_INVALID, "%s: bits, depth or links is NULL", fn);
     if (!d.n_seqs || !d.n_tokens) return TG_OK;
     DeviceOf dev(as_stream(stream));
     if (dev.rc) return dev.rc;
-    PROFILED("draft_tree", as_stream(stream), tg::launch_draft_tree(d, bits, depth, as_stream(stream)));
+    PROFILED("draft_tree", as_stream(stream), tg::launch_draft_tree(d, bits, depth, links, as_stream(stream)));
     return TG_OK;
 }
 
@@ -2685,8 +2686,8 @@ extern "C" size_t tg_verify_workspace(const tg_draft_trees *t, int vocab) {
     return verify_shape("tg_verify_workspace", t, vocab, &d) ? 0 : tg::verify_workspace(d, vocab);
 }
 
-extern "C" int tg_verify_dev(const tg_draft_trees *t, int type, const void *logits, int64_t stride, const void *draft,
-                             int64_t draft_stride, int vocab, const int32_t *tokens, const double *u,
+extern "C" int tg_verify_dev(const tg_draft_trees *t, const int32_t *links, int type, const void *logits,
+                             int64_t stride, const void *draft, int64_t draft_stride, int vocab, const int32_t *tokens, const double *u,
                              float temperature, const float *temperatures, int32_t *out_tokens, int32_t *path,
                              int32_t *count, void *workspace, size_t workspace_bytes, void *stream) {
     const char *fn = "tg_verify_dev";
@@ -2695,7 +2696,7 @@ extern "C" int tg_verify_dev(const tg_draft_trees *t, int type, const void *logi
     if (rc) return rc;
     if (type != TG_T_F32 && type != TG_T_F16 && type != TG_T_BF16)
         return set_err(TG_E_INVALID, "%s: element type %d", fn, type);
-    if (!out_tokens || !path || !count || (d.n_tokens && (!logits || !tokens || !u)))
+    if (!out_tokens || !path || !count || (d.n_tokens && (!links || !logits || !tokens || !u)))
         return set_err(TG_E_INVALID, "%s: a NULL pointer", fn);
     if (stride < vocab || (draft && draft_stride < vocab))
         return set_err(TG_E_INVALID, "%s: rows overlap (logits %lld, draft %lld apart)", fn, (long long)stride, (long long)draft_stride);
@@ -2711,7 +2712,7 @@ extern "C" int tg_verify_dev(const tg_draft_trees *t, int type, const void *logi
     DeviceOf dev(as_stream(stream));
     if (dev.rc) return dev.rc;
     tg::VerifyArgs a{};
-    a.t = d, a.logits = logits, a.stride = stride, a.draft = draft, a.draft_stride = draft_stride, a.vocab = vocab;
+    a.t = d, a.links = links, a.logits = logits, a.stride = stride, a.draft = draft, a.draft_stride = draft_stride, a.vocab = vocab;
     a.tokens = tokens, a.u = u, a.temps = temperatures, a.temp = temperature;
     a.out = out_tokens, a.path = path, a.count = count;
     PROFILED("verify", as_stream(stream), tg::launch_verify(a, type, workspace, as_stream(stream)));

@@ -33,12 +33,21 @@ TG_DEV int parent_of(const DraftTrees &t, int lo, int j) {
 // A block per sequence, a thread per node, which walks to its root through the parents in LDS and sets the bits of what it
 // meets, one word after the other.  Bound by latency: the rows' bounds, the parents, then a read of LDS a step, 1 us for
 // trees of ordinary depth.
-__global__ __launch_bounds__(256) void k_draft_tree(DraftTrees t, uint32_t *bits, int32_t *depth) {
+__global__ __launch_bounds__(256) void k_draft_tree(DraftTrees t, uint32_t *bits, int32_t *depth, int32_t *links) {
     __shared__ int16_t par[DT_NODES];
+    __shared__ uint8_t kids[DT_NODES];
     const TreeRows r = tree_rows(t, blockIdx.x);
     const int n = min(r.n, t.max_nodes), words = (t.max_nodes + 31) / 32;
-    for (int j = threadIdx.x; j < n; j += 256) par[j] = (int16_t)parent_of(t, r.lo, j);
+    for (int j = threadIdx.x; j < n; j += 256) par[j] = (int16_t)parent_of(t, r.lo, j), kids[j] = 0;
     __syncthreads();
+    for (int j = threadIdx.x; j < n; j += 256)
+        if (par[j] >= 0) kids[par[j]] = 1;
+    __syncthreads();
+    // rows before the first and behind the last sequence are no nodes either
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < r.lo; i += 256) links[i] = -1;
+    if (blockIdx.x == gridDim.x - 1)
+        for (int i = r.lo + r.n + threadIdx.x; i < t.n_tokens; i += 256) links[i] = -1;
     for (int j = threadIdx.x; j < r.n; j += 256) {
         uint32_t *out = bits + (size_t)(r.lo + j) * words;
         int d = -1, a = j < n ? j : DT_BAD, w = words;  // words from w on are written
@@ -59,11 +68,12 @@ __global__ __launch_bounds__(256) void k_draft_tree(DraftTrees t, uint32_t *bits
             d = -1;
         }
         depth[r.lo + j] = d;
+        links[r.lo + j] = d < 0 ? -1 : 2 * (int)blockIdx.x + kids[j];
     }
 }
 
-hipError_t launch_draft_tree(const DraftTrees &t, uint32_t *bits, int32_t *depth, hipStream_t st) {
-    TG_LAUNCH(k_draft_tree, dim3((unsigned)t.n_seqs), dim3(256), 0, st, t, bits, depth);
+hipError_t launch_draft_tree(const DraftTrees &t, uint32_t *bits, int32_t *depth, int32_t *links, hipStream_t st) {
+    TG_LAUNCH(k_draft_tree, dim3((unsigned)t.n_seqs), dim3(256), 0, st, t, bits, depth, links);
     return hipGetLastError();
 }
 
@@ -77,9 +87,10 @@ hipError_t launch_draft_tree(const DraftTrees &t, uint32_t *bits, int32_t *depth
 // before them had), and what is left is p without them.
 //
 // Whatever a random number decides is decided in 64 bits: probabilities, their sums and running sums.
-constexpr int V_CHUNK = 8192;  // values of a row to a block of the first launch
+constexpr int V_CHUNK = 4096;  // values of a row to a block of the first launch
 constexpr int V_PIECE = 2048;  // ... whose sum is kept
 constexpr int V_PER = V_CHUNK / V_PIECE;
+constexpr uint64_t V_ABSENT = ~0ull;  // in the place of a sum that is not there yet: a NaN that no sum is
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -217,12 +228,6 @@ TG_DEV T half_of(T v, int lane) {
 }
 TG_DEV double half_add(double v, int lane) { return half_of(wave_upto(v, 0.0, true, v_plus), lane); }
 TG_DEV float half_max(float v, int lane) { return half_of(wave_upto(v, -INFINITY, true, v_most), lane); }
-TG_DEV int wave_count(int v) {
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) v += __shfl_xor(v, m);
-    return uni(v);
-}
-
 // over the four waves of a block, in order; `sm` is 4 values that nothing else uses until the next barrier
 TG_DEV double block_add(double v, double *sm) {
     v = wave_add(v);
@@ -255,25 +260,17 @@ __global__ __launch_bounds__(256) void k_verify_rows(VerifyArgs a) {
         load_stretch<TYPE, V_PER, V_PIECE>(p, chunk * V_CHUNK + threadIdx.x * 8, (chunk + 1) * V_CHUNK, a.vocab, v);
     };
     if (a.early) load();
-    if (!of)
-        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < a.meet_words; i += (size_t)gridDim.x * 256) a.meet[i] = 0;
-    if (threadIdx.x < V_TABLE) exp_table(two, threadIdx.x);
-    int s = 0;
-    for (int j = lane; j < a.t.n_seqs; j += 64) s += a.t.cu[j + 1] <= row;
-    s = wave_count(s);
-    if (s >= a.t.n_seqs) return;
-    const TreeRows r = tree_rows(a.t, s);
-    const float t = uni(temperature_of(a, s));
-    const int node = row - r.lo, n = min(r.n, a.t.max_nodes);
-    if (node < 0 || node >= n) return;
-    const bool greedy = !(t > 0.0f);
-    if (greedy) {
-        if (of) return;
-    } else {
-        bool kid = false;
-        for (int j = node + 1 + lane; j < n; j += 64) kid |= parent_of(a.t, r.lo, j) == node;
-        if (!__ballot(kid)) return;
+    if (!of) {
+        const size_t all = (size_t)gridDim.x * 256, me = (size_t)blockIdx.x * 256 + threadIdx.x;
+        for (size_t i = me; i < a.meet_words; i += all) a.meet[i] = 0;
+        for (size_t i = me; i < (size_t)a.t.n_seqs * a.pieces; i += all) a.swept_sum[i] = V_ABSENT, a.swept_top[i] = (uint32_t)V_ABSENT;
     }
+    if (threadIdx.x < V_TABLE) exp_table(two, threadIdx.x);
+    const int link = uni(a.links[row]);  // twice the sequence, and whether something follows
+    if (link < 0 || link / 2 >= a.t.n_seqs) return;
+    const float t = uni(temperature_of(a, link / 2));
+    const bool greedy = !(t > 0.0f);
+    if (greedy ? of : !(link & 1)) return;
     if (!a.early) load();
     bool bad = false;
 #pragma unroll
@@ -315,9 +312,8 @@ __global__ __launch_bounds__(256) void k_verify_rows(VerifyArgs a) {
         const int k = threadIdx.x;
         double z = ((smd[0][k] + smd[1][k]) + smd[2][k]) + smd[3][k];
         if (chunk * V_PER + k < a.pieces) a.sum[at_row * a.pieces + chunk * V_PER + k] = z;
-        static_assert(V_PER == 4, "");
-        z += __shfl_xor(z, 1);
-        z += __shfl_xor(z, 2);
+#pragma unroll
+        for (int m = 1; m < V_PER; m *= 2) z += __shfl_xor(z, m);
         if (k == 0) a.whole[at_row * a.chunks + chunk] = z;
     }
 }
@@ -329,13 +325,13 @@ struct Sweep {
 };
 // How the blocks of one sequence's walk meet: the first to begin leads, the others help with its sweeps.  The leader
 // writes what a sweep is, then its number to `number`; every block that sees it (the leader too) takes pieces from its
-// counter until there are none, and counts those it has done.  Only the leader waits for something that others do, and only for
-// pieces that running blocks have taken; helpers wait for the leader, which runs.  So a walk ends however few of its blocks the
-// device runs at a time.
+// counter until there are none, and puts each one's sum where the leader sees that it is there.  Only the leader waits for something
+// that others do, and only for pieces that running blocks have taken; helpers wait for the leader, which runs.  So a walk ends
+// however few of its blocks the device runs at a time.
 struct Meeting {
     uint32_t ticket, number;
     Sweep sweep;
-    uint32_t taken_done[];  // [max_nodes + 2][2]
+    uint32_t taken[];  // [max_nodes + 2]
 };
 constexpr uint32_t V_END = ~0u;
 // What blocks hand to each other goes past the caches of an XCD, and what is to be seen first is waited for (a release at
@@ -350,11 +346,11 @@ template <int TYPE>
 struct Walk {
     const void *logits, *draft;
     int64_t stride, draft_stride;
-    int vocab, pieces, helpers;
+    int vocab, pieces;
     Exp64 exp64;
     Meeting *meet;
-    float *top;   // of a sweep's pieces: the largest value of each
-    double *sum;  // ... the sums
+    uint64_t *sums;  // of a sweep's pieces, as their bits
+    uint32_t *tops;  // the largest value of each, likewise
     float *smf;
     double *smd;
     uint32_t *smu;
@@ -386,16 +382,16 @@ struct Walk {
             if (m > -INFINITY && m < INFINITY)
 #pragma unroll
                 for (int e = 0; e < 8; e++) z += exp64((double)v[0][e] - m);
-            if (threadIdx.x == 0) show(top + k, m);
+            if (threadIdx.x == 0) show(tops + k, __float_as_uint(m));
         }
         z = block_add(z, smd);
-        if (threadIdx.x == 0) show(sum + k, z);
+        if (threadIdx.x == 0) show(sums + k, __builtin_bit_cast(uint64_t, z));
     }
     TG_DEV double rest(const Sweep &w, float v, float q) const {
         return fmax(exp64((double)v - w.Mp) * w.ip - exp64((double)q - w.Mq) * w.iq, 0.0);
     }
     TG_DEV void claim(uint32_t number) const {  // thread 0's
-        *smu = __hip_atomic_fetch_add(meet->taken_done + 2 * number, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *smu = __hip_atomic_fetch_add(meet->taken + number, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     // takes pieces of sweep `number` until there are none; the first is claimed
     TG_DEV void take(const Sweep &w, uint32_t number) const {
@@ -405,11 +401,7 @@ struct Walk {
             __syncthreads();
             if (k >= (uint32_t)pieces) return;
             piece(w, (int)k);
-            if (threadIdx.x == 0) {
-                shown();  // the piece's sum before it counts
-                __hip_atomic_fetch_add(meet->taken_done + 2 * number + 1, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                claim(number);
-            }
+            if (threadIdx.x == 0) claim(number);
         }
     }
     TG_DEV void help() const {
@@ -431,47 +423,59 @@ struct Walk {
             take(w, number);
         }
     }
-    // the leader's: a whole sweep
-    TG_DEV void lead(const Sweep &w, uint32_t number) const {
+    // the leader's: what the next sweep is, ahead of it where that is known
+    TG_DEV void announce(const Sweep &w) const {
+        if (threadIdx.x != 0) return;
+        show(&meet->sweep.row, w.row), show(&meet->sweep.Mp, w.Mp), show(&meet->sweep.ip, w.ip);
+        show(&meet->sweep.Mq, w.Mq), show(&meet->sweep.iq, w.iq);
+    }
+    // ... and a whole sweep that was announced: its pieces' sums to `sum`, their largest values to `top`
+    TG_DEV void lead(const Sweep &w, uint32_t number, double *sum, float *top) const {
+        shown();  // all of this block's, the marks in the places of the last sums among them
         __syncthreads();
-        if (!helpers) {
-            for (int k = 0; k < pieces; k++) piece(w, k);
-            shown();
-            __syncthreads();
-            return;
-        }
         if (threadIdx.x == 0) {
-            show(&meet->sweep.row, w.row), show(&meet->sweep.Mp, w.Mp), show(&meet->sweep.ip, w.ip);
-            show(&meet->sweep.Mq, w.Mq), show(&meet->sweep.iq, w.iq);
-            shown();
             show(&meet->number, number);
             claim(number);
         }
         take(w, number);
-        if (threadIdx.x == 0)
-            while (seen_now(meet->taken_done + 2 * number + 1) != (uint32_t)pieces) __builtin_amdgcn_s_sleep(1);
+        for (int k0 = 0; k0 < pieces; k0 += 256) {
+            const int k = min(k0 + (int)threadIdx.x, pieces - 1);
+            uint64_t z;
+            while (__ballot((z = seen_now(sums + k)) == V_ABSENT)) __builtin_amdgcn_s_sleep(1);
+            sum[k] = __builtin_bit_cast(double, z);
+            if (!uni((int)w.row & 1)) {
+                uint32_t m;
+                while (__ballot((m = seen_now(tops + k)) == (uint32_t)V_ABSENT)) __builtin_amdgcn_s_sleep(1);
+                top[k] = __uint_as_float(m);
+            }
+        }
         __syncthreads();
+        for (int k = threadIdx.x; k < pieces; k += 256) {
+            show(sums + k, (uint64_t)V_ABSENT);
+            if (!uni((int)w.row & 1)) show(tops + k, (uint32_t)V_ABSENT);
+        }
     }
 };
 
 // LDS of a walk, for `nodes` of them and rows of `pieces`
 struct WalkNodes {
-    double *u, *e, *inv;  // random numbers; exponentials of the nodes' logits at their parents; 1 / the rows' sums of those
-    double *weight;       // of the pieces of what is left
-    float *x, *top;       // the nodes' logits at their parents; the rows' largest values (e, inv, x, top: target's, then draft's)
+    double *u;        // random numbers
+    double *e, *inv;  // the nodes' logits at their parents, then exponentials of those; 1 / the rows' sums of exponentials
+    double *weight;   // of the pieces of what is left
+    float *top;       // the rows' largest values (e, inv, top: target's, then draft's)
+    float *most;      // of a sweep's pieces
+    uint16_t *list;   // in its place: pieces to be summed again
     int *tok;
     int16_t *par, *way;
-    uint8_t *again;       // an earlier sibling has the same token
-    uint16_t *list;       // pieces to be summed again
+    uint8_t *again;   // an earlier sibling has the same token
     TG_DEV WalkNodes(uint8_t *lds, int nodes, int pieces) {
         u = reinterpret_cast<double *>(lds), e = u + nodes, inv = e + 2 * nodes, weight = inv + 2 * nodes;
-        x = reinterpret_cast<float *>(weight + pieces), top = x + 2 * nodes;
-        tok = reinterpret_cast<int *>(top + 2 * nodes);
+        top = reinterpret_cast<float *>(weight + pieces), most = top + 2 * nodes, list = reinterpret_cast<uint16_t *>(most);
+        tok = reinterpret_cast<int *>(most + pieces);
         par = reinterpret_cast<int16_t *>(tok + nodes), way = par + nodes;
-        list = reinterpret_cast<uint16_t *>(way + nodes);
-        again = reinterpret_cast<uint8_t *>(list + pieces);
+        again = reinterpret_cast<uint8_t *>(way + nodes);
     }
-    static size_t bytes(int nodes, int pieces) { return (size_t)nodes * (5 * 8 + 5 * 4 + 2 * 2 + 1) + (size_t)pieces * (8 + 2); }
+    static constexpr size_t bytes(int nodes, int pieces) { return (size_t)nodes * (5 * 8 + 3 * 4 + 2 * 2 + 1) + (size_t)pieces * (8 + 4); }
 };
 
 // A sequence's walk: one block leads, the others help with sums over whole rows.  What decides where the leader goes is the
@@ -493,98 +497,98 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
     const bool greedy = !(t > 0.0f), with_q = a.draft && !greedy;
     if (tid < V_TABLE) exp_table(two, tid);
     const Exp64 exp64{factor_of(t), two};
-    const Walk<TYPE> walk{a.logits, a.draft, a.stride, a.draft_stride, V, a.pieces, a.team - 1, exp64, meet,
-                          a.swept_top + (size_t)s * a.pieces, a.swept_sum + (size_t)s * a.pieces, smf, smd, &smu};
+    const Walk<TYPE> walk{a.logits, a.draft, a.stride, a.draft_stride, V, a.pieces, exp64, meet,
+                          a.swept_sum + (size_t)s * a.pieces, a.swept_top + (size_t)s * a.pieces, smf, smd, &smu};
     __syncthreads();
     if (a.team > 1 && uni((int)smu)) {
         walk.help();
         return;
     }
-    const int n = uni(min(r.n, a.t.max_nodes)), lo = uni(r.lo);
-    const int N = a.t.max_nodes;
+    const int n = uni(min(r.n, a.t.max_nodes)), lo = uni(r.lo), N = a.t.max_nodes;
     const WalkNodes d(lds, N, a.pieces);
 
-    // Largest values and sums of the rows of nodes j0 .. j0 + 63, from those of their chunks: half a wave to a row, the
-    // next one's on their way.  Of rows that nothing follows they are whatever the memory holds, and not used.  For a
-    // greedy sequence the first of the largest stands in the place of the draft's logits.
-    const int l = lane % 32, each = with_q ? 2 : 1;
-    struct Part {
-        float m;
-        double z;
-    };
-    auto part = [&](int j0, int i) {
-        Part c{-INFINITY, 0.0};
-        const int j = j0 + i / each;
-        if (i < 64 * each && j < n && l < a.chunks) {
-            const size_t at = ((size_t)(lo + j) * 2 + i % each) * a.chunks + l;
-            c.m = a.top[at];
-            if (!greedy) c.z = a.whole[at];
-        }
-        return c;
-    };
-    auto join = [&](int j0, Part c) {
-        const int units = min(n - j0, 64) * each;
-        for (int i0 = 2 * wave; i0 < units; i0 += 8) {
-            const int i = i0 + lane / 32, j = j0 + i / each, of = i % each;
-            const bool live = i < units;
-            const Part next = part(j0, i + 8);
-            const size_t at = ((size_t)(lo + j) * 2 + of) * a.chunks;
-            float m = c.m;
-            for (int k = 32; k < a.chunks; k += 32)
-                if (live && k + l < a.chunks) m = fmaxf(m, a.top[at + k + l]);
-            m = half_max(m, lane);
-            if (live && l == 0) d.top[of * N + j] = m;
-            if (greedy) {
-                int best = INT32_MAX;
-                for (int k = 0; k < a.chunks; k += 32)
-                    if (live && k + l < a.chunks && a.top[at + k + l] == m) best = min(best, a.arg[(size_t)(lo + j) * a.chunks + k + l]);
+    // Largest values and sums of the rows of nodes j0 .. j0 + 63, from those of their chunks: half a wave to a row, four
+    // rows at a time.  Of rows that nothing follows they are whatever the memory holds, and not used.  For a greedy
+    // sequence the first of the largest stands in the place of the draft's logits.
+    auto join = [&](int j0) {
+        constexpr int B = 4;  // rows of a half wave at a time
+        const int l = lane % 32, each = with_q ? 2 : 1, units = min(n - j0, 64) * each;
+        for (int i0 = 2 * wave; i0 < units; i0 += 8 * B) {
+            float m[B][2];
+            double z[B][2];
+            size_t at[B];
 #pragma unroll
-                for (int k = 1; k < 32; k *= 2) best = min(best, __shfl_xor(best, k));
-                if (live && l == 0) d.x[N + j] = __int_as_float(best);
-            } else {
-                double z = c.z * exp64((double)c.m - m);
-                for (int k = 32; k < a.chunks; k += 32)
-                    if (live && k + l < a.chunks) z += a.whole[at + k + l] * exp64((double)a.top[at + k + l] - m);
-                z = half_add(z, lane);
-                if (live && l == 0) d.inv[of * N + j] = 1.0 / z;
+            for (int b = 0; b < B; b++) {
+                const int i = min(i0 + 8 * b + lane / 32, units - 1);
+                at[b] = ((size_t)(lo + j0 + i / each) * 2 + i % each) * a.chunks;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int k = min(l + 32 * h, a.chunks - 1);
+                    m[b][h] = a.top[at[b] + k];
+                    z[b][h] = a.whole[at[b] + k];
+                }
             }
-            c = next;
+#pragma unroll
+            for (int b = 0; b < B; b++) {
+                const int i = min(i0 + 8 * b + lane / 32, units - 1), j = j0 + i / each + i % each * N;
+                // the last lanes have the last chunk again: it counts once
+                const bool one = l < a.chunks, more = l + 32 < a.chunks;
+                float t = fmaxf(m[b][0], m[b][1]);
+                for (int k = 64 + l; k < a.chunks + l; k += 32) t = k < a.chunks ? fmaxf(t, a.top[at[b] + k]) : t;
+                t = half_max(t, lane);
+                if (l == 0) d.top[j] = t;
+                if (greedy) {
+                    int best = INT32_MAX;
+                    for (int k = l; k < a.chunks + l; k += 32)
+                        if (k < a.chunks && a.top[at[b] + k] == t) best = min(best, a.arg[at[b] / 2 + k]);
+#pragma unroll
+                    for (int k = 1; k < 32; k *= 2) best = min(best, __shfl_xor(best, k));
+                    if (l == 0) d.e[N + j] = best;
+                } else {
+                    double y = one ? z[b][0] * exp64((double)m[b][0] - t) : 0.0;
+                    y += more ? z[b][1] * exp64((double)m[b][1] - t) : 0.0;
+                    for (int k = 64 + l; k < a.chunks + l; k += 32) y += k < a.chunks ? a.whole[at[b] + k] * exp64((double)a.top[at[b] + k] - t) : 0.0;
+                    y = half_add(y, lane);
+                    if (l == 0) d.inv[j] = 1.0 / y;
+                }
+            }
         }
         __syncthreads();
         if (greedy) return;
         for (int j = j0 + 1 + tid; j < n; j += 256) {
             const int p = d.par[j];
             if (p < j0 || p >= j0 + 64) continue;
-            d.e[j] = exp64((double)d.x[j] - d.top[p]);
-            if (with_q) d.e[N + j] = exp64((double)d.x[N + j] - d.top[N + p]);
+            d.e[j] = exp64(d.e[j] - d.top[p]);
+            if (with_q) d.e[N + j] = exp64(d.e[N + j] - d.top[N + p]);
         }
         __syncthreads();
     };
-    Part first = part(0, 2 * wave + lane / 32);
     for (int j = tid; j < n; j += 256) {
         const int p = parent_of(a.t, lo, j), x = a.tokens[lo + j];
         const bool ok = p >= 0 && x >= 0 && x < V;
-        d.par[j] = (int16_t)p, d.tok[j] = x, d.u[j] = a.u[lo + j], d.again[j] = 0;
+        d.par[j] = (int16_t)p, d.tok[j] = x, d.u[j] = a.u[lo + j];
         if (!greedy) {
-            d.x[j] = ok ? load1<TYPE>(walk.row_p(lo + p), x) : -INFINITY;
-            if (with_q) d.x[N + j] = ok ? load1<TYPE>(walk.row_q(lo + p), x) : -INFINITY;
+            d.e[j] = ok ? load1<TYPE>(walk.row_p(lo + p), x) : -INFINITY;
+            if (with_q) d.e[N + j] = ok ? load1<TYPE>(walk.row_q(lo + p), x) : -INFINITY;
         }
     }
     __syncthreads();
+    if (!greedy && !with_q) {
+        for (int j = tid; j < n; j += 256) {
+            const int p = d.par[j], x = d.tok[j];
+            bool again = x < 0 || x >= V;
+            for (int k = max(p, 0) + 1; k < j; k++) again |= d.par[k] == p && d.tok[k] == x;
+            d.again[j] = again;
+        }
+        __syncthreads();
+    }
     // the next child of `node` behind j, or -1: the same in every wave, like all that follows
     auto child = [&](int node, int j) {
         for (int k = j + 1; k < n; k += 64) {
-            const uint64_t m = __ballot(k + lane < n && d.par[k + lane < n ? k + lane : 0] == node);
+            const uint64_t m = __ballot(k + lane < n && d.par[min(k + lane, n - 1)] == node);
             if (m) return k + __builtin_ctzll(m);
         }
         return -1;
-    };
-    // is there a child of `node` before j with its token
-    auto earlier = [&](int node, int j) {
-        const int x = uni(d.tok[j]);
-        for (int k = node + 1; k < j; k += 64)
-            if (__ballot(k + lane < j && d.par[k + lane < j ? k + lane : 0] == node && d.tok[k + lane < j ? k + lane : 0] == x)) return true;
-        return false;
     };
     auto no_number = [](float m) { return m == INFINITY || m == -INFINITY; };
     auto total_of = [&]() {  // of the pieces' weights
@@ -600,73 +604,89 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
         const int row = lo + at, kid = child(at, at);
         int yes = -1;
         if (at >= joined) {
-            join(at, at ? part(at, 2 * wave + lane / 32) : first);
+            join(at);
             joined = at + 64;
         }
         if (greedy) {
             if (no_number(uni(d.top[at]))) break;
-            const int best = uni(__float_as_int(d.x[N + at]));
-            for (int k = kid; k >= 0 && yes < 0; k = child(at, k))
-                if (uni(d.tok[k]) == best) yes = k;
-            if (yes < 0) next = best;
+            next = uni((int)d.e[N + at]);
+            for (int k = at + 1; k < n && yes < 0; k += 64) {
+                const int j = min(k + lane, n - 1);
+                const uint64_t m = __ballot(k + lane < n && d.par[j] == at && d.tok[j] == next);
+                if (m) yes = k + __builtin_ctzll(m);
+            }
+            if (yes >= 0) next = -1;
         } else {
-            double Mp = 0, ip = 1, Mq = 0, iq = 1, c = 0;
+            Sweep w{2 * (uint64_t)row, 0.0, 1.0, 0.0, 1.0};
+            double c = 0.0;
             if (kid >= 0) {
-                Mp = d.top[at], ip = d.inv[at];
-                if (with_q) Mq = d.top[N + at], iq = d.inv[N + at];
-                if (no_number(uni((float)Mp)) || no_number(uni((float)Mq))) break;
+                w.Mp = d.top[at], w.ip = d.inv[at];
+                if (with_q) w.row++, w.Mq = d.top[N + at], w.iq = d.inv[N + at];
+                if (no_number(uni((float)w.Mp)) || no_number(uni((float)w.Mq))) break;
+            }
+            const double iq = w.iq;
+            if (with_q || kid < 0) walk.announce(w);  // with the c of the first that is rejected, 1
+            if (with_q) {
                 double left = 1.0;
                 for (int k = kid, after; k >= 0; k = after) {
                     after = child(at, k);
-                    const double px = d.e[k] * ip;
-                    if (with_q) {
-                        const double qx = d.e[N + k] * iq;
-                        if (sure(d.u[k] * left * qx < px - c * qx)) {
-                            yes = k;
-                            break;
-                        }
-                        c += left;
-                        if (after >= 0) {
-                            walk.lead({2 * (uint64_t)row + 1, Mp, ip, Mq, c * iq}, ++sweeps);
-                            double z = 0.0;
-                            for (int k0 = lane; k0 < a.pieces; k0 += 64) z += seen_now(walk.sum + k0);
-                            left = wave_add(z);
-                        }
-                    } else if (earlier(at, k)) {  // rejected already
-                        if (tid == 0) d.again[k] = 1;
-                    } else {
-                        if (sure(px > 0.0 && d.u[k] * left < px)) {
-                            yes = k;
-                            break;
-                        }
-                        left -= px;
+                    const double px = d.e[k] * w.ip, qx = d.e[N + k] * iq;
+                    if (sure(d.u[k] * left * qx < px - c * qx)) {
+                        yes = k;
+                        break;
                     }
+                    c += left;
+                    w.iq = c * iq;
+                    if (after >= 0) {
+                        if (c != 1.0) walk.announce(w);
+                        walk.lead(w, ++sweeps, d.weight, d.most);
+                        left = total_of();
+                    }
+                }
+            } else {
+                // side by side: each candidate with what those before it have left
+                double left = 1.0;
+                for (int k = at + 1; k < n && yes < 0 && kid >= 0; k += 64) {
+                    const int j = min(k + lane, n - 1);
+                    const double px = k + lane < n && d.par[j] == at && !d.again[j] ? d.e[j] * w.ip : 0.0, up = sums_upto(px);
+                    const uint64_t m = __ballot(px > 0.0 && d.u[j] * (left - (up - px)) < px);
+                    if (m) yes = k + __builtin_ctzll(m);
+                    left -= of_lane(up, 63);
                 }
             }
             if (yes < 0) {
                 if (!sure(d.u[0] >= 0.0 && d.u[0] < 1.0)) break;
-                // what is left, by pieces: of the row of a leaf and of p - c q by a sweep, else by the row's own sums
-                Sweep w{2 * (uint64_t)row, Mp, ip, Mq, c * iq};
+                // what is left, by pieces: of p - c q and of the row of a leaf by a sweep, else by the row's own sums
                 bool of_rest = with_q && kid >= 0, without = !with_q && kid >= 0;
                 auto own_weights = [&]() {
                     __syncthreads();
                     for (int k = tid; k < a.pieces; k += 256)
-                        d.weight[k] = a.sum[(size_t)row * 2 * a.pieces + k] * exp64((double)a.top[(size_t)row * 2 * a.chunks + k / V_PER] - Mp);
+                        d.weight[k] = a.sum[(size_t)row * 2 * a.pieces + k] * exp64((double)a.top[(size_t)row * 2 * a.chunks + k / V_PER] - w.Mp);
                     __syncthreads();
                 };
+                // the candidates that were rejected (all), one after the other: their tokens and exponentials
+                auto rejected = [&](auto f) {
+                    for (int k = at + 1; k < n; k += 64) {
+                        const int j = min(k + lane, n - 1), x = d.tok[j];
+                        const double e = d.e[j];
+                        for (uint64_t m = __ballot(k + lane < n && d.par[j] == at && !d.again[j]); m; m &= m - 1) {
+                            const int i = __builtin_ctzll(m);
+                            f(__builtin_amdgcn_readlane(x, i), of_lane(e, i));
+                        }
+                    }
+                };
                 if (of_rest) {
-                    w.row++;
-                    walk.lead(w, ++sweeps);
-                    for (int k = tid; k < a.pieces; k += 256) d.weight[k] = seen_now(walk.sum + k);
-                    __syncthreads();
+                    if (c != 1.0) walk.announce(w);
+                    walk.lead(w, ++sweeps, d.weight, d.most);
                 } else if (kid < 0) {
-                    walk.lead(w, ++sweeps);
+                    w.row &= ~1ull;
+                    walk.lead(w, ++sweeps, d.weight, d.most);
                     float m = -INFINITY;
-                    for (int k = lane; k < a.pieces; k += 64) m = fmaxf(m, seen_now(walk.top + k));
+                    for (int k = lane; k < a.pieces; k += 64) m = fmaxf(m, d.most[k]);
                     m = uni(wave_max(m));
                     if (no_number(m)) break;
-                    w.Mp = Mp = m;
-                    for (int k = tid; k < a.pieces; k += 256) d.weight[k] = seen_now(walk.sum + k) * exp64((double)seen_now(walk.top + k) - Mp);
+                    w.Mp = m;
+                    for (int k = tid; k < a.pieces; k += 256) d.weight[k] *= exp64((double)d.most[k] - w.Mp);
                     __syncthreads();
                 } else {
                     // without the rejected tokens, which are taken off.  A piece of which less than a 16th is left, so that
@@ -678,8 +698,7 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
                         const int k = min(k0 + tid, a.pieces - 1);
                         const double z = d.weight[k];
                         double y = z;
-                        for (int j = kid; j >= 0; j = child(at, j))
-                            y -= d.tok[j] >= 0 && d.tok[j] < V && d.tok[j] / V_PIECE == k && !d.again[j] ? d.e[j] : 0.0;
+                        rejected([&](int x, double e) { y -= x / V_PIECE == k ? e : 0.0; });
                         if (k0 + tid < a.pieces) {
                             d.weight[k] = y;
                             if (y < z / 16) d.list[atomicAdd(&listed, 1)] = (uint16_t)k;
@@ -692,16 +711,16 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
                         float v[4][8];
                         load_stretch<TYPE, 4, 512>(walk.row_p(row), k * V_PIECE + lane * 8, (k + 1) * V_PIECE, V, v);
                         uint32_t o[4] = {0, 0, 0, 0};
-                        for (int j = kid; j >= 0; j = child(at, j)) {
-                            const int x = d.tok[j] - k * V_PIECE;
+                        rejected([&](int x, double) {
+                            x -= k * V_PIECE;
 #pragma unroll
                             for (int h = 0; h < 4; h++) o[h] |= x >= 0 && x >> 3 == h * 64 + lane ? 1u << (x & 7) : 0u;
-                        }
+                        });
                         double z = 0.0;
 #pragma unroll
                         for (int h = 0; h < 4; h++)
 #pragma unroll
-                            for (int e = 0; e < 8; e++) z += o[h] >> e & 1 ? 0.0 : exp64((double)v[h][e] - Mp);
+                            for (int e = 0; e < 8; e++) z += o[h] >> e & 1 ? 0.0 : exp64((double)v[h][e] - w.Mp);
                         z = wave_add(z);
                         if (lane == 0) d.weight[k] = z;
                     }
@@ -735,16 +754,16 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
                 if (of_rest) walk.load_piece(walk.row_q(row), piece, q);
                 uint32_t o = 0;
                 if (without)
-                    for (int j = kid; j >= 0; j = child(at, j)) {
-                        const int x = d.tok[j] - piece * V_PIECE;
+                    rejected([&](int x, double) {
+                        x -= piece * V_PIECE;
                         o |= x >= 0 && x >> 3 == tid ? 1u << (x & 7) : 0u;
-                    }
+                    });
                 if (of_rest) {
 #pragma unroll
                     for (int e = 0; e < 8; e++) z[e] = walk.rest(w, v[0][e], q[0][e]);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) z[e] = o >> e & 1 ? 0.0 : exp64((double)v[0][e] - Mp);
+                    for (int e = 0; e < 8; e++) z[e] = o >> e & 1 ? 0.0 : exp64((double)v[0][e] - w.Mp);
                 }
 #pragma unroll
                 for (int e = 0; e < 8; e++) mine += z[e];
@@ -781,8 +800,8 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
     __syncthreads();
     if (a.team > 1 && tid == 0) show(&meet->number, V_END);
     if (!n) kept = 0;
-    int32_t *out = a.out + (size_t)s * a.t.max_nodes, *path = a.path + (size_t)s * a.t.max_nodes;
-    for (int j = tid; j < a.t.max_nodes; j += 256) {
+    int32_t *out = a.out + (size_t)s * N, *path = a.path + (size_t)s * N;
+    for (int j = tid; j < N; j += 256) {
         path[j] = j < kept ? d.way[j] : -1;
         out[j] = j + 1 < kept ? d.tok[d.way[j + 1]] : j + 1 == kept ? next : -1;
     }
@@ -795,7 +814,7 @@ static size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 static size_t verify_layout(VerifyArgs &a, uint8_t *ws) {
     a.chunks = (a.vocab + V_CHUNK - 1) / V_CHUNK, a.pieces = (a.vocab + V_PIECE - 1) / V_PIECE;
     // 8-byte aligned words of one sequence
-    a.meet_words = (sizeof(Meeting) / 4 + 2 * (a.t.max_nodes + 2) + 1) / 2 * 2 * (size_t)a.t.n_seqs;
+    a.meet_words = (sizeof(Meeting) / 4 + a.t.max_nodes + 2 + 1) / 2 * 2 * (size_t)a.t.n_seqs;
     size_t n = 0;
     auto part = [&](auto *&p, size_t count) {
         p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(ws + n);
@@ -814,6 +833,8 @@ static size_t verify_layout(VerifyArgs &a, uint8_t *ws) {
 bool verify_fits(const DraftTrees &t, int vocab) {
     return (int64_t)t.n_tokens * ((vocab + V_CHUNK - 1) / V_CHUNK) <= UINT32_MAX / 256;
 }
+
+static_assert(WalkNodes::bytes(DT_NODES, (1 << 20) / V_PIECE) + 1024 <= 65536, "a walk's LDS");
 
 size_t verify_workspace(const DraftTrees &t, int vocab) {
     VerifyArgs a{};

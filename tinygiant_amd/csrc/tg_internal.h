@@ -430,9 +430,10 @@ struct DraftTrees {
     const int32_t *cu, *parent;
     int n_seqs, n_tokens, max_nodes;
 };
-hipError_t launch_draft_tree(const DraftTrees &t, uint32_t *bits, int32_t *depth, hipStream_t st);
+hipError_t launch_draft_tree(const DraftTrees &t, uint32_t *bits, int32_t *depth, int32_t *links, hipStream_t st);
 struct VerifyArgs {
     DraftTrees t;
+    const int32_t *links;
     const void *logits;
     int64_t stride;
     const void *draft;
@@ -451,8 +452,8 @@ struct VerifyArgs {
     double *whole;     // [n_tokens][target, draft][chunks]
     float *top;        // [n_tokens][target, draft][chunks]
     int *arg;          // [n_tokens][chunks]
-    double *swept_sum; // [n_seqs][pieces]
-    float *swept_top;
+    uint64_t *swept_sum;  // [n_seqs][2][pieces]
+    uint32_t *swept_top;
     uint32_t *meet;    // [n_seqs] of Meeting
     size_t meet_words;
 };

@@ -63,6 +63,7 @@ class DraftTree:
         self.words = (self.max_nodes + 31) // 32
         self.bits = torch.empty((self.n_tokens, self.words), dtype=torch.int32, device=self.device)
         self.depth = torch.empty(self.n_tokens, dtype=torch.int32, device=self.device)
+        self.links = torch.empty_like(self.depth)  # for verify
         self.build()
 
     def _trees(self) -> _Trees:
@@ -72,7 +73,8 @@ class DraftTree:
     def build(self) -> "DraftTree":
         """bits and depth from cu and parent as they now are."""
         if self.n_tokens and self.n_seqs:
-            run_on(self.depth, "tg_draft_tree_dev", ctypes.byref(self._trees()), self.bits.data_ptr(), self.depth.data_ptr())
+            run_on(self.depth, "tg_draft_tree_dev", ctypes.byref(self._trees()), self.bits.data_ptr(), self.depth.data_ptr(),
+                   self.links.data_ptr())
         return self
 
 
@@ -146,7 +148,7 @@ def verify(logits, tokens, u, tree: DraftTree, draft=None, temperature=1.0) -> V
         ref = ctypes.byref(t)
         n = require_lib().tg_verify_workspace(ref, V)
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        run_on(logits, "tg_verify_dev", ref, TYPES[logits.dtype], logits.data_ptr(), stride,
+        run_on(logits, "tg_verify_dev", ref, tree.links.data_ptr(), TYPES[logits.dtype], logits.data_ptr(), stride,
                None if draft is None else draft.data_ptr(), dstride, V, tokens.data_ptr(), u.data_ptr(), temp, temps,
                out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), ws.data_ptr() if n else None, n)
     return Verified(*out)
