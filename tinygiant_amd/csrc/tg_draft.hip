@@ -482,7 +482,7 @@ struct WalkNodes {
 // same in all of its lanes, and told so to the compiler (uni, sure): with branches by lanes, what it moved between registers behind
 // a loop was moved with all lanes off, and lost (rejected tokens of some waves were drawn).
 template <int TYPE>
-__global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
+__global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ double smd[4], two[V_TABLE];
     __shared__ float smf[4];
@@ -511,50 +511,59 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
     // rows at a time.  Of rows that nothing follows they are whatever the memory holds, and not used.  For a greedy
     // sequence the first of the largest stands in the place of the draft's logits.
     auto join = [&](int j0) {
-        constexpr int B = 4;  // rows of a half wave at a time
-        const int l = lane % 32, each = with_q ? 2 : 1, units = min(n - j0, 64) * each;
+        const int l = lane % 32, two_rows = with_q, units = min(n - j0, 64) << two_rows;
+        // of the unit that a half wave has: its place among the rows' parts; among the nodes'
+        auto row_at = [&](int i) { return ((size_t)(lo + j0 + (i >> two_rows)) * 2 + (i & two_rows)) * a.chunks; };
+        auto node_at = [&](int i) { return j0 + (i >> two_rows) + (i & two_rows) * N; };
+        if (greedy) {
+#pragma unroll 1
+            for (int i0 = 2 * wave; i0 < units; i0 += 8) {
+                const int i = min(i0 + lane / 32, units - 1);
+                const float *top = a.top + row_at(i);
+                float m = -INFINITY;
+                for (int k = l; k < a.chunks + l; k += 32) m = fmaxf(m, top[min(k, a.chunks - 1)]);
+                m = half_max(m, lane);
+                int best = INT32_MAX;
+                for (int k = l; k < a.chunks + l; k += 32)
+                    if (k < a.chunks && top[k] == m) best = min(best, a.arg[row_at(i) / 2 + k]);
+#pragma unroll
+                for (int k = 1; k < 32; k *= 2) best = min(best, __shfl_xor(best, k));
+                if (l == 0) d.top[node_at(i)] = m, d.e[N + j0 + i] = best;
+            }
+            __syncthreads();
+            return;
+        }
+        constexpr int B = 4;
+#pragma unroll 1
         for (int i0 = 2 * wave; i0 < units; i0 += 8 * B) {
             float m[B][2];
             double z[B][2];
-            size_t at[B];
 #pragma unroll
-            for (int b = 0; b < B; b++) {
-                const int i = min(i0 + 8 * b + lane / 32, units - 1);
-                at[b] = ((size_t)(lo + j0 + i / each) * 2 + i % each) * a.chunks;
+            for (int b = 0; b < B; b++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int k = min(l + 32 * h, a.chunks - 1);
-                    m[b][h] = a.top[at[b] + k];
-                    z[b][h] = a.whole[at[b] + k];
+                    const size_t at = row_at(min(i0 + 8 * b + lane / 32, units - 1)) + min(l + 32 * h, a.chunks - 1);
+                    m[b][h] = a.top[at];
+                    z[b][h] = l + 32 * h < a.chunks ? a.whole[at] : 0.0;
                 }
-            }
 #pragma unroll
             for (int b = 0; b < B; b++) {
-                const int i = min(i0 + 8 * b + lane / 32, units - 1), j = j0 + i / each + i % each * N;
-                // the last lanes have the last chunk again: it counts once
-                const bool one = l < a.chunks, more = l + 32 < a.chunks;
+                if (i0 + 8 * b >= units) break;
+                const int i = min(i0 + 8 * b + lane / 32, units - 1);
                 float t = fmaxf(m[b][0], m[b][1]);
-                for (int k = 64 + l; k < a.chunks + l; k += 32) t = k < a.chunks ? fmaxf(t, a.top[at[b] + k]) : t;
+                if (a.chunks > 64)
+                    for (int k = 64 + l; k < a.chunks + l; k += 32) t = fmaxf(t, a.top[row_at(i) + min(k, a.chunks - 1)]);
                 t = half_max(t, lane);
-                if (l == 0) d.top[j] = t;
-                if (greedy) {
-                    int best = INT32_MAX;
-                    for (int k = l; k < a.chunks + l; k += 32)
-                        if (k < a.chunks && a.top[at[b] + k] == t) best = min(best, a.arg[at[b] / 2 + k]);
-#pragma unroll
-                    for (int k = 1; k < 32; k *= 2) best = min(best, __shfl_xor(best, k));
-                    if (l == 0) d.e[N + j] = best;
-                } else {
-                    double y = one ? z[b][0] * exp64((double)m[b][0] - t) : 0.0;
-                    y += more ? z[b][1] * exp64((double)m[b][1] - t) : 0.0;
-                    for (int k = 64 + l; k < a.chunks + l; k += 32) y += k < a.chunks ? a.whole[at[b] + k] * exp64((double)a.top[at[b] + k] - t) : 0.0;
-                    y = half_add(y, lane);
-                    if (l == 0) d.inv[j] = 1.0 / y;
-                }
+                double y = z[b][0] * exp64((double)m[b][0] - t) + z[b][1] * exp64((double)m[b][1] - t);
+                if (a.chunks > 64)
+#pragma unroll 1
+                    for (int k = 64 + l; k < a.chunks + l; k += 32)
+                        y += k < a.chunks ? a.whole[row_at(i) + k] * exp64((double)a.top[row_at(i) + k] - t) : 0.0;
+                y = half_add(y, lane);
+                if (l == 0) d.top[node_at(i)] = t, d.inv[node_at(i)] = 1.0 / y;
             }
         }
         __syncthreads();
-        if (greedy) return;
         for (int j = j0 + 1 + tid; j < n; j += 256) {
             const int p = d.par[j];
             if (p < j0 || p >= j0 + 64) continue;
@@ -573,15 +582,6 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
         }
     }
     __syncthreads();
-    if (!greedy && !with_q) {
-        for (int j = tid; j < n; j += 256) {
-            const int p = d.par[j], x = d.tok[j];
-            bool again = x < 0 || x >= V;
-            for (int k = max(p, 0) + 1; k < j; k++) again |= d.par[k] == p && d.tok[k] == x;
-            d.again[j] = again;
-        }
-        __syncthreads();
-    }
     // the next child of `node` behind j, or -1: the same in every wave, like all that follows
     auto child = [&](int node, int j) {
         for (int k = j + 1; k < n; k += 64) {
@@ -625,38 +625,53 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
                 if (no_number(uni((float)w.Mp)) || no_number(uni((float)w.Mq))) break;
             }
             const double iq = w.iq;
-            if (with_q || kid < 0) walk.announce(w);  // with the c of the first that is rejected, 1
-            if (with_q) {
+            if (with_q || kid < 0) {
+                // each child that is rejected leaves a sweep's sums, by pieces: to the next one, or to be drawn from; as
+                // does the row of a leaf
+                walk.announce(w);  // with the c of the first that is rejected, 1
                 double left = 1.0;
-                for (int k = kid, after; k >= 0; k = after) {
-                    after = child(at, k);
-                    const double px = d.e[k] * w.ip, qx = d.e[N + k] * iq;
-                    if (sure(d.u[k] * left * qx < px - c * qx)) {
-                        yes = k;
-                        break;
-                    }
-                    c += left;
-                    w.iq = c * iq;
-                    if (after >= 0) {
+                for (int k = kid;;) {
+                    if (k >= 0) {
+                        const double px = d.e[k] * w.ip, qx = d.e[N + k] * iq;
+                        if (sure(d.u[k] * left * qx < px - c * qx)) {
+                            yes = k;
+                            break;
+                        }
+                        c += left;
+                        w.iq = c * iq;
                         if (c != 1.0) walk.announce(w);
-                        walk.lead(w, ++sweeps, d.weight, d.most);
-                        left = total_of();
+                        k = child(at, k);
                     }
+                    walk.lead(w, ++sweeps, d.weight, d.most);
+                    if (k < 0) break;
+                    left = total_of();
                 }
             } else {
-                // side by side: each candidate with what those before it have left
+                // side by side: each candidate with what those before it have left; one whose token was asked before, or is
+                // none, has nothing
                 double left = 1.0;
-                for (int k = at + 1; k < n && yes < 0 && kid >= 0; k += 64) {
-                    const int j = min(k + lane, n - 1);
-                    const double px = k + lane < n && d.par[j] == at && !d.again[j] ? d.e[j] * w.ip : 0.0, up = sums_upto(px);
+                for (int k = at + 1; k < n && yes < 0; k += 64) {
+                    const int j = min(k + lane, n - 1), x = d.tok[j];
+                    const bool mine = k + lane < n && d.par[j] == at;
+                    bool again = x < 0 || x >= V;
+                    for (int i = at + 1; i <= k; i += 64) {
+                        const int y = d.tok[min(i + lane, n - 1)];
+                        for (uint64_t m = __ballot(i + lane < n && d.par[min(i + lane, n - 1)] == at); m; m &= m - 1) {
+                            const int f = __builtin_ctzll(m);
+                            again |= i + f < k + lane && __builtin_amdgcn_readlane(y, f) == x;
+                        }
+                    }
+                    if (mine) d.again[j] = again;
+                    const double px = mine && !again ? d.e[j] * w.ip : 0.0, up = sums_upto(px);
                     const uint64_t m = __ballot(px > 0.0 && d.u[j] * (left - (up - px)) < px);
                     if (m) yes = k + __builtin_ctzll(m);
                     left -= of_lane(up, 63);
                 }
+                __syncthreads();
             }
             if (yes < 0) {
                 if (!sure(d.u[0] >= 0.0 && d.u[0] < 1.0)) break;
-                // what is left, by pieces: of p - c q and of the row of a leaf by a sweep, else by the row's own sums
+                // what is left, by pieces: a sweep's sums, or the row's own
                 bool of_rest = with_q && kid >= 0, without = !with_q && kid >= 0;
                 auto own_weights = [&]() {
                     __syncthreads();
@@ -675,12 +690,7 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
                         }
                     }
                 };
-                if (of_rest) {
-                    if (c != 1.0) walk.announce(w);
-                    walk.lead(w, ++sweeps, d.weight, d.most);
-                } else if (kid < 0) {
-                    w.row &= ~1ull;
-                    walk.lead(w, ++sweeps, d.weight, d.most);
+                if (kid < 0) {
                     float m = -INFINITY;
                     for (int k = lane; k < a.pieces; k += 64) m = fmaxf(m, d.most[k]);
                     m = uni(wave_max(m));
@@ -688,7 +698,7 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
                     w.Mp = m;
                     for (int k = tid; k < a.pieces; k += 256) d.weight[k] *= exp64((double)d.most[k] - w.Mp);
                     __syncthreads();
-                } else {
+                } else if (without) {
                     // without the rejected tokens, which are taken off.  A piece of which less than a 16th is left, so that
                     // what is left could be off by more than 2^-48, is summed again without them, by one wave.
                     own_weights();
@@ -708,19 +718,19 @@ __global__ __launch_bounds__(256, 3) void k_verify_walk(VerifyArgs a) {
                     const int lists = uni(listed);
                     for (int i = wave; i < lists; i += 4) {
                         const int k = uni(d.list[i]);
-                        float v[4][8];
-                        load_stretch<TYPE, 4, 512>(walk.row_p(row), k * V_PIECE + lane * 8, (k + 1) * V_PIECE, V, v);
-                        uint32_t o[4] = {0, 0, 0, 0};
-                        rejected([&](int x, double) {
-                            x -= k * V_PIECE;
-#pragma unroll
-                            for (int h = 0; h < 4; h++) o[h] |= x >= 0 && x >> 3 == h * 64 + lane ? 1u << (x & 7) : 0u;
-                        });
                         double z = 0.0;
+#pragma unroll 1
+                        for (int h = 0; h < 4; h++) {
+                            float v[1][8];
+                            load_stretch<TYPE, 1, 0>(walk.row_p(row), k * V_PIECE + h * 512 + lane * 8, (k + 1) * V_PIECE, V, v);
+                            uint32_t o = 0;
+                            rejected([&](int x, double) {
+                                x -= k * V_PIECE + h * 512;
+                                o |= x >= 0 && x >> 3 == lane ? 1u << (x & 7) : 0u;
+                            });
 #pragma unroll
-                        for (int h = 0; h < 4; h++)
-#pragma unroll
-                            for (int e = 0; e < 8; e++) z += o[h] >> e & 1 ? 0.0 : exp64((double)v[h][e] - w.Mp);
+                            for (int e = 0; e < 8; e++) z += o >> e & 1 ? 0.0 : exp64((double)v[0][e] - w.Mp);
+                        }
                         z = wave_add(z);
                         if (lane == 0) d.weight[k] = z;
                     }
@@ -847,7 +857,7 @@ hipError_t launch_verify(VerifyArgs a, int type, void *ws, hipStream_t st) {
     const dim3 grid((unsigned)(a.t.n_tokens * a.chunks), a.draft ? 2 : 1);
     // blocks to a walk: as many as the row has pieces, but what the device holds at once for all walks at the most; one
     // where nothing is swept
-    a.team = grid.x && (a.temps || a.temp > 0.0f) ? std::max(1, std::min(a.pieces, 768 / a.t.n_seqs)) : 1;
+    a.team = grid.x && (a.temps || a.temp > 0.0f) ? std::max(1, std::min(a.pieces, 1024 / a.t.n_seqs)) : 1;
     a.early = grid.x * grid.y <= 1024;
     auto launch = [&](auto T) {
         constexpr int TYPE = decltype(T)::value;
