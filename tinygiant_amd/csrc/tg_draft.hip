@@ -90,7 +90,8 @@ hipError_t launch_draft_tree(const DraftTrees &t, uint32_t *bits, int32_t *depth
 constexpr int V_CHUNK = 4096;  // values of a row to a block of the first launch
 constexpr int V_PIECE = 2048;  // ... whose sum is kept
 constexpr int V_PER = V_CHUNK / V_PIECE;
-constexpr uint64_t V_ABSENT = ~0ull;  // in the place of a sum that is not there yet: a NaN that no sum is
+constexpr uint64_t V_ABSENT = ~0ull;  // in the place of what is not there yet: a NaN that no number of a walk is
+constexpr int V_WORDS = 5;            // of a sweep
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -262,7 +263,9 @@ __global__ __launch_bounds__(256) void k_verify_rows(VerifyArgs a) {
     if (a.early) load();
     if (!of) {
         const size_t all = (size_t)gridDim.x * 256, me = (size_t)blockIdx.x * 256 + threadIdx.x;
-        for (size_t i = me; i < a.meet_words; i += all) a.meet[i] = 0;
+        const size_t numbers = (size_t)a.t.n_seqs * (a.t.max_nodes + 2);
+        for (size_t i = me; i < numbers; i += all) a.taken[i] = 0;
+        for (size_t i = me; i < numbers * V_WORDS; i += all) a.sweeps[i] = V_ABSENT;
         for (size_t i = me; i < (size_t)a.t.n_seqs * a.pieces; i += all) a.swept_sum[i] = V_ABSENT, a.swept_top[i] = (uint32_t)V_ABSENT;
     }
     if (threadIdx.x < V_TABLE) exp_table(two, threadIdx.x);
@@ -323,17 +326,13 @@ struct Sweep {
     uint64_t row;           // times 2; + 1: sums of max(p - c q, 0); else of exp((v - largest) / T), each piece by itself
     double Mp, ip, Mq, iq;  // p = exp((v - Mp) / T) ip, c q likewise
 };
-// How the blocks of one sequence's walk meet: the first to begin leads, the others help with its sweeps.  The leader
-// writes what a sweep is, then its number to `number`; every block that sees it (the leader too) takes pieces from its
-// counter until there are none, and puts each one's sum where the leader sees that it is there.  Only the leader waits for something
-// that others do, and only for pieces that running blocks have taken; helpers wait for the leader, which runs.  So a walk ends
-// however few of its blocks the device runs at a time.
-struct Meeting {
-    uint32_t ticket, number;
-    Sweep sweep;
-    uint32_t taken[];  // [max_nodes + 2]
-};
-constexpr uint32_t V_END = ~0u;
+// How the blocks of one sequence's walk meet: the first to begin (taken[0] says which) leads, the others help with its
+// sweeps.  A sweep has a number, from 1 on, five words that say what it is, and a counter that pieces are taken from.
+// Each block takes its first piece before it knows what the sweep is; words and sums are waited for one by one, in places
+// that are written once.  Only the leader waits for something that others do, and only for pieces that running
+// blocks have taken; helpers wait for the leader, which runs.  So a walk ends however few of its blocks the device runs at a
+// time.
+constexpr uint64_t V_END = ~1ull;  // in the place of a sweep's row: there are no more
 // What blocks hand to each other goes past the caches of an XCD, and what is to be seen first is waited for (a release at
 // the device's scope writes back a whole L2).
 template <class T>
@@ -347,8 +346,10 @@ struct Walk {
     const void *logits, *draft;
     int64_t stride, draft_stride;
     int vocab, pieces;
+    bool ahead;      // pieces are taken before the last one is summed
     Exp64 exp64;
-    Meeting *meet;
+    uint32_t *taken;
+    uint64_t *sweeps;
     uint64_t *sums;  // of a sweep's pieces, as their bits
     uint32_t *tops;  // the largest value of each, likewise
     float *smf;
@@ -360,17 +361,27 @@ struct Walk {
     TG_DEV void load_piece(const void *row, int k, float v[1][8]) const {
         load_stretch<TYPE, 1, 0>(row, k * V_PIECE + (int)threadIdx.x * 8, (k + 1) * V_PIECE, vocab, v);
     }
+    TG_DEV void load_both(int row, int k, float v[2][8]) const {
+        const int i = k * V_PIECE + (int)threadIdx.x * 8;
+        if ((k + 1) * V_PIECE <= vocab) {  // one branch around the loads of both
+            load8<TYPE>(row_p(row), i, v[0]);
+            load8<TYPE>(row_q(row), i, v[1]);
+        } else {
+            load_piece(row_p(row), k, v);
+            load_piece(row_q(row), k, v + 1);
+        }
+    }
     // piece k of a sweep, by one block
     TG_DEV void piece(const Sweep &w, int k) const {
         const int row = uni((int)(w.row >> 1));
-        float v[1][8], q[1][8];
-        load_piece(row_p(row), k, v);
+        float v[2][8];
         double z = 0.0;
         if (uni((int)w.row & 1)) {
-            load_piece(row_q(row), k, q);
+            load_both(row, k, v);
 #pragma unroll
-            for (int e = 0; e < 8; e++) z += rest(w, v[0][e], q[0][e]);
+            for (int e = 0; e < 8; e++) z += rest(w, v[0][e], v[1][e]);
         } else {
+            load_piece(row_p(row), k, v);
             float m = -INFINITY;
             bool bad = false;
 #pragma unroll
@@ -390,54 +401,52 @@ struct Walk {
     TG_DEV double rest(const Sweep &w, float v, float q) const {
         return fmax(exp64((double)v - w.Mp) * w.ip - exp64((double)q - w.Mq) * w.iq, 0.0);
     }
-    TG_DEV void claim(uint32_t number) const {  // thread 0's
-        *smu = __hip_atomic_fetch_add(meet->taken + number, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    // takes pieces of sweep `number` until there are none; the first is claimed
-    TG_DEV void take(const Sweep &w, uint32_t number) const {
+    TG_DEV uint32_t claim(uint32_t number) const { return __hip_atomic_fetch_add(taken + number, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+    // takes pieces of sweep `number` until there are none; thread 0 has the first
+    TG_DEV void take(const Sweep &w, uint32_t number, uint32_t mine) const {
         for (;;) {
             __syncthreads();
-            const uint32_t k = uni((int)*smu);
+            if (threadIdx.x == 0) *smu = mine;
             __syncthreads();
+            const uint32_t k = uni((int)*smu);
             if (k >= (uint32_t)pieces) return;
+            if (ahead && threadIdx.x == 0) mine = claim(number);
             piece(w, (int)k);
-            if (threadIdx.x == 0) claim(number);
+            if (!ahead && threadIdx.x == 0) mine = claim(number);
         }
     }
     TG_DEV void help() const {
-        for (uint32_t number = 0;;) {
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                uint32_t now;
-                while ((now = seen_now(&meet->number)) == number) __builtin_amdgcn_s_sleep(2);
-                *smu = now;
+        for (uint32_t number = 1;; number++) {
+            uint32_t mine = 0;
+            if (threadIdx.x == 0) mine = claim(number);
+            uint64_t x[V_WORDS];
+            for (;;) {
+                bool there = true;
+#pragma unroll
+                for (int i = 0; i < V_WORDS; i++) {
+                    x[i] = seen_now(sweeps + (size_t)number * V_WORDS + i);
+                    there &= x[i] != V_ABSENT;
+                }
+                if (__ballot(x[0] == V_END)) return;
+                if (__ballot(there)) break;
+                __builtin_amdgcn_s_sleep(2);
             }
-            __syncthreads();
-            number = uni((int)*smu);
-            __syncthreads();
-            if (number == V_END) return;
-            // this sweep's as long as pieces of it can be taken: a later one's is not worked on
-            const Sweep w{seen_now(&meet->sweep.row), seen_now(&meet->sweep.Mp), seen_now(&meet->sweep.ip), seen_now(&meet->sweep.Mq),
-                          seen_now(&meet->sweep.iq)};
-            if (threadIdx.x == 0) claim(number);
-            take(w, number);
+            take({x[0], __builtin_bit_cast(double, x[1]), __builtin_bit_cast(double, x[2]), __builtin_bit_cast(double, x[3]),
+                  __builtin_bit_cast(double, x[4])}, number, mine);
         }
     }
-    // the leader's: what the next sweep is, ahead of it where that is known
-    TG_DEV void announce(const Sweep &w) const {
-        if (threadIdx.x != 0) return;
-        show(&meet->sweep.row, w.row), show(&meet->sweep.Mp, w.Mp), show(&meet->sweep.ip, w.ip);
-        show(&meet->sweep.Mq, w.Mq), show(&meet->sweep.iq, w.iq);
-    }
-    // ... and a whole sweep that was announced: its pieces' sums to `sum`, their largest values to `top`
+    // the leader's: a whole sweep, its pieces' sums to `sum`, their largest values to `top`
     TG_DEV void lead(const Sweep &w, uint32_t number, double *sum, float *top) const {
         shown();  // all of this block's, the marks in the places of the last sums among them
         __syncthreads();
+        uint32_t mine = 0;
         if (threadIdx.x == 0) {
-            show(&meet->number, number);
-            claim(number);
+            uint64_t *x = sweeps + (size_t)number * V_WORDS;
+            show(x, w.row), show(x + 1, __builtin_bit_cast(uint64_t, w.Mp)), show(x + 2, __builtin_bit_cast(uint64_t, w.ip));
+            show(x + 3, __builtin_bit_cast(uint64_t, w.Mq)), show(x + 4, __builtin_bit_cast(uint64_t, w.iq));
+            mine = claim(number);
         }
-        take(w, number);
+        take(w, number, mine);
         for (int k0 = 0; k0 < pieces; k0 += 256) {
             const int k = min(k0 + (int)threadIdx.x, pieces - 1);
             uint64_t z;
@@ -487,18 +496,20 @@ __global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
     __shared__ double smd[4], two[V_TABLE];
     __shared__ float smf[4];
     __shared__ int hits[4], lasts[4];
+    __shared__ uint8_t inner[4][64];
     __shared__ uint32_t smu;
     __shared__ int listed;
     const int tid = threadIdx.x, lane = tid % 64, wave = uni(tid / 64), s = blockIdx.x % a.t.n_seqs, V = a.vocab;
-    Meeting *meet = reinterpret_cast<Meeting *>(a.meet + s * (a.meet_words / a.t.n_seqs));
-    if (a.team > 1 && tid == 0) smu = __hip_atomic_fetch_add(&meet->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    uint32_t *taken = a.taken + (size_t)s * (a.t.max_nodes + 2);
+    if (a.team > 1 && tid == 0) smu = __hip_atomic_fetch_add(taken, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const TreeRows r = tree_rows(a.t, s);
     const float t = uni(temperature_of(a, s));
     const bool greedy = !(t > 0.0f), with_q = a.draft && !greedy;
     if (tid < V_TABLE) exp_table(two, tid);
     const Exp64 exp64{factor_of(t), two};
-    const Walk<TYPE> walk{a.logits, a.draft, a.stride, a.draft_stride, V, a.pieces, exp64, meet,
-                          a.swept_sum + (size_t)s * a.pieces, a.swept_top + (size_t)s * a.pieces, smf, smd, &smu};
+    const Walk<TYPE> walk{a.logits, a.draft, a.stride, a.draft_stride, V, a.pieces, a.pieces > 2 * a.team, exp64, taken,
+                          a.sweeps + (size_t)s * (a.t.max_nodes + 2) * V_WORDS, a.swept_sum + (size_t)s * a.pieces,
+                          a.swept_top + (size_t)s * a.pieces, smf, smd, &smu};
     __syncthreads();
     if (a.team > 1 && uni((int)smu)) {
         walk.help();
@@ -508,13 +519,18 @@ __global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
     const WalkNodes d(lds, N, a.pieces);
 
     // Largest values and sums of the rows of nodes j0 .. j0 + 63, from those of their chunks: half a wave to a row, four
-    // rows at a time.  Of rows that nothing follows they are whatever the memory holds, and not used.  For a greedy
-    // sequence the first of the largest stands in the place of the draft's logits.
+    // rows at a time.  For a greedy sequence the first of the largest stands in the place of the draft's logits.
     auto join = [&](int j0) {
-        const int l = lane % 32, two_rows = with_q, units = min(n - j0, 64) << two_rows;
+        // those that something follows, of greedy sequences all
+        const int link = j0 + lane < n ? a.links[lo + j0 + lane] : -1;
+        const bool asked = j0 + lane < n && (greedy || link & 1);
+        const uint64_t asks = __ballot(asked);
+        if (asked) inner[wave][__builtin_popcountll(asks & ((1ull << lane) - 1))] = (uint8_t)lane;
+        wave_lds_sync();
+        const int l = lane % 32, two_rows = with_q, units = __builtin_popcountll(asks) << two_rows;
         // of the unit that a half wave has: its place among the rows' parts; among the nodes'
-        auto row_at = [&](int i) { return ((size_t)(lo + j0 + (i >> two_rows)) * 2 + (i & two_rows)) * a.chunks; };
-        auto node_at = [&](int i) { return j0 + (i >> two_rows) + (i & two_rows) * N; };
+        auto row_at = [&](int i) { return ((size_t)(lo + j0 + inner[wave][i >> two_rows]) * 2 + (i & two_rows)) * a.chunks; };
+        auto node_at = [&](int i) { return j0 + inner[wave][i >> two_rows] + (i & two_rows) * N; };
         if (greedy) {
 #pragma unroll 1
             for (int i0 = 2 * wave; i0 < units; i0 += 8) {
@@ -528,7 +544,7 @@ __global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
                     if (k < a.chunks && top[k] == m) best = min(best, a.arg[row_at(i) / 2 + k]);
 #pragma unroll
                 for (int k = 1; k < 32; k *= 2) best = min(best, __shfl_xor(best, k));
-                if (l == 0) d.top[node_at(i)] = m, d.e[N + j0 + i] = best;
+                if (l == 0) d.top[node_at(i)] = m, d.e[N + node_at(i)] = best;
             }
             __syncthreads();
             return;
@@ -628,7 +644,6 @@ __global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
             if (with_q || kid < 0) {
                 // each child that is rejected leaves a sweep's sums, by pieces: to the next one, or to be drawn from; as
                 // does the row of a leaf
-                walk.announce(w);  // with the c of the first that is rejected, 1
                 double left = 1.0;
                 for (int k = kid;;) {
                     if (k >= 0) {
@@ -639,7 +654,6 @@ __global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
                         }
                         c += left;
                         w.iq = c * iq;
-                        if (c != 1.0) walk.announce(w);
                         k = child(at, k);
                     }
                     walk.lead(w, ++sweeps, d.weight, d.most);
@@ -808,7 +822,7 @@ __global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
         kept++;
     }
     __syncthreads();
-    if (a.team > 1 && tid == 0) show(&meet->number, V_END);
+    if (a.team > 1 && tid == 0) show(walk.sweeps + (size_t)(sweeps + 1) * V_WORDS, (uint64_t)V_END);
     if (!n) kept = 0;
     int32_t *out = a.out + (size_t)s * N, *path = a.path + (size_t)s * N;
     for (int j = tid; j < N; j += 256) {
@@ -823,8 +837,6 @@ static size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // Where the workspace's parts are; its size.
 static size_t verify_layout(VerifyArgs &a, uint8_t *ws) {
     a.chunks = (a.vocab + V_CHUNK - 1) / V_CHUNK, a.pieces = (a.vocab + V_PIECE - 1) / V_PIECE;
-    // 8-byte aligned words of one sequence
-    a.meet_words = (sizeof(Meeting) / 4 + a.t.max_nodes + 2 + 1) / 2 * 2 * (size_t)a.t.n_seqs;
     size_t n = 0;
     auto part = [&](auto *&p, size_t count) {
         p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(ws + n);
@@ -836,7 +848,8 @@ static size_t verify_layout(VerifyArgs &a, uint8_t *ws) {
     part(a.arg, (size_t)a.t.n_tokens * a.chunks);
     part(a.swept_sum, (size_t)a.t.n_seqs * a.pieces);
     part(a.swept_top, (size_t)a.t.n_seqs * a.pieces);
-    part(a.meet, a.meet_words);
+    part(a.sweeps, (size_t)a.t.n_seqs * (a.t.max_nodes + 2) * V_WORDS);
+    part(a.taken, (size_t)a.t.n_seqs * (a.t.max_nodes + 2));
     return n;
 }
 
@@ -844,7 +857,7 @@ bool verify_fits(const DraftTrees &t, int vocab) {
     return (int64_t)t.n_tokens * ((vocab + V_CHUNK - 1) / V_CHUNK) <= UINT32_MAX / 256;
 }
 
-static_assert(WalkNodes::bytes(DT_NODES, (1 << 20) / V_PIECE) + 1024 <= 65536, "a walk's LDS");
+static_assert(WalkNodes::bytes(DT_NODES, (1 << 20) / V_PIECE) + 768 <= 65536, "a walk's LDS");
 
 size_t verify_workspace(const DraftTrees &t, int vocab) {
     VerifyArgs a{};

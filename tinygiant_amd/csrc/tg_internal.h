@@ -454,8 +454,8 @@ struct VerifyArgs {
     int *arg;          // [n_tokens][chunks]
     uint64_t *swept_sum;  // [n_seqs][2][pieces]
     uint32_t *swept_top;
-    uint32_t *meet;    // [n_seqs] of Meeting
-    size_t meet_words;
+    uint64_t *sweeps;     // [n_seqs][max_nodes + 2][5]
+    uint32_t *taken;      // [n_seqs][max_nodes + 2]
 };
 bool verify_fits(const DraftTrees &t, int vocab);  // in the threads of a launch
 size_t verify_workspace(const DraftTrees &t, int vocab);
