@@ -90,8 +90,7 @@ hipError_t launch_draft_tree(const DraftTrees &t, uint32_t *bits, int32_t *depth
 constexpr int V_CHUNK = 4096;  // values of a row to a block of the first launch
 constexpr int V_PIECE = 2048;  // ... whose sum is kept
 constexpr int V_PER = V_CHUNK / V_PIECE;
-constexpr uint64_t V_ABSENT = ~0ull;  // in the place of what is not there yet: a NaN that no number of a walk is
-constexpr int V_WORDS = 5;            // of a sweep
+constexpr int V_ROUNDS = 8;    // sweeps that have launches of their own
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -146,38 +145,40 @@ TG_DEV const void *row_of(const void *p, int64_t stride, int row) {
     return static_cast<const uint8_t *>(p) + (int64_t)row * stride * (TYPE == TG_T_F32 ? 4 : 2);
 }
 
-// Exponentials of what is 0 or below, to some 2^-50: exp(d / T) = 2^(y / 32), y = d 32 log2(e) / T, by the nearest whole
-// number n of y from a table of 2^(j / 32) and the power of 2, and the rest f, at most 1/2, by the Taylor polynomial of
-// 2^(f / 32) of degree 6 (what it leaves out is below 2^-57).  Below 2^-1021 the result is 0.  14 operations on doubles; without the
-// table, by the remainder of ln 2 and degree 13, 26.
+// Exponentials of what is 0 or below, to some 2^-51: exp(d / T) = 2^(y / 32), y = d 32 log2(e) / T, is 2^(j / 32) from a
+// table times the power of 2 that the nearest whole number n = 32 i + j of y gives, times 2^(f / 32) for the rest f, at most 1/2, by
+// the polynomial of degree 5 that has its values at the six Chebyshev nodes (off by 2^-52.6, the constant rounded to 1).
+// Below 2^-1021 the result is 0.  13 operations on doubles; by the remainder of ln 2 and Taylor's polynomial 26.
 constexpr int V_TABLE = 32;
 struct Exp64 {
-    double by;          // 32 log2(e) / T
-    const double *two;  // 2^(j / 32)
+    double by, least;     // 32 log2(e) / T; the least d whose exponential is not 0
+    const uint64_t *two;  // 2^(j / 32), its exponent's half less what n brings into it of j
     TG_DEV double operator()(double d) const {
-        const double y = d * by, t = y + 6755399441055744.0, f = y - (t - 6755399441055744.0);  // 1.5 2^52: its unit is 1
+        constexpr double ONES = 6755399441055744.0;  // 1.5 2^52: its unit is 1
+        const double t = __builtin_fma(d, by, ONES), f = __builtin_fma(d, by, -(t - ONES));
         const int n = (int)__builtin_bit_cast(uint64_t, t);
-        double p = 1.4345655584131934e-13;  // (ln 2 / 32)^i / i!
-        p = __builtin_fma(p, f, 3.973709984549416e-11);
-        p = __builtin_fma(p, f, 9.172562701824643e-09);
-        p = __builtin_fma(p, f, 1.693850972437182e-06);
-        p = __builtin_fma(p, f, 0.0002345961982022468);
+        double p = 3.9737266313166245e-11;
+        p = __builtin_fma(p, f, 9.172616498159851e-09);
+        p = __builtin_fma(p, f, 1.6938509724215757e-06);
+        p = __builtin_fma(p, f, 0.0002345961981972034);
         p = __builtin_fma(p, f, 0.02166084939249829);
         p = __builtin_fma(p, f, 1.0);
-        const uint64_t w = __builtin_bit_cast(uint64_t, two[n & (V_TABLE - 1)]) + ((uint64_t)(uint32_t)(n >> 5) << 52);
-        const double r = __builtin_bit_cast(double, w) * p;
-        return y > -32.0 * 1021.0 ? r : 0.0;
+        const uint64_t w = two[n & (V_TABLE - 1)];
+        const uint32_t hi = (uint32_t)(w >> 32) + ((uint32_t)n << 15);
+        const double r = __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)w) * p;
+        return d > least ? r : 0.0;
     }
 };
+TG_DEV Exp64 exp_of(double by, const uint64_t *two) { return {by, -32.0 * 1021.0 / by, two}; }
 // the table, by repeated square roots of 2: 2^(j / 32) is the product of those of j's bits
-TG_DEV void exp_table(double *two, int j) {
+TG_DEV void exp_table(uint64_t *two, int j) {
     double r = 1.0;
     if (j & 16) r *= 1.4142135623730951;
     if (j & 8) r *= 1.189207115002721;
     if (j & 4) r *= 1.0905077326652577;
     if (j & 2) r *= 1.0442737824274138;
     if (j & 1) r *= 1.0218971486541166;
-    two[j] = r;
+    two[j] = __builtin_bit_cast(uint64_t, r) - ((uint64_t)j << 47);
 }
 
 // the sequence's temperature; 32 log2(e) / T, so that -inf times it stays -inf
@@ -247,11 +248,12 @@ TG_DEV float block_max(float v, float *sm) {
 
 // The largest value of each chunk of the rows that a walk may ask (those that something follows, of greedy sequences
 // all), of the chunk and its pieces the sums of exp((v - largest) / T), or the place of the first of the largest.  NaN
-// or +inf: the largest is +inf.  The first blocks also clear what the walks' blocks meet by.
+// or +inf: the largest is +inf.
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_verify_rows(VerifyArgs a) {
     __shared__ float sm[4];
-    __shared__ double smd[4][V_PER], two[V_TABLE];
+    __shared__ double smd[4][V_PER];
+    __shared__ uint64_t two[V_TABLE];
     __shared__ int first;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks, of = blockIdx.y;
@@ -261,13 +263,6 @@ __global__ __launch_bounds__(256) void k_verify_rows(VerifyArgs a) {
         load_stretch<TYPE, V_PER, V_PIECE>(p, chunk * V_CHUNK + threadIdx.x * 8, (chunk + 1) * V_CHUNK, a.vocab, v);
     };
     if (a.early) load();
-    if (!of) {
-        const size_t all = (size_t)gridDim.x * 256, me = (size_t)blockIdx.x * 256 + threadIdx.x;
-        const size_t numbers = (size_t)a.t.n_seqs * (a.t.max_nodes + 2);
-        for (size_t i = me; i < numbers; i += all) a.taken[i] = 0;
-        for (size_t i = me; i < numbers * V_WORDS; i += all) a.sweeps[i] = V_ABSENT;
-        for (size_t i = me; i < (size_t)a.t.n_seqs * a.pieces; i += all) a.swept_sum[i] = V_ABSENT, a.swept_top[i] = (uint32_t)V_ABSENT;
-    }
     if (threadIdx.x < V_TABLE) exp_table(two, threadIdx.x);
     const int link = uni(a.links[row]);  // twice the sequence, and whether something follows
     if (link < 0 || link / 2 >= a.t.n_seqs) return;
@@ -300,7 +295,7 @@ __global__ __launch_bounds__(256) void k_verify_rows(VerifyArgs a) {
         return;
     }
     if (m == INFINITY) return;
-    const Exp64 exp64{factor_of(t), two};
+    const Exp64 exp64 = exp_of(factor_of(t), two);
 #pragma unroll
     for (int k = 0; k < V_PER; k++) {
         double sum = 0.0;
@@ -321,44 +316,21 @@ __global__ __launch_bounds__(256) void k_verify_rows(VerifyArgs a) {
     }
 }
 
-// What a walk asks of all the pieces of a row at once
-struct Sweep {
-    uint64_t row;           // times 2; + 1: sums of max(p - c q, 0); else of exp((v - largest) / T), each piece by itself
-    double Mp, ip, Mq, iq;  // p = exp((v - Mp) / T) ip, c q likewise
-};
-// How the blocks of one sequence's walk meet: the first to begin (taken[0] says which) leads, the others help with its
-// sweeps.  A sweep has a number, from 1 on, five words that say what it is, and a counter that pieces are taken from.
-// Each block takes its first piece before it knows what the sweep is; words and sums are waited for one by one, in places
-// that are written once.  Only the leader waits for something that others do, and only for pieces that running
-// blocks have taken; helpers wait for the leader, which runs.  So a walk ends however few of its blocks the device runs at a
-// time.
-constexpr uint64_t V_END = ~1ull;  // in the place of a sweep's row: there are no more
-// What blocks hand to each other goes past the caches of an XCD, and what is to be seen first is waited for (a release at
-// the device's scope writes back a whole L2).
-template <class T>
-TG_DEV T seen_now(const T *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-template <class T>
-TG_DEV void show(T *p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-TG_DEV void shown() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt 0: this thread's stores are acknowledged
-
+// One piece of a sweep, by a block: the sum of max(p - c q, 0) over it, or (leaf) its largest value and the sum of exp((v -
+// largest) / T).
 template <int TYPE>
-struct Walk {
+struct Pieces {
     const void *logits, *draft;
     int64_t stride, draft_stride;
-    int vocab, pieces;
-    bool ahead;      // pieces are taken before the last one is summed
+    int vocab;
     Exp64 exp64;
-    uint32_t *taken;
-    uint64_t *sweeps;
-    uint64_t *sums;  // of a sweep's pieces, as their bits
-    uint32_t *tops;  // the largest value of each, likewise
     float *smf;
     double *smd;
-    uint32_t *smu;
-
+    TG_DEV Pieces(const VerifyArgs &a, const Exp64 &e, float *f, double *d)
+        : logits(a.logits), draft(a.draft), stride(a.stride), draft_stride(a.draft_stride), vocab(a.vocab), exp64(e), smf(f), smd(d) {}
     TG_DEV const void *row_p(int row) const { return row_of<TYPE>(logits, stride, row); }
     TG_DEV const void *row_q(int row) const { return row_of<TYPE>(draft, draft_stride, row); }
-    TG_DEV void load_piece(const void *row, int k, float v[1][8]) const {
+    TG_DEV void load(const void *row, int k, float v[1][8]) const {
         load_stretch<TYPE, 1, 0>(row, k * V_PIECE + (int)threadIdx.x * 8, (k + 1) * V_PIECE, vocab, v);
     }
     TG_DEV void load_both(int row, int k, float v[2][8]) const {
@@ -367,21 +339,22 @@ struct Walk {
             load8<TYPE>(row_p(row), i, v[0]);
             load8<TYPE>(row_q(row), i, v[1]);
         } else {
-            load_piece(row_p(row), k, v);
-            load_piece(row_q(row), k, v + 1);
+            load(row_p(row), k, v);
+            load(row_q(row), k, v + 1);
         }
     }
-    // piece k of a sweep, by one block
-    TG_DEV void piece(const Sweep &w, int k) const {
-        const int row = uni((int)(w.row >> 1));
+    TG_DEV double rest(const WalkState &w, float v, float q) const {
+        return fmax(exp64((double)v - w.Mp) * w.ip - exp64((double)q - w.Mq) * w.iq, 0.0);
+    }
+    TG_DEV void operator()(const WalkState &w, int k, double &sum, float &top) const {
         float v[2][8];
         double z = 0.0;
-        if (uni((int)w.row & 1)) {
-            load_both(row, k, v);
+        if (!uni(w.leaf)) {
+            load_both(uni(w.row), k, v);
 #pragma unroll
             for (int e = 0; e < 8; e++) z += rest(w, v[0][e], v[1][e]);
         } else {
-            load_piece(row_p(row), k, v);
+            load(row_p(uni(w.row)), k, v);
             float m = -INFINITY;
             bool bad = false;
 #pragma unroll
@@ -389,82 +362,35 @@ struct Walk {
                 bad |= !(v[0][e] < INFINITY);
                 m = fmaxf(m, v[0][e]);
             }
-            m = block_max(bad ? INFINITY : m, smf);
-            if (m > -INFINITY && m < INFINITY)
+            top = block_max(bad ? INFINITY : m, smf);
+            if (top > -INFINITY && top < INFINITY)
 #pragma unroll
-                for (int e = 0; e < 8; e++) z += exp64((double)v[0][e] - m);
-            if (threadIdx.x == 0) show(tops + k, __float_as_uint(m));
+                for (int e = 0; e < 8; e++) z += exp64((double)v[0][e] - top);
         }
-        z = block_add(z, smd);
-        if (threadIdx.x == 0) show(sums + k, __builtin_bit_cast(uint64_t, z));
-    }
-    TG_DEV double rest(const Sweep &w, float v, float q) const {
-        return fmax(exp64((double)v - w.Mp) * w.ip - exp64((double)q - w.Mq) * w.iq, 0.0);
-    }
-    TG_DEV uint32_t claim(uint32_t number) const { return __hip_atomic_fetch_add(taken + number, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-    // takes pieces of sweep `number` until there are none; thread 0 has the first
-    TG_DEV void take(const Sweep &w, uint32_t number, uint32_t mine) const {
-        for (;;) {
-            __syncthreads();
-            if (threadIdx.x == 0) *smu = mine;
-            __syncthreads();
-            const uint32_t k = uni((int)*smu);
-            if (k >= (uint32_t)pieces) return;
-            if (ahead && threadIdx.x == 0) mine = claim(number);
-            piece(w, (int)k);
-            if (!ahead && threadIdx.x == 0) mine = claim(number);
-        }
-    }
-    TG_DEV void help() const {
-        for (uint32_t number = 1;; number++) {
-            uint32_t mine = 0;
-            if (threadIdx.x == 0) mine = claim(number);
-            uint64_t x[V_WORDS];
-            for (;;) {
-                bool there = true;
-#pragma unroll
-                for (int i = 0; i < V_WORDS; i++) {
-                    x[i] = seen_now(sweeps + (size_t)number * V_WORDS + i);
-                    there &= x[i] != V_ABSENT;
-                }
-                if (__ballot(x[0] == V_END)) return;
-                if (__ballot(there)) break;
-                __builtin_amdgcn_s_sleep(2);
-            }
-            take({x[0], __builtin_bit_cast(double, x[1]), __builtin_bit_cast(double, x[2]), __builtin_bit_cast(double, x[3]),
-                  __builtin_bit_cast(double, x[4])}, number, mine);
-        }
-    }
-    // the leader's: a whole sweep, its pieces' sums to `sum`, their largest values to `top`
-    TG_DEV void lead(const Sweep &w, uint32_t number, double *sum, float *top) const {
-        shown();  // all of this block's, the marks in the places of the last sums among them
-        __syncthreads();
-        uint32_t mine = 0;
-        if (threadIdx.x == 0) {
-            uint64_t *x = sweeps + (size_t)number * V_WORDS;
-            show(x, w.row), show(x + 1, __builtin_bit_cast(uint64_t, w.Mp)), show(x + 2, __builtin_bit_cast(uint64_t, w.ip));
-            show(x + 3, __builtin_bit_cast(uint64_t, w.Mq)), show(x + 4, __builtin_bit_cast(uint64_t, w.iq));
-            mine = claim(number);
-        }
-        take(w, number, mine);
-        for (int k0 = 0; k0 < pieces; k0 += 256) {
-            const int k = min(k0 + (int)threadIdx.x, pieces - 1);
-            uint64_t z;
-            while (__ballot((z = seen_now(sums + k)) == V_ABSENT)) __builtin_amdgcn_s_sleep(1);
-            sum[k] = __builtin_bit_cast(double, z);
-            if (!uni((int)w.row & 1)) {
-                uint32_t m;
-                while (__ballot((m = seen_now(tops + k)) == (uint32_t)V_ABSENT)) __builtin_amdgcn_s_sleep(1);
-                top[k] = __uint_as_float(m);
-            }
-        }
-        __syncthreads();
-        for (int k = threadIdx.x; k < pieces; k += 256) {
-            show(sums + k, (uint64_t)V_ABSENT);
-            if (!uni((int)w.row & 1)) show(tops + k, (uint32_t)V_ABSENT);
-        }
+        sum = block_add(z, smd);
     }
 };
+
+// The sweeps that the walks of the last launch ask for: a block to a piece, of all sequences.  Bound by the exponentials, 16
+// of 13 operations in 64 bits to a thread, and where few sequences ask by the latency of a launch, the state, the row and two joins.
+template <int TYPE>
+__global__ __launch_bounds__(256) void k_verify_sweep(VerifyArgs a) {
+    __shared__ float smf[4];
+    __shared__ double smd[4];
+    __shared__ uint64_t two[V_TABLE];
+    const int k = blockIdx.x / a.t.n_seqs, s = blockIdx.x - k * a.t.n_seqs;
+    const WalkState &w = a.states[s];
+    if (!uni(w.asks)) return;
+    if (threadIdx.x < V_TABLE) exp_table(two, threadIdx.x);
+    __syncthreads();
+    const Pieces<TYPE> piece(a, exp_of(factor_of(uni(temperature_of(a, s))), two), smf, smd);
+    double z;
+    float m;
+    piece(w, k, z, m);
+    if (threadIdx.x != 0) return;
+    a.swept_sum[(size_t)s * a.pieces + k] = z;
+    if (w.leaf) a.swept_top[(size_t)s * a.pieces + k] = m;
+}
 
 // LDS of a walk, for `nodes` of them and rows of `pieces`
 struct WalkNodes {
@@ -484,39 +410,35 @@ struct WalkNodes {
         par = reinterpret_cast<int16_t *>(tok + nodes), way = par + nodes;
         again = reinterpret_cast<uint8_t *>(way + nodes);
     }
-    static constexpr size_t bytes(int nodes, int pieces) { return (size_t)nodes * (5 * 8 + 3 * 4 + 2 * 2 + 1) + (size_t)pieces * (8 + 4); }
+    static constexpr size_t bytes(int nodes, int pieces) { return ((size_t)nodes * (5 * 8 + 3 * 4 + 2 * 2 + 1) + (size_t)pieces * (8 + 4) + 15) / 16 * 16; }
 };
 
-// A sequence's walk: one block leads, the others help with sums over whole rows.  What decides where the leader goes is the
-// same in all of its lanes, and told so to the compiler (uni, sure): with branches by lanes, what it moved between registers behind
-// a loop was moved with all lanes off, and lost (rejected tokens of some waves were drawn).
+// A sequence's walk, by one block, up to the next sum over a whole row that it needs (what rejected siblings drawn from q
+// leave, the row of a leaf): it asks for a sweep of it and leaves what it knows in memory, for the launch behind the sweep to
+// go on from.  So no block waits for another.  With `alone` the block does its sweeps itself, a piece after the other.
+// What decides where the walk goes is the same in all of its lanes, and told so to the compiler (uni, sure): with branches by
+// lanes, what it moved between registers behind a loop was moved with all lanes off, and lost (rejected tokens were drawn).
 template <int TYPE>
-__global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
+__global__ __launch_bounds__(256, 2) void k_verify_walk(VerifyArgs a, bool begin, bool alone) {
     extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ double smd[4], two[V_TABLE];
+    __shared__ double smd[4];
+    __shared__ uint64_t two[V_TABLE];
     __shared__ float smf[4];
     __shared__ int hits[4], lasts[4];
     __shared__ uint8_t inner[4][64];
-    __shared__ uint32_t smu;
     __shared__ int listed;
-    const int tid = threadIdx.x, lane = tid % 64, wave = uni(tid / 64), s = blockIdx.x % a.t.n_seqs, V = a.vocab;
-    uint32_t *taken = a.taken + (size_t)s * (a.t.max_nodes + 2);
-    if (a.team > 1 && tid == 0) smu = __hip_atomic_fetch_add(taken, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int tid = threadIdx.x, lane = tid % 64, wave = uni(tid / 64), s = blockIdx.x, V = a.vocab, N = a.t.max_nodes;
+    WalkState w = a.states[s];
+    if (!begin && !uni(w.asks)) return;
     const TreeRows r = tree_rows(a.t, s);
     const float t = uni(temperature_of(a, s));
     const bool greedy = !(t > 0.0f), with_q = a.draft && !greedy;
     if (tid < V_TABLE) exp_table(two, tid);
-    const Exp64 exp64{factor_of(t), two};
-    const Walk<TYPE> walk{a.logits, a.draft, a.stride, a.draft_stride, V, a.pieces, a.pieces > 2 * a.team, exp64, taken,
-                          a.sweeps + (size_t)s * (a.t.max_nodes + 2) * V_WORDS, a.swept_sum + (size_t)s * a.pieces,
-                          a.swept_top + (size_t)s * a.pieces, smf, smd, &smu};
-    __syncthreads();
-    if (a.team > 1 && uni((int)smu)) {
-        walk.help();
-        return;
-    }
-    const int n = uni(min(r.n, a.t.max_nodes)), lo = uni(r.lo), N = a.t.max_nodes;
+    const Exp64 exp64 = exp_of(factor_of(t), two);
+    const Pieces<TYPE> piece_of(a, exp64, smf, smd);
+    const int n = uni(min(r.n, N)), lo = uni(r.lo);
     const WalkNodes d(lds, N, a.pieces);
+    u32x4 *held = reinterpret_cast<u32x4 *>(a.held + (size_t)s * a.held_bytes);
 
     // Largest values and sums of the rows of nodes j0 .. j0 + 63, from those of their chunks: half a wave to a row, four
     // rows at a time.  For a greedy sequence the first of the largest stands in the place of the draft's logits.
@@ -588,13 +510,23 @@ __global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
         }
         __syncthreads();
     };
-    for (int j = tid; j < n; j += 256) {
-        const int p = parent_of(a.t, lo, j), x = a.tokens[lo + j];
-        const bool ok = p >= 0 && x >= 0 && x < V;
-        d.par[j] = (int16_t)p, d.tok[j] = x, d.u[j] = a.u[lo + j];
-        if (!greedy) {
-            d.e[j] = ok ? load1<TYPE>(walk.row_p(lo + p), x) : -INFINITY;
-            if (with_q) d.e[N + j] = ok ? load1<TYPE>(walk.row_q(lo + p), x) : -INFINITY;
+    if (begin) {
+        for (int j = tid; j < n; j += 256) {
+            const int p = parent_of(a.t, lo, j), x = a.tokens[lo + j];
+            const bool ok = p >= 0 && x >= 0 && x < V;
+            d.par[j] = (int16_t)p, d.tok[j] = x, d.u[j] = a.u[lo + j];
+            if (!greedy) {
+                d.e[j] = ok ? load1<TYPE>(piece_of.row_p(lo + p), x) : -INFINITY;
+                if (with_q) d.e[N + j] = ok ? load1<TYPE>(piece_of.row_q(lo + p), x) : -INFINITY;
+            }
+        }
+        if (tid == 0) d.way[0] = 0;
+    } else {
+        for (int i = tid; i < a.held_bytes / 16; i += 256) reinterpret_cast<u32x4 *>(lds)[i] = held[i];
+        __syncthreads();
+        for (int k = tid; k < a.pieces; k += 256) {
+            d.weight[k] = a.swept_sum[(size_t)s * a.pieces + k];
+            if (w.leaf) d.most[k] = a.swept_top[(size_t)s * a.pieces + k];
         }
     }
     __syncthreads();
@@ -613,10 +545,9 @@ __global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
         return wave_add(z);
     };
 
-    int at = 0, kept = 1, next = -1, joined = 0;
-    uint32_t sweeps = 0;
-    if (tid == 0) d.way[0] = 0;
-    while (n) {
+    int at = begin ? 0 : uni(w.at), kept = begin ? 1 : uni(w.kept), joined = begin ? 0 : uni(w.joined), next = -1;
+    bool swept = !begin;  // this launch goes on behind a sweep
+    for (; kept <= n;) {
         const int row = lo + at, kid = child(at, at);
         int yes = -1;
         if (at >= joined) {
@@ -633,30 +564,48 @@ __global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
             }
             if (yes >= 0) next = -1;
         } else {
-            Sweep w{2 * (uint64_t)row, 0.0, 1.0, 0.0, 1.0};
-            double c = 0.0;
+            w.row = row, w.leaf = kid < 0;
+            w.Mp = 0.0, w.ip = 1.0, w.Mq = 0.0;
+            double iq = 1.0;
             if (kid >= 0) {
                 w.Mp = d.top[at], w.ip = d.inv[at];
-                if (with_q) w.row++, w.Mq = d.top[N + at], w.iq = d.inv[N + at];
+                if (with_q) w.Mq = d.top[N + at], iq = d.inv[N + at];
                 if (no_number(uni((float)w.Mp)) || no_number(uni((float)w.Mq))) break;
             }
-            const double iq = w.iq;
             if (with_q || kid < 0) {
                 // each child that is rejected leaves a sweep's sums, by pieces: to the next one, or to be drawn from; as
                 // does the row of a leaf
-                double left = 1.0;
-                for (int k = kid;;) {
-                    if (k >= 0) {
-                        const double px = d.e[k] * w.ip, qx = d.e[N + k] * iq;
-                        if (sure(d.u[k] * left * qx < px - c * qx)) {
-                            yes = k;
-                            break;
+                double c = swept ? w.c : 0.0, left = 1.0;
+                int k = swept ? uni(w.k) : kid;
+                for (;;) {
+                    if (!swept) {
+                        if (k >= 0) {
+                            const double px = d.e[k] * w.ip, qx = d.e[N + k] * iq;
+                            if (sure(d.u[k] * left * qx < px - c * qx)) {
+                                yes = k;
+                                break;
+                            }
+                            c += left;
+                            k = child(at, k);
                         }
-                        c += left;
                         w.iq = c * iq;
-                        k = child(at, k);
+                        if (!alone) {
+                            __syncthreads();
+                            for (int i = tid; i < a.held_bytes / 16; i += 256) held[i] = reinterpret_cast<u32x4 *>(lds)[i];
+                            w.c = c, w.k = k, w.at = at, w.kept = kept, w.joined = joined, w.asks = 1;
+                            if (tid == 0) a.states[s] = w;
+                            return;
+                        }
+                        for (int i = 0; i < a.pieces; i++) {
+                            double z;
+                            float m;
+                            piece_of(w, i, z, m);
+                            if (tid == 0) d.weight[i] = z, d.most[i] = m;
+                        }
+                        __syncthreads();
                     }
-                    walk.lead(w, ++sweeps, d.weight, d.most);
+                    swept = false;
+                    w.iq = c * iq;
                     if (k < 0) break;
                     left = total_of();
                 }
@@ -736,7 +685,7 @@ __global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
 #pragma unroll 1
                         for (int h = 0; h < 4; h++) {
                             float v[1][8];
-                            load_stretch<TYPE, 1, 0>(walk.row_p(row), k * V_PIECE + h * 512 + lane * 8, (k + 1) * V_PIECE, V, v);
+                            load_stretch<TYPE, 1, 0>(piece_of.row_p(row), k * V_PIECE + h * 512 + lane * 8, (k + 1) * V_PIECE, V, v);
                             uint32_t o = 0;
                             rejected([&](int x, double) {
                                 x -= k * V_PIECE + h * 512;
@@ -774,8 +723,8 @@ __global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
                 if (behind) piece = last;
                 float v[1][8], q[1][8];
                 double z[8], mine = 0.0;
-                walk.load_piece(walk.row_p(row), piece, v);
-                if (of_rest) walk.load_piece(walk.row_q(row), piece, q);
+                piece_of.load(piece_of.row_p(row), piece, v);
+                if (of_rest) piece_of.load(piece_of.row_q(row), piece, q);
                 uint32_t o = 0;
                 if (without)
                     rejected([&](int x, double) {
@@ -784,7 +733,7 @@ __global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
                     });
                 if (of_rest) {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) z[e] = walk.rest(w, v[0][e], q[0][e]);
+                    for (int e = 0; e < 8; e++) z[e] = piece_of.rest(w, v[0][e], q[0][e]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; e++) z[e] = o >> e & 1 ? 0.0 : exp64((double)v[0][e] - w.Mp);
@@ -822,7 +771,7 @@ __global__ __launch_bounds__(256, 4) void k_verify_walk(VerifyArgs a) {
         kept++;
     }
     __syncthreads();
-    if (a.team > 1 && tid == 0) show(walk.sweeps + (size_t)(sweeps + 1) * V_WORDS, (uint64_t)V_END);
+    if (tid == 0) a.states[s].asks = 0;
     if (!n) kept = 0;
     int32_t *out = a.out + (size_t)s * N, *path = a.path + (size_t)s * N;
     for (int j = tid; j < N; j += 256) {
@@ -848,13 +797,15 @@ static size_t verify_layout(VerifyArgs &a, uint8_t *ws) {
     part(a.arg, (size_t)a.t.n_tokens * a.chunks);
     part(a.swept_sum, (size_t)a.t.n_seqs * a.pieces);
     part(a.swept_top, (size_t)a.t.n_seqs * a.pieces);
-    part(a.sweeps, (size_t)a.t.n_seqs * (a.t.max_nodes + 2) * V_WORDS);
-    part(a.taken, (size_t)a.t.n_seqs * (a.t.max_nodes + 2));
+    part(a.states, (size_t)a.t.n_seqs);
+    a.held_bytes = WalkNodes::bytes(a.t.max_nodes, a.pieces);
+    part(a.held, (size_t)a.t.n_seqs * a.held_bytes);
     return n;
 }
 
 bool verify_fits(const DraftTrees &t, int vocab) {
-    return (int64_t)t.n_tokens * ((vocab + V_CHUNK - 1) / V_CHUNK) <= UINT32_MAX / 256;
+    return (int64_t)t.n_tokens * ((vocab + V_CHUNK - 1) / V_CHUNK) <= UINT32_MAX / 256 &&
+           (int64_t)t.n_seqs * ((vocab + V_PIECE - 1) / V_PIECE) <= UINT32_MAX / 256;
 }
 
 static_assert(WalkNodes::bytes(DT_NODES, (1 << 20) / V_PIECE) + 768 <= 65536, "a walk's LDS");
@@ -868,14 +819,20 @@ size_t verify_workspace(const DraftTrees &t, int vocab) {
 hipError_t launch_verify(VerifyArgs a, int type, void *ws, hipStream_t st) {
     verify_layout(a, static_cast<uint8_t *>(ws));
     const dim3 grid((unsigned)(a.t.n_tokens * a.chunks), a.draft ? 2 : 1);
-    // blocks to a walk: as many as the row has pieces, but what the device holds at once for all walks at the most; one
-    // where nothing is swept
-    a.team = grid.x && (a.temps || a.temp > 0.0f) ? std::max(1, std::min(a.pieces, 1024 / a.t.n_seqs)) : 1;
     a.early = grid.x * grid.y <= 1024;
+    // Sweeps: none where all are greedy; one where a walk ends with its first, as every one without a draft model's logits
+    // and every chain's does; of trees as many as a walk may have, but V_ROUNDS at the most, the rest by the walk's block
+    // alone.  (4 trees of 26 nodes drawn from a draft model, 151936 tokens: TIMES)
+    const int rounds = !grid.x || (!a.temps && !(a.temp > 0.0f)) ? 0 : !a.draft || !a.t.parent ? 1 : std::min(V_ROUNDS, a.t.max_nodes);
     auto launch = [&](auto T) {
         constexpr int TYPE = decltype(T)::value;
+        const size_t lds = WalkNodes::bytes(a.t.max_nodes, a.pieces);
         if (grid.x) TG_LAUNCH(k_verify_rows<TYPE>, grid, dim3(256), 0, st, a);
-        TG_LAUNCH(k_verify_walk<TYPE>, dim3((unsigned)(a.t.n_seqs * a.team)), dim3(256), WalkNodes::bytes(a.t.max_nodes, a.pieces), st, a);
+        TG_LAUNCH(k_verify_walk<TYPE>, dim3((unsigned)a.t.n_seqs), dim3(256), lds, st, a, true, rounds == 0);
+        for (int i = 1; i <= rounds; i++) {
+            TG_LAUNCH(k_verify_sweep<TYPE>, dim3((unsigned)(a.t.n_seqs * a.pieces)), dim3(256), 0, st, a);
+            TG_LAUNCH(k_verify_walk<TYPE>, dim3((unsigned)a.t.n_seqs), dim3(256), lds, st, a, false, i == rounds);
+        }
     };
     if (type == TG_T_F32) launch(std::integral_constant<int, TG_T_F32>{});
     else if (type == TG_T_F16) launch(std::integral_constant<int, TG_T_F16>{});

@@ -431,6 +431,14 @@ struct DraftTrees {
     int n_seqs, n_tokens, max_nodes;
 };
 hipError_t launch_draft_tree(const DraftTrees &t, uint32_t *bits, int32_t *depth, int32_t *links, hipStream_t st);
+// A sequence's walk between two launches
+struct WalkState {
+    int asks;                   // it needs a sweep, of
+    int row, leaf;              // the sum of max(p - c q, 0), or of a leaf's p
+    int at, k, kept, joined;    // its node, the child to be asked next (-1: none), nodes kept, nodes whose rows are joined
+    double Mp, ip, Mq, iq;      // p = exp((v - Mp) / T) ip, c q likewise
+    double c;
+};
 struct VerifyArgs {
     DraftTrees t;
     const int32_t *links;
@@ -444,7 +452,6 @@ struct VerifyArgs {
     const float *temps;
     float temp;
     int32_t *out, *path, *count;
-    int team;          // blocks of a walk
     bool early;        // rows are loaded before it is known whether they are asked for
     // the workspace
     int chunks, pieces;
@@ -452,10 +459,11 @@ struct VerifyArgs {
     double *whole;     // [n_tokens][target, draft][chunks]
     float *top;        // [n_tokens][target, draft][chunks]
     int *arg;          // [n_tokens][chunks]
-    uint64_t *swept_sum;  // [n_seqs][2][pieces]
-    uint32_t *swept_top;
-    uint64_t *sweeps;     // [n_seqs][max_nodes + 2][5]
-    uint32_t *taken;      // [n_seqs][max_nodes + 2]
+    double *swept_sum; // [n_seqs][pieces]
+    float *swept_top;
+    WalkState *states; // [n_seqs]
+    uint8_t *held;     // [n_seqs][held_bytes]: the walks' nodes between two launches
+    size_t held_bytes;
 };
 bool verify_fits(const DraftTrees &t, int vocab);  // in the threads of a launch
 size_t verify_workspace(const DraftTrees &t, int vocab);
