@@ -371,26 +371,13 @@ struct Pieces {
     }
 };
 
-// The sweeps that the walks of the last launch ask for: a block to a piece, of all sequences.  Bound by the exponentials, 16
-// of 13 operations in 64 bits to a thread, and where few sequences ask by the latency of a launch, the state, the row and two joins.
-template <int TYPE>
-__global__ __launch_bounds__(256) void k_verify_sweep(VerifyArgs a) {
-    __shared__ float smf[4];
-    __shared__ double smd[4];
-    __shared__ uint64_t two[V_TABLE];
-    const int k = blockIdx.x / a.t.n_seqs, s = blockIdx.x - k * a.t.n_seqs;
-    const WalkState &w = a.states[s];
-    if (!uni(w.asks)) return;
-    if (threadIdx.x < V_TABLE) exp_table(two, threadIdx.x);
-    __syncthreads();
-    const Pieces<TYPE> piece(a, exp_of(factor_of(uni(temperature_of(a, s))), two), smf, smd);
-    double z;
-    float m;
-    piece(w, k, z, m);
-    if (threadIdx.x != 0) return;
-    a.swept_sum[(size_t)s * a.pieces + k] = z;
-    if (w.leaf) a.swept_top[(size_t)s * a.pieces + k] = m;
-}
+// What blocks hand to each other goes past the caches of an XCD, and what is to be seen first is waited for (a release at
+// the device's scope writes back a whole L2).
+template <class T>
+TG_DEV T seen_now(const T *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <class T>
+TG_DEV void show(T *p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+TG_DEV void shown() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt 0: this thread's stores are acknowledged
 
 // LDS of a walk, for `nodes` of them and rows of `pieces`
 struct WalkNodes {
@@ -414,28 +401,22 @@ struct WalkNodes {
 };
 
 // A sequence's walk, by one block, up to the next sum over a whole row that it needs (what rejected siblings drawn from q
-// leave, the row of a leaf): it asks for a sweep of it and leaves what it knows in memory, for the launch behind the sweep to
-// go on from.  So no block waits for another.  With `alone` the block does its sweeps itself, a piece after the other.
+// leave, the row of a leaf): it asks for a sweep of it and leaves what it knows in memory.  The next launch has a block to
+// each piece, and the last of them to be done goes on with the walk: no block waits for another.  With `alone` the block does its
+// sweeps itself, a piece after the other.
 // What decides where the walk goes is the same in all of its lanes, and told so to the compiler (uni, sure): with branches by
 // lanes, what it moved between registers behind a loop was moved with all lanes off, and lost (rejected tokens were drawn).
 template <int TYPE>
-__global__ __launch_bounds__(256, 2) void k_verify_walk(VerifyArgs a, bool begin, bool alone) {
+TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &piece_of, bool begin, bool alone) {
     extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ double smd[4];
-    __shared__ uint64_t two[V_TABLE];
-    __shared__ float smf[4];
     __shared__ int hits[4], lasts[4];
     __shared__ uint8_t inner[4][64];
     __shared__ int listed;
-    const int tid = threadIdx.x, lane = tid % 64, wave = uni(tid / 64), s = blockIdx.x, V = a.vocab, N = a.t.max_nodes;
-    WalkState w = a.states[s];
-    if (!begin && !uni(w.asks)) return;
+    const int tid = threadIdx.x, lane = tid % 64, wave = uni(tid / 64), V = a.vocab, N = a.t.max_nodes;
     const TreeRows r = tree_rows(a.t, s);
-    const float t = uni(temperature_of(a, s));
-    const bool greedy = !(t > 0.0f), with_q = a.draft && !greedy;
-    if (tid < V_TABLE) exp_table(two, tid);
-    const Exp64 exp64 = exp_of(factor_of(t), two);
-    const Pieces<TYPE> piece_of(a, exp64, smf, smd);
+    const bool greedy = !(uni(temperature_of(a, s)) > 0.0f), with_q = a.draft && !greedy;
+    const Exp64 exp64 = piece_of.exp64;
+    double *smd = piece_of.smd;
     const int n = uni(min(r.n, N)), lo = uni(r.lo);
     const WalkNodes d(lds, N, a.pieces);
     u32x4 *held = reinterpret_cast<u32x4 *>(a.held + (size_t)s * a.held_bytes);
@@ -525,8 +506,8 @@ __global__ __launch_bounds__(256, 2) void k_verify_walk(VerifyArgs a, bool begin
         for (int i = tid; i < a.held_bytes / 16; i += 256) reinterpret_cast<u32x4 *>(lds)[i] = held[i];
         __syncthreads();
         for (int k = tid; k < a.pieces; k += 256) {
-            d.weight[k] = a.swept_sum[(size_t)s * a.pieces + k];
-            if (w.leaf) d.most[k] = a.swept_top[(size_t)s * a.pieces + k];
+            d.weight[k] = seen_now(a.swept_sum + (size_t)s * a.pieces + k);
+            if (w.leaf) d.most[k] = seen_now(a.swept_top + (size_t)s * a.pieces + k);
         }
     }
     __syncthreads();
@@ -781,6 +762,44 @@ __global__ __launch_bounds__(256, 2) void k_verify_walk(VerifyArgs a, bool begin
     if (tid == 0) a.count[s] = kept;
 }
 
+template <int TYPE>
+__global__ __launch_bounds__(256, 2) void k_verify_walk(VerifyArgs a, bool alone) {
+    __shared__ float smf[4];
+    __shared__ double smd[4];
+    __shared__ uint64_t two[V_TABLE];
+    const int s = blockIdx.x;
+    if (threadIdx.x < V_TABLE) exp_table(two, threadIdx.x);
+    if (threadIdx.x == 0) a.swept[s] = 0;
+    walk<TYPE>(a, s, WalkState{}, Pieces<TYPE>(a, exp_of(factor_of(uni(temperature_of(a, s))), two), smf, smd), true, alone);
+}
+
+// The sweeps that the walks of the last launch ask for, a block to a piece of a sequence's row, and the walks behind them.
+template <int TYPE>
+__global__ __launch_bounds__(256, 3) void k_verify_sweep(VerifyArgs a, bool alone) {
+    __shared__ float smf[4];
+    __shared__ double smd[4];
+    __shared__ uint64_t two[V_TABLE];
+    __shared__ int last;
+    const int k = blockIdx.x / a.t.n_seqs, s = blockIdx.x - k * a.t.n_seqs;
+    const WalkState w = a.states[s];
+    if (!uni(w.asks)) return;
+    if (threadIdx.x < V_TABLE) exp_table(two, threadIdx.x);
+    __syncthreads();
+    const Pieces<TYPE> piece_of(a, exp_of(factor_of(uni(temperature_of(a, s))), two), smf, smd);
+    double z;
+    float m;
+    piece_of(w, k, z, m);
+    if (threadIdx.x == 0) {
+        show(a.swept_sum + (size_t)s * a.pieces + k, z);
+        if (w.leaf) show(a.swept_top + (size_t)s * a.pieces + k, m);
+        shown();
+        last = __hip_atomic_fetch_add(a.swept + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.pieces - 1;
+        if (last) a.swept[s] = 0;  // for the next launch
+    }
+    __syncthreads();
+    if (uni(last)) walk<TYPE>(a, s, w, piece_of, false, alone);
+}
+
 static size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Where the workspace's parts are; its size.
@@ -797,6 +816,7 @@ static size_t verify_layout(VerifyArgs &a, uint8_t *ws) {
     part(a.arg, (size_t)a.t.n_tokens * a.chunks);
     part(a.swept_sum, (size_t)a.t.n_seqs * a.pieces);
     part(a.swept_top, (size_t)a.t.n_seqs * a.pieces);
+    part(a.swept, (size_t)a.t.n_seqs);
     part(a.states, (size_t)a.t.n_seqs);
     a.held_bytes = WalkNodes::bytes(a.t.max_nodes, a.pieces);
     part(a.held, (size_t)a.t.n_seqs * a.held_bytes);
@@ -822,17 +842,15 @@ hipError_t launch_verify(VerifyArgs a, int type, void *ws, hipStream_t st) {
     a.early = grid.x * grid.y <= 1024;
     // Sweeps: none where all are greedy; one where a walk ends with its first, as every one without a draft model's logits
     // and every chain's does; of trees as many as a walk may have, but V_ROUNDS at the most, the rest by the walk's block
-    // alone.  (4 trees of 26 nodes drawn from a draft model, 151936 tokens: TIMES)
+    // alone, which takes a tenth of a ms each.  (4 trees of 26 nodes drawn from a draft model, 151936 tokens, of whose walks few need
+    // more than 6: 60 us with 4, 64 with 8, 86 with 12.)
     const int rounds = !grid.x || (!a.temps && !(a.temp > 0.0f)) ? 0 : !a.draft || !a.t.parent ? 1 : std::min(V_ROUNDS, a.t.max_nodes);
     auto launch = [&](auto T) {
         constexpr int TYPE = decltype(T)::value;
         const size_t lds = WalkNodes::bytes(a.t.max_nodes, a.pieces);
         if (grid.x) TG_LAUNCH(k_verify_rows<TYPE>, grid, dim3(256), 0, st, a);
-        TG_LAUNCH(k_verify_walk<TYPE>, dim3((unsigned)a.t.n_seqs), dim3(256), lds, st, a, true, rounds == 0);
-        for (int i = 1; i <= rounds; i++) {
-            TG_LAUNCH(k_verify_sweep<TYPE>, dim3((unsigned)(a.t.n_seqs * a.pieces)), dim3(256), 0, st, a);
-            TG_LAUNCH(k_verify_walk<TYPE>, dim3((unsigned)a.t.n_seqs), dim3(256), lds, st, a, false, i == rounds);
-        }
+        TG_LAUNCH(k_verify_walk<TYPE>, dim3((unsigned)a.t.n_seqs), dim3(256), lds, st, a, rounds == 0);
+        for (int i = 1; i <= rounds; i++) TG_LAUNCH(k_verify_sweep<TYPE>, dim3((unsigned)(a.t.n_seqs * a.pieces)), dim3(256), lds, st, a, i == rounds);
     };
     if (type == TG_T_F32) launch(std::integral_constant<int, TG_T_F32>{});
     else if (type == TG_T_F16) launch(std::integral_constant<int, TG_T_F16>{});

@@ -461,6 +461,7 @@ struct VerifyArgs {
     int *arg;          // [n_tokens][chunks]
     double *swept_sum; // [n_seqs][pieces]
     float *swept_top;
+    int *swept;        // [n_seqs]: pieces of a sweep that are done
     WalkState *states; // [n_seqs]
     uint8_t *held;     // [n_seqs][held_bytes]: the walks' nodes between two launches
     size_t held_bytes;
