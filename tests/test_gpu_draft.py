@@ -161,7 +161,7 @@ ATTEND = [
     (256, 1, 5, 16, [257, 130, 3], [7, 60, 3], "f16", 64),
     (256, 2, 16, 48, [500], [24], "bf16", 24),
     (128, 1, 24, 128, [300, 77], [5, 30], "f16", 64),
-    (128, 4, 8, 64, [190], [190], "bf16", 200),                     # a tree that is all there is, in wide tiles
+    (128, 4, 8, 64, [190], [190], "bf16", 200),                     # a tree that is all there is
     (128, 2, 8, 16, [300, 17, 128], [300, 17, 100], "f16", 320),
     (64, 2, 4, 32, [1000], [257], "f16", 257),
     (64, 1, 1, 16, [400], [400], "bf16", 400),
@@ -170,9 +170,19 @@ ATTEND = [
     (64, 8, 2, 16, [12 + i % 37 for i in range(80)] + [3000, 1700], [1 + i % 12 for i in range(82)], "f16", 16),
     (128, 2, 8, 16, [3000, 40], [64, 40], "bf16", 64),
     (64, 4, 4, 64, [5000], [33], "bf16", 64),
-    (128, 2, 8, 32, [900, 700, 33, 0, 1500, 64, 5, 6, 7, 8], [600, 1, 33, 0, 1, 2, 1, 1, 1, 1], "bf16", 640),  # two launches
+    (128, 2, 8, 32, [900, 700, 33, 0, 1500, 64, 5, 6, 7, 8], [600, 1, 33, 0, 1, 2, 1, 1, 1, 1], "bf16", 640),
     (128, 1, 16, 48, [1777, 1300], [1024, 300], "f16", 1024),
     (64, 1, 4, 16, [1000, 50], [100, 50], "bf16", 33),              # nodes behind max_nodes are NaN
+    # in wide tiles
+    (128, 8, 8, 16, [190, 100], [190, 60], "bf16", 200),
+    (128, 8, 8, 64, [300, 17, 128], [300, 17, 100], "f16", 320),
+    (64, 16, 4, 32, [1000], [400], "bf16", 400),
+    (64, 8, 8, 16, [300, 150], [280, 150], "f16", 300),
+    (256, 8, 8, 64, [333, 64], [200, 64], "bf16", 200),
+    (128, 8, 8, 64, [3000, 40], [300, 40], "bf16", 512),            # split
+    (64, 8, 8, 32, [2500], [300], "f16", 300),
+    (128, 8, 8, 16, [100, 5], [200, 9], "bf16", 200),
+    (64, 8, 8, 16, [400, 50], [300, 50], "bf16", 33),
 ]
 
 
@@ -189,23 +199,27 @@ def test_attend(case):
     check_tree_attend(s, parents, q, qn, out, max_nodes=most)
 
 
-@pytest.mark.parametrize("lens,news,G,dt", [([300, 9, 70], [20, 9, 1], 8, "bf16"), ([900, 300], [200, 100], 8, "f16"), ([5000], [5], 16, "f16")])
-def test_a_chain_is_ordinary_attention(lens, news, G, dt):
-    """Bit for bit, whichever way the chain is given."""
+@pytest.mark.parametrize("lens,news,G,dt,same", [([300, 9, 70], [20, 9, 1], 8, "bf16", True), ([900, 300], [200, 100], 8, "f16", False),
+                                                 ([5000], [5], 16, "f16", True), ([2100] * 8, [100] * 8, 8, "bf16", True)])
+def test_a_chain_is_ordinary_attention(lens, news, G, dt, same):
+    """Bit for bit where the same kernel takes either, whichever way the chain is given."""
     from tinygiant_amd.draft import DraftTree
     gpu_note(f"attend chain {lens}")
     s = Setup(61, 128, 2, 16, lens, news)
-    q, _ = s.rows(2 * G, dt)
+    q, qn = s.rows(2 * G, dt)
     want = s.kv.attend(0, q, s.batch)
-    for tree in (tree_of(s, [list(range(-1, n - 1)) for n in news], 200), DraftTree(s.batch.cu, s.T, max_nodes=256)):
-        assert torch.equal(s.kv.attend(0, q, s.batch, tree=tree), want)
+    chains = [list(range(-1, n - 1)) for n in news]
+    a, b = (s.kv.attend(0, q, s.batch, tree=tree) for tree in (tree_of(s, chains, 200), DraftTree(s.batch.cu, s.T, max_nodes=256)))
+    assert torch.equal(a, b)
+    assert not same or torch.equal(a, want)
+    check_tree_attend(s, chains, q, qn, a)
 
 
-@pytest.mark.parametrize("news", [[6, 5], [150, 140]])
-def test_attend_rows_that_are_no_nodes(news):
+@pytest.mark.parametrize("news,n_kv,G", [([6, 5], 1, 4), ([150, 140], 1, 4), ([190, 180], 8, 8)])
+def test_attend_rows_that_are_no_nodes(news, n_kv, G):
     """They are NaN, and tokens that a row does not see may hold anything."""
     gpu_note(f"attend no nodes {news}")
-    s = Setup(62, 64, 1, 16, [200, 190], news)
+    s = Setup(62, 64, n_kv, 16, [200, 190], news)
     parents = [random_tree(s.rng, n) for n in news]
     parents[0][3] = 3
     parents[1][4] = -5
@@ -220,7 +234,7 @@ def test_attend_rows_that_are_no_nodes(news):
                 tile[:, places[4]] = 0x7E00
                 tile[:, places[5]] = 0x7C00
     s.kv.pages.copy_(dev(s.all))
-    q, qn = s.rows(4, "f16")
+    q, qn = s.rows(n_kv * G, "f16")
     out = s.kv.attend(0, q, s.batch, tree=tree_of(s, parents, 160))
     clean = [[a is not None for a in R.ancestors(p)] for p in parents]
     # the oracle multiplies hidden values by 0: give it finite ones

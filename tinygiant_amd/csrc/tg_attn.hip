@@ -1647,8 +1647,31 @@ static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len, bool many,
 // single tokens after 8192, 32 heads over 4: 133 us, 274 in one launch; after 4000 122 and 147; 8 chunks of 128, where
 // the second launch finds nothing to do: 84 and 79.  So a row's roundings are those of the kernel that its call's
 // numbers choose, not of the row alone.
-static int attn_plans(const KvBatch &b, int n_heads, int max_len, bool bf16, AttnPlan p[2]) {
+//
+// Trees have few rows next to long sequences, and rarely fill the card: what counts is the longest block of either kernel, in
+// narrow steps of 32 tokens, of which a wide one of 64 takes 7 (fp16 10, heads of 256 11).  A narrow tile costs 12
+// steps beside its own, a wide block 6, and 16 of its steps at the least.  Of 519 sizes (1 to 48 sequences of 8 to 200 nodes
+// after 500 to 30000 tokens, all head sizes, 1 to 16 heads to a key head) that chose the faster but for 1% of the time in the mean and 1.36
+// times at the most.  D = 128, bf16, 32 heads over 4, few and many: 1 tree of 16 nodes after 2000 21 and 67 us, after
+// 30000 41 and 53; 1 of 200 after 8000 99 and 60; 4 of 64 after 2000 35 and 71, after 8000 99 and 58; 48 of 8 after 8000 172 and 261,
+// of 31 509 and 262.  One launch for all: 32 trees of 16 nodes in the mean after 4200 123 us, each by the kernel that suits it, in two
+// launches, 129; 64 of 32 after 1000 154 and 187.
+static bool tree_wide(const KvBatch &b, int n_heads, int max_len, bool bf16) {
+    const AttnPlan few = attn_plan(b, n_heads, max_len, false, 0, INT32_MAX), many = attn_plan(b, n_heads, max_len, true, 0, INT32_MAX);
+    const int width = b.D == 256 ? 11 : bf16 ? 7 : 10;
+    const double all = (double)b.n_tokens * (n_heads / b.n_kv), seqs = 0.5 * b.n_seqs;
+    const double blocks = std::max(1, (b.D == 256 ? 256 : 512) / b.n_kv), wide_blocks = std::max(1, 256 / b.n_kv);
+    const double narrow = (all / few.cols + seqs) * (max_len / 32.0 + 12.0) / blocks;
+    const double steps = max_len / 64.0, rounds = (all / many.cols + seqs) / wide_blocks;
+    return narrow > width * (many.share ? std::max(16.0, rounds * steps) : std::max(1.0, rounds) * steps) + 6.0;
+}
+
+static int attn_plans(const KvBatch &b, int n_heads, int max_len, bool bf16, bool tree, AttnPlan p[2]) {
     const int64_t all = (int64_t)b.n_tokens * (n_heads / b.n_kv);
+    if (tree) {
+        p[0] = attn_plan(b, n_heads, max_len, (b.D < 256 || bf16) && tree_wide(b, n_heads, max_len, bf16), 0, INT32_MAX);
+        return 1;
+    }
     const int few = bf16 ? 128 : 192;
     const bool many = (b.D < 256 || bf16) && all >= few * (int64_t)b.n_seqs;
     const bool both = many && b.n_seqs > 8 && 2 * (int64_t)b.n_tokens < (int64_t)b.n_seqs * max_len;
@@ -1664,9 +1687,9 @@ static size_t attn_join_bytes(const KvBatch &b, const AttnPlan &p) {
 // Enough for rows of either type; a call's launches use it one after the other.
 size_t attn_workspace(const KvBatch &b, int n_heads, int max_len) {
     size_t most = 0;
-    for (const bool bf16 : {false, true}) {
+    for (const int kind : {0, 1, 2, 3}) {
         AttnPlan p[2];
-        for (int i = attn_plans(b, n_heads, max_len, bf16, p) - 1; i >= 0; i--)
+        for (int i = attn_plans(b, n_heads, max_len, kind & 1, kind & 2, p) - 1; i >= 0; i--)
             if (p[i].share) most = std::max(most, attn_join_bytes(b, p[i]) + (size_t)p[i].parts * b.n_kv * (p[i].cols * (b.D + 2)) * sizeof(float));
     }
     return most;
@@ -1698,7 +1721,7 @@ static hipError_t attn_launch(const KvBatch &b, KvRows q, int G, float scale, co
 hipError_t launch_attn(const KvBatch &b, int type, KvRows q, int n_heads, float scale, void *out, int64_t out_stride,
                        int max_len, void *ws, hipStream_t st) {
     AttnPlan plans[2];
-    const int n = attn_plans(b, n_heads, max_len, type == TG_T_BF16, plans), G = n_heads / b.n_kv;
+    const int n = attn_plans(b, n_heads, max_len, type == TG_T_BF16, b.bits, plans), G = n_heads / b.n_kv;
     hipError_t e = hipSuccess;
     for (int i = 0; i < n && e == hipSuccess; i++) {
         const AttnPlan &p = plans[i];
