@@ -90,7 +90,7 @@ hipError_t launch_draft_tree(const DraftTrees &t, uint32_t *bits, int32_t *depth
 constexpr int V_CHUNK = 4096;  // values of a row to a block of the first launch
 constexpr int V_PIECE = 2048;  // ... whose sum is kept
 constexpr int V_PER = V_CHUNK / V_PIECE;
-constexpr int V_ROUNDS = 8;    // sweeps that have launches of their own
+constexpr int V_ROUNDS = 12;     // sweeps that have launches of their own
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -843,7 +843,7 @@ hipError_t launch_verify(VerifyArgs a, int type, void *ws, hipStream_t st) {
     // Sweeps: none where all are greedy; one where a walk ends with its first, as every one without a draft model's logits
     // and every chain's does; of trees as many as a walk may have, but V_ROUNDS at the most, the rest by the walk's block
     // alone, which takes a tenth of a ms each.  (4 trees of 26 nodes drawn from a draft model, 151936 tokens, of whose walks few need
-    // more than 6: 60 us with 4, 64 with 8, 86 with 12.)
+    // more than 8 and none of 40 more than 10: 60 us where 4 are enough, 82 with 12; an idle launch takes 1.7.)
     const int rounds = !grid.x || (!a.temps && !(a.temp > 0.0f)) ? 0 : !a.draft || !a.t.parent ? 1 : std::min(V_ROUNDS, a.t.max_nodes);
     auto launch = [&](auto T) {
         constexpr int TYPE = decltype(T)::value;
