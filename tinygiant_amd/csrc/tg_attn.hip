@@ -312,9 +312,11 @@ __global__ __launch_bounds__(256) void k_kv_read(KvBatch b, _Float16 *k, _Float1
 // ================================================================ keep
 // The token that a walk through a draft tree kept as its i-th to place i of the tree, codes and scales as they are.  A
 // wave has one key head of one sequence and layer and goes through the places in order: entry i comes from path[i] >= i,
-// so no place is written before what it held is read.
+// so no place is written before what it held is read, and entries may be read together.
 //
-// Bound by latency: cu and kv_len, path and count, the table, and the entries themselves, one after the other.
+// Bound by latency where there are few: cu and kv_len, path and count, the table, and the entries themselves (1 user, 48 layers of 4
+// heads of 128: 4.3 us); otherwise by lines: of 144 bytes of a token and head, codes lie in some ten lines of a tile, read and written
+// (64 users: 18 us, some 20 lines of 128 bytes an entry, 5 TB/s).  The lengths by themselves in a launch behind it: 1 user 10.1 us a call, 6.6 so.
 template <int D>
 __global__ __launch_bounds__(256) void k_kv_keep(KvBatch b, KeepArgs a) {
     constexpr int NG = D / 32, KW = D / 8, VH = D / 4, ITEMS = KW + VH + 2 * NG;  // K words, V halfwords, scales of a token
@@ -325,6 +327,7 @@ __global__ __launch_bounds__(256) void k_kv_keep(KvBatch b, KeepArgs a) {
     if (layer >= a.n_layers) return;
     const int lo = max(b.cu[s], 0), n = max(b.cu[s + 1], lo) - lo, base = max(b.kv_len[s], 0) - n;
     const int count = min(max(a.count[s], 0), min(n, a.path_cols));
+    if (a.kv_len && a.kv_len != b.kv_len && layer == 0 && hk == 0 && lane == 0) a.kv_len[s] = max(base + count, 0);
     uint8_t *pages = b.pages + layer * a.layer_bytes;
     // bytes of this lane's items in token r's tile: V's as halfwords, K's as words
     auto at = [&](int item, int r) {
@@ -340,30 +343,46 @@ __global__ __launch_bounds__(256) void k_kv_keep(KvBatch b, KeepArgs a) {
         const int i = i0 + lane, from = i < count ? a.path[(int64_t)s * a.path_stride + i] : i;
         const int to_page = i < count && from != i ? page_of(b, s, base + i) : -1;
         const int from_page = to_page >= 0 && from > i && from < n ? page_of(b, s, base + from) : -1;
-        for (uint64_t todo = __ballot(to_page >= 0); todo; todo &= todo - 1) {
-            const int e = __builtin_ctzll(todo);
-            const int tp = __builtin_amdgcn_readlane(to_page, e), fp = __builtin_amdgcn_readlane(from_page, e);
-            const int t = base + i0 + e, f = base + __builtin_amdgcn_readlane(from, e);
-            uint8_t *tt = pages + tile_at<D>(b, tp, hk, t % b.page_tokens / 16);
-            const uint8_t *ft = fp < 0 ? tt : pages + tile_at<D>(b, fp, hk, f % b.page_tokens / 16);
+        // four entries at a time, all of their loads before the first store
+        for (uint64_t todo = __ballot(to_page >= 0); todo;) {
+            uint32_t v[4][PER];
+            uint8_t *tt[4];
+            int t[4], live[4];
 #pragma unroll
-            for (int k = 0; k < PER; k++) {
-                const int item = lane + 64 * k;
-                if (item >= ITEMS) break;
-                const int to = at(item, t % 16), fr = at(item, (fp < 0 ? t : f) % 16);
-                if (item < KW) {
-                    *reinterpret_cast<uint32_t *>(tt + to) = *reinterpret_cast<const uint32_t *>(ft + fr);
-                } else {
-                    // an entry that is none: NaN for scales
-                    const uint16_t v = *reinterpret_cast<const uint16_t *>(ft + fr);
-                    *reinterpret_cast<uint16_t *>(tt + to) = fp < 0 && item >= KW + VH ? (uint16_t)0x7E00 : v;
+            for (int q = 0; q < 4; q++) {
+                live[q] = todo != 0;
+                const int e = todo ? __builtin_ctzll(todo) : 0;
+                todo &= todo - 1;
+                const int tp = __builtin_amdgcn_readlane(to_page, e), fp = __builtin_amdgcn_readlane(from_page, e);
+                t[q] = base + i0 + e;
+                const int f = base + __builtin_amdgcn_readlane(from, e);
+                if (!live[q]) continue;
+                tt[q] = pages + tile_at<D>(b, tp, hk, t[q] % b.page_tokens / 16);
+                const uint8_t *ft = fp < 0 ? tt[q] : pages + tile_at<D>(b, fp, hk, f % b.page_tokens / 16);
+#pragma unroll
+                for (int k = 0; k < PER; k++) {
+                    const int item = min(lane + 64 * k, ITEMS - 1), fr = at(item, (fp < 0 ? t[q] : f) % 16);
+                    if (item < KW) v[q][k] = *reinterpret_cast<const uint32_t *>(ft + fr);
+                    else v[q][k] = *reinterpret_cast<const uint16_t *>(ft + fr);
+                    if (fp < 0 && item >= KW + VH) v[q][k] = 0x7E00;  // an entry that is none: NaN for scales
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (!live[q]) break;
+#pragma unroll
+                for (int k = 0; k < PER; k++) {
+                    const int item = lane + 64 * k, to = at(item, t[q] % 16);
+                    if (item >= ITEMS) break;
+                    if (item < KW) *reinterpret_cast<uint32_t *>(tt[q] + to) = v[q][k];
+                    else *reinterpret_cast<uint16_t *>(tt[q] + to) = (uint16_t)v[q][k];
                 }
             }
         }
     }
 }
 
-// The lengths by themselves: they may stand where the ones before do.
+// The lengths where they take the place of the ones before, which every other block reads: a launch of their own.
 __global__ __launch_bounds__(256) void k_kv_keep_len(KvBatch b, KeepArgs a) {
     const int s = blockIdx.x * 256 + threadIdx.x;
     if (s >= b.n_seqs) return;
@@ -1595,7 +1614,7 @@ hipError_t launch_kv_keep(const KvBatch &b, const KeepArgs &a, hipStream_t st) {
     const int64_t grid = ((int64_t)b.n_seqs * b.n_kv * a.n_layers + 3) / 4;
     if (grid > UINT32_MAX / 256) return hipErrorInvalidValue;
     if (a.n_layers) TG_BY_DIM(b.D, TG_LAUNCH(k_kv_keep<DIM>, dim3((unsigned)grid), dim3(256), 0, st, b, a));
-    if (a.kv_len) TG_LAUNCH(k_kv_keep_len, dim3((b.n_seqs + 255) / 256), dim3(256), 0, st, b, a);
+    if (a.kv_len && (a.kv_len == b.kv_len || !a.n_layers)) TG_LAUNCH(k_kv_keep_len, dim3((b.n_seqs + 255) / 256), dim3(256), 0, st, b, a);
     return hipGetLastError();
 }
 
