@@ -8,6 +8,7 @@ include/tinygiant.h.  Python side:
   arena     HBMExpertArena (tinygiant/cache.py's role, in HBM)
   moe       MoEBlock (tinygiant/engine.py:229-258 on the GPU)
   attn      PagedKV / KVBatch (paged Q4_0 KV cache and attention over it; tinygiant/engine.py:199-227 on the GPU)
+  draft     DraftTree / verify (steps over trees of drafted tokens; tinygiant/engine.py:317-409 generates a token a pass)
   linear    matmul_i8 (int8 projections around it)
   relayout  Q4_0 expert-contiguous cache files (tinygiant/relayout.py)
 """
