@@ -1,7 +1,7 @@
 """Draft trees restated in numpy: what a node sees, which drafted tokens a
 target's probabilities keep, and the cache afterwards.
 
-TEST INFRASTRUCTURE ONLY: the checker that tests/ compare libtinygiant's
+TEST INFRASTRUCTURE ONLY: the oracle that tests/ compare libtinygiant's
 tg_draft_tree_dev, tg_verify_dev and tg_kv_keep_q4_dev with.  Nothing in the
 product imports it.  Everything is computed in float64, step by step as the
 operators are defined.
