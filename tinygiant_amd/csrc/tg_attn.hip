@@ -1429,17 +1429,30 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
             }
             lds_barrier();
         }
-        matrix(0, false_type{}, true_type{});
-        lds_barrier();
-        vector(0);
-        lds_barrier();
-        for (int i = 1; i < steps; i++) {
-            matrix(i, true_type{}, true_type{});
+        // a wave without columns, of which trees leave many, does its share of the codes alone: 16 trees of 16 nodes, half a tile
+        // each, after 8000 tokens 71 us, 84 with all of the products
+        if (TREE && f0 >= ncol) {
+            for (int i = 0; i < steps; i++) {
+                const int next = i + (late ? 2 : 1);
+                pages(next);
+                fetch(next);
+                lds_barrier();
+                if (next < steps) spread(next);
+                lds_barrier();
+            }
+        } else {
+            matrix(0, false_type{}, true_type{});
             lds_barrier();
-            vector(i);
+            vector(0);
             lds_barrier();
+            for (int i = 1; i < steps; i++) {
+                matrix(i, true_type{}, true_type{});
+                lds_barrier();
+                vector(i);
+                lds_barrier();
+            }
+            matrix(steps, true_type{}, false_type{});
         }
-        matrix(steps, true_type{}, false_type{});
         if (!late) lds_barrier();
         lds_barrier();
     }
@@ -1668,16 +1681,16 @@ static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len, bool many,
 // numbers choose, not of the row alone.
 //
 // Trees have few rows next to long sequences, and rarely fill the card: what counts is the longest block of either kernel, in
-// narrow steps of 32 tokens, of which a wide one of 64 takes 7 (fp16 10, heads of 256 11).  A narrow tile costs 12
+// narrow steps of 32 tokens, of which a wide one of 64 takes 7 (fp16 10, at heads of 64 6.5; heads of 256 8).  A narrow tile costs 12
 // steps beside its own, a wide block 6, and 16 of its steps at the least.  Of 519 sizes (1 to 48 sequences of 8 to 200 nodes
-// after 500 to 30000 tokens, all head sizes, 1 to 16 heads to a key head) that chose the faster but for 1% of the time in the mean and 1.36
-// times at the most.  D = 128, bf16, 32 heads over 4, few and many: 1 tree of 16 nodes after 2000 21 and 67 us, after
-// 30000 41 and 53; 1 of 200 after 8000 99 and 60; 4 of 64 after 2000 35 and 71, after 8000 99 and 58; 48 of 8 after 8000 172 and 261,
+// after 500 to 30000 tokens, all head sizes, 1 to 16 heads to a key head) that chose the faster but for 1% of the time in the mean and 1.5
+// times at the most.  D = 128, bf16, 32 heads over 4, few and many: 1 tree of 16 nodes after 2000 21 and 58 us, after
+// 8000 27 and 43; 1 of 200 after 8000 99 and 60; 4 of 64 after 2000 36 and 71, after 8000 99 and 58; 48 of 8 after 8000 171 and 232,
 // of 31 509 and 262.  One launch for all: 32 trees of 16 nodes in the mean after 4200 123 us, each by the kernel that suits it, in two
 // launches, 129; 64 of 32 after 1000 154 and 187.
 static bool tree_wide(const KvBatch &b, int n_heads, int max_len, bool bf16) {
     const AttnPlan few = attn_plan(b, n_heads, max_len, false, 0, INT32_MAX), many = attn_plan(b, n_heads, max_len, true, 0, INT32_MAX);
-    const int width = b.D == 256 ? 11 : bf16 ? 7 : 10;
+    const double width = b.D == 256 ? 8 : bf16 ? 7 : b.D == 64 ? 6.5 : 10;
     const double all = (double)b.n_tokens * (n_heads / b.n_kv), seqs = 0.5 * b.n_seqs;
     const double blocks = std::max(1, (b.D == 256 ? 256 : 512) / b.n_kv), wide_blocks = std::max(1, 256 / b.n_kv);
     const double narrow = (all / few.cols + seqs) * (max_len / 32.0 + 12.0) / blocks;
