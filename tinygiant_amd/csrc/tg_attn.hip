@@ -311,20 +311,22 @@ __global__ __launch_bounds__(256) void k_kv_read(KvBatch b, _Float16 *k, _Float1
 
 // ================================================================ keep
 // The token that a walk through a draft tree kept as its i-th to place i of the tree, codes and scales as they are.  A
-// wave has one key head of one sequence and layer and goes through the places in order: entry i comes from path[i] >= i,
-// so no place is written before what it held is read, and entries may be read together.
+// wave has one key head of one sequence in KEEP_LAYERS layers and goes through the places in order: entry i comes from path[i] >=
+// i, so no place is written before what it held is read.
 //
-// Bound by latency where there are few: cu and kv_len, path and count, the table, and the entries themselves (1 user, 48 layers of 4
-// heads of 128: 4.3 us); otherwise by lines: of 144 bytes of a token and head, codes lie in some ten lines of a tile, read and written
-// (64 users: 18 us, some 20 lines of 128 bytes an entry, 5 TB/s).  The lengths by themselves in a launch behind it: 1 user 10.1 us a call, 6.6 so.
+// Bound by latency: cu and kv_len, path and count, the table, and the entries themselves, of all its layers at once.
+// 64 users, 48 layers of 4 heads of 128, a layer to a wave 18.2 us (more waves than the card holds at once, entries four at a
+// time), four layers 10.5; 1 user 4.6 either way.  The lengths by a launch of their own: 1 user 10.1 us a call, 6.6 so.
+constexpr int KEEP_LAYERS = 4;
 template <int D>
 __global__ __launch_bounds__(256) void k_kv_keep(KvBatch b, KeepArgs a) {
     constexpr int NG = D / 32, KW = D / 8, VH = D / 4, ITEMS = KW + VH + 2 * NG;  // K words, V halfwords, scales of a token
     constexpr int PER = (ITEMS + 63) / 64;
     const int lane = threadIdx.x % 64;
     const uint32_t unit = blockIdx.x * 4 + uni(threadIdx.x / 64), pair = unit / b.n_kv;  // below 2^26, as the launch checks
-    const int hk = unit - pair * b.n_kv, layer = pair / b.n_seqs, s = pair - layer * b.n_seqs;
-    if (layer >= a.n_layers) return;
+    const int hk = unit - pair * b.n_kv, group = pair / b.n_seqs, s = pair - group * b.n_seqs;
+    const int layer = group * KEEP_LAYERS, layers = min(KEEP_LAYERS, a.n_layers - layer);
+    if (layers <= 0) return;
     const int lo = max(b.cu[s], 0), n = max(b.cu[s + 1], lo) - lo, base = max(b.kv_len[s], 0) - n;
     const int count = min(max(a.count[s], 0), min(n, a.path_cols));
     if (a.kv_len && a.kv_len != b.kv_len && layer == 0 && hk == 0 && lane == 0) a.kv_len[s] = max(base + count, 0);
@@ -343,39 +345,33 @@ __global__ __launch_bounds__(256) void k_kv_keep(KvBatch b, KeepArgs a) {
         const int i = i0 + lane, from = i < count ? a.path[(int64_t)s * a.path_stride + i] : i;
         const int to_page = i < count && from != i ? page_of(b, s, base + i) : -1;
         const int from_page = to_page >= 0 && from > i && from < n ? page_of(b, s, base + from) : -1;
-        // four entries at a time, all of their loads before the first store
-        for (uint64_t todo = __ballot(to_page >= 0); todo;) {
-            uint32_t v[4][PER];
-            uint8_t *tt[4];
-            int t[4], live[4];
+        for (uint64_t todo = __ballot(to_page >= 0); todo; todo &= todo - 1) {
+            const int e = __builtin_ctzll(todo);
+            const int tp = __builtin_amdgcn_readlane(to_page, e), fp = __builtin_amdgcn_readlane(from_page, e);
+            const int t = base + i0 + e, f = fp < 0 ? t : base + __builtin_amdgcn_readlane(from, e);
+            uint8_t *tt = pages + tile_at<D>(b, tp, hk, t % b.page_tokens / 16);
+            const uint8_t *ft = pages + tile_at<D>(b, fp < 0 ? tp : fp, hk, f % b.page_tokens / 16);
+            uint32_t v[KEEP_LAYERS][PER];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                live[q] = todo != 0;
-                const int e = todo ? __builtin_ctzll(todo) : 0;
-                todo &= todo - 1;
-                const int tp = __builtin_amdgcn_readlane(to_page, e), fp = __builtin_amdgcn_readlane(from_page, e);
-                t[q] = base + i0 + e;
-                const int f = base + __builtin_amdgcn_readlane(from, e);
-                if (!live[q]) continue;
-                tt[q] = pages + tile_at<D>(b, tp, hk, t[q] % b.page_tokens / 16);
-                const uint8_t *ft = fp < 0 ? tt[q] : pages + tile_at<D>(b, fp, hk, f % b.page_tokens / 16);
+            for (int q = 0; q < KEEP_LAYERS; q++)
 #pragma unroll
                 for (int k = 0; k < PER; k++) {
-                    const int item = min(lane + 64 * k, ITEMS - 1), fr = at(item, (fp < 0 ? t[q] : f) % 16);
-                    if (item < KW) v[q][k] = *reinterpret_cast<const uint32_t *>(ft + fr);
-                    else v[q][k] = *reinterpret_cast<const uint16_t *>(ft + fr);
+                    const int item = min(lane + 64 * k, ITEMS - 1);
+                    const uint8_t *p = ft + min(q, layers - 1) * a.layer_bytes + at(item, f % 16);
+                    if (item < KW) v[q][k] = *reinterpret_cast<const uint32_t *>(p);
+                    else v[q][k] = *reinterpret_cast<const uint16_t *>(p);
                     if (fp < 0 && item >= KW + VH) v[q][k] = 0x7E00;  // an entry that is none: NaN for scales
                 }
-            }
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if (!live[q]) break;
+            for (int q = 0; q < KEEP_LAYERS; q++) {
+                if (q >= layers) break;
 #pragma unroll
                 for (int k = 0; k < PER; k++) {
-                    const int item = lane + 64 * k, to = at(item, t[q] % 16);
+                    const int item = lane + 64 * k;
                     if (item >= ITEMS) break;
-                    if (item < KW) *reinterpret_cast<uint32_t *>(tt[q] + to) = v[q][k];
-                    else *reinterpret_cast<uint16_t *>(tt[q] + to) = (uint16_t)v[q][k];
+                    uint8_t *p = tt + q * a.layer_bytes + at(item, t % 16);
+                    if (item < KW) *reinterpret_cast<uint32_t *>(p) = v[q][k];
+                    else *reinterpret_cast<uint16_t *>(p) = (uint16_t)v[q][k];
                 }
             }
         }
@@ -1624,7 +1620,7 @@ hipError_t launch_kv_read(const KvBatch &b, void *k, void *v, hipStream_t st) {
 }
 
 hipError_t launch_kv_keep(const KvBatch &b, const KeepArgs &a, hipStream_t st) {
-    const int64_t grid = ((int64_t)b.n_seqs * b.n_kv * a.n_layers + 3) / 4;
+    const int64_t grid = ((int64_t)b.n_seqs * b.n_kv * ((a.n_layers + KEEP_LAYERS - 1) / KEEP_LAYERS) + 3) / 4;
     if (grid > UINT32_MAX / 256) return hipErrorInvalidValue;
     if (a.n_layers) TG_BY_DIM(b.D, TG_LAUNCH(k_kv_keep<DIM>, dim3((unsigned)grid), dim3(256), 0, st, b, a));
     if (a.kv_len && (a.kv_len == b.kv_len || !a.n_layers)) TG_LAUNCH(k_kv_keep_len, dim3((b.n_seqs + 255) / 256), dim3(256), 0, st, b, a);

@@ -779,7 +779,7 @@ __global__ __launch_bounds__(256, 2) void k_verify_walk(VerifyArgs a, bool alone
 
 // The sweeps that the walks of the last launch ask for, a block to a piece of a sequence's row, and the walks behind them.
 // Bound by latencies, the state, the rows, two joins, the count and then the walk's own: 11 us of a sweep of 4 sequences, 28 of one of 32
-// pairs of rows of 151936 (17.5 alone, half of it the exponentials, and the walk's launch behind it 9).  Four blocks to a CU in place of three put 16
+// pairs of rows of 151936 (17.5 alone, and the walk's launch behind it 9).  Four blocks to a CU in place of three put 16
 // registers to scratch: 4 drawn trees 118 us, 82 so.
 template <int TYPE>
 __global__ __launch_bounds__(256, 3) void k_verify_sweep(VerifyArgs a, bool alone) {
