@@ -767,14 +767,14 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(256, 2) void k_verify_walk(VerifyArgs a, bool alone) {
+__global__ __launch_bounds__(256, 2) void k_verify_walk(VerifyArgs a) {
     __shared__ float smf[4];
     __shared__ double smd[4];
     __shared__ uint64_t two[V_TABLE];
     const int s = blockIdx.x;
     if (threadIdx.x < V_TABLE) exp_table(two, threadIdx.x);
     if (threadIdx.x == 0) a.swept[s] = 0;
-    walk<TYPE>(a, s, WalkState{}, Pieces<TYPE>(a, exp_of(factor_of(uni(temperature_of(a, s))), two), smf, smd), true, alone);
+    walk<TYPE>(a, s, WalkState{}, Pieces<TYPE>(a, exp_of(factor_of(uni(temperature_of(a, s))), two), smf, smd), true, false);
 }
 
 // The sweeps that the walks of the last launch ask for, a block to a piece of a sequence's row, and the walks behind them.
@@ -856,7 +856,7 @@ hipError_t launch_verify(VerifyArgs a, int type, void *ws, hipStream_t st) {
         constexpr int TYPE = decltype(T)::value;
         const size_t lds = WalkNodes::bytes(a.t.max_nodes, a.pieces);
         if (grid.x) TG_LAUNCH(k_verify_rows<TYPE>, grid, dim3(256), 0, st, a);
-        TG_LAUNCH(k_verify_walk<TYPE>, dim3((unsigned)a.t.n_seqs), dim3(256), lds, st, a, rounds == 0);
+        TG_LAUNCH(k_verify_walk<TYPE>, dim3((unsigned)a.t.n_seqs), dim3(256), lds, st, a);
         for (int i = 1; i <= rounds; i++) TG_LAUNCH(k_verify_sweep<TYPE>, dim3((unsigned)(a.t.n_seqs * a.pieces)), dim3(256), lds, st, a, i == rounds);
     };
     if (type == TG_T_F32) launch(std::integral_constant<int, TG_T_F32>{});
