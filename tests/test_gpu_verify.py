@@ -193,6 +193,19 @@ def test_everything_rejected():
     assert got.tokens[:, 0].tolist() == [int(np.searchsorted(np.cumsum(p[i]), u, side="right")) for i, u in ((0, 0.4), (1, 0.9))]
 
 
+def test_more_rejections_than_sweeps_have_launches():
+    """Siblings that the target never says: 23 sums over the row, and 19 before one that it may."""
+    gpu_note("verify many rejections")
+    for seed in range(4):
+        s = Step(310 + seed, [24, 9, 24], 5000, "f32", True, 1.0, "tree", 24)
+        s.parents[0], s.parents[2] = [-1] + [0] * 23, [-1] + [0] * 20 + [1, 20, 20]
+        for i, last in ((0, 24), (2, 20)):
+            s.logits[s.cu[i], torch.from_numpy(s.tokens[s.cu[i] + 1:s.cu[i] + last]).long()] = -np.inf
+        got = s.run()
+        s.check(got)
+        assert int(got.count[0]) == 1
+
+
 @pytest.mark.parametrize("with_draft", [True, False])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), "all -inf"])
 def test_rows_that_are_no_logits(bad, with_draft):
