@@ -661,10 +661,16 @@ TG_DEV uint32_t tree_window(const uint32_t *bits, int words, int j) {
     const int w = j >> 5;
     return __builtin_amdgcn_alignbit(tree_word(bits, words, w + 1), tree_word(bits, words, w), j & 31);
 }
-// A token that a row of a tree does not see; the row's own place, where its own bit is clear, says that it is no node of
-// the tree, and makes NaN of it.
-TG_DEV float tree_hides(float s, bool seen, int t, int pos) {
-    return t > pos ? -INFINITY : seen ? s : t == pos ? __builtin_nanf("") : -INFINITY;
+// The last place that a row at place p visits.  Rows of a tree that are behind the table visit the first place there, as far as
+// tokens_seen goes: unlike causal ones they need not see the token that is missing there.
+template <bool TREE>
+TG_DEV int last_place(const KvBatch &b, int p) {
+    return TREE ? min(p, b.table_cols * b.page_tokens) : p;
+}
+// A token that a row of a tree does not see.  Its last place, if it does not see that, says that the row is no node of the
+// tree or that its own token is behind the table, and makes NaN of it.
+TG_DEV float tree_hides(float s, bool seen, int t, int last) {
+    return t > last ? -INFINITY : seen ? s : t == last ? __builtin_nanf("") : -INFINITY;
 }
 
 // One step of 32 tokens of one key head as a lane holds it: tiles x = 0, 1
@@ -745,7 +751,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_attn_sp
         const int f = ct.tile * 16 + c, last = min(ct.n * G - 1, ct.tile * 16 + 15);
         const bool col = f < ct.n * G;
         const int row = ct.lo + (col ? f / G : 0), head = hk * G + (col ? f % G : 0);
-        const int pos = col ? ct.len - ct.n + f / G : -1;
+        const int pos = col ? last_place<TREE>(b, ct.len - ct.n + f / G) : -1;
         // what every column sees ends at the first one's position, of trees before their first node
         const int seen = uni(tokens_seen(b, ct, last / G)), all = uni(ct.len - ct.n + (TREE ? -1 : (ct.tile * 16) / G));
         const bool first = ct.at <= over;
@@ -1151,7 +1157,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
     for (int c = 0; c < NC; c++) {
         const int f = f0 + 16 * c + c16;
         const bool col = f < ncol;
-        pos[c] = col ? ct.len - ct.n + f / G : -1;
+        pos[c] = col ? last_place<TREE>(b, ct.len - ct.n + f / G) : -1;
         const uint16_t *qp = static_cast<const uint16_t *>(q.p) + (int64_t)(ct.lo + (col ? f / G : 0)) * q.stride +
                              (int64_t)(hk * G + (col ? f % G : 0)) * D;
 #pragma unroll
