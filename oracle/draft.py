@@ -55,7 +55,7 @@ def walk(logits, tokens, u, parent, t, draft=None, max_nodes=1024):
     be drawn).  Each rejected sibling leaves norm(max(r - q, 0)) of what was left, or r without its token where no one
     drew it."""
     V, n = logits.shape[1], min(len(parent), max_nodes)
-    if not n:
+    if not n or parent[0] != -1:
         return [], []
     at, path, out = 0, [0], []
     while True:

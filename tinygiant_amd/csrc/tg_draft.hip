@@ -430,7 +430,7 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
     auto join = [&](int j0) {
         // those that something follows, of greedy sequences all
         const int link = j0 + lane < n ? a.links[lo + j0 + lane] : -1;
-        const bool asked = j0 + lane < n && (greedy || link & 1);
+        const bool asked = link >= 0 && (greedy || link & 1);
         const uint64_t asks = __ballot(asked);
         if (asked) inner[wave][__builtin_popcountll(asks & ((1ull << lane) - 1))] = (uint8_t)lane;
         wave_lds_sync();
@@ -495,7 +495,9 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
         }
         __syncthreads();
     };
+    bool none = !n;  // or node 0 is no node, so that none of the rows was summed
     if (begin) {
+        none = none || a.links[lo] < 0;
         for (int j = tid; j < n; j += 256) {
             const int p = parent_of(a.t, lo, j), x = a.tokens[lo + j];
             const bool ok = p >= 0 && x >= 0 && x < V;
@@ -532,7 +534,8 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
 
     int at = begin ? 0 : uni(w.at), kept = begin ? 1 : uni(w.kept), joined = begin ? 0 : uni(w.joined), next = -1;
     bool swept = !begin;  // this launch goes on behind a sweep
-    for (; kept <= n;) {
+    none = sure(none);
+    for (; kept <= n && !none;) {
         const int row = lo + at, kid = child(at, at);
         int yes = -1;
         if (at >= joined) {
@@ -757,7 +760,7 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
     }
     __syncthreads();
     if (tid == 0) a.states[s].asks = 0;
-    if (!n) kept = 0;
+    if (none) kept = 0;
     int32_t *out = a.out + (size_t)s * N, *path = a.path + (size_t)s * N;
     for (int j = tid; j < N; j += 256) {
         path[j] = j < kept ? d.way[j] : -1;
