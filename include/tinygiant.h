@@ -541,9 +541,12 @@ int tg_kv_append_tree_q4_dev(const tg_kv_batch *b, const int32_t *depth,
                              const float *rope_sin, int max_pos, void *stream);
 /* tg_attn_q4_dev for nodes: a row sees the tokens before the batch's, and of
  * the batch's those whose bits are set among its words (1 to 32 a row) up to
- * itself.  A row whose own bit is clear is NaN.  Everything else, the
- * workspace too, as there; with the bits of a chain the results are its, but
- * for roundings where a tree's sizes choose another kernel. */
+ * itself.  A row whose own bit is clear is NaN.  workspace: at least
+ * tg_attn_tree_q4_workspace bytes.  Everything else as there; with the bits of
+ * a chain the results are its, but for roundings where a tree's sizes choose
+ * another kernel. */
+size_t tg_attn_tree_q4_workspace(const tg_kv_batch *b, int n_heads,
+                                 int max_len);
 int tg_attn_tree_q4_dev(const tg_kv_batch *b, const uint32_t *bits, int words,
                         int type, const void *q, int64_t q_stride, int n_heads,
                         float scale, void *out, int64_t out_stride,

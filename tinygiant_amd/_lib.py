@@ -108,6 +108,7 @@ NEW_SYMBOLS = [
     ("tg_attn_q4_dev", CI, [VP, CI, VP, I64, CI, CF, VP, I64, CI, VP, SZ, VP]),
     ("tg_draft_tree_dev", CI, [VP, VP, VP, VP, VP]),
     ("tg_kv_append_tree_q4_dev", CI, [VP, VP, CI, VP, I64, VP, I64, VP, I64, VP, I64, CI, VP, VP, CF, VP, VP, CI, VP]),
+    ("tg_attn_tree_q4_workspace", SZ, [VP, CI, CI]),
     ("tg_attn_tree_q4_dev", CI, [VP, VP, CI, CI, VP, I64, CI, CF, VP, I64, CI, VP, SZ, VP]),
     ("tg_kv_keep_q4_dev", CI, [VP, CI, I64, VP, I64, CI, VP, VP, VP]),
     ("tg_verify_workspace", SZ, [VP, CI]),

@@ -257,7 +257,8 @@ class PagedKV:
         if not T or not batch.n_seqs:
             return out
         ref = ctypes.byref(b)
-        n = require_lib().tg_attn_q4_workspace(ref, heads, batch.max_len)
+        size = require_lib().tg_attn_q4_workspace if tree is None else require_lib().tg_attn_tree_q4_workspace
+        n = size(ref, heads, batch.max_len)
         ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         args = (TYPES[dt], q.data_ptr(), qs, heads, D ** -0.5 if scale is None else float(scale), out.data_ptr(), os_,
                 batch.max_len, ws.data_ptr() if n else None, n)

@@ -2601,7 +2601,13 @@ static int attn_args(const char *fn, const tg_kv_batch *b, int n_heads, int *max
 extern "C" size_t tg_attn_q4_workspace(const tg_kv_batch *b, int n_heads, int max_len) {
     tg::KvBatch kb;
     if (attn_args("tg_attn_q4_workspace", b, n_heads, &max_len, &kb)) return 0;
-    return tg::attn_workspace(kb, n_heads, max_len);
+    return tg::attn_workspace(kb, n_heads, max_len, false);
+}
+
+extern "C" size_t tg_attn_tree_q4_workspace(const tg_kv_batch *b, int n_heads, int max_len) {
+    tg::KvBatch kb;
+    if (attn_args("tg_attn_tree_q4_workspace", b, n_heads, &max_len, &kb)) return 0;
+    return tg::attn_workspace(kb, n_heads, max_len, true);
 }
 
 static int attn(const char *fn, const tg_kv_batch *b, const uint32_t *bits, int words, int type, const void *q,
@@ -2617,7 +2623,7 @@ static int attn(const char *fn, const tg_kv_batch *b, const uint32_t *bits, int 
     if ((rc = kv_rows(fn, "out", out, out_stride, n_heads, kb.D, type, 8))) return rc;
     if (!(scale > 0.0f && scale < INFINITY)) return set_err(TG_E_INVALID, "%s: scale %g", fn, (double)scale);
     if (!kb.n_tokens || !kb.n_seqs) return TG_OK;
-    const size_t need = tg::attn_workspace(kb, n_heads, max_len);
+    const size_t need = tg::attn_workspace(kb, n_heads, max_len, bits);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return set_err(TG_E_INVALID, "%s: workspace of %zu bytes, %zu and 16-byte alignment needed", fn,
                        workspace ? workspace_bytes : (size_t)0, need);

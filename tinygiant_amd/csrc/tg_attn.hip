@@ -1719,11 +1719,11 @@ static size_t attn_join_bytes(const KvBatch &b, const AttnPlan &p) {
 }
 
 // Enough for rows of either type; a call's launches use it one after the other.
-size_t attn_workspace(const KvBatch &b, int n_heads, int max_len) {
+size_t attn_workspace(const KvBatch &b, int n_heads, int max_len, bool tree) {
     size_t most = 0;
-    for (const int kind : {0, 1, 2, 3}) {
+    for (const bool bf16 : {false, true}) {
         AttnPlan p[2];
-        for (int i = attn_plans(b, n_heads, max_len, kind & 1, kind & 2, p) - 1; i >= 0; i--)
+        for (int i = attn_plans(b, n_heads, max_len, bf16, tree, p) - 1; i >= 0; i--)
             if (p[i].share) most = std::max(most, attn_join_bytes(b, p[i]) + (size_t)p[i].parts * b.n_kv * (p[i].cols * (b.D + 2)) * sizeof(float));
     }
     return most;

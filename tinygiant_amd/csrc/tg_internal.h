@@ -412,7 +412,7 @@ struct AppendArgs {
 };
 hipError_t launch_kv_append(const KvBatch &b, int type, const AppendArgs &a, hipStream_t st);
 hipError_t launch_kv_read(const KvBatch &b, void *k, void *v, hipStream_t st);
-size_t attn_workspace(const KvBatch &b, int n_heads, int max_len);
+size_t attn_workspace(const KvBatch &b, int n_heads, int max_len, bool tree);
 hipError_t launch_attn(const KvBatch &b, int type, KvRows q, int n_heads, float scale, void *out, int64_t out_stride,
                        int max_len, void *ws, hipStream_t st);
 // Entries of the tokens path[s][0 .. count[s]) of the sequences' last cu[s + 1] - cu[s] tokens to the first places of
