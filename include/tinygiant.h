@@ -577,7 +577,8 @@ int tg_kv_keep_q4_dev(const tg_kv_batch *b, int n_layers, int64_t layer_bytes,
  * running sum of what p has become (as it was at first where nothing is
  * left) passes u[cu[s]] times the whole.  T of 0 or below (or NaN): p is 1 at
  * the first of the largest logits, and draft and u count for nothing.  As
- * decided in 64 bits.
+ * decided in 64 bits, in which a token that is less likely than 2^-1000 times
+ * the likeliest may count for nothing.
  * out_tokens, path [n_seqs][max_nodes], count [n_seqs]: path[s][0..count[s])
  * are the kept nodes, node 0 first; out_tokens[s] the tokens of those behind
  * it, then the next token; -1 behind them.  The next token is -1 where a row

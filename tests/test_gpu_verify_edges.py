@@ -31,3 +31,23 @@ def test_a_sequence_whose_first_node_is_none(with_draft, t):
         got = s.run()
         s.check(got)
         assert got.count.tolist()[1:4] == [0, 0, 0] and int(got.count[5]) == 0 and int(got.count[0]) >= 1
+
+
+@pytest.mark.parametrize("gap", [7.2, 7.3])
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_a_random_number_of_0_draws_a_token(gap, dt):
+    """Values of which a chunk's own largest is exp(-500) of the row's, and others before it that are nothing next to that:
+    a number of 0 draws the first token whose exponential is one of 64 bits' normal numbers."""
+    gpu_note(f"verify u of 0 {gap}")
+    for kids in (0, 1):
+        s = Step(910, [1 + kids, 1 + kids], 9000, dt, False, 0.01, "chain", 2, ban=0.0)
+        x = torch.full((s.T, 9000), -gap)
+        x[:, 2048 + 77] = -5.0
+        x[:, 5000] = 0.0
+        s.logits = x.to(s.dt)
+        s.tokens[:] = 7000                     # not kept: nothing of a chance
+        s.u[:] = 0.5
+        s.u[s.cu[:-1]] = 0.0
+        got = s.run()
+        assert got.count.tolist() == [1, 1]
+        assert got.tokens[:, 0].tolist() == [2048 + 77] * 2

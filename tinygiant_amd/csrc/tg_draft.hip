@@ -624,10 +624,15 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
                 if (!sure(d.u[0] >= 0.0 && d.u[0] < 1.0)) break;
                 // what is left, by pieces: a sweep's sums, or the row's own
                 bool of_rest = with_q && kid >= 0, without = !with_q && kid >= 0;
+                // A piece's sum is relative to its chunk's largest value: one that is next to nothing may be of elements that
+                // are each 0 next to the row's largest.  From 2^-1000 on it has one of 2^-1011 at least, and, where less than
+                // 15 / 16 are taken off below, of 2^-1015, which Exp64 does not make 0.
                 auto own_weights = [&]() {
                     __syncthreads();
-                    for (int k = tid; k < a.pieces; k += 256)
-                        d.weight[k] = a.sum[(size_t)row * 2 * a.pieces + k] * exp64((double)a.top[(size_t)row * 2 * a.chunks + k / V_PER] - w.Mp);
+                    for (int k = tid; k < a.pieces; k += 256) {
+                        const double z = a.sum[(size_t)row * 2 * a.pieces + k] * exp64((double)a.top[(size_t)row * 2 * a.chunks + k / V_PER] - w.Mp);
+                        d.weight[k] = z < 0x1p-1000 ? 0.0 : z;
+                    }
                     __syncthreads();
                 };
                 // the candidates that were rejected (all), one after the other: their tokens and exponentials
