@@ -408,8 +408,9 @@ struct WalkNodes {
 // leave, the row of a leaf): it asks for a sweep of it and leaves what it knows in memory.  The next launch has a block to
 // each piece, and the last of them to be done goes on with the walk: no block waits for another.  With `alone` the block does its
 // sweeps itself, a piece after the other.
-// What decides where the walk goes is the same in all of its lanes, and told so to the compiler (uni, sure): with branches by
-// lanes, what it moved between registers behind a loop was moved with all lanes off, and lost (rejected tokens were drawn).
+// What decides where the walk goes is the same in all of its lanes, and told so to the compiler (uni, sure), and every loop
+// has a counter that is the same in all of them (each, by_lanes): with loops that lanes left one after the other, what it
+// moved between registers behind such a loop was moved with all lanes off, and lost (rejected tokens were drawn).
 template <int TYPE>
 TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &piece_of, bool begin, bool alone) {
     extern __shared__ __align__(16) uint8_t lds[];
@@ -424,6 +425,18 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
     const int n = uni(min(r.n, N)), lo = uni(r.lo);
     const WalkNodes d(lds, N, a.pieces);
     u32x4 *held = reinterpret_cast<u32x4 *>(a.held + (size_t)s * a.held_bytes);
+    // f(i) for each i below n, by the block, or from `first` on by `width` lanes: the loop itself is the same in all lanes
+    auto each = [&](int n, auto f) {
+#pragma unroll 1
+        for (int i0 = 0; i0 < n; i0 += 256)
+            if (i0 + tid < n) f(i0 + tid);
+    };
+    auto by_lanes = [&](int first, int n, int lane, int width, auto f) {
+#pragma unroll 1
+        for (int i0 = first; i0 < n; i0 += width)
+            if (i0 + lane < n) f(i0 + lane);
+    };
+    auto copy = [&](u32x4 *to, const u32x4 *from) { each((int)(a.held_bytes / 16), [&](int i) { to[i] = from[i]; }); };
 
     // Largest values and sums of the rows of nodes j0 .. j0 + 63, from those of their chunks: half a wave to a row, four
     // rows at a time.  For a greedy sequence the first of the largest stands in the place of the draft's logits.
@@ -444,11 +457,12 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
                 const int i = min(i0 + lane / 32, units - 1);
                 const float *top = a.top + row_at(i);
                 float m = -INFINITY;
-                for (int k = l; k < a.chunks + l; k += 32) m = fmaxf(m, top[min(k, a.chunks - 1)]);
+                by_lanes(0, a.chunks, l, 32, [&](int k) { m = fmaxf(m, top[k]); });
                 m = half_max(m, lane);
                 int best = INT32_MAX;
-                for (int k = l; k < a.chunks + l; k += 32)
-                    if (k < a.chunks && top[k] == m) best = min(best, a.arg[row_at(i) / 2 + k]);
+                by_lanes(0, a.chunks, l, 32, [&](int k) {
+                    if (top[k] == m) best = min(best, a.arg[row_at(i) / 2 + k]);
+                });
 #pragma unroll
                 for (int k = 1; k < 32; k *= 2) best = min(best, __shfl_xor(best, k));
                 if (l == 0) d.top[node_at(i)] = m, d.e[N + node_at(i)] = best;
@@ -474,31 +488,27 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
                 if (i0 + 8 * b >= units) break;
                 const int i = min(i0 + 8 * b + lane / 32, units - 1);
                 float t = fmaxf(m[b][0], m[b][1]);
-                if (a.chunks > 64)
-                    for (int k = 64 + l; k < a.chunks + l; k += 32) t = fmaxf(t, a.top[row_at(i) + min(k, a.chunks - 1)]);
+                by_lanes(64, a.chunks, l, 32, [&](int k) { t = fmaxf(t, a.top[row_at(i) + k]); });
                 t = half_max(t, lane);
                 double y = z[b][0] * exp64((double)m[b][0] - t) + z[b][1] * exp64((double)m[b][1] - t);
-                if (a.chunks > 64)
-#pragma unroll 1
-                    for (int k = 64 + l; k < a.chunks + l; k += 32)
-                        y += k < a.chunks ? a.whole[row_at(i) + k] * exp64((double)a.top[row_at(i) + k] - t) : 0.0;
+                by_lanes(64, a.chunks, l, 32, [&](int k) { y += a.whole[row_at(i) + k] * exp64((double)a.top[row_at(i) + k] - t); });
                 y = half_add(y, lane);
                 if (l == 0) d.top[node_at(i)] = t, d.inv[node_at(i)] = 1.0 / y;
             }
         }
         __syncthreads();
-        for (int j = j0 + 1 + tid; j < n; j += 256) {
+        each(n, [&](int j) {
             const int p = d.par[j];
-            if (p < j0 || p >= j0 + 64) continue;
+            if (p < j0 || p >= j0 + 64) return;
             d.e[j] = exp64(d.e[j] - d.top[p]);
             if (with_q) d.e[N + j] = exp64(d.e[N + j] - d.top[N + p]);
-        }
+        });
         __syncthreads();
     };
     bool none = !n;  // or node 0 is no node, so that none of the rows was summed
     if (begin) {
         none = none || a.links[lo] < 0;
-        for (int j = tid; j < n; j += 256) {
+        each(n, [&](int j) {
             const int p = parent_of(a.t, lo, j), x = a.tokens[lo + j];
             const bool ok = p >= 0 && x >= 0 && x < V;
             d.par[j] = (int16_t)p, d.tok[j] = x, d.u[j] = a.u[lo + j];
@@ -506,15 +516,15 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
                 d.e[j] = ok ? load1<TYPE>(piece_of.row_p(lo + p), x) : -INFINITY;
                 if (with_q) d.e[N + j] = ok ? load1<TYPE>(piece_of.row_q(lo + p), x) : -INFINITY;
             }
-        }
+        });
         if (tid == 0) d.way[0] = 0;
     } else {
-        for (int i = tid; i < a.held_bytes / 16; i += 256) reinterpret_cast<u32x4 *>(lds)[i] = held[i];
+        copy(reinterpret_cast<u32x4 *>(lds), held);
         __syncthreads();
-        for (int k = tid; k < a.pieces; k += 256) {
+        each(a.pieces, [&](int k) {
             d.weight[k] = seen_now(a.swept_sum + (size_t)s * a.pieces + k);
             if (w.leaf) d.most[k] = seen_now(a.swept_top + (size_t)s * a.pieces + k);
-        }
+        });
     }
     __syncthreads();
     // the next child of `node` behind j, or -1: the same in every wave, like all that follows
@@ -528,7 +538,7 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
     auto no_number = [](float m) { return m == INFINITY || m == -INFINITY; };
     auto total_of = [&]() {  // of the pieces' weights
         double z = 0.0;
-        for (int k = lane; k < a.pieces; k += 64) z += d.weight[k];
+        by_lanes(0, a.pieces, lane, 64, [&](int k) { z += d.weight[k]; });
         return wave_add(z);
     };
 
@@ -579,7 +589,7 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
                         w.iq = c * iq;
                         if (!alone) {
                             __syncthreads();
-                            for (int i = tid; i < a.held_bytes / 16; i += 256) held[i] = reinterpret_cast<u32x4 *>(lds)[i];
+                            copy(held, reinterpret_cast<u32x4 *>(lds));
                             w.c = c, w.k = k, w.at = at, w.kept = kept, w.joined = joined, w.asks = 1;
                             if (tid == 0) a.states[s] = w;
                             return;
@@ -629,10 +639,10 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
                 // 15 / 16 are taken off below, of 2^-1015, which Exp64 does not make 0.
                 auto own_weights = [&]() {
                     __syncthreads();
-                    for (int k = tid; k < a.pieces; k += 256) {
+                    each(a.pieces, [&](int k) {
                         const double z = a.sum[(size_t)row * 2 * a.pieces + k] * exp64((double)a.top[(size_t)row * 2 * a.chunks + k / V_PER] - w.Mp);
                         d.weight[k] = z < 0x1p-1000 ? 0.0 : z;
-                    }
+                    });
                     __syncthreads();
                 };
                 // the candidates that were rejected (all), one after the other: their tokens and exponentials
@@ -648,11 +658,11 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
                 };
                 if (kid < 0) {
                     float m = -INFINITY;
-                    for (int k = lane; k < a.pieces; k += 64) m = fmaxf(m, d.most[k]);
+                    by_lanes(0, a.pieces, lane, 64, [&](int k) { m = fmaxf(m, d.most[k]); });
                     m = uni(wave_max(m));
                     if (no_number(m)) break;
                     w.Mp = m;
-                    for (int k = tid; k < a.pieces; k += 256) d.weight[k] *= exp64((double)d.most[k] - w.Mp);
+                    each(a.pieces, [&](int k) { d.weight[k] *= exp64((double)d.most[k] - w.Mp); });
                     __syncthreads();
                 } else if (without) {
                     // without the rejected tokens, which are taken off.  A piece of which less than a 16th is left, so that
@@ -767,10 +777,10 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
     if (tid == 0) a.states[s].asks = 0;
     if (none) kept = 0;
     int32_t *out = a.out + (size_t)s * N, *path = a.path + (size_t)s * N;
-    for (int j = tid; j < N; j += 256) {
+    each(N, [&](int j) {
         path[j] = j < kept ? d.way[j] : -1;
         out[j] = j + 1 < kept ? d.tok[d.way[j + 1]] : j + 1 == kept ? next : -1;
-    }
+    });
     if (tid == 0) a.count[s] = kept;
 }
 
