@@ -1,9 +1,10 @@
-"""Draft trees at the edges of what a cache holds, on the GPU: trees that go on behind the page table's end, and pages that
-are not there, in the tokens before a tree and inside it."""
+"""Draft trees at the edges of what a cache holds, on the GPU: trees that go on behind the page table's end, pages that are
+not there, in the tokens before a tree and inside it, and entries kept in more layers than a wave takes at once."""
 import numpy as np
 import pytest
 import torch
 
+from oracle import attn as A
 from oracle import draft as R
 from tests.conftest import gpu_note
 from tests.test_gpu_attn import Setup, dev
@@ -107,3 +108,35 @@ def test_a_second_tree_behind_a_table_of_768_tokens():
     kv.append(0, None, new, new, b, tree=tree)
     nan = torch.isnan(kv.attend(0, q, b, tree=tree).float()).flatten(1)
     assert nan[cu[1] + first:].all() and not nan[:cu[1] + first].any()
+
+
+@pytest.mark.parametrize("D,n_kv,page,lens,news,layers,layer,n_layers", [
+    (128, 4, 16, [60, 9], [16, 3], 5, 0, 5), (64, 3, 32, [200, 70, 40, 33], [33, 9, 0, 30], 8, 0, 8), (256, 1, 16, [90, 300], [64, 5], 9, 0, 9),
+    (128, 2, 48, [100 + 3 * i for i in range(20)], [1 + i % 9 for i in range(20)], 7, 1, 6), (64, 2, 16, [50, 31], [9, 4], 11, 2, 7)], ids=str)
+def test_keep_of_many_layers(D, n_kv, page, lens, news, layers, layer, n_layers):
+    """More layers than a wave has at once, groups that are full and that are not; the layers beside them stay as they were."""
+    gpu_note(f"keep {layers} layers from {layer} on {n_layers}")
+    s = Setup(layers, D, n_kv, page, lens, news, layers=layers)
+    paths, count = np.full((len(lens), max(news)), 999, np.int32), np.zeros(len(lens), np.int32)
+    for i, n in enumerate(news):
+        kept = sorted(s.rng.choice(n, size=s.rng.integers(1, n + 1), replace=False)) if n else []
+        paths[i, :len(kept)], count[i] = kept, len(kept)
+    s.kv.keep(s.batch, dev(paths), dev(count), layer=layer, n_layers=n_layers)
+    for at in range(layer, layer + n_layers):
+        c = A.Cache(len(s.cache.pages), page, n_kv, D, s.all[at])
+        for i, n in enumerate(lens):
+            R.keep(c, s.table[i], n, news[i], paths[i, :count[i]])
+    assert np.array_equal(s.kv.pages.cpu().numpy(), s.all)
+
+
+@pytest.mark.parametrize("case", SIZES + [(128, 4, 8, 64, 9000, 40, "bf16")], ids=str)
+def test_the_same_tree_gives_the_same_bits(case):
+    D, n_kv, G, page, n, new, dt = case
+    gpu_note(f"attend tree again {case}")
+    s = Setup(n, D, n_kv, page, [n, n // 2, 11], [new, 7, 3])
+    q, _ = s.rows(n_kv * G, dt)
+    tree = tree_of(s, [random_tree(s.rng, k) for k in (new, 7, 3)], 320)
+    want = s.kv.attend(0, q, s.batch, tree=tree)
+    for _ in range(4):
+        s.rows(n_kv * G, dt)[0].sum().item()
+        assert torch.equal(s.kv.attend(0, q, s.batch, tree=tree), want)

@@ -1,8 +1,10 @@
 """Verification of drafted tokens at the edges of what its arguments may hold, on the GPU."""
+import numpy as np
 import pytest
 import torch
 
 from tests.conftest import gpu_note
+from tests.test_gpu_attn import dev
 from tests.test_gpu_verify import Step
 
 pytestmark = pytest.mark.gpu
@@ -51,3 +53,45 @@ def test_a_random_number_of_0_draws_a_token(gap, dt):
         got = s.run()
         assert got.count.tolist() == [1, 1]
         assert got.tokens[:, 0].tolist() == [2048 + 77] * 2
+
+
+@pytest.mark.parametrize("V,with_draft,t", [(262145, True, 1.0), (262145, False, 0.7), (262145, True, 0.0), (600001, True, 0.8),
+                                            (600001, False, 1.0), (600001, False, 0.0), (1 << 20, True, [0.0, 1.0, 0.5])])
+def test_more_chunks_than_lanes(V, with_draft, t):
+    """Rows of more than 64 chunks (from 262145 tokens on) and 256 pieces: what decides stands behind them, the largest
+    value, kept drafts and the token that is drawn."""
+    gpu_note(f"verify {V} {with_draft} {t}")
+    s = Step(V % 1000, [4, 3, 1], V, "f32", with_draft, t, "tree", 4, ban=0.0)
+    for x in (s.logits, s.draft):
+        if x is not None:
+            x[:, 262143:] += 3.0 if V > 262145 else 16.0
+    if V > 262145:
+        at = s.rng.integers(262144, V, s.T)
+        s.logits[torch.arange(s.T), torch.from_numpy(at)] = 14.0
+        for i, p in enumerate(s.parents):
+            for j in range(1, s.nodes[i]):
+                if j % 2:
+                    s.tokens[s.cu[i] + j] = at[s.cu[i] + p[j]]
+    s.u[s.cu[:-1]] = [0.999, 0.97, 0.9999]
+    got = s.run()
+    count = s.check(got)
+    last = got.tokens.cpu().numpy()[np.arange(3), count - 1]
+    assert (last >= 262143).all(), last
+
+
+@pytest.mark.parametrize("with_draft,t", [(True, 1.0), (False, 1.0), (True, 0.0)])
+def test_trees_of_fewer_rows_than_counted(with_draft, t):
+    """Rows that end before cu does: a tree whose first nodes are there is walked over those, one of which none is there has
+    count 0."""
+    from tinygiant_amd.draft import DraftTree
+    gpu_note(f"verify cut off {with_draft} {t}")
+    for T in (0, 1, 9, 13, 14):
+        s = Step(920, [9, 5, 4], 700, "f32", with_draft, t, "tree", 9)
+        tree = DraftTree(dev(s.cu), T, dev(np.concatenate(s.parents).astype(np.int32)[:T]), max_nodes=9)
+        used_memory(0x7F)
+        got = s.run(logits=s.logits[:T].cuda(), tokens=dev(s.tokens[:T]), u=dev(s.u[:T]), draft=s.draft[:T].cuda() if with_draft else None, tree=tree)
+        s.nodes = [max(0, min(n, T - at)) for n, at in zip(s.nodes, s.cu)]
+        s.parents = [p[:n] for p, n in zip(s.parents, s.nodes)]
+        whole, s.cu = s.cu, np.concatenate([[0], np.cumsum(s.nodes)]).astype(np.int32)
+        assert (s.cu[1:] == np.minimum(whole[1:], T)).all()
+        s.check(got)
