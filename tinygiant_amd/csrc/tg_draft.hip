@@ -251,8 +251,9 @@ TG_DEV float block_max(float v, float *sm) {
 // or +inf: the largest is +inf.
 //
 // Bound by reading where there are rows enough: 64 chains of up to 7 nodes, 151936 tokens, fp32, target's and draft's rows: 33 us, 5 TB/s;
-// 5 rows of 304 KB of each 5.4 us, launch, load and two joins.  Chunks of 4096 against 2048 and 8192: 35.4, 43.6 and 36.7 us, 5.2, 4.6 and 6.9.  Rows are loaded before it
-// is known whether they are asked for where all blocks are there at once: one latency less.
+// 5 rows of 304 KB of each 5.4 us, launch, load and two joins.  Chunks of 4096 against 2048 and 8192: 35.4, 43.6 and 36.7 us, 5.2, 4.6 and 6.9.  Rows
+// loaded before it is known whether they are asked for: chains of 5, 13 and 54, bf16, 5.4, 8.4 and 20.0 us, 5.3, 7.7 and 20.2
+// so; trees of 13 and 54, fp32, most of whose nodes nothing follows, 6.3 and 15.2, 5.5 and 13.4 so.
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_verify_rows(VerifyArgs a) {
     __shared__ float sm[4];
@@ -263,17 +264,13 @@ __global__ __launch_bounds__(256) void k_verify_rows(VerifyArgs a) {
     const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks, of = blockIdx.y;
     const void *p = of ? row_of<TYPE>(a.draft, a.draft_stride, row) : row_of<TYPE>(a.logits, a.stride, row);
     float v[V_PER][8], m = -INFINITY;
-    auto load = [&]() {
-        load_stretch<TYPE, V_PER, V_PIECE>(p, chunk * V_CHUNK + threadIdx.x * 8, (chunk + 1) * V_CHUNK, a.vocab, v);
-    };
-    if (a.early) load();
     if (threadIdx.x < V_TABLE) exp_table(two, threadIdx.x);
     const int link = uni(a.links[row]);  // twice the sequence, and whether something follows
     if (link < 0 || link / 2 >= a.t.n_seqs) return;
     const float t = uni(temperature_of(a, link / 2));
     const bool greedy = !(t > 0.0f);
     if (greedy ? of : !(link & 1)) return;
-    if (!a.early) load();
+    load_stretch<TYPE, V_PER, V_PIECE>(p, chunk * V_CHUNK + threadIdx.x * 8, (chunk + 1) * V_CHUNK, a.vocab, v);
     bool bad = false;
 #pragma unroll
     for (int k = 0; k < V_PER; k++)
@@ -864,7 +861,6 @@ size_t verify_workspace(const DraftTrees &t, int vocab) {
 hipError_t launch_verify(VerifyArgs a, int type, void *ws, hipStream_t st) {
     verify_layout(a, static_cast<uint8_t *>(ws));
     const dim3 grid((unsigned)(a.t.n_tokens * a.chunks), a.draft ? 2 : 1);
-    a.early = grid.x * grid.y <= 1024;
     // Sweeps: none where all are greedy; one where a walk ends with its first, as every one without a draft model's logits
     // and every chain's does; of trees as many as a walk may have, but V_ROUNDS at the most, the rest by the walk's block
     // alone, which takes a tenth of a ms each.  (4 trees of 26 nodes drawn from a draft model, 151936 tokens, of whose walks few need

@@ -452,7 +452,6 @@ struct VerifyArgs {
     const float *temps;
     float temp;
     int32_t *out, *path, *count;
-    bool early;        // rows are loaded before it is known whether they are asked for
     // the workspace
     int chunks, pieces;
     double *sum;       // [n_tokens][target, draft][pieces]
