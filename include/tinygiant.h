@@ -556,43 +556,45 @@ int tg_attn_tree_q4_dev(const tg_kv_batch *b, const uint32_t *bits, int words,
  * path_stride apart): the i-th one's entry is moved, as it is, from its own
  * place to that of node i, in n_layers layers from pages on, layer_bytes
  * apart.  path[s][i] is at least i, as a walk from node 0 leaves it; an entry
- * that is below i or no row of the sequence makes NaN of the token at place i.  kv_len (n_seqs, NULL: none; may be the
- * batch's own, but overlap it in no other way) gets the sequences' lengths
- * without the nodes that were not kept.  n_tokens counts for nothing; pages
- * that a call moves tokens in or out of belong to one sequence. */
+ * that is below i or no row of the sequence makes NaN of the token at place i.
+ * kv_len (n_seqs, NULL: none; may be the batch's own, but overlap it in no
+ * other way) gets the sequences' lengths without the nodes that were not kept.
+ * n_tokens counts for nothing; pages that a call moves tokens in or out of
+ * belong to one sequence. */
 int tg_kv_keep_q4_dev(const tg_kv_batch *b, int n_layers, int64_t layer_bytes,
                       const int32_t *path, int64_t path_stride, int path_cols,
                       const int32_t *count, int32_t *kv_len, void *stream);
 /* Which drafted tokens a target keeps.  links are tg_draft_tree_dev's of the
- * same trees.  logits [n_tokens][vocab] (any element
- * type, rows stride elements apart) are the target's after each row, draft
- * (NULL, or the same type and shape) those of the model that the tokens were
- * drawn from, tokens[row] the drafts, u[row] random numbers in [0, 1).  With p
- * = softmax(logits / T), q = softmax(draft / T), T temperature, or
- * temperatures[s] where given: from node 0 on, the children of a node are
- * asked in order.  The first one x is kept where u q(x) < p(x); one that is not
- * makes max(p - q, 0), divided by its sum, the p of the next (without draft: kept where u <
- * p(x), and p without x, divided by its sum).  The walk goes on at a kept
- * child.  Where none is, or a node has none, the next token is the first whose
- * running sum of what p has become (as it was at first where nothing is
- * left) passes u[cu[s]] times the whole.  T of 0 or below (or NaN): p is 1 at
- * the first of the largest logits, and draft and u count for nothing.  As
- * decided in 64 bits, in which a token that is less likely than 2^-1000 times
- * the likeliest may count for nothing.
+ * same trees, whose cu and parent this call reads again: they have not changed
+ * since.  logits [n_tokens][vocab] (any element type, rows stride elements
+ * apart) are the target's after each row, draft (NULL, or the same type and
+ * shape) those of the model that the tokens were drawn from, tokens[row] the
+ * drafts, u[row] random numbers in [0, 1).  With p = softmax(logits / T), q =
+ * softmax(draft / T), T temperature, or temperatures[s] where given: from node
+ * 0 on, the children of a node are asked in order.  The first one x is kept
+ * where u q(x) < p(x); one that is not makes max(p - q, 0), divided by its
+ * sum, the p of the next (without draft: kept where u < p(x), and p without x,
+ * divided by its sum).  The walk goes on at a kept child.  Where none is, or a
+ * node has none, the next token is the first whose running sum of what p has
+ * become (as it was at first where nothing is left) passes u[cu[s]] times the
+ * whole.  T of 0 or below (or NaN): p is 1 at the first of the largest logits,
+ * and draft and u count for nothing.  As decided in 64 bits, in which a token
+ * that is less likely than 2^-1000 times the likeliest may count for nothing.
  * out_tokens, path [n_seqs][max_nodes], count [n_seqs]: path[s][0..count[s])
  * are the kept nodes, node 0 first; out_tokens[s] the tokens of those behind
  * it, then the next token; -1 behind them.  The next token is -1 where a row
  * that it, or the choice of a child, is decided by holds NaN or +inf or
- * nothing but -inf, or where u[cu[s]] is not in [0, 1).  Draft tokens outside the vocabulary
- * are not kept.  A sequence without rows, or whose node 0 is not part of its
- * tree: count 0.  vocab up to 2^20.
- * temperature is below infinity.  workspace: at least tg_verify_workspace
- * bytes, 16-byte aligned, free again when the call's work is done. */
+ * nothing but -inf, or where u[cu[s]] is not in [0, 1).  Draft tokens outside
+ * the vocabulary are not kept.  A sequence without rows, or whose node 0 is
+ * not part of its tree: count 0.  vocab up to 2^20.  temperature is below
+ * infinity.  workspace: at least tg_verify_workspace bytes, 16-byte aligned,
+ * free again when the call's work is done. */
 size_t tg_verify_workspace(const tg_draft_trees *t, int vocab);
 int tg_verify_dev(const tg_draft_trees *t, const int32_t *links, int type,
                   const void *logits, int64_t stride, const void *draft,
-                  int64_t draft_stride, int vocab, const int32_t *tokens, const double *u,
-                  float temperature, const float *temperatures,
+                  int64_t draft_stride, int vocab, const int32_t *tokens,
+                  const double *u, float temperature,
+                  const float *temperatures,
                   int32_t *out_tokens, int32_t *path, int32_t *count,
                   void *workspace, size_t workspace_bytes, void *stream);
 /* out [M][N] = x [M][K] times int8 weights w [N][K] (scale w_scale[n] per

@@ -311,12 +311,13 @@ __global__ __launch_bounds__(256) void k_kv_read(KvBatch b, _Float16 *k, _Float1
 
 // ================================================================ keep
 // The token that a walk through a draft tree kept as its i-th to place i of the tree, codes and scales as they are.  A
-// wave has one key head of one sequence in KEEP_LAYERS layers and goes through the places in order: entry i comes from path[i] >=
-// i, so no place is written before what it held is read.
+// wave has one key head of one sequence in KEEP_LAYERS layers and goes through the places in order: entry i comes from
+// path[i] >= i, so no place is written before what it held is read.
 //
-// Bound by latency: cu and kv_len, path and count, the table, and the entries themselves, of all its layers at once.
-// 64 users, 48 layers of 4 heads of 128, a layer to a wave 18.2 us (more waves than the card holds at once, entries four at a
-// time), four layers 10.5; 1 user 4.6 either way.  The lengths by a launch of their own: 1 user 10.1 us a call, 6.6 so.
+// Bound by latency: cu and kv_len, path and count, the table, and then the entries, those of all its layers at once but
+// one after the other, 0.6 us each: 1 user, 48 layers of 4 heads of 128, 4 entries moved 5.8 us, 16 13, 64 44, 256 166.
+// 64 users with a few each, a layer to a wave 18.2 us (more waves than the card holds at once, entries four at a time),
+// four layers 10.5; 1 user 4.6 either way.  The lengths by a launch of their own: 1 user 10.1 us a call, 6.6 so.
 constexpr int KEEP_LAYERS = 4;
 template <int D>
 __global__ __launch_bounds__(256) void k_kv_keep(KvBatch b, KeepArgs a) {
@@ -661,14 +662,14 @@ TG_DEV uint32_t tree_window(const uint32_t *bits, int words, int j) {
     const int w = j >> 5;
     return __builtin_amdgcn_alignbit(tree_word(bits, words, w + 1), tree_word(bits, words, w), j & 31);
 }
-// The last place that a row at place p visits.  Rows of a tree that are behind the table visit the first place there, as far as
-// tokens_seen goes: unlike causal ones they need not see the token that is missing there.
+// The last place that a row at place p visits.  Rows of a tree that are behind the table visit the first place there,
+// as far as tokens_seen goes: unlike causal ones they need not see the token that is missing there.
 template <bool TREE>
 TG_DEV int last_place(const KvBatch &b, int p) {
     return TREE ? min(p, b.table_cols * b.page_tokens) : p;
 }
-// A token that a row of a tree does not see.  Its last place, if it does not see that, says that the row is no node of the
-// tree or that its own token is behind the table, and makes NaN of it.
+// A token that a row of a tree does not see.  Its last place, if it does not see that, says that the row is no node of
+// the tree or that its own token is behind the table, and makes NaN of it.
 TG_DEV float tree_hides(float s, bool seen, int t, int last) {
     return t > last ? -INFINITY : seen ? s : t == last ? __builtin_nanf("") : -INFINITY;
 }
@@ -1431,8 +1432,8 @@ __global__ __launch_bounds__(512, 2) void k_attn_tile(KvBatch b, KvRows q, int G
             }
             lds_barrier();
         }
-        // a wave without columns, of which trees leave many, does its share of the codes alone: 16 trees of 16 nodes, half a tile
-        // each, after 8000 tokens 71 us, 84 with all of the products
+        // a wave without columns, of which trees leave many, does its share of the codes alone: 16 trees of 16 nodes,
+        // half a tile each, after 8000 tokens 71 us, 84 with all of the products
         if (TREE && f0 >= ncol) {
             for (int i = 0; i < steps; i++) {
                 const int next = i + (late ? 2 : 1);
@@ -1668,28 +1669,28 @@ static AttnPlan attn_plan(const KvBatch &b, int n_heads, int max_len, bool many,
     return p;
 }
 
-// The launches of a call, one or two.  The mean number of columns of a sequence says which kernel takes all of
-// them.  16 sequences of up to 4096
-// tokens, D = 128, few against many: 64 columns 42 and 50 us, 96 51 and 52, 128 53 and 54, 256 88 and 59; one of
-// 16000: 128 43 and 56, 256 51 and 61; 200 of up to 1000: 128 117 and 129, 256 203 and 127; D = 64, 16 of up to
-// 8192: 64 72 and 88, 128 87 and 89.  fp16, whose many take longer: D = 128, 128 columns 56 and 74, 192 73 and 74,
-// 256 88 and 76; D = 64 128 88 and 109, 192 114 and 111, 256 137 and 114.  D = 256, bf16, 16 of up to 4096: 64 columns 55
-// and 72, 128 78 and 78, 192 103 and 83; fp16 has no wide tiles, its remainders do not fit LDS.
+// The launches of a call, one or two.  The mean number of columns of a sequence says which kernel takes all of them.
+// 16 sequences of up to 4096 tokens, D = 128, few against many: 64 columns 42 and 50 us, 96 51 and 52, 128 53 and 54,
+// 256 88 and 59; one of 16000: 128 43 and 56, 256 51 and 61; 200 of up to 1000: 128 117 and 129, 256 203 and 127; D =
+// 64, 16 of up to 8192: 64 72 and 88, 128 87 and 89.  fp16, whose many take longer: D = 128, 128 columns 56 and 74, 192
+// 73 and 74, 256 88 and 76; D = 64 128 88 and 109, 192 114 and 111, 256 137 and 114.  D = 256, bf16, 16 of up to 4096:
+// 64 columns 55 and 72, 128 78 and 78, 192 103 and 83; fp16 has no wide tiles, its remainders do not fit LDS.
 //
-// Where that is many, and the rows are so few next to the lengths that not all of more than 8 sequences can be prompts, single
-// tokens may be among them, to which a wide tile is a waste: each kernel takes those that are its.  A prompt of 2000 and 32
-// single tokens after 8192, 32 heads over 4: 133 us, 274 in one launch; after 4000 122 and 147; 8 chunks of 128, where
-// the second launch finds nothing to do: 84 and 79.  So a row's roundings are those of the kernel that its call's
-// numbers choose, not of the row alone.
+// Where that is many, and the rows are so few next to the lengths that not all of more than 8 sequences can be prompts,
+// single tokens may be among them, to which a wide tile is a waste: each kernel takes those that are its.  A prompt of
+// 2000 and 32 single tokens after 8192, 32 heads over 4: 133 us, 274 in one launch; after 4000 122 and 147; 8 chunks of
+// 128, where the second launch finds nothing to do: 84 and 79.  So a row's roundings are those of the kernel that its
+// call's numbers choose, not of the row alone.
 //
-// Trees have few rows next to long sequences, and rarely fill the card: what counts is the longest block of either kernel, in
-// narrow steps of 32 tokens, of which a wide one of 64 takes 7 (fp16 10, at heads of 64 6.5; heads of 256 8).  A narrow tile costs 12
-// steps beside its own, a wide block 6, and 16 of its steps at the least.  Of 519 sizes (1 to 48 sequences of 8 to 200 nodes
-// after 500 to 30000 tokens, all head sizes, 1 to 16 heads to a key head) that chose the faster but for 1% of the time in the mean and 1.5
-// times at the most.  D = 128, bf16, 32 heads over 4, few and many: 1 tree of 16 nodes after 2000 21 and 58 us, after
-// 8000 27 and 43; 1 of 200 after 8000 99 and 60; 4 of 64 after 2000 36 and 71, after 8000 99 and 58; 48 of 8 after 8000 171 and 232,
-// of 31 509 and 262.  One launch for all: 32 trees of 16 nodes in the mean after 4200 123 us, each by the kernel that suits it, in two
-// launches, 129; 64 of 32 after 1000 154 and 187.
+// Trees have few rows next to long sequences, and rarely fill the card: what counts is the longest block of either
+// kernel, in narrow steps of 32 tokens, of which a wide one of 64 takes 7 (fp16 10, at heads of 64 6.5; heads of 256
+// 8).  A narrow tile costs 12 steps beside its own, a wide block 6, and 16 of its steps at the least.  Of 519 sizes (1
+// to 48 sequences of 8 to 200 nodes after 500 to 30000 tokens, all head sizes, 1 to 16 heads to a key head) that chose
+// the faster but for 1% of the time in the mean and 1.5 times at the most.  D = 128, bf16, 32 heads over 4, few and
+// many: 1 tree of 16 nodes after 2000 21 and 58 us, after 8000 27 and 43; 1 of 200 after 8000 99 and 60; 4 of 64 after
+// 2000 36 and 71, after 8000 99 and 58; 48 of 8 after 8000 171 and 232, of 31 509 and 262.  One launch for all: 32
+// trees of 16 nodes in the mean after 4200 123 us, each by the kernel that suits it, in two launches, 129; 64 of 32
+// after 1000 154 and 187.
 static bool tree_wide(const KvBatch &b, int n_heads, int max_len, bool bf16) {
     const AttnPlan few = attn_plan(b, n_heads, max_len, false, 0, INT32_MAX), many = attn_plan(b, n_heads, max_len, true, 0, INT32_MAX);
     const double width = b.D == 256 ? 8 : bf16 ? 7 : b.D == 64 ? 6.5 : 10;

@@ -1,9 +1,8 @@
-// tg_draft.hip -- trees of drafted tokens on the device: which nodes each one
-// sees and how deep it stands, and which of the drafts a target's
-// probabilities keep.
+// tg_draft.hip -- trees of drafted tokens on the device: which nodes each one sees and how deep it stands, and which of
+// the drafts a target's probabilities keep.
 //
-// Node j of a sequence is row cu[s] + j of the batch; its parent is a node
-// before it, so a walk towards the root only goes down in j.
+// Node j of a sequence is row cu[s] + j of the batch; its parent is a node before it, so a walk towards the root only
+// goes down in j.
 #include "tg_device.h"
 #include "tg_internal.h"
 
@@ -30,9 +29,12 @@ TG_DEV int parent_of(const DraftTrees &t, int lo, int j) {
     return p >= DT_NONE && p < j ? p : DT_BAD;
 }
 
-// A block per sequence, a thread per node, which walks to its root through the parents in LDS and sets the bits of what it
-// meets, one word after the other.  Bound by latency: the rows' bounds, the parents, then a read of LDS a step, 1 us for
-// trees of ordinary depth.
+// A block per sequence, a thread per node, which walks to its root through the parents in LDS and sets the bits of what
+// it meets, one word after the other.  Bound by latency: the rows' bounds, the parents, then a dependent read of LDS a
+// step, so by the depth, and from 257 nodes on by the depths of the up to four nodes of a thread and the words that it
+// writes.  One tree of 16 nodes, 4 deep, 2.0 us (a launch that does nothing takes 1.7); 37 of up to 61, 7 deep, 3.3;
+// one of 512, 9 deep, 7.0, of 1024 21.6.  Chains, with parents or without: 5 nodes 1.9 us, 16 2.6, 64 7.5, 256 30, 1024
+// 291.
 __global__ __launch_bounds__(256) void k_draft_tree(DraftTrees t, uint32_t *bits, int32_t *depth, int32_t *links) {
     __shared__ int16_t par[DT_NODES];
     __shared__ uint8_t kids[DT_NODES];
@@ -80,11 +82,11 @@ hipError_t launch_draft_tree(const DraftTrees &t, uint32_t *bits, int32_t *depth
 // ================================================================ verification
 // One sequence's walk.  At a node, p = softmax(target's logits / T) and q the same of the draft's.  Its children x were
 // drawn from q, one after the other: x stays with probability r(x) / q(x) at the most 1, where r = p for the first, and
-// each one that does not stay leaves max(r - q, 0) / its sum for the next, so that whichever stays, or the token that is
-// drawn of what is left in the end, is distributed as p.  In closed form r = max(p - c q, 0) / Z with c = 0, Z = 1 at
-// first; one that does not stay makes c + Z of c, and Z the sum of max(p - c q, 0) for the new c: one number is kept of all
-// that were asked.  Without q the children are candidates that no one drew, kept with probability p(x) / (1 - what those
-// before them had), and what is left is p without them.
+// each one that does not stay leaves max(r - q, 0) / its sum for the next, so that whichever stays, or the token that
+// is drawn of what is left in the end, is distributed as p.  In closed form r = max(p - c q, 0) / Z with c = 0, Z = 1
+// at first; one that does not stay makes c + Z of c, and Z the sum of max(p - c q, 0) for the new c: one number is kept
+// of all that were asked.  Without q the children are candidates that no one drew, kept with probability p(x) / (1 -
+// what those before them had), and what is left is p without them.
 //
 // Whatever a random number decides is decided in 64 bits: probabilities, their sums and running sums.
 constexpr int V_CHUNK = 4096;  // values of a row to a block of the first launch
@@ -122,8 +124,8 @@ TG_DEV void load8(const void *row, int i, float v[8]) {
         }
     }
 }
-// N times 8 values, STEP apart, of a stretch of the row that ends at `end`: one branch around all of the loads, and a value
-// at a time, -inf behind the row's end, where the stretch passes it
+// N times 8 values, STEP apart, of a stretch of the row that ends at `end`: one branch around all of the loads, and a
+// value at a time, -inf behind the row's end, where the stretch passes it
 template <int TYPE, int N, int STEP>
 TG_DEV void load_stretch(const void *row, int i, int end, int V, float v[N][8]) {
     if (end <= V) {
@@ -145,10 +147,11 @@ TG_DEV const void *row_of(const void *p, int64_t stride, int row) {
     return static_cast<const uint8_t *>(p) + (int64_t)row * stride * (TYPE == TG_T_F32 ? 4 : 2);
 }
 
-// Exponentials of what is 0 or below, to some 2^-51: exp(d / T) = 2^(y / 32), y = d 32 log2(e) / T, is 2^(j / 32) from a
-// table times the power of 2 that the nearest whole number n = 32 i + j of y gives, times 2^(f / 32) for the rest f, at most 1/2, by
-// the polynomial of degree 5 that has its values at the six Chebyshev nodes (off by 2^-52.6, the constant rounded to 1).
-// Below 2^-1021 the result is 0.  13 operations on doubles; by the remainder of ln 2 and Taylor's polynomial 26.
+// Exponentials of what is 0 or below, to some 2^-51: exp(d / T) = 2^(y / 32), y = d 32 log2(e) / T, is 2^(j / 32) from
+// a table times the power of 2 that the nearest whole number n = 32 i + j of y gives, times 2^(f / 32) for the rest f,
+// at most 1/2, by the polynomial of degree 5 that has its values at the six Chebyshev nodes (off by 2^-52.6, the
+// constant rounded to 1).  Below 2^-1021 the result is 0.  13 operations on doubles; by the remainder of ln 2 and
+// Taylor's polynomial 26.
 constexpr int V_TABLE = 32;
 struct Exp64 {
     double by, least;     // 32 log2(e) / T; the least d whose exponential is not 0
@@ -250,10 +253,11 @@ TG_DEV float block_max(float v, float *sm) {
 // all), of the chunk and its pieces the sums of exp((v - largest) / T), or the place of the first of the largest.  NaN
 // or +inf: the largest is +inf.
 //
-// Bound by reading where there are rows enough: 64 chains of up to 7 nodes, 151936 tokens, fp32, target's and draft's rows: 33 us, 5 TB/s;
-// 5 rows of 304 KB of each 5.4 us, launch, load and two joins.  Chunks of 4096 against 2048 and 8192: 35.4, 43.6 and 36.7 us, 5.2, 4.6 and 6.9.  Rows
-// loaded before it is known whether they are asked for: chains of 5, 13 and 54, bf16, 5.4, 8.4 and 20.0 us, 5.3, 7.7 and 20.2
-// so; trees of 13 and 54, fp32, most of whose nodes nothing follows, 6.3 and 15.2, 5.5 and 13.4 so.
+// Bound by reading where there are rows enough: 64 chains of up to 7 nodes, 151936 tokens, fp32, target's and draft's
+// rows: 33 us, 5 TB/s; 5 rows of 304 KB of each 5.4 us, launch, load and two joins.  Chunks of 4096 against 2048 and
+// 8192: 35.4, 43.6 and 36.7 us, 5.2, 4.6 and 6.9.  Rows loaded before it is known whether they are asked for: chains of
+// 5, 13 and 54, bf16, 5.4, 8.4 and 20.0 us, 5.3, 7.7 and 20.2 so; trees of 13 and 54, fp32, most of whose nodes nothing
+// follows, 6.3 and 15.2, 5.5 and 13.4 so.
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_verify_rows(VerifyArgs a) {
     __shared__ float sm[4];
@@ -317,8 +321,8 @@ __global__ __launch_bounds__(256) void k_verify_rows(VerifyArgs a) {
     }
 }
 
-// One piece of a sweep, by a block: the sum of max(p - c q, 0) over it, or (leaf) its largest value and the sum of exp((v -
-// largest) / T).
+// One piece of a sweep, by a block: the sum of max(p - c q, 0) over it, or (leaf) its largest value and the sum of
+// exp((v - largest) / T).
 template <int TYPE>
 struct Pieces {
     const void *logits, *draft;
@@ -372,8 +376,8 @@ struct Pieces {
     }
 };
 
-// What blocks hand to each other goes past the caches of an XCD, and what is to be seen first is waited for (a release at
-// the device's scope writes back a whole L2).
+// What blocks hand to each other goes past the caches of an XCD, and what is to be seen first is waited for (a release
+// at the device's scope writes back a whole L2).
 template <class T>
 TG_DEV T seen_now(const T *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <class T>
@@ -401,13 +405,13 @@ struct WalkNodes {
     static constexpr size_t bytes(int nodes, int pieces) { return ((size_t)nodes * (5 * 8 + 3 * 4 + 2 * 2 + 1) + (size_t)pieces * (8 + 4) + 15) / 16 * 16; }
 };
 
-// A sequence's walk, by one block, up to the next sum over a whole row that it needs (what rejected siblings drawn from q
-// leave, the row of a leaf): it asks for a sweep of it and leaves what it knows in memory.  The next launch has a block to
-// each piece, and the last of them to be done goes on with the walk: no block waits for another.  With `alone` the block does its
-// sweeps itself, a piece after the other.
-// What decides where the walk goes is the same in all of its lanes, and told so to the compiler (uni, sure), and every loop
-// has a counter that is the same in all of them (each, by_lanes): with loops that lanes left one after the other, what it
-// moved between registers behind such a loop was moved with all lanes off, and lost (rejected tokens were drawn).
+// A sequence's walk, by one block, up to the next sum over a whole row that it needs (what rejected siblings drawn from
+// q leave, the row of a leaf): it asks for a sweep of it and leaves what it knows in memory.  The next launch has a
+// block to each piece, and the last of them to be done goes on with the walk: no block waits for another.  With `alone`
+// the block does its sweeps itself, a piece after the other.  What decides where the walk goes is the same in all of
+// its lanes, and told so to the compiler (uni, sure), and every loop has a counter that is the same in all of them
+// (each, by_lanes): with loops that lanes left one after the other, what it moved between registers behind such a loop
+// was moved with all lanes off, and lost (rejected tokens were drawn).
 template <int TYPE>
 TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &piece_of, bool begin, bool alone) {
     extern __shared__ __align__(16) uint8_t lds[];
@@ -422,7 +426,8 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
     const int n = uni(min(r.n, N)), lo = uni(r.lo);
     const WalkNodes d(lds, N, a.pieces);
     u32x4 *held = reinterpret_cast<u32x4 *>(a.held + (size_t)s * a.held_bytes);
-    // f(i) for each i below n, by the block, or from `first` on by `width` lanes: the loop itself is the same in all lanes
+    // f(i) for each i below n, by the block, or from `first` on by `width` lanes: the loop itself is the same in all
+    // lanes
     auto each = [&](int n, auto f) {
 #pragma unroll 1
         for (int i0 = 0; i0 < n; i0 += 256)
@@ -435,8 +440,8 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
     };
     auto copy = [&](u32x4 *to, const u32x4 *from) { each((int)(a.held_bytes / 16), [&](int i) { to[i] = from[i]; }); };
 
-    // Largest values and sums of the rows of nodes j0 .. j0 + 63, from those of their chunks: half a wave to a row, four
-    // rows at a time.  For a greedy sequence the first of the largest stands in the place of the draft's logits.
+    // Largest values and sums of the rows of nodes j0 .. j0 + 63, from those of their chunks: half a wave to a row,
+    // four rows at a time.  For a greedy sequence the first of the largest stands in the place of the draft's logits.
     auto join = [&](int j0) {
         // those that something follows, of greedy sequences all
         const int link = j0 + lane < n ? a.links[lo + j0 + lane] : -1;
@@ -568,8 +573,8 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
                 if (no_number(uni((float)w.Mp)) || no_number(uni((float)w.Mq))) break;
             }
             if (with_q || kid < 0) {
-                // each child that is rejected leaves a sweep's sums, by pieces: to the next one, or to be drawn from; as
-                // does the row of a leaf
+                // each child that is rejected leaves a sweep's sums, by pieces: to the next one, or to be drawn from;
+                // as does the row of a leaf
                 double c = swept ? w.c : 0.0, left = 1.0;
                 int k = swept ? uni(w.k) : kid;
                 for (;;) {
@@ -605,8 +610,8 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
                     left = total_of();
                 }
             } else {
-                // side by side: each candidate with what those before it have left; one whose token was asked before, or is
-                // none, has nothing
+                // side by side: each candidate with what those before it have left; one whose token was asked before,
+                // or is none, has nothing
                 double left = 1.0;
                 for (int k = at + 1; k < n && yes < 0; k += 64) {
                     const int j = min(k + lane, n - 1), x = d.tok[j];
@@ -631,9 +636,9 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
                 if (!sure(d.u[0] >= 0.0 && d.u[0] < 1.0)) break;
                 // what is left, by pieces: a sweep's sums, or the row's own
                 bool of_rest = with_q && kid >= 0, without = !with_q && kid >= 0;
-                // A piece's sum is relative to its chunk's largest value: one that is next to nothing may be of elements that
-                // are each 0 next to the row's largest.  From 2^-1000 on it has one of 2^-1011 at least, and, where less than
-                // 15 / 16 are taken off below, of 2^-1015, which Exp64 does not make 0.
+                // A piece's sum is relative to its chunk's largest value: one that is next to nothing may be of
+                // elements that are each 0 next to the row's largest.  From 2^-1000 on it has one of 2^-1011 at least,
+                // and, where less than 15 / 16 are taken off below, of 2^-1015, which Exp64 does not make 0.
                 auto own_weights = [&]() {
                     __syncthreads();
                     each(a.pieces, [&](int k) {
@@ -662,8 +667,8 @@ TG_DEV void walk(const VerifyArgs &a, int s, WalkState w, const Pieces<TYPE> &pi
                     each(a.pieces, [&](int k) { d.weight[k] *= exp64((double)d.most[k] - w.Mp); });
                     __syncthreads();
                 } else if (without) {
-                    // without the rejected tokens, which are taken off.  A piece of which less than a 16th is left, so that
-                    // what is left could be off by more than 2^-48, is summed again without them, by one wave.
+                    // without the rejected tokens, which are taken off.  A piece of which less than a 16th is left, so
+                    // that what is left could be off by more than 2^-48, is summed again without them, by one wave.
                     own_weights();
                     if (tid == 0) listed = 0;
                     __syncthreads();
@@ -792,10 +797,10 @@ __global__ __launch_bounds__(256, 2) void k_verify_walk(VerifyArgs a) {
     walk<TYPE>(a, s, WalkState{}, Pieces<TYPE>(a, exp_of(factor_of(uni(temperature_of(a, s))), two), smf, smd), true, false);
 }
 
-// The sweeps that the walks of the last launch ask for, a block to a piece of a sequence's row, and the walks behind them.
-// Bound by latencies, the state, the rows, two joins, the count and then the walk's own: 11 us of a sweep of 4 sequences, 28 of one of 32
-// pairs of rows of 151936 (17.5 alone, and the walk's launch behind it 9).  Four blocks to a CU in place of three put 16
-// registers to scratch: 4 drawn trees 118 us, 82 so.
+// The sweeps that the walks of the last launch ask for, a block to a piece of a sequence's row, and the walks behind
+// them.  Bound by latencies, the state, the rows, two joins, the count and then the walk's own: 11 us of a sweep of 4
+// sequences, 28 of one of 32 pairs of rows of 151936 (17.5 alone, and the walk's launch behind it 9).  Four blocks to a
+// CU in place of three put 16 registers to scratch: 4 drawn trees 118 us, 82 so.
 template <int TYPE>
 __global__ __launch_bounds__(256, 3) void k_verify_sweep(VerifyArgs a, bool alone) {
     __shared__ float smf[4];
@@ -861,10 +866,12 @@ size_t verify_workspace(const DraftTrees &t, int vocab) {
 hipError_t launch_verify(VerifyArgs a, int type, void *ws, hipStream_t st) {
     verify_layout(a, static_cast<uint8_t *>(ws));
     const dim3 grid((unsigned)(a.t.n_tokens * a.chunks), a.draft ? 2 : 1);
-    // Sweeps: none where all are greedy; one where a walk ends with its first, as every one without a draft model's logits
-    // and every chain's does; of trees as many as a walk may have, but V_ROUNDS at the most, the rest by the walk's block
-    // alone, which takes a tenth of a ms each.  (4 trees of 26 nodes drawn from a draft model, 151936 tokens, of whose walks few need
-    // more than 8 and none of 40 more than 10: 60 us where 4 are enough, 82 with 12; an idle launch takes 1.7.)
+    // Sweeps: none where all are greedy; one where a walk ends with its first, as every one without a draft model's
+    // logits and every chain's does; of trees as many as a walk may have, but V_ROUNDS at the most, the rest by the
+    // walk's block alone, which takes a tenth of a ms each.  What 40 calls each need, with siblings drawn from a draft
+    // model: 4 trees of 26 nodes 4 in the mean, 9 at the most; one of 26 2 and 6; one of 5 1 and 2; 64 of 16 8 and 9;
+    // 16 of 64 9 and 13, one more than there are launches in 4 of the 40.  An idle launch takes 1.7 us: the first of
+    // these would take 60 us with 4 where those are enough, and takes 70 to 82 with 12.
     const int rounds = !grid.x || (!a.temps && !(a.temp > 0.0f)) ? 0 : !a.draft || !a.t.parent ? 1 : std::min(V_ROUNDS, a.t.max_nodes);
     auto launch = [&](auto T) {
         constexpr int TYPE = decltype(T)::value;

@@ -42,9 +42,10 @@ class DraftTree:
     its words: node i; itself and those it follows), depth [n_tokens] int32
     how many it follows.  Rows that are no nodes (a parent that is no node
     before them, nodes from max_nodes on) have no bits and depth -1; what
-    attends them is NaN and nothing of them is appended.  The tensors are read
-    when build() is called: again after they were rewritten in place, which may be
-    captured into a graph."""
+    attends them is NaN and nothing of them is appended.  cu and parent are
+    read by build() and by verify: call build() again, which may be captured
+    into a graph, after they were rewritten in place, and do not rewrite them
+    between it and verify."""
 
     def __init__(self, cu, n_tokens: int, parent=None, max_nodes: int = 64):
         _index(cu, "cu", 1)
@@ -71,7 +72,7 @@ class DraftTree:
                       self.n_tokens, self.max_nodes)
 
     def build(self) -> "DraftTree":
-        """bits and depth from cu and parent as they now are."""
+        """bits, depth and links from cu and parent as they now are."""
         if self.n_tokens and self.n_seqs:
             run_on(self.depth, "tg_draft_tree_dev", ctypes.byref(self._trees()), self.bits.data_ptr(), self.depth.data_ptr(),
                    self.links.data_ptr())
