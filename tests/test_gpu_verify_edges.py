@@ -79,6 +79,14 @@ def test_more_chunks_than_lanes(V, with_draft, t):
     assert (last >= 262143).all(), last
 
 
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_the_largest_vocabulary_and_the_most_nodes(with_draft):
+    """2^20 tokens and trees that may have 1024 nodes: what a walk holds is as large as it gets."""
+    gpu_note(f"verify 2^20, 1024 {with_draft}")
+    s = Step(930, [3, 2], 1 << 20, "bf16", with_draft, 1.0, "tree", 1024, ban=0.0)
+    s.check(s.run())
+
+
 @pytest.mark.parametrize("with_draft,t", [(True, 1.0), (False, 1.0), (True, 0.0)])
 def test_trees_of_fewer_rows_than_counted(with_draft, t):
     """Rows that end before cu does: a tree whose first nodes are there is walked over those, one of which none is there has
