@@ -103,3 +103,15 @@ def test_trees_of_fewer_rows_than_counted(with_draft, t):
         whole, s.cu = s.cu, np.concatenate([[0], np.cumsum(s.nodes)]).astype(np.int32)
         assert (s.cu[1:] == np.minimum(whole[1:], T)).all()
         s.check(got)
+
+
+def test_logits_of_no_rows_have_any_strides():
+    from tinygiant_amd.draft import DraftTree, verify
+    gpu_note("verify no rows")
+    i, u = torch.zeros(0, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.float64, device="cuda")
+    tree = DraftTree(dev(np.zeros(3, np.int32)), 0, max_nodes=5)
+    for strides in ((0, 0), (9, 1), (1, 7)):
+        x = torch.zeros(0, device="cuda").as_strided((0, 9), strides)
+        for draft in (None, x):
+            got = verify(x, i, u, tree, draft=draft)
+            assert got.count.tolist() == [0, 0] and (got.tokens == -1).all() and (got.path == -1).all()

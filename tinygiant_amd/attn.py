@@ -151,13 +151,15 @@ class PagedKV:
             raise TypeError(f"{name} must be a {dtype} tensor on {self.device}")
         D, shape, stride = self.head_dim, t.shape, t.stride()
         if len(shape) == 3:
-            ok = shape[1] == heads and shape[2] == D and stride[2] == 1 and (heads == 1 or stride[1] == D)
+            ok = shape[1] == heads and shape[2] == D
+            packed = stride[2] == 1 and (heads == 1 or stride[1] == D)
         else:
-            ok = len(shape) == 2 and shape[1] == heads * D and stride[1] == 1
-        if not ok or shape[0] != n_tokens:
+            ok = len(shape) == 2 and shape[1] == heads * D
+            packed = ok and stride[1] == 1
+        if not ok or shape[0] != n_tokens or (n_tokens and not packed):
             raise ValueError(f"{name} of shape {tuple(shape)}, strides {stride}: "
                              f"[{n_tokens}, {heads}, {D}] with packed heads needed")
-        return heads * D if n_tokens == 1 else stride[0]  # of one row the stride is any
+        return heads * D if n_tokens <= 1 else stride[0]  # of one row the stride is any, of none all are
 
     def _heads(self, q):
         D = self.head_dim

@@ -94,7 +94,7 @@ def _logits(t, name, like=None):
         raise TypeError(f"{name} must be a [rows, vocab] float32, float16 or bfloat16 CUDA (HIP) tensor")
     if like is not None and (t.dtype != like.dtype or t.shape != like.shape or t.device != like.device):
         raise ValueError(f"{name} is {t.dtype} {tuple(t.shape)} on {t.device}, the logits {like.dtype} {tuple(like.shape)} on {like.device}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    if t.shape[0] and t.shape[1] > 1 and t.stride(1) != 1:  # of no rows the strides are any
         raise ValueError(f"{name} must have contiguous rows, its strides are {t.stride()}")
     return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
 
