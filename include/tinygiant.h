@@ -584,11 +584,12 @@ int tg_kv_keep_q4_dev(const tg_kv_batch *b, int n_layers, int64_t layer_bytes,
  * are the kept nodes, node 0 first; out_tokens[s] the tokens of those behind
  * it, then the next token; -1 behind them.  The next token is -1 where a row
  * that it, or the choice of a child, is decided by holds NaN or +inf or
- * nothing but -inf, or where u[cu[s]] is not in [0, 1).  Draft tokens outside
- * the vocabulary are not kept.  A sequence without rows, or whose node 0 is
- * not part of its tree: count 0.  vocab up to 2^20.  temperature is below
- * infinity.  workspace: at least tg_verify_workspace bytes, 16-byte aligned,
- * free again when the call's work is done. */
+ * nothing but -inf, or where u[cu[s]] is not in [0, 1); a draft whose u is not
+ * may stay or not.  Draft tokens outside the vocabulary are not kept.  A
+ * sequence without rows, or whose node 0 is not part of its tree: count 0.
+ * vocab up to 2^20.  temperature is below infinity.  workspace: at least
+ * tg_verify_workspace bytes, 16-byte aligned, free again when the call's work
+ * is done. */
 size_t tg_verify_workspace(const tg_draft_trees *t, int vocab);
 int tg_verify_dev(const tg_draft_trees *t, const int32_t *links, int type,
                   const void *logits, int64_t stride, const void *draft,

@@ -72,7 +72,7 @@ def walk(logits, tokens, u, parent, t, draft=None, max_nodes=1024):
                 if q is not None:
                     rest = np.maximum(share - q, 0)
                 continue
-            if u[j] * (1.0 if q is None else q[x]) < share[x]:
+            if (u[j] * (1.0 if q is None else q[x]) if t > 0 else 0.0) < share[x]:
                 at = j
                 break
             rest = rest.copy()

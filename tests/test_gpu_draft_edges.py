@@ -140,3 +140,17 @@ def test_the_same_tree_gives_the_same_bits(case):
     for _ in range(4):
         s.rows(n_kv * G, dt)[0].sum().item()
         assert torch.equal(s.kv.attend(0, q, s.batch, tree=tree), want)
+
+
+def test_one_column_of_any_stride():
+    """Of a path of one column, or a page table of one, the columns' stride counts for nothing."""
+    from tinygiant_amd.attn import KVBatch
+    gpu_note("keep and attend, one column")
+    s = Setup(8, 64, 2, 64, [40, 33, 64], [6, 9, 1])
+    table, path = (dev(x).reshape(1, -1).t() for x in (s.table, np.zeros(3, np.int32)))
+    assert table.stride() == path.stride() == (1, 3)
+    b = KVBatch(s.batch.cu, s.batch.kv_len, table, max_len=64)
+    q, _ = s.rows(4, "f16")
+    assert torch.equal(s.kv.attend(0, q, b), s.kv.attend(0, q, s.batch))
+    got = s.kv.keep(b, path, dev(np.ones(3, np.int32)), kv_len=torch.zeros(3, dtype=torch.int32, device="cuda"))
+    assert got.tolist() == [35, 25, 64]

@@ -115,3 +115,19 @@ def test_logits_of_no_rows_have_any_strides():
         for draft in (None, x):
             got = verify(x, i, u, tree, draft=draft)
             assert got.count.tolist() == [0, 0] and (got.tokens == -1).all() and (got.path == -1).all()
+
+
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_random_numbers_count_for_nothing_where_a_sequence_is_greedy(with_draft):
+    gpu_note(f"verify greedy u {with_draft}")
+    for u in (0.0, 1.0, 2.0, -1.0, float("nan"), float("inf")):
+        s = Step(940, [12, 30, 1, 5], 40, "f32", with_draft, [0.0, -2.0, float("nan"), 0.0], "tree", 30, spread=1.0)
+        for i, p in enumerate(s.parents):       # children that are the largest logits' tokens, so that walks are long
+            for j in range(1, len(p)):
+                if j % 2:
+                    s.tokens[s.cu[i] + j] = int(s.logits[s.cu[i] + p[j]].argmax())
+        want = s.run()
+        s.u[:] = u
+        got = s.run()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and int(got.count.max()) > 2
+        s.check(got)

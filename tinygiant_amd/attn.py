@@ -99,7 +99,7 @@ class KVBatch:
         n = kv_len.numel()
         if cu.numel() != n + 1 or table.shape[0] != n:
             raise ValueError(f"{n} sequences, {cu.numel()} row bounds, {table.shape[0]} table rows")
-        if not cu.is_contiguous() or not kv_len.is_contiguous() or (table.numel() and table.stride(1) != 1):
+        if not cu.is_contiguous() or not kv_len.is_contiguous() or (table.numel() and table.shape[1] > 1 and table.stride(1) != 1):
             raise TypeError("cu, kv_len and the rows of table must be contiguous")
         table_stride(table)
         if not cu.device == kv_len.device == table.device:
@@ -290,7 +290,7 @@ class PagedKV:
             raise ValueError(f"path on {path.device}, count on {count.device}, batch on {batch.device}, pages on {self.device}")
         if path.shape[0] != n or count.numel() != n or not cols:
             raise ValueError(f"{n} sequences, {count.numel()} counts, path of shape {tuple(path.shape)}")
-        if path.stride(1) != 1 or not count.is_contiguous():
+        if (cols > 1 and path.stride(1) != 1) or not count.is_contiguous():
             raise TypeError("count and the rows of path must be contiguous")
         stride = max(path.stride(0), cols) if n == 1 else path.stride(0)
         if kv_len is not None:

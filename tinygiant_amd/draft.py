@@ -119,8 +119,8 @@ def verify(logits, tokens, u, tree: DraftTree, draft=None, temperature=1.0) -> V
     tinygiant/engine.py:348-357, at top_p 1).  Decisions are those of 64-bit
     arithmetic.  Rows that hold NaN or +inf, or nothing but -inf: the next
     token is -1 where they decide (Sampler's errors, which a call that does
-    not wait cannot raise), as it is where node 0's u is not in [0, 1).  Drafts
-    outside the vocabulary do not stay.  A sequence without rows, or whose node
+    not wait cannot raise), as it is where node 0's u is not in [0, 1); a draft
+    whose u is not may stay or not.  Drafts outside the vocabulary do not stay.  A sequence without rows, or whose node
     0 is no node (its parent is not -1), has count 0."""
     stride = _logits(logits, "logits")
     dev, (T, V) = logits.device, logits.shape
