@@ -871,7 +871,7 @@ hipError_t launch_verify(VerifyArgs a, int type, void *ws, hipStream_t st) {
     // walk's block alone, which takes a tenth of a ms each.  What 40 calls each need, with siblings drawn from a draft
     // model: 4 trees of 26 nodes 4 in the mean, 9 at the most; one of 26 2 and 6; one of 5 1 and 2; 64 of 16 8 and 9;
     // 16 of 64 9 and 13, one more than there are launches in 4 of the 40.  An idle launch takes 1.7 us: the first of
-    // these would take 60 us with 4 where those are enough, and takes 70 to 82 with 12.
+    // these would take 60 us with 4 where those are enough, and takes 66 to 90, by its inputs, with 12.
     const int rounds = !grid.x || (!a.temps && !(a.temp > 0.0f)) ? 0 : !a.draft || !a.t.parent ? 1 : std::min(V_ROUNDS, a.t.max_nodes);
     auto launch = [&](auto T) {
         constexpr int TYPE = decltype(T)::value;
